@@ -54,6 +54,10 @@ typedef enum {
   LMX_FMT_INT8 = 7
 } lmx_format;
 
+/* Element types of activations where a call takes more than fp32 (the calls
+ * with float pointers take fp32 only). */
+typedef enum { LMX_F32 = 0, LMX_F16 = 1, LMX_BF16 = 2 } lmx_type;
+
 /* Activation rotation applied inside the GEMV before the table build. */
 #define LMX_ROTATE_NONE 0u
 /* Blockwise FWHT-256 with 1/16 scaling over the zero-padded activations,
@@ -177,6 +181,28 @@ int lmx_gemv(const lmx_weight *w, const float *x, float *y, size_t batch,
  * quant_bits <= 2, none otherwise; then y += bias when bias is not NULL. */
 int lmx_linear(const lmx_weight *w, const float *bias, const float *x,
                float *y, size_t batch, void *stream);
+/* A linear layer in 8-bit integers (no counterpart in the reference, whose
+ * activations stay fp32): every row of x [batch][cols] is rounded to codes c =
+ * round(127 x / amax) of its largest magnitude amax (ties to even, exactly), and
+ *   y[b][r] = (sum_k c[b][k] w[r][k]) * (amax[b] / 127) * w_scale[r] + bias[r],
+ * the sum exact, the rest fp32, rounded once to y's type.  w: signed bytes, row
+ * r at w + r * w_stride (w and w_stride multiples of 16; cols any number up to
+ * 131072; the bytes between cols and w_stride are not used); x, bias (or NULL)
+ * and y [batch][rows] have elements of `type` (lmx_type) and their own alignment
+ * only.  A row of x with an element that is not finite gives NaN.  y does not
+ * overlap x.  workspace: lmx_linear_i8_workspace bytes, 16-byte aligned, in any
+ * state; calls that may overlap in time need workspaces of their own.  Nothing
+ * is allocated: calls can be captured into a HIP graph. */
+int lmx_linear_i8_workspace(size_t rows, size_t cols, size_t batch, size_t *bytes);
+int lmx_linear_i8(const int8_t *w, size_t w_stride, const float *w_scale,
+                  const void *bias, const void *x, void *y, int type,
+                  size_t rows, size_t cols, size_t batch, void *workspace,
+                  size_t workspace_bytes, void *stream);
+/* The codes and scales of an 8-bit handle with one scale per row (group 0), as
+ * lmx_linear_i8 takes them: w [rows][w_stride] (bytes past cols set to 0),
+ * w_scale [rows], device buffers of the caller. */
+int lmx_weight_codes_i8(const lmx_weight *w, int8_t *codes, size_t w_stride,
+                        float *scales, void *stream);
 /* In-place blockwise FWHT-256 (transform.hpp:19 apply_hadamard_rotation);
  * n a multiple of 256 (whole chunks only, as the reference). */
 int lmx_fwht256(float *x, size_t n, void *stream);

@@ -34,7 +34,7 @@ EXPORTS = [
     "lmx_weight_create", "lmx_weight_from_blocks", "lmx_weight_destroy", "lmx_weight_info",
     "lmx_weight_kernel_config", "lmx_weight_read_tiles", "lmx_gemv", "lmx_linear", "lmx_fwht256",
     "lmx_precompute_luts", "lmx_extract_indices", "lmx_hbm_read_probe", "lmx_hbm_read_probe_shape",
-    "lmx_hbm_read_probe_tiles",
+    "lmx_hbm_read_probe_tiles", "lmx_linear_i8_workspace", "lmx_linear_i8", "lmx_weight_codes_i8",
     # include/lutmac_hip_compat.h
     "lmx_host_gemv", "lmx_host_lut_linear", "lmx_host_apply_hadamard_rotation",
     "lmx_host_precompute_luts", "lmx_host_precompute_lut", "lmx_host_extract_indices", "lmx_host_forget",
@@ -47,7 +47,12 @@ EXPORTS = [
     "lmx_quantize_int4", "lmx_quantize", "lmx_synth_int4_normal", "lmx_synth_normal",
     # include/lutmac_model.h
     "lmx_model_load", "lmx_model_destroy", "lmx_model_config", "lmx_model_decoder", "lmx_model_weight_format",
+    # include/lutmac_kv8.h
+    "lmx_kv8_append", "lmx_kv8_attention_workspace", "lmx_kv8_attention",
 ]
+
+# lmx_type (include/lutmac_hip.h): activations of the calls that take more than fp32
+F32, F16, BF16 = range(3)
 
 
 class DecoderConfigC(ctypes.Structure):
@@ -58,6 +63,19 @@ class DecoderConfigC(ctypes.Structure):
                 ("rope_theta", ctypes.c_float), ("rope_mode", ctypes.c_int), ("rope_factor", ctypes.c_float),
                 ("rope_low_freq_factor", ctypes.c_float), ("rope_high_freq_factor", ctypes.c_float),
                 ("rope_orig_max_pos", ctypes.c_size_t)]
+
+
+class Kv8CacheC(ctypes.Structure):
+    """lmx_kv8_cache (include/lutmac_kv8.h)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("n_pages", ctypes.c_size_t), ("n_kv_heads", ctypes.c_size_t),
+                ("head_dim", ctypes.c_size_t)]
+
+
+class Kv8BatchC(ctypes.Structure):
+    """lmx_kv8_batch (include/lutmac_kv8.h)."""
+    _fields_ = [("offsets", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("pages", ctypes.c_void_p),
+                ("n_seqs", ctypes.c_size_t), ("max_pages", ctypes.c_size_t), ("n_rows", ctypes.c_size_t)]
 
 
 class LmxError(RuntimeError):
@@ -129,6 +147,12 @@ _SIGS = {
     "lmx_host_precompute_lut": ([_p, _p], _i),
     "lmx_decoder_set_repetition_penalty": ([_p, ctypes.c_float], _i),
     "lmx_host_extract_indices": ([_p, _p, _sz, _p, _p], _i),
+    "lmx_linear_i8_workspace": ([_sz, _sz, _sz, ctypes.POINTER(_sz)], _i),
+    "lmx_linear_i8": ([_p, _sz, _p, _p, _p, _p, _i, _sz, _sz, _sz, _p, _sz, _p], _i),
+    "lmx_weight_codes_i8": ([_p, _p, _sz, _p, _p], _i),
+    "lmx_kv8_append": ([_p, _p, _i, _p, _sz, _p, _sz, _p, _sz, _p, _sz, _sz, _p, _sz, _p], _i),
+    "lmx_kv8_attention_workspace": ([_p, _p, _sz, ctypes.POINTER(_sz)], _i),
+    "lmx_kv8_attention": ([_p, _p, _i, _p, _sz, _sz, ctypes.c_float, _p, _sz, _p, _sz, _p], _i),
 }
 
 _LIB = None
@@ -198,6 +222,30 @@ def _current_stream():
 
 def _stream_ptr(stream):
     return _current_stream() if stream is None else stream.cuda_stream
+
+
+_TYPES = None
+
+
+def _types():
+    global _TYPES
+    if _TYPES is None:
+        import torch
+        _TYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+    return _TYPES
+
+
+def _on_current_device(*tensors):
+    """Raises unless the tensors (None: skipped) are on torch's current device,
+    where the calls launch."""
+    import torch
+    for t in tensors:
+        if t is not None and not t.is_cuda:
+            raise ValueError(f"expected device tensors, got one on {t.device}")
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != here:
+            raise ValueError(f"expected tensors on the current device cuda:{here}, got one on {t.device}")
 
 
 # ---- host-only helpers -----------------------------------------------------
@@ -386,6 +434,16 @@ class Weight:
                                _stream_ptr(stream)))
         return y
 
+    def codes_i8(self, stream=None):
+        """(codes [rows, cols] int8, scales [rows] fp32) of an 8-bit handle with one
+        scale per row, on the device, as linear_i8 takes them."""
+        import torch
+        width = -(-self.cols // 16) * 16
+        codes = torch.empty(self.rows, width, dtype=torch.int8, device="cuda")
+        scales = torch.empty(self.rows, dtype=torch.float32, device="cuda")
+        check(lib().lmx_weight_codes_i8(self._h, codes.data_ptr(), width, scales.data_ptr(), _stream_ptr(stream)))
+        return codes[:, :self.cols], scales
+
     def close(self):
         if self._h:
             lib().lmx_weight_destroy(self._h)
@@ -396,6 +454,50 @@ class Weight:
             self.close()
         except Exception:
             pass
+
+
+def linear_i8(x, w, w_scale, bias=None, y=None, workspace=None, stream=None):
+    """Linear layer in 8-bit integers (lmx_linear_i8): x [..., cols] fp32, fp16 or
+    bf16, w [rows, cols] int8 whose rows start on multiples of 16 bytes (any row
+    stride that is one), w_scale [rows] fp32, bias [rows] of x's type.  Returns
+    [..., rows] of x's type.  workspace: a uint8 tensor of at least
+    linear_i8_workspace bytes that no overlapping call uses (default: torch
+    allocates one for the call)."""
+    import torch
+    kind = _types().get(x.dtype)
+    if kind is None:
+        raise LmxError(ERR_UNSUPPORTED_FORMAT, f"x is {x.dtype}: float32, float16 or bfloat16")
+    if w.dim() != 2 or w.dtype != torch.int8 or w.stride(1) != 1:
+        raise ValueError("w: int8 [rows, cols] with neighbouring columns side by side")
+    rows, cols = w.shape
+    if x.dim() == 0 or x.shape[-1] != cols or not x.is_contiguous():
+        raise ValueError(f"x {tuple(x.shape)}: contiguous, {cols} values a row")
+    if w_scale.dtype != torch.float32 or w_scale.shape != (rows,) or not w_scale.is_contiguous():
+        raise ValueError(f"w_scale: contiguous float32 [{rows}]")
+    if bias is not None and (bias.dtype != x.dtype or bias.shape != (rows,) or not bias.is_contiguous()):
+        raise ValueError(f"bias: contiguous {x.dtype} [{rows}]")
+    batch = x.numel() // cols
+    if y is None:
+        y = torch.empty(*x.shape[:-1], rows, dtype=x.dtype, device=x.device)
+    elif y.dtype != x.dtype or y.numel() != batch * rows or not y.is_contiguous():
+        raise ValueError(f"y: contiguous {x.dtype}, {batch} x {rows}")
+    need = linear_i8_workspace(rows, cols, batch)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+    _on_current_device(x, w, w_scale, bias, y, workspace)
+    # (the stride of a single row says nothing)
+    stride = w.stride(0) if rows > 1 else -(-cols // 16) * 16
+    check(lib().lmx_linear_i8(w.data_ptr(), stride, w_scale.data_ptr(), None if bias is None else bias.data_ptr(),
+                              x.data_ptr(), y.data_ptr(), kind, rows, cols, batch, workspace.data_ptr(),
+                              workspace.numel() * workspace.element_size(), _stream_ptr(stream)))
+    return y
+
+
+def linear_i8_workspace(rows, cols, batch):
+    """Bytes of workspace of a linear_i8 call."""
+    n = ctypes.c_size_t()
+    check(lib().lmx_linear_i8_workspace(rows, cols, batch, ctypes.byref(n)))
+    return n.value
 
 
 def fwht256(x, stream=None):

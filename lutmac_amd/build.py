@@ -33,6 +33,8 @@ SOURCES = [
     ("lmx_probe.hip", True),
     ("lmx_noalloc.hip", True),
     ("lmx_decode.hip", True),
+    ("lmx_kv8.hip", True),
+    ("lmx_i8.hip", True),
     ("lmx_capi.cpp", False),
     ("lmx_repack.cpp", False),
     ("lut_gemm_compat.cpp", False),

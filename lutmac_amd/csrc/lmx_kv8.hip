@@ -1,0 +1,637 @@
+// lmx_kv8.hip -- the 8-bit paged KV cache (include/lutmac_kv8.h): rotation and
+// append, and attention of a few rows per sequence over it.
+#include <algorithm>
+#include <cmath>
+
+#include "lmx_kv8.hpp"
+
+namespace lmx {
+namespace {
+
+// ---------------------------------------------------------------------------
+// Append.  A unit is one 16-token block of a sequence that receives rows; a
+// workgroup takes one unit of one KV head's keys, one KV head's values or one
+// query head, its 16 groups of 16 lanes a token each.  The block's scale needs
+// every value before any code, so the values wait in registers (in 64 bits: a
+// rotation or quotient next to a border between two codes has to fall on the
+// right side whatever the order of operations).
+struct AppendArgs {
+  Kv8Args c;
+  const void *k, *v, *q;
+  void *q_out;
+  size_t k_stride, v_stride, q_stride, q_out_stride;
+  const float2 *rope;
+  int rope_n;
+};
+
+// The rotated pairs (d0 + i, d0 + i + HD / 2) of a row.
+template <class T, int HD>
+__device__ __forceinline__ void rotated(const T *row, const float2 *rope, int pos, int d0, double (&x)[HD / 32],
+                                        double (&y)[HD / 32]) {
+  constexpr int E = HD / 32;
+  float a[E], b[E];
+  load_floats<E>(row + d0, a);
+  load_floats<E>(row + d0 + HD / 2, b);
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    x[i] = a[i], y[i] = b[i];
+    if (rope) {
+      const float2 t = rope[size_t(pos) * (HD / 2) + d0 + i];
+      const double c = t.x, s = t.y;
+      x[i] = a[i] * c - b[i] * s;
+      y[i] = a[i] * s + b[i] * c;
+    }
+  }
+}
+
+__device__ __forceinline__ double wave_max(double v) {
+#pragma unroll
+  for (int d = 32; d; d >>= 1) v = fmax(v, __shfl_xor(v, d, kWave));
+  return v;
+}
+
+// The block's scale from its new values' largest magnitude and whether all of
+// them are finite; every thread of the workgroup calls it.
+__device__ __forceinline__ float block_scale(double top, bool finite, const float *scale, bool kept, float &was) {
+  __shared__ double tops[4];
+  was = *scale;   // (before the barrier: thread 0 writes it afterwards)
+  top = wave_max(top);
+  if ((threadIdx.x & (kWave - 1)) == 0) tops[threadIdx.x / kWave] = top;
+  const bool all = __syncthreads_and(finite);
+  top = fmax(fmax(tops[0], tops[1]), fmax(tops[2], tops[3]));
+  float now = fmaxf(float(top / 127.0), 0x1p-100f);
+  if (kept) now = was != was ? was : fmaxf(now, was);
+  return all && now < INFINITY ? now : __builtin_nanf("");
+}
+
+// (a NaN scale leaves the codes 0)
+__device__ __forceinline__ int code_of(double x, double scale, double inverse) {
+  return scale == scale ? int(round_quotient(x, scale, inverse)) : 0;
+}
+
+template <class T, int HD>
+__global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
+  constexpr int E = HD / 32, VE = HD / 16;
+  __shared__ __attribute__((aligned(16))) uint8_t cod[HD][kBlock];
+  const int lane = threadIdx.x & (kWave - 1), tk = int(threadIdx.x) >> 4, part = int(threadIdx.x) & 15;
+  int first = 0;
+  const int seq = unit_sequence(a.c, int(blockIdx.x), 1, 2, lane, first);
+  if (seq < 0) return;
+  const SeqRows r(a.c, seq);
+  const int from = max(r.start, 0);   // rows before position 0 have no place
+  const int block = from / kBlock + (int(blockIdx.x) - first);
+  if (r.n == 0 || block >= (r.len + kBlock - 1) / kBlock) return;
+  const int pos = block * kBlock + tk;
+  const bool live = pos >= from && pos < r.len && (!a.rope || pos < a.rope_n);
+  const size_t row = size_t(r.r0 + (live ? pos - r.start : from - r.start));
+  const int role = int(blockIdx.y), n_kv = a.c.n_kv;
+  if (role >= 2 * n_kv) {   // a query head
+    if (!live) return;
+    const int head = role - 2 * n_kv;
+    double x[E], y[E];
+    rotated<T, HD>(static_cast<const T *>(a.q) + row * a.q_stride + size_t(head) * HD, a.rope, pos, part * E, x, y);
+    T *out = static_cast<T *>(a.q_out) + row * a.q_out_stride + size_t(head) * HD + part * E;
+    float f[E], g[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) f[i] = narrow<T>(x[i]), g[i] = narrow<T>(y[i]);
+    store_floats<E>(out, f);
+    store_floats<E>(out + HD / 2, g);
+    return;
+  }
+  const int pi = block / kPageBlocks, sub = block % kPageBlocks;
+  if (pi >= a.c.max_pages) return;
+  const int page = a.c.pages[size_t(seq) * a.c.max_pages + pi];
+  if (!page_ok(a.c, page)) return;
+  const int kept = max(from - block * kBlock, 0);   // earlier tokens of the block
+  const int last = min(r.len, a.rope ? a.rope_n : r.len) - block * kBlock;   // tokens of the block with the rows
+  if (last <= kept) return;
+  double top = 0.0;
+  bool finite = true;
+  float was;
+  if (role < n_kv) {
+    const size_t ph = size_t(page) * n_kv + role;
+    double x[E], y[E];
+    if (live) {
+      rotated<T, HD>(static_cast<const T *>(a.k) + row * a.k_stride + size_t(role) * HD, a.rope, pos, part * E, x, y);
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        top = fmax(top, fmax(fabs(x[i]), fabs(y[i])));
+        finite = finite && fabs(x[i]) < INFINITY && fabs(y[i]) < INFINITY;
+      }
+    }
+    float *scale = a.c.k_scale + ph * kPageBlocks + sub;
+    const float now = block_scale(top, finite, scale, kept > 0, was);
+    const double inv = 1.0 / double(now);
+    int8_t *dst = a.c.k + (ph * kPage + sub * kBlock + tk) * HD + part * E;
+    if (live || (tk < kept && now == now && now != was)) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        int8_t *p = dst + h * (HD / 2);
+        typedef int8_t bytes __attribute__((ext_vector_type(E)));
+        bytes c = *reinterpret_cast<bytes *>(p);
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+          c[i] = int8_t(code_of(live ? (h ? y[i] : x[i]) : double(int(c[i])) * double(was), now, inv));
+        *reinterpret_cast<bytes *>(p) = c;
+      }
+    }
+    if (threadIdx.x == 0) *scale = now;
+    return;
+  }
+  const int head = role - n_kv;
+  const size_t ph = size_t(page) * n_kv + head;
+  float x[VE];
+  if (live) {
+    load_floats<VE>(static_cast<const T *>(a.v) + row * a.v_stride + size_t(head) * HD + part * VE, x);
+#pragma unroll
+    for (int i = 0; i < VE; ++i) {
+      top = fmax(top, fabs(double(x[i])));
+      finite = finite && fabsf(x[i]) < INFINITY;
+    }
+  }
+  float *scale = a.c.v_scale + ph * kPageBlocks + sub;
+  const float now = block_scale(top, finite, scale, kept > 0, was);
+  const double inv = 1.0 / double(now);
+  if (live) {
+#pragma unroll
+    for (int i = 0; i < VE; ++i) cod[part * VE + i][tk] = uint8_t(code_of(x[i], now, inv));
+  }
+  __syncthreads();
+  if (threadIdx.x < HD) {   // one dimension's 16 tokens: earlier ones rescaled, later ones left
+    int8_t *p = a.c.v + (ph * HD + threadIdx.x) * kPage + sub * kBlock;
+    typedef int8_t bytes __attribute__((ext_vector_type(16)));
+    bytes c = *reinterpret_cast<const bytes *>(cod[threadIdx.x]);
+    if (kept > 0 || last < kBlock) {
+      const bytes old = *reinterpret_cast<const bytes *>(p);
+      const bool rescale = now == now && now != was;
+#pragma unroll
+      for (int t = 0; t < kBlock; ++t) {
+        if (t < kept) c[t] = rescale ? int8_t(code_of(double(int(old[t])) * double(was), now, inv)) : old[t];
+        else if (t >= last) c[t] = old[t];
+      }
+    }
+    *reinterpret_cast<bytes *>(p) = c;
+  }
+  if (threadIdx.x == 0) *scale = now;
+}
+
+// ---------------------------------------------------------------------------
+// Attention of up to 16 rows (a row: one query head of one token) of one KV
+// head per workgroup, on the 8-bit matrix cores with exact products.
+//
+// A query row becomes fixed point of ND signed-byte digits relative to a power
+// of two; S^T = K Q^T digit by digit (v_mfma_i32_16x16x64_i8, sums from the bits
+// of 1.5 * 2^23, so the sum is a float that differs from it by the sum); the
+// weights p become fixed point the same way, and O^T = V^T P^T.  No code is
+// converted, and cache bytes go from memory straight into the operand
+// registers:
+//   K operand, tile t: lane (i, g) holds dimensions 64 m + 16 g .. + 15 of token
+//     16 (i / 4) + 4 t + i % 4, so that of S^T tile t lane (column j, g) gets the
+//     tokens 16 g + 4 t + 0..3 -- over the four tiles the 16 tokens of block g,
+//     in order: one K and one V scale per lane, and P^T's operand in place.
+//   V operand: lane (i, g) holds tokens 16 g .. + 15 of dimension 16 h + i.
+// Weights are relative to the running maximum of score + log2 of the V scale's
+// power of two (what bounds the fixed point); the rest of the scale is
+// multiplied in as the digits are made.
+//
+// The 4 waves take pages in turn, grid.z parts ("splits") a share of them;
+// (m, l, o) of the waves merge in LDS, of the parts in kv8_merge_kernel.
+struct AttnArgs {
+  Kv8Args c;
+  const void *q;
+  void *out;
+  size_t q_stride, out_stride;
+  float scale;       // softmax scale * log2(e)
+  int splits;
+  float *part_o;     // [units][n_kv][splits][16][HD]
+  float2 *part_ml;   // [units][n_kv][splits][16]
+};
+
+constexpr float kMagic = 12582912.0f;   // 1.5 * 2^23
+// The sums of weights carry 2^kSumExp, so that V scales from 2^-100 to 2^120
+// leave them in range (22 bits of weight, 2^24 tokens).
+constexpr int kSumExp = -24;
+__device__ __forceinline__ float inverse_sum(float l) { return l == 0.0f ? 0.0f : 0x1p-24f / l; }
+
+// ND digit sums (from kMagic) -> the fixed-point sum, rounded once.
+template <int ND>
+__device__ __forceinline__ float join(const float (&d)[ND]) {
+  const float lo = fmaf(d[1], 256.0f, -257.0f * kMagic) + d[0];
+  if constexpr (ND == 2) return lo;
+  else return fmaf(d[2] - kMagic, 65536.0f, lo);
+}
+
+// Four fixed-point values, each in the low bits of a word, 128 added to every
+// digit but the top one -> dword d of the result: their digits d.
+template <int ND>
+__device__ __forceinline__ void digit_words(const uint32_t (&u)[4], uint32_t (&w)[ND]) {
+  const uint32_t a = __builtin_amdgcn_perm(u[1], u[0], 0x05010400u), c = __builtin_amdgcn_perm(u[3], u[2], 0x05010400u);
+  w[0] = __builtin_amdgcn_perm(c, a, 0x05040100u) ^ 0x80808080u;
+  w[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+  if constexpr (ND == 3) {
+    w[1] ^= 0x80808080u;
+    const uint32_t b = __builtin_amdgcn_perm(u[1], u[0], 0x0C0C0602u), e = __builtin_amdgcn_perm(u[3], u[2], 0x0C0C0602u);
+    w[2] = __builtin_amdgcn_perm(e, b, 0x05040100u);
+  }
+}
+
+template <int ND> struct Digits;
+// carry: 128 for every digit below the top; q_bits: |q| <= 2^q_bits; p_exp: the
+// largest weight is 2^p_exp, so that weight + carry stays below 2^22 (three
+// digits: below the window of kMagic) or 2^15 (two)
+template <> struct Digits<2> { static constexpr int carry = 0x80, q_bits = 14; static constexpr float p_exp = 14.98f; };
+template <> struct Digits<3> { static constexpr int carry = 0x8080, q_bits = 22; static constexpr float p_exp = 21.98f; };
+
+// A row's 16 contiguous elements of step m -> its digit words; f: the power of
+// two of the fixed point.
+template <int ND>
+__device__ __forceinline__ void query_digits(const float (&x)[16], float f, v4i (&w)[ND]) {
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    uint32_t u[4], d[ND];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = uint32_t(__float2int_rn(x[4 * b + i] * f) + Digits<ND>::carry);
+    digit_words<ND>(u, d);
+#pragma unroll
+    for (int j = 0; j < ND; ++j) w[j][b] = int(d[j]);
+  }
+}
+
+template <class T, int HD, int ND>
+__global__ __launch_bounds__(256) void kv8_rows_kernel(AttnArgs a) {
+  constexpr int W = 4, M = HD / 64, H = HD / 16;
+  __shared__ float os[W][16][HD + 4];
+  __shared__ float ms[W][16], ls[W][16];
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
+  const int j = lane & 15, g = lane >> 4;
+  const int kvh = int(blockIdx.y), group = a.c.group;
+  int first = 0;
+  const int seq = unit_sequence(a.c, int(blockIdx.x), group, 1, lane, first);
+  if (seq < 0) return;
+  const SeqRows r(a.c, seq);
+  const int tile0 = (int(blockIdx.x) - first) * 16, rows = r.n * group;   // (< 2^31: checked by the host)
+  if (tile0 >= rows) return;
+  // row i of the sequence: query head kvh * group + i % group of token i / group
+  const int i = tile0 + j;
+  const int t = min(i, rows - 1) / group;
+  const int see = min(r.len, a.c.max_pages * kPage) - 1;   // the last token with a place
+  const int first_pos = min(r.start + tile0 / group, see), last_pos = min(r.start + min(tile0 + 15, rows - 1) / group, see);
+  const int limit = min(r.start + t, see);
+  const int n_pages = last_pos < 0 ? 0 : last_pos / kPage + 1;
+  const int part = int(blockIdx.z);
+  const int p0 = int((long long)n_pages * part / a.splits), p1 = int((long long)n_pages * (part + 1) / a.splits);
+
+  // query digits, this lane's 16 dimensions of every 64-dimension step
+  const T *q = static_cast<const T *>(a.q) + size_t(r.r0 + t) * a.q_stride + size_t(kvh * group + min(i, rows - 1) % group) * HD;
+  v4i qd[M][ND];
+  float qs;
+  {
+    float x[M][16];
+    uint32_t top = 0;
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      load_floats<16>(q + 64 * m + 16 * g, x[m]);
+#pragma unroll
+      for (int d = 0; d < 16; ++d) top = max(top, __float_as_uint(x[m][d]) & 0x7FFFFFFFu);
+    }
+    top = max(top, lane_xor_u32<16>(top, lane));
+    top = max(top, lane_xor_u32<32>(top, lane));
+    const bool finite = top < 0x7F800000u;
+    const int e = max(int(top >> 23), 29) - 126;   // |x| < 2^e
+    const float f = finite ? __builtin_amdgcn_ldexpf(1.0f, Digits<ND>::q_bits - e) : 0.0f;
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+#pragma unroll
+      for (int d = 0; d < 16; ++d) x[m][d] = finite ? x[m][d] : 0.0f;
+      query_digits<ND>(x[m], f, qd[m]);
+    }
+    qs = finite ? __builtin_amdgcn_ldexpf(a.scale, e - Digits<ND>::q_bits) : __builtin_nanf("");
+  }
+
+  float mref = -INFINITY, l = 0.0f;
+  float o[H][4];
+#pragma unroll
+  for (int h = 0; h < H; ++h)
+#pragma unroll
+    for (int v = 0; v < 4; ++v) o[h][v] = 0.0f;
+  const v4i zero = {__float_as_int(kMagic), __float_as_int(kMagic), __float_as_int(kMagic), __float_as_int(kMagic)};
+  const int *table = a.c.pages + size_t(seq) * a.c.max_pages;
+  for (int p = p0 + wave; p < p1; p += W) {
+    const int page = __builtin_amdgcn_readfirstlane(table[p]);
+    if (!page_ok(a.c, page)) continue;
+    const size_t ph = size_t(page) * a.c.n_kv + kvh;
+    const int8_t *kp = a.c.k + ph * kPage * HD + (16 * (j >> 2) + (j & 3)) * HD + 16 * g;
+    const int8_t *vp = a.c.v + ph * HD * kPage + j * kPage + 16 * g;
+    v4i kb[4][M], vb[H];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int m = 0; m < M; ++m) kb[u][m] = *reinterpret_cast<const v4i *>(kp + 4 * u * HD + 64 * m);
+    float ks = a.c.k_scale[ph * kPageBlocks + g], vs = a.c.v_scale[ph * kPageBlocks + g];
+#pragma unroll
+    for (int h = 0; h < H; ++h) vb[h] = *reinterpret_cast<const v4i *>(vp + h * 16 * kPage);
+    const int t0 = p * kPage + 16 * g;   // this lane's first token
+    if (t0 > last_pos) ks = 0.0f, vs = 0.0f;   // nothing of the block is seen: its scales may hold anything
+    const int ex = vs != 0.0f ? __builtin_amdgcn_frexp_expf(vs) : 0;
+    const float mant = __builtin_amdgcn_frexp_mantf(vs), fex = float(ex), c = qs * ks;
+    float y[4][4], top = -INFINITY;
+    const bool masked = p * kPage + kPage - 1 > first_pos;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      v4i s[ND];
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        s[d] = zero;
+#pragma unroll
+        for (int m = 0; m < M; ++m) s[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kb[u][m], qd[m][d], s[d], 0, 0, 0);
+      }
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        float d[ND];
+#pragma unroll
+        for (int n = 0; n < ND; ++n) d[n] = __int_as_float(s[n][v]);
+        y[u][v] = fmaf(join<ND>(d), c, fex);
+        if (masked && t0 + 4 * u + v > limit) y[u][v] = -INFINITY;
+        top = fmaxf(top, y[u][v]);
+      }
+    }
+    top = fmaxf(top, lane_xor<16>(top, lane));
+    top = fmaxf(top, lane_xor<32>(top, lane));
+    const float mn = fmaxf(mref, top), base = mn == -INFINITY ? 0.0f : mn;
+    const float keep = __builtin_amdgcn_exp2f(mref - base);
+    const float off = Digits<ND>::p_exp - base;
+    mref = mn;
+    v4i pd[ND];
+    float sum = 0.0f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      uint32_t w[4], dw[ND];
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const float e = __builtin_amdgcn_exp2f(y[u][v] + off);
+        sum += e;
+        w[v] = __float_as_uint(fmaf(e, mant, kMagic + float(Digits<ND>::carry)));
+      }
+      digit_words<ND>(w, dw);
+      if constexpr (ND == 3) dw[2] ^= 0x40404040u;   // (kMagic's own bit 22)
+#pragma unroll
+      for (int d = 0; d < ND; ++d) pd[d][u] = int(dw[d]);
+    }
+    // (a block whose scale is not finite gives NaN to the rows that see it)
+    const float unit = vs - vs == 0.0f ? __builtin_amdgcn_ldexpf(1.0f, kSumExp - ex) : __builtin_nanf("");
+    l *= keep;
+    if (sum != 0.0f) l = fmaf(sum, unit, l);
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      v4i s[ND];
+#pragma unroll
+      for (int d = 0; d < ND; ++d) s[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vb[h], pd[d], zero, 0, 0, 0);
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        float d[ND];
+#pragma unroll
+        for (int n = 0; n < ND; ++n) d[n] = __int_as_float(s[n][v]);
+        o[h][v] = fmaf(o[h][v], keep, join<ND>(d));
+      }
+    }
+  }
+  l += lane_xor<16>(l, lane);
+  l += lane_xor<32>(l, lane);
+  if (g == 0) ms[wave][j] = mref, ls[wave][j] = l;
+#pragma unroll
+  for (int h = 0; h < H; ++h)
+    *reinterpret_cast<float4 *>(&os[wave][j][16 * h + 4 * g]) = make_float4(o[h][0], o[h][1], o[h][2], o[h][3]);
+  __syncthreads();
+  // thread (row, 1/16 of the dimensions) merges the waves
+  constexpr int E = HD / 16;
+  const int row = int(threadIdx.x) >> 4, d0 = (int(threadIdx.x) & 15) * E;
+  float mx = ms[0][row];
+#pragma unroll
+  for (int w = 1; w < W; ++w) mx = fmaxf(mx, ms[w][row]);
+  float sum = 0.0f, acc[E];
+#pragma unroll
+  for (int d = 0; d < E; ++d) acc[d] = 0.0f;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    const float f = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ms[w][row] - mx);   // (1: a sum that is NaN stays so)
+    sum += f * ls[w][row];
+#pragma unroll
+    for (int d = 0; d < E; ++d) acc[d] = fmaf(f, os[w][row][d0 + d], acc[d]);
+  }
+  if (a.splits > 1) {
+    const size_t at = ((size_t(blockIdx.x) * a.c.n_kv + kvh) * a.splits + part) * 16 + row;
+    if ((threadIdx.x & 15) == 0) a.part_ml[at] = make_float2(mx, sum);
+    store_floats<E>(a.part_o + at * HD + d0, acc);
+    return;
+  }
+  if (tile0 + row >= rows) return;
+  const float inv = inverse_sum(sum);
+#pragma unroll
+  for (int d = 0; d < E; ++d) acc[d] *= inv;
+  T *out = static_cast<T *>(a.out) + size_t(r.r0 + (tile0 + row) / group) * a.out_stride +
+           size_t(kvh * group + (tile0 + row) % group) * HD + d0;
+  store_floats<E>(out, acc);
+}
+
+// The parts of a split unit: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.
+template <class T, int HD>
+__global__ __launch_bounds__(256) void kv8_merge_kernel(AttnArgs a) {
+  constexpr int E = HD / 16;
+  const int lane = threadIdx.x & (kWave - 1), kvh = int(blockIdx.y), group = a.c.group;
+  int first = 0;
+  const int seq = unit_sequence(a.c, int(blockIdx.x), group, 1, lane, first);
+  if (seq < 0) return;
+  const SeqRows r(a.c, seq);
+  const int row = int(threadIdx.x) >> 4, d0 = (int(threadIdx.x) & 15) * E;
+  const int i = (int(blockIdx.x) - first) * 16 + row;
+  if (i >= r.n * group) return;
+  const size_t at = (size_t(blockIdx.x) * a.c.n_kv + kvh) * a.splits * 16 + row;
+  float mx = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) mx = fmaxf(mx, a.part_ml[at + size_t(s) * 16].x);
+  float sum = 0.0f, acc[E];
+#pragma unroll
+  for (int d = 0; d < E; ++d) acc[d] = 0.0f;
+  for (int s = 0; s < a.splits; ++s) {
+    const float2 ml = a.part_ml[at + size_t(s) * 16];
+    const float f = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ml.x - mx);
+    sum += f * ml.y;
+    float o[E];
+    load_floats<E>(a.part_o + (at + size_t(s) * 16) * HD + d0, o);
+#pragma unroll
+    for (int d = 0; d < E; ++d) acc[d] = fmaf(f, o[d], acc[d]);
+  }
+  const float inv = inverse_sum(sum);
+#pragma unroll
+  for (int d = 0; d < E; ++d) acc[d] *= inv;
+  store_floats<E>(static_cast<T *>(a.out) + size_t(r.r0 + i / group) * a.out_stride + size_t(kvh * group + i % group) * HD + d0,
+                  acc);
+}
+
+// ---- host side ----
+
+int launch_err(const char *what) {
+  hipError_t e = hipGetLastError();
+  return e == hipSuccess ? LMX_OK : fail(LMX_ERR_LAUNCH_FAILED, "%s launch: %s", what, hipGetErrorString(e));
+}
+
+int check_sizes(const lmx_kv8_cache *c, const lmx_kv8_batch *b, size_t n_heads) {
+  if (!c || !b) return fail(LMX_ERR_INVALID_ARGUMENT, "cache or batch is NULL");
+  if (c->head_dim != 64 && c->head_dim != 128) return fail(LMX_ERR_INVALID_ARGUMENT, "head_dim %zu must be 64 or 128", c->head_dim);
+  if (c->n_kv_heads == 0 || c->n_kv_heads > 512) return fail(LMX_ERR_INVALID_ARGUMENT, "%zu KV heads", c->n_kv_heads);
+  if (c->n_pages == 0 || c->n_pages >= (1u << 31)) return fail(LMX_ERR_INVALID_ARGUMENT, "%zu pages", c->n_pages);
+  if (b->n_seqs > (1u << 20) || b->max_pages > (1u << 24) || b->n_rows > (1u << 24))
+    return fail(LMX_ERR_INVALID_ARGUMENT, "%zu sequences of up to %zu pages, %zu rows: at most 2^20, 2^24, 2^24", b->n_seqs,
+                b->max_pages, b->n_rows);
+  if (n_heads == 0 || n_heads % c->n_kv_heads || n_heads / c->n_kv_heads > 64)
+    return fail(LMX_ERR_INVALID_ARGUMENT, "%zu query heads must be a multiple of %zu KV heads, at most 64 times", n_heads,
+                c->n_kv_heads);
+  return LMX_OK;
+}
+
+int check_pointers(const lmx_kv8_cache *c, const lmx_kv8_batch *b) {
+  if (!c->k || !c->v || !c->k_scale || !c->v_scale) return fail(LMX_ERR_INVALID_ARGUMENT, "cache pointer is NULL");
+  if (!b->offsets || !b->lengths || (b->max_pages && !b->pages)) return fail(LMX_ERR_INVALID_ARGUMENT, "batch pointer is NULL");
+  if ((reinterpret_cast<size_t>(c->k) | reinterpret_cast<size_t>(c->v)) % 16)
+    return fail(LMX_ERR_INVALID_ARGUMENT, "cache codes must be 16-byte aligned");
+  return LMX_OK;
+}
+
+// A row array: 16-byte aligned rows that do not run into each other.
+int check_rows(const char *what, const void *p, size_t stride, size_t width, int type, size_t rows) {
+  if (!p) return fail(LMX_ERR_INVALID_ARGUMENT, "%s is NULL", what);
+  if (reinterpret_cast<size_t>(p) % 16 || stride * type_bytes(type) % 16)
+    return fail(LMX_ERR_INVALID_ARGUMENT, "%s: pointer and row stride must be multiples of 16 bytes", what);
+  if (stride < width && rows > 1) return fail(LMX_ERR_INVALID_ARGUMENT, "%s: row stride %zu is less than a row's %zu", what, stride, width);
+  return LMX_OK;
+}
+
+Kv8Args kv8_args(const lmx_kv8_cache *c, const lmx_kv8_batch *b, size_t n_heads) {
+  Kv8Args a{};
+  a.k = c->k, a.v = c->v, a.k_scale = c->k_scale, a.v_scale = c->v_scale;
+  a.offsets = b->offsets, a.lengths = b->lengths, a.pages = b->pages;
+  a.n_pages = int(c->n_pages), a.n_kv = int(c->n_kv_heads);
+  a.n_seqs = int(b->n_seqs), a.max_pages = int(b->max_pages), a.n_rows = int(b->n_rows);
+  a.n_heads = int(n_heads), a.group = int(n_heads / c->n_kv_heads);
+  return a;
+}
+
+// Work units of 16 rows that a call may have (unit_sequence).
+size_t row_units(const lmx_kv8_batch *b, size_t group) { return b->n_rows * group / 16 + b->n_seqs; }
+
+// Parts of a unit's pages: as many as bring the grid to about three workgroups
+// per CU, of four pages at least (one per wave).
+int split_count(const lmx_kv8_cache *c, const lmx_kv8_batch *b, size_t group) {
+  const size_t wgs = row_units(b, group) * c->n_kv_heads, want = 768;
+  if (wgs == 0) return 1;
+  const size_t s = std::min<size_t>(want / wgs, b->max_pages / 4);
+  return int(std::max<size_t>(1, std::min<size_t>(s, 64)));
+}
+
+size_t workspace_bytes(const lmx_kv8_cache *c, const lmx_kv8_batch *b, size_t n_heads) {
+  const size_t group = n_heads / c->n_kv_heads;
+  const int splits = split_count(c, b, group);
+  if (splits == 1) return 0;
+  return row_units(b, group) * c->n_kv_heads * size_t(splits) * 16 * (c->head_dim + 2) * sizeof(float);
+}
+
+template <class T, int HD>
+int launch_attention(const AttnArgs &a, size_t units, hipStream_t st) {
+  constexpr int ND = sizeof(T) == 4 ? 3 : 2;
+  const dim3 grid(unsigned(units), unsigned(a.c.n_kv), unsigned(a.splits));
+  kv8_rows_kernel<T, HD, ND><<<grid, dim3(256), 0, st>>>(a);
+  int r = launch_err("kv8 attention");
+  if (r || a.splits == 1) return r;
+  kv8_merge_kernel<T, HD><<<dim3(unsigned(units), unsigned(a.c.n_kv)), dim3(256), 0, st>>>(a);
+  return launch_err("kv8 merge");
+}
+
+template <class T>
+int launch_append(const AppendArgs &a, size_t hd, dim3 grid, hipStream_t st) {
+  if (hd == 64) kv8_append_kernel<T, 64><<<grid, dim3(256), 0, st>>>(a);
+  else kv8_append_kernel<T, 128><<<grid, dim3(256), 0, st>>>(a);
+  return launch_err("kv8 append");
+}
+
+}  // namespace
+}  // namespace lmx
+
+using namespace lmx;
+
+extern "C" {
+
+int lmx_kv8_append(const lmx_kv8_cache *cache, const lmx_kv8_batch *batch, int type, const void *k, size_t k_stride,
+                   const void *v, size_t v_stride, const void *q, size_t q_stride, void *q_out, size_t q_out_stride,
+                   size_t n_heads, const float *rope, size_t rope_positions, void *stream) {
+  int r = check_sizes(cache, batch, q ? n_heads : cache ? cache->n_kv_heads : 1);
+  if (r) return r;
+  if (!type_bytes(type)) return fail(LMX_ERR_UNSUPPORTED_FORMAT, "unknown element type %d", type);
+  if (batch->n_seqs == 0 || batch->n_rows == 0) return LMX_OK;
+  const size_t kvw = cache->n_kv_heads * cache->head_dim, qw = n_heads * cache->head_dim, rows = batch->n_rows;
+  if ((r = check_pointers(cache, batch)) || (r = check_rows("k", k, k_stride, kvw, type, rows)) ||
+      (r = check_rows("v", v, v_stride, kvw, type, rows)))
+    return r;
+  if (q && ((r = check_rows("q", q, q_stride, qw, type, rows)) || (r = check_rows("q_out", q_out, q_out_stride, qw, type, rows))))
+    return r;
+  if (rope && (rope_positions == 0 || rope_positions >= (1u << 31) || reinterpret_cast<size_t>(rope) % 8))
+    return fail(LMX_ERR_INVALID_ARGUMENT, "rotation table of %zu positions, or not 8-byte aligned", rope_positions);
+  AppendArgs a{};
+  a.c = kv8_args(cache, batch, q ? n_heads : cache->n_kv_heads);
+  a.k = k, a.v = v, a.q = q, a.q_out = q_out;
+  a.k_stride = k_stride, a.v_stride = v_stride, a.q_stride = q_stride, a.q_out_stride = q_out_stride;
+  a.rope = reinterpret_cast<const float2 *>(rope);
+  a.rope_n = rope ? int(rope_positions) : 0;
+  // a sequence of n rows touches at most n / 16 + 2 blocks, rounded down
+  const dim3 grid(unsigned(rows / kBlock + 2 * batch->n_seqs), unsigned(2 * cache->n_kv_heads + (q ? n_heads : 0)));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  switch (type) {
+  case LMX_F32: return launch_append<float>(a, cache->head_dim, grid, st);
+  case LMX_F16: return launch_append<f16>(a, cache->head_dim, grid, st);
+  default: return launch_append<bf16>(a, cache->head_dim, grid, st);
+  }
+}
+
+int lmx_kv8_attention_workspace(const lmx_kv8_cache *cache, const lmx_kv8_batch *batch, size_t n_heads, size_t *bytes) {
+  if (!bytes) return fail(LMX_ERR_INVALID_ARGUMENT, "bytes is NULL");
+  const int r = check_sizes(cache, batch, n_heads);
+  if (r) return r;
+  *bytes = workspace_bytes(cache, batch, n_heads);
+  return LMX_OK;
+}
+
+int lmx_kv8_attention(const lmx_kv8_cache *cache, const lmx_kv8_batch *batch, int type, const void *q, size_t q_stride,
+                      size_t n_heads, float scale, void *out, size_t out_stride, void *workspace, size_t workspace_size,
+                      void *stream) {
+  int r = check_sizes(cache, batch, n_heads);
+  if (r) return r;
+  if (!type_bytes(type)) return fail(LMX_ERR_UNSUPPORTED_FORMAT, "unknown element type %d", type);
+  if (!(scale > 0.0f) || !(scale < INFINITY)) return fail(LMX_ERR_INVALID_ARGUMENT, "scale %g must be positive and finite", double(scale));
+  if (batch->n_seqs == 0 || batch->n_rows == 0) return LMX_OK;
+  const size_t qw = n_heads * cache->head_dim, need = workspace_bytes(cache, batch, n_heads);
+  if ((r = check_pointers(cache, batch)) || (r = check_rows("q", q, q_stride, qw, type, batch->n_rows)) ||
+      (r = check_rows("out", out, out_stride, qw, type, batch->n_rows)))
+    return r;
+  if (need && (!workspace || workspace_size < need || reinterpret_cast<size_t>(workspace) % 16))
+    return fail(LMX_ERR_INVALID_ARGUMENT, "workspace of %zu bytes at %p: %zu bytes, 16-byte aligned, are needed", workspace_size,
+                workspace, need);
+  AttnArgs a{};
+  a.c = kv8_args(cache, batch, n_heads);
+  a.q = q, a.out = out, a.q_stride = q_stride, a.out_stride = out_stride;
+  a.scale = scale * 1.44269504088896340736f;
+  a.splits = split_count(cache, batch, size_t(a.c.group));
+  const size_t units = row_units(batch, size_t(a.c.group));
+  if (a.splits > 1) {
+    a.part_o = static_cast<float *>(workspace);
+    a.part_ml = reinterpret_cast<float2 *>(a.part_o + units * cache->n_kv_heads * size_t(a.splits) * 16 * cache->head_dim);
+  }
+  hipStream_t st = static_cast<hipStream_t>(stream);
+#define LMX_KV8_ATTENTION(T) \
+  return cache->head_dim == 64 ? launch_attention<T, 64>(a, units, st) : launch_attention<T, 128>(a, units, st)
+  switch (type) {
+  case LMX_F32: LMX_KV8_ATTENTION(float);
+  case LMX_F16: LMX_KV8_ATTENTION(f16);
+  default: LMX_KV8_ATTENTION(bf16);
+  }
+#undef LMX_KV8_ATTENTION
+}
+
+}  // extern "C"
