@@ -87,17 +87,18 @@ int lmx_kv8_append(const lmx_kv8_cache *cache, const lmx_kv8_batch *batch,
 /* Bytes of workspace that lmx_kv8_attention needs for a call of these sizes
  * (pointers are not looked at; 0 is possible). */
 int lmx_kv8_attention_workspace(const lmx_kv8_cache *cache,
-                                const lmx_kv8_batch *batch, size_t n_heads,
-                                size_t *bytes);
+                                const lmx_kv8_batch *batch, int type,
+                                size_t n_heads, size_t *bytes);
 /* Attention of the rows' queries (row r at q + r * q_stride, [n_heads]
  * [head_dim], rotated) over their sequences' cached tokens up to their own
  * positions: out = softmax(scale * q . k) v, query head h reading KV head
  * h / (n_heads / n_kv_heads).  A row that sees nothing gets zeros.  out
  * (out_stride; elements of `type`) may be q.
  * Queries become fixed point relative to a power of two at or above the
- * largest of their head (2^-15 of it, for fp32 2^-23), weights of the values
- * 2^-14 (2^-21) of the largest; products with the codes are exact, sums and
- * softmax statistics fp32.  A query head with an element that is not finite
+ * largest of their head (rounded to 2^-15 of it, for fp32 2^-23), weights of
+ * the values rounded to 2^-12 (2^-22) of the largest or finer; products with the codes are exact, sums and
+ * softmax statistics fp32.  V scales below 2^-60 of the largest in reach lose
+ * bits like the small values of one block do.  A query head with an element that is not finite
  * gives NaN.
  * workspace: lmx_kv8_attention_workspace bytes, 16-byte aligned, in any state;
  * calls that may overlap in time need workspaces of their own. */

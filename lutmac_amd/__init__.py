@@ -151,7 +151,7 @@ _SIGS = {
     "lmx_linear_i8": ([_p, _sz, _p, _p, _p, _p, _i, _sz, _sz, _sz, _p, _sz, _p], _i),
     "lmx_weight_codes_i8": ([_p, _p, _sz, _p, _p], _i),
     "lmx_kv8_append": ([_p, _p, _i, _p, _sz, _p, _sz, _p, _sz, _p, _sz, _sz, _p, _sz, _p], _i),
-    "lmx_kv8_attention_workspace": ([_p, _p, _sz, ctypes.POINTER(_sz)], _i),
+    "lmx_kv8_attention_workspace": ([_p, _p, _i, _sz, ctypes.POINTER(_sz)], _i),
     "lmx_kv8_attention": ([_p, _p, _i, _p, _sz, _sz, ctypes.c_float, _p, _sz, _p, _sz, _p], _i),
 }
 
@@ -235,17 +235,19 @@ def _types():
     return _TYPES
 
 
-def _on_current_device(*tensors):
-    """Raises unless the tensors (None: skipped) are on torch's current device,
-    where the calls launch."""
-    import torch
-    for t in tensors:
-        if t is not None and not t.is_cuda:
-            raise ValueError(f"expected device tensors, got one on {t.device}")
-    here = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.device.index != here:
-            raise ValueError(f"expected tensors on the current device cuda:{here}, got one on {t.device}")
+_CURRENT_DEVICE = None
+
+
+def _current_device():
+    """Index of torch's current device, where the calls launch; -1 without a GPU."""
+    global _CURRENT_DEVICE
+    if _CURRENT_DEVICE is None:
+        import torch
+        if not torch.cuda.is_available():
+            return -1
+        torch.cuda.init()
+        _CURRENT_DEVICE = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+    return _CURRENT_DEVICE()
 
 
 # ---- host-only helpers -----------------------------------------------------
@@ -464,32 +466,40 @@ def linear_i8(x, w, w_scale, bias=None, y=None, workspace=None, stream=None):
     linear_i8_workspace bytes that no overlapping call uses (default: torch
     allocates one for the call)."""
     import torch
-    kind = _types().get(x.dtype)
+    dtype = x.dtype
+    kind = _types().get(dtype)
     if kind is None:
-        raise LmxError(ERR_UNSUPPORTED_FORMAT, f"x is {x.dtype}: float32, float16 or bfloat16")
-    if w.dim() != 2 or w.dtype != torch.int8 or w.stride(1) != 1:
+        raise LmxError(ERR_UNSUPPORTED_FORMAT, f"x is {dtype}: float32, float16 or bfloat16")
+    if w.dim() != 2 or w.dtype is not torch.int8 or w.stride(1) != 1:
         raise ValueError("w: int8 [rows, cols] with neighbouring columns side by side")
     rows, cols = w.shape
     if x.dim() == 0 or x.shape[-1] != cols or not x.is_contiguous():
         raise ValueError(f"x {tuple(x.shape)}: contiguous, {cols} values a row")
-    if w_scale.dtype != torch.float32 or w_scale.shape != (rows,) or not w_scale.is_contiguous():
+    if w_scale.dtype is not torch.float32 or w_scale.shape != (rows,) or not w_scale.is_contiguous():
         raise ValueError(f"w_scale: contiguous float32 [{rows}]")
-    if bias is not None and (bias.dtype != x.dtype or bias.shape != (rows,) or not bias.is_contiguous()):
-        raise ValueError(f"bias: contiguous {x.dtype} [{rows}]")
-    batch = x.numel() // cols
+    bp = None
+    if bias is not None:
+        if bias.dtype is not dtype or bias.shape != (rows,) or not bias.is_contiguous():
+            raise ValueError(f"bias: contiguous {dtype} [{rows}]")
+        bp = bias.data_ptr()
+    batch = x.numel() // cols if cols else 0
     if y is None:
-        y = torch.empty(*x.shape[:-1], rows, dtype=x.dtype, device=x.device)
-    elif y.dtype != x.dtype or y.numel() != batch * rows or not y.is_contiguous():
-        raise ValueError(f"y: contiguous {x.dtype}, {batch} x {rows}")
-    need = linear_i8_workspace(rows, cols, batch)
+        y = x.new_empty((batch, rows) if x.dim() == 2 else (*x.shape[:-1], rows))
+    elif y.dtype is not dtype or y.numel() != batch * rows or not y.is_contiguous():
+        raise ValueError(f"y: contiguous {dtype}, {batch} x {rows}")
     if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
-    _on_current_device(x, w, w_scale, bias, y, workspace)
+        size = linear_i8_workspace(rows, cols, batch)
+        workspace = torch.empty(size, dtype=torch.uint8, device=x.device)
+    else:
+        size = workspace.numel() * workspace.element_size()
+    here = _current_device()
+    for t in (x, w, w_scale, bias, y, workspace):
+        if t is not None and (t.get_device() != here or here < 0):
+            raise ValueError(f"expected tensors on the current device, got one on {t.device}")
     # (the stride of a single row says nothing)
-    stride = w.stride(0) if rows > 1 else -(-cols // 16) * 16
-    check(lib().lmx_linear_i8(w.data_ptr(), stride, w_scale.data_ptr(), None if bias is None else bias.data_ptr(),
-                              x.data_ptr(), y.data_ptr(), kind, rows, cols, batch, workspace.data_ptr(),
-                              workspace.numel() * workspace.element_size(), _stream_ptr(stream)))
+    check(lib().lmx_linear_i8(w.data_ptr(), w.stride(0) if rows > 1 else -(-cols // 16) * 16, w_scale.data_ptr(), bp,
+                              x.data_ptr(), y.data_ptr(), kind, rows, cols, batch, workspace.data_ptr(), size,
+                              _stream_ptr(stream)))
     return y
 
 

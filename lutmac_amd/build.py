@@ -34,6 +34,7 @@ SOURCES = [
     ("lmx_noalloc.hip", True),
     ("lmx_decode.hip", True),
     ("lmx_kv8.hip", True),
+    ("lmx_kv8_prompt.hip", True),
     ("lmx_i8.hip", True),
     ("lmx_capi.cpp", False),
     ("lmx_repack.cpp", False),

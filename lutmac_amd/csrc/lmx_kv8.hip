@@ -192,71 +192,10 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
 //   V operand: lane (i, g) holds tokens 16 g .. + 15 of dimension 16 h + i.
 // Weights are relative to the running maximum of score + log2 of the V scale's
 // power of two (what bounds the fixed point); the rest of the scale is
-// multiplied in as the digits are made.
+// multiplied in as the digits are made (see value_exponent).
 //
 // The 4 waves take pages in turn, grid.z parts ("splits") a share of them;
 // (m, l, o) of the waves merge in LDS, of the parts in kv8_merge_kernel.
-struct AttnArgs {
-  Kv8Args c;
-  const void *q;
-  void *out;
-  size_t q_stride, out_stride;
-  float scale;       // softmax scale * log2(e)
-  int splits;
-  float *part_o;     // [units][n_kv][splits][16][HD]
-  float2 *part_ml;   // [units][n_kv][splits][16]
-};
-
-constexpr float kMagic = 12582912.0f;   // 1.5 * 2^23
-// The sums of weights carry 2^kSumExp, so that V scales from 2^-100 to 2^120
-// leave them in range (22 bits of weight, 2^24 tokens).
-constexpr int kSumExp = -24;
-__device__ __forceinline__ float inverse_sum(float l) { return l == 0.0f ? 0.0f : 0x1p-24f / l; }
-
-// ND digit sums (from kMagic) -> the fixed-point sum, rounded once.
-template <int ND>
-__device__ __forceinline__ float join(const float (&d)[ND]) {
-  const float lo = fmaf(d[1], 256.0f, -257.0f * kMagic) + d[0];
-  if constexpr (ND == 2) return lo;
-  else return fmaf(d[2] - kMagic, 65536.0f, lo);
-}
-
-// Four fixed-point values, each in the low bits of a word, 128 added to every
-// digit but the top one -> dword d of the result: their digits d.
-template <int ND>
-__device__ __forceinline__ void digit_words(const uint32_t (&u)[4], uint32_t (&w)[ND]) {
-  const uint32_t a = __builtin_amdgcn_perm(u[1], u[0], 0x05010400u), c = __builtin_amdgcn_perm(u[3], u[2], 0x05010400u);
-  w[0] = __builtin_amdgcn_perm(c, a, 0x05040100u) ^ 0x80808080u;
-  w[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
-  if constexpr (ND == 3) {
-    w[1] ^= 0x80808080u;
-    const uint32_t b = __builtin_amdgcn_perm(u[1], u[0], 0x0C0C0602u), e = __builtin_amdgcn_perm(u[3], u[2], 0x0C0C0602u);
-    w[2] = __builtin_amdgcn_perm(e, b, 0x05040100u);
-  }
-}
-
-template <int ND> struct Digits;
-// carry: 128 for every digit below the top; q_bits: |q| <= 2^q_bits; p_exp: the
-// largest weight is 2^p_exp, so that weight + carry stays below 2^22 (three
-// digits: below the window of kMagic) or 2^15 (two)
-template <> struct Digits<2> { static constexpr int carry = 0x80, q_bits = 14; static constexpr float p_exp = 14.98f; };
-template <> struct Digits<3> { static constexpr int carry = 0x8080, q_bits = 22; static constexpr float p_exp = 21.98f; };
-
-// A row's 16 contiguous elements of step m -> its digit words; f: the power of
-// two of the fixed point.
-template <int ND>
-__device__ __forceinline__ void query_digits(const float (&x)[16], float f, v4i (&w)[ND]) {
-#pragma unroll
-  for (int b = 0; b < 4; ++b) {
-    uint32_t u[4], d[ND];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = uint32_t(__float2int_rn(x[4 * b + i] * f) + Digits<ND>::carry);
-    digit_words<ND>(u, d);
-#pragma unroll
-    for (int j = 0; j < ND; ++j) w[j][b] = int(d[j]);
-  }
-}
-
 template <class T, int HD, int ND>
 __global__ __launch_bounds__(256) void kv8_rows_kernel(AttnArgs a) {
   constexpr int W = 4, M = HD / 64, H = HD / 16;
@@ -309,6 +248,7 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(AttnArgs a) {
   }
 
   float mref = -INFINITY, l = 0.0f;
+  int exmax = kLeastExp + kExpSpan;
   float o[H][4];
 #pragma unroll
   for (int h = 0; h < H; ++h)
@@ -332,8 +272,11 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(AttnArgs a) {
     for (int h = 0; h < H; ++h) vb[h] = *reinterpret_cast<const v4i *>(vp + h * 16 * kPage);
     const int t0 = p * kPage + 16 * g;   // this lane's first token
     if (t0 > last_pos) ks = 0.0f, vs = 0.0f;   // nothing of the block is seen: its scales may hold anything
-    const int ex = vs != 0.0f ? __builtin_amdgcn_frexp_expf(vs) : 0;
-    const float mant = __builtin_amdgcn_frexp_mantf(vs), fex = float(ex), c = qs * ks;
+    int ex = value_exponent(vs);
+    exmax = max(exmax, max(ex, lane_xor_int<16>(ex, lane)));
+    exmax = max(exmax, lane_xor_int<32>(exmax, lane));
+    ex = max(ex, exmax - kExpSpan);
+    const float mant = __builtin_amdgcn_ldexpf(vs, -ex), fex = float(ex), c = qs * ks;
     float y[4][4], top = -INFINITY;
     const bool masked = p * kPage + kPage - 1 > first_pos;
 #pragma unroll
@@ -358,7 +301,7 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(AttnArgs a) {
     top = fmaxf(top, lane_xor<16>(top, lane));
     top = fmaxf(top, lane_xor<32>(top, lane));
     const float mn = fmaxf(mref, top), base = mn == -INFINITY ? 0.0f : mn;
-    const float keep = __builtin_amdgcn_exp2f(mref - base);
+    const float root = __builtin_amdgcn_exp2f(0.5f * (mref - base)), keep = root * root;
     const float off = Digits<ND>::p_exp - base;
     mref = mn;
     v4i pd[ND];
@@ -379,7 +322,7 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(AttnArgs a) {
     }
     // (a block whose scale is not finite gives NaN to the rows that see it)
     const float unit = vs - vs == 0.0f ? __builtin_amdgcn_ldexpf(1.0f, kSumExp - ex) : __builtin_nanf("");
-    l *= keep;
+    l = l * root * root;   // (keep alone may underflow where l is large)
     if (sum != 0.0f) l = fmaf(sum, unit, l);
 #pragma unroll
     for (int h = 0; h < H; ++h) {
@@ -413,8 +356,9 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(AttnArgs a) {
   for (int d = 0; d < E; ++d) acc[d] = 0.0f;
 #pragma unroll
   for (int w = 0; w < W; ++w) {
-    const float f = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ms[w][row] - mx);   // (1: a sum that is NaN stays so)
-    sum += f * ls[w][row];
+    // (1: a sum that is NaN stays so)
+    const float root = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(0.5f * (ms[w][row] - mx)), f = root * root;
+    sum += ls[w][row] * root * root;
 #pragma unroll
     for (int d = 0; d < E; ++d) acc[d] = fmaf(f, os[w][row][d0 + d], acc[d]);
   }
@@ -434,29 +378,29 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(AttnArgs a) {
 }
 
 // The parts of a split unit: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.
-template <class T, int HD>
+template <class T, int HD, int ROWS>
 __global__ __launch_bounds__(256) void kv8_merge_kernel(AttnArgs a) {
   constexpr int E = HD / 16;
   const int lane = threadIdx.x & (kWave - 1), kvh = int(blockIdx.y), group = a.c.group;
   int first = 0;
-  const int seq = unit_sequence(a.c, int(blockIdx.x), group, 1, lane, first);
+  const int seq = unit_sequence(a.c, int(blockIdx.x), group, 1, lane, first, ROWS);
   if (seq < 0) return;
   const SeqRows r(a.c, seq);
-  const int row = int(threadIdx.x) >> 4, d0 = (int(threadIdx.x) & 15) * E;
-  const int i = (int(blockIdx.x) - first) * 16 + row;
+  const int row = int(blockIdx.z) * 16 + (int(threadIdx.x) >> 4), d0 = (int(threadIdx.x) & 15) * E;
+  const int i = (int(blockIdx.x) - first) * ROWS + row;
   if (i >= r.n * group) return;
-  const size_t at = (size_t(blockIdx.x) * a.c.n_kv + kvh) * a.splits * 16 + row;
+  const size_t at = (size_t(blockIdx.x) * a.c.n_kv + kvh) * a.splits * ROWS + row;
   float mx = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) mx = fmaxf(mx, a.part_ml[at + size_t(s) * 16].x);
+  for (int s = 0; s < a.splits; ++s) mx = fmaxf(mx, a.part_ml[at + size_t(s) * ROWS].x);
   float sum = 0.0f, acc[E];
 #pragma unroll
   for (int d = 0; d < E; ++d) acc[d] = 0.0f;
   for (int s = 0; s < a.splits; ++s) {
-    const float2 ml = a.part_ml[at + size_t(s) * 16];
-    const float f = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ml.x - mx);
-    sum += f * ml.y;
+    const float2 ml = a.part_ml[at + size_t(s) * ROWS];
+    const float root = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(0.5f * (ml.x - mx)), f = root * root;
+    sum += ml.y * root * root;
     float o[E];
-    load_floats<E>(a.part_o + (at + size_t(s) * 16) * HD + d0, o);
+    load_floats<E>(a.part_o + (at + size_t(s) * ROWS) * HD + d0, o);
 #pragma unroll
     for (int d = 0; d < E; ++d) acc[d] = fmaf(f, o[d], acc[d]);
   }
@@ -515,33 +459,48 @@ Kv8Args kv8_args(const lmx_kv8_cache *c, const lmx_kv8_batch *b, size_t n_heads)
   return a;
 }
 
-// Work units of 16 rows that a call may have (unit_sequence).
-size_t row_units(const lmx_kv8_batch *b, size_t group) { return b->n_rows * group / 16 + b->n_seqs; }
+// How a call is split over the device, from its sizes alone (lengths are known
+// to the kernels only).
+struct Plan {
+  size_t rows;     // of a work unit: 16 (kv8_rows_kernel) or kPromptRows
+  size_t units;    // at most
+  int splits;      // parts of a unit's pages
+};
 
-// Parts of a unit's pages: as many as bring the grid to about three workgroups
-// per CU, of four pages at least (one per wave).
-int split_count(const lmx_kv8_cache *c, const lmx_kv8_batch *b, size_t group) {
-  const size_t wgs = row_units(b, group) * c->n_kv_heads, want = 768;
-  if (wgs == 0) return 1;
-  const size_t s = std::min<size_t>(want / wgs, b->max_pages / 4);
-  return int(std::max<size_t>(1, std::min<size_t>(s, 64)));
+Plan plan(const lmx_kv8_cache *c, const lmx_kv8_batch *b, size_t n_heads, int type) {
+  const size_t group = n_heads / c->n_kv_heads;
+  Plan p{};
+  p.rows = type != LMX_F32 && b->n_rows * group >= 64 * b->n_seqs ? kPromptRows : 16;
+  p.units = b->n_rows * group / p.rows + b->n_seqs;
+  // As many parts as bring the grid to about three workgroups per CU (prompts:
+  // two), of four pages at least (one per wave; prompts: 8).
+  const size_t wgs = p.units * c->n_kv_heads, want = p.rows == 16 ? 768 : 512;
+  const size_t s = std::min<size_t>(want / wgs, b->max_pages / (p.rows == 16 ? 4 : 8));
+  p.splits = int(std::max<size_t>(1, std::min<size_t>(s, 64)));
+  return p;
 }
 
-size_t workspace_bytes(const lmx_kv8_cache *c, const lmx_kv8_batch *b, size_t n_heads) {
-  const size_t group = n_heads / c->n_kv_heads;
-  const int splits = split_count(c, b, group);
-  if (splits == 1) return 0;
-  return row_units(b, group) * c->n_kv_heads * size_t(splits) * 16 * (c->head_dim + 2) * sizeof(float);
+size_t workspace_bytes(const lmx_kv8_cache *c, const lmx_kv8_batch *b, size_t n_heads, int type) {
+  if (b->n_seqs == 0 || b->n_rows == 0) return 0;
+  const Plan p = plan(c, b, n_heads, type);
+  if (p.splits == 1) return 0;
+  return p.units * c->n_kv_heads * size_t(p.splits) * p.rows * (c->head_dim + 2) * sizeof(float);
 }
 
 template <class T, int HD>
-int launch_attention(const AttnArgs &a, size_t units, hipStream_t st) {
+int launch_attention(const AttnArgs &a, int type, const Plan &p, hipStream_t st) {
   constexpr int ND = sizeof(T) == 4 ? 3 : 2;
-  const dim3 grid(unsigned(units), unsigned(a.c.n_kv), unsigned(a.splits));
-  kv8_rows_kernel<T, HD, ND><<<grid, dim3(256), 0, st>>>(a);
-  int r = launch_err("kv8 attention");
+  const dim3 grid(unsigned(p.units), unsigned(a.c.n_kv), unsigned(a.splits));
+  int r;
+  if (p.rows == 16) {
+    kv8_rows_kernel<T, HD, ND><<<grid, dim3(256), 0, st>>>(a);
+    r = launch_err("kv8 attention");
+  } else {
+    r = launch_prompt(a, type, HD, p.units, st);
+  }
   if (r || a.splits == 1) return r;
-  kv8_merge_kernel<T, HD><<<dim3(unsigned(units), unsigned(a.c.n_kv)), dim3(256), 0, st>>>(a);
+  if (p.rows == 16) kv8_merge_kernel<T, HD, 16><<<dim3(grid.x, grid.y, 1), dim3(256), 0, st>>>(a);
+  else kv8_merge_kernel<T, HD, kPromptRows><<<dim3(grid.x, grid.y, kPromptRows / 16), dim3(256), 0, st>>>(a);
   return launch_err("kv8 merge");
 }
 
@@ -590,11 +549,13 @@ int lmx_kv8_append(const lmx_kv8_cache *cache, const lmx_kv8_batch *batch, int t
   }
 }
 
-int lmx_kv8_attention_workspace(const lmx_kv8_cache *cache, const lmx_kv8_batch *batch, size_t n_heads, size_t *bytes) {
+int lmx_kv8_attention_workspace(const lmx_kv8_cache *cache, const lmx_kv8_batch *batch, int type, size_t n_heads,
+                                size_t *bytes) {
   if (!bytes) return fail(LMX_ERR_INVALID_ARGUMENT, "bytes is NULL");
   const int r = check_sizes(cache, batch, n_heads);
   if (r) return r;
-  *bytes = workspace_bytes(cache, batch, n_heads);
+  if (!type_bytes(type)) return fail(LMX_ERR_UNSUPPORTED_FORMAT, "unknown element type %d", type);
+  *bytes = workspace_bytes(cache, batch, n_heads, type);
   return LMX_OK;
 }
 
@@ -606,7 +567,7 @@ int lmx_kv8_attention(const lmx_kv8_cache *cache, const lmx_kv8_batch *batch, in
   if (!type_bytes(type)) return fail(LMX_ERR_UNSUPPORTED_FORMAT, "unknown element type %d", type);
   if (!(scale > 0.0f) || !(scale < INFINITY)) return fail(LMX_ERR_INVALID_ARGUMENT, "scale %g must be positive and finite", double(scale));
   if (batch->n_seqs == 0 || batch->n_rows == 0) return LMX_OK;
-  const size_t qw = n_heads * cache->head_dim, need = workspace_bytes(cache, batch, n_heads);
+  const size_t qw = n_heads * cache->head_dim, need = workspace_bytes(cache, batch, n_heads, type);
   if ((r = check_pointers(cache, batch)) || (r = check_rows("q", q, q_stride, qw, type, batch->n_rows)) ||
       (r = check_rows("out", out, out_stride, qw, type, batch->n_rows)))
     return r;
@@ -617,15 +578,15 @@ int lmx_kv8_attention(const lmx_kv8_cache *cache, const lmx_kv8_batch *batch, in
   a.c = kv8_args(cache, batch, n_heads);
   a.q = q, a.out = out, a.q_stride = q_stride, a.out_stride = out_stride;
   a.scale = scale * 1.44269504088896340736f;
-  a.splits = split_count(cache, batch, size_t(a.c.group));
-  const size_t units = row_units(batch, size_t(a.c.group));
+  const Plan p = plan(cache, batch, n_heads, type);
+  a.splits = p.splits;
   if (a.splits > 1) {
     a.part_o = static_cast<float *>(workspace);
-    a.part_ml = reinterpret_cast<float2 *>(a.part_o + units * cache->n_kv_heads * size_t(a.splits) * 16 * cache->head_dim);
+    a.part_ml = reinterpret_cast<float2 *>(a.part_o + p.units * cache->n_kv_heads * size_t(a.splits) * p.rows * cache->head_dim);
   }
   hipStream_t st = static_cast<hipStream_t>(stream);
 #define LMX_KV8_ATTENTION(T) \
-  return cache->head_dim == 64 ? launch_attention<T, 64>(a, units, st) : launch_attention<T, 128>(a, units, st)
+  return cache->head_dim == 64 ? launch_attention<T, 64>(a, type, p, st) : launch_attention<T, 128>(a, type, p, st)
   switch (type) {
   case LMX_F32: LMX_KV8_ATTENTION(float);
   case LMX_F16: LMX_KV8_ATTENTION(f16);

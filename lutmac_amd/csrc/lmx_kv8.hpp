@@ -26,12 +26,14 @@ struct Kv8Args {
 };
 
 // The sequence that work unit u belongs to, where sequence s begins at unit
-// floor(offsets[s] * mul / 16) + s * per (at least its units follow, and less
-// than `per` more): -1 past the last.  The wave looks at 64 sequences a load.
-__device__ __forceinline__ int unit_sequence(const Kv8Args &a, int u, int mul, int per, int lane, int &first) {
+// floor(offsets[s] * mul / size) + s * per (at least its units of `size` follow,
+// and at most `per` more): -1 past the last.  The wave looks at 64 sequences a
+// load.
+__device__ __forceinline__ int unit_sequence(const Kv8Args &a, int u, int mul, int per, int lane, int &first,
+                                             int size = 16) {
   int lo = 0, n = a.n_seqs;
   const auto begin = [&](int s) {
-    return int((static_cast<long long>(min(max(a.offsets[s], 0), a.n_rows)) * mul) >> 4) + s * per;
+    return min(max(a.offsets[s], 0), a.n_rows) * mul / size + s * per;   // (below 2^31: at most 2^24 rows, 64 heads)
   };
   while (true) {
     const int step = (n + kWave - 1) / kWave, s = lo + lane * step;
@@ -59,6 +61,82 @@ struct SeqRows {
 };
 
 __device__ __forceinline__ bool page_ok(const Kv8Args &a, int page) { return page >= 0 && page < a.n_pages; }
+
+struct AttnArgs {
+  Kv8Args c;
+  const void *q;
+  void *out;
+  size_t q_stride, out_stride;
+  float scale;       // softmax scale * log2(e)
+  int splits;
+  float *part_o;     // [units][n_kv][splits][16][HD]
+  float2 *part_ml;   // [units][n_kv][splits][16]
+};
+
+constexpr float kMagic = 12582912.0f;   // 1.5 * 2^23
+// The sums of weights carry 2^kSumExp, so that V scales from 2^-100 to 2^120
+// leave them in range (22 bits of weight, 2^24 tokens).
+constexpr int kSumExp = -24;
+__device__ __forceinline__ float inverse_sum(float l) { return l == 0.0f ? 0.0f : 0x1p-24f / l; }
+
+// ND digit sums (from kMagic) -> the fixed-point sum, rounded once.
+template <int ND>
+__device__ __forceinline__ float join(const float (&d)[ND]) {
+  const float lo = fmaf(d[1], 256.0f, -257.0f * kMagic) + d[0];
+  if constexpr (ND == 2) return lo;
+  else return fmaf(d[2] - kMagic, 65536.0f, lo);
+}
+
+// Four fixed-point values, each in the low bits of a word, 128 added to every
+// digit but the top one -> dword d of the result: their digits d.
+template <int ND>
+__device__ __forceinline__ void digit_words(const uint32_t (&u)[4], uint32_t (&w)[ND]) {
+  const uint32_t a = __builtin_amdgcn_perm(u[1], u[0], 0x05010400u), c = __builtin_amdgcn_perm(u[3], u[2], 0x05010400u);
+  w[0] = __builtin_amdgcn_perm(c, a, 0x05040100u) ^ 0x80808080u;
+  w[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+  if constexpr (ND == 3) {
+    w[1] ^= 0x80808080u;
+    const uint32_t b = __builtin_amdgcn_perm(u[1], u[0], 0x0C0C0602u), e = __builtin_amdgcn_perm(u[3], u[2], 0x0C0C0602u);
+    w[2] = __builtin_amdgcn_perm(e, b, 0x05040100u);
+  }
+}
+
+// A weight enters the fixed point as p 2^ex with ex its V scale's power of two,
+// which the rest of the scale, scale 2^-ex, then multiplies.  Scales far below
+// the largest so far (kExpSpan) share its exponent less that, so that their
+// weights, small next to that reference, do not underflow in the sum of weights.
+constexpr int kLeastExp = -100, kExpSpan = 60;
+__device__ __forceinline__ int value_exponent(float scale) {
+  return scale != 0.0f ? max(__builtin_amdgcn_frexp_expf(scale), kLeastExp) : kLeastExp;
+}
+template <int D>
+__device__ __forceinline__ int lane_xor_int(int v, int lane) { return int(lane_xor_u32<D>(uint32_t(v), lane)); }
+
+template <int ND> struct Digits;
+// carry: 128 for every digit below the top; q_bits: |q| <= 2^q_bits; p_exp: the
+// largest weight is 2^p_exp, so that weight + carry stays below 2^22 (three
+// digits: below the window of kMagic) or 2^15 (two)
+template <> struct Digits<2> { static constexpr int carry = 0x80, q_bits = 14; static constexpr float p_exp = 14.98f; };
+template <> struct Digits<3> { static constexpr int carry = 0x8080, q_bits = 22; static constexpr float p_exp = 21.98f; };
+
+// A row's 16 contiguous elements of step m -> its digit words; f: the power of
+// two of the fixed point.
+template <int ND>
+__device__ __forceinline__ void query_digits(const float (&x)[16], float f, v4i (&w)[ND]) {
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    uint32_t u[4], d[ND];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = uint32_t(__float2int_rn(x[4 * b + i] * f) + Digits<ND>::carry);
+    digit_words<ND>(u, d);
+#pragma unroll
+    for (int j = 0; j < ND; ++j) w[j][b] = int(d[j]);
+  }
+}
+
+// Many rows per sequence, 16-bit types (lmx_kv8_prompt.hip).
+constexpr int kPromptRows = 128;   // rows (query heads of tokens) per workgroup
+int launch_prompt(const AttnArgs &a, int type, size_t hd, size_t units, hipStream_t st);
 
 }  // namespace lmx
 

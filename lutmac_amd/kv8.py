@@ -14,12 +14,10 @@ offsets, lengths and pages are int32 and read when the work runs, so a captured
 call follows what they hold at each replay.
 """
 import ctypes
-import math
 
 import torch
 
-from . import (ERR_UNSUPPORTED_FORMAT, Kv8BatchC, Kv8CacheC, LmxError, _on_current_device, _stream_ptr, _types, check,
-               lib)
+from . import (ERR_UNSUPPORTED_FORMAT, Kv8BatchC, Kv8CacheC, LmxError, _current_device, _stream_ptr, _types, check, lib)
 
 PAGE, BLOCK = 64, 16
 
@@ -33,16 +31,20 @@ def rope_table(positions, head_dim, theta=10000.0, factor=1.0, device="cuda"):
     return torch.stack([angle.cos(), angle.sin()], -1).float().to(device)
 
 
-def _rows(name, t, kind, heads, head_dim, rows=None):
+def _bad(name, t, want):
+    raise ValueError(f"{name}: {t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device}, expected {want}")
+
+
+def _rows(name, t, dtype, heads, head_dim, rows):
     """Checks a row tensor [rows, heads, head_dim], rows any stride apart; returns its row stride."""
-    if _types().get(t.dtype) != kind:
-        raise ValueError(f"{name} is {t.dtype}: the rows of a call have one type")
-    if t.dim() != 3 or t.shape[2] != head_dim or (heads and t.shape[1] != heads) or (rows is not None and t.shape[0] != rows):
-        raise ValueError(f"{name} {tuple(t.shape)}: expected [{rows if rows is not None else 'rows'}, {heads or 'heads'}, {head_dim}]")
-    if t.numel() and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != head_dim)):
-        raise ValueError(f"{name}: the heads of a row must lie side by side")
-    # (a single row's stride says nothing)
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * head_dim
+    # (written for speed: every call checks four of them)
+    if t.dtype is not dtype or t.dim() != 3:
+        _bad(name, t, f"{dtype} [rows, heads, {head_dim}]")
+    n, h, d = t.shape
+    row, head, one = t.stride()
+    if n != rows or h != heads or d != head_dim or (n and (one != 1 or (h > 1 and head != head_dim))):
+        _bad(name, t, f"[{rows}, {heads}, {head_dim}] with a row's heads side by side")
+    return row if n > 1 else h * d   # (a single row's stride says nothing)
 
 
 class KvCache8:
@@ -51,21 +53,19 @@ class KvCache8:
     v_scale fp32 [pages, kv_heads, 4]; value = code * scale."""
 
     def __init__(self, k, v, k_scale, v_scale):
-        if k.dim() != 4 or k.shape[2] != PAGE or k.shape[3] not in (64, 128):
-            raise ValueError(f"k {tuple(k.shape)}: expected [pages, kv_heads, {PAGE}, 64 or 128]")
+        if k.dim() != 4 or k.dtype is not torch.int8 or not k.is_contiguous() or k.shape[2] != PAGE or k.shape[3] not in (64, 128):
+            _bad("k", k, f"contiguous int8 [pages, kv_heads, {PAGE}, 64 or 128]")
         pages, heads, _, hd = k.shape
-        if v.shape != (pages, heads, hd, PAGE):
-            raise ValueError(f"v {tuple(v.shape)}: expected {(pages, heads, hd, PAGE)}")
-        if k.dtype != torch.int8 or v.dtype != torch.int8:
-            raise ValueError("codes must be int8")
+        if v.dtype is not torch.int8 or v.shape != (pages, heads, hd, PAGE) or not v.is_contiguous():
+            _bad("v", v, f"contiguous int8 {(pages, heads, hd, PAGE)}")
         for s in (k_scale, v_scale):
-            if s.shape != (pages, heads, PAGE // BLOCK) or s.dtype != torch.float32:
-                raise ValueError(f"scales must be float32 {(pages, heads, PAGE // BLOCK)}")
-        for t in (k, v, k_scale, v_scale):
-            if not t.is_contiguous():
-                raise ValueError("cache tensors must be contiguous")
+            if s.dtype is not torch.float32 or s.shape != (pages, heads, PAGE // BLOCK) or not s.is_contiguous():
+                _bad("scales", s, f"contiguous float32 {(pages, heads, PAGE // BLOCK)}")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.n_pages, self.n_kv_heads, self.head_dim = pages, heads, hd
+        self._device = k.get_device()
+        if v.get_device() != self._device or k_scale.get_device() != self._device or v_scale.get_device() != self._device:
+            raise ValueError("the cache's tensors must be on one device")
         self._c = Kv8CacheC(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, heads, hd)
 
     @classmethod
@@ -76,43 +76,56 @@ class KvCache8:
         return cls(zeros(torch.int8, PAGE, head_dim), zeros(torch.int8, head_dim, PAGE), zeros(torch.float32, PAGE // BLOCK),
                    zeros(torch.float32, PAGE // BLOCK))
 
-    def _batch(self, offsets, lengths, pages, rows):
-        for name, t, dim in (("offsets", offsets, 1), ("lengths", lengths, 1), ("pages", pages, 2)):
-            if t.dtype != torch.int32 or t.dim() != dim or not t.is_contiguous():
-                raise ValueError(f"{name}: contiguous int32 of {dim} dimension(s)")
+    def _batch(self, offsets, lengths, pages, rows, *others):
+        """The call's batch, after checking that all its tensors are on the current device."""
+        if offsets.dtype is not torch.int32 or lengths.dtype is not torch.int32 or pages.dtype is not torch.int32 or \
+                offsets.dim() != 1 or lengths.dim() != 1 or pages.dim() != 2 or \
+                not (offsets.is_contiguous() and lengths.is_contiguous() and pages.is_contiguous()):
+            for name, t, dim in (("offsets", offsets, 1), ("lengths", lengths, 1), ("pages", pages, 2)):
+                if t.dtype is not torch.int32 or t.dim() != dim or not t.is_contiguous():
+                    _bad(name, t, f"contiguous int32 of {dim} dimension(s)")
         n = lengths.shape[0]
-        if offsets.shape[0] != n + 1 or pages.shape[0] != n:
+        listed, width = pages.shape
+        if offsets.shape[0] != n + 1 or listed != n:
             raise ValueError(f"{n} lengths need {n + 1} offsets and {n} page table rows")
-        return Kv8BatchC(offsets.data_ptr(), lengths.data_ptr(), pages.data_ptr(), n, pages.shape[1], rows)
+        device = self._device
+        for t in (offsets, lengths, pages) + others:
+            if t is not None and t.get_device() != device:
+                raise ValueError(f"expected tensors on the cache's device, got one on {t.device}")
+        if device < 0 or device != _current_device():
+            raise ValueError(f"expected tensors on the current device, the cache is on {self.k.device}")
+        return Kv8BatchC(offsets.data_ptr(), lengths.data_ptr(), pages.data_ptr(), n, width, rows)
 
     def append(self, k, v, offsets, lengths, pages, rope=None, q=None, q_out=None, stream=None):
         """lmx_kv8_append: k and v [rows, kv_heads, head_dim] rotated (k) to their
         positions and appended; returns q [rows, heads, head_dim] rotated, in q_out
         (which may be q; default a new tensor), or None without q.  rope: fp32
         [positions, head_dim // 2, 2] (rope_table), or None."""
-        kind = _types().get(k.dtype)
+        dtype, hd, rows = k.dtype, self.head_dim, k.shape[0] if k.dim() else 0
+        kind = _types().get(dtype)
         if kind is None:
             raise LmxError(ERR_UNSUPPORTED_FORMAT, f"k is {k.dtype}: float32, float16 or bfloat16")
-        hd, rows = self.head_dim, k.shape[0]
-        ks, vs = _rows("k", k, kind, self.n_kv_heads, hd), _rows("v", v, kind, self.n_kv_heads, hd, rows)
+        ks, vs = _rows("k", k, dtype, self.n_kv_heads, hd, rows), _rows("v", v, dtype, self.n_kv_heads, hd, rows)
         heads = qs = os = 0
+        qp = op = rp = None
         if q is not None:
-            heads = q.shape[1]
-            qs = _rows("q", q, kind, heads, hd, rows)
+            heads = q.shape[1] if q.dim() == 3 else 0
+            qs = _rows("q", q, dtype, heads, hd, rows)
             if q_out is None:
-                q_out = torch.empty(rows, heads, hd, dtype=q.dtype, device=q.device)
-            os = _rows("q_out", q_out, kind, heads, hd, rows)
+                q_out, os = torch.empty_like(q, memory_format=torch.contiguous_format), heads * hd
+            else:
+                os = _rows("q_out", q_out, dtype, heads, hd, rows)
+            qp, op = q.data_ptr(), q_out.data_ptr()
         elif q_out is not None:
             raise ValueError("q_out without q")
-        if rope is not None and (rope.dtype != torch.float32 or rope.dim() != 3 or rope.shape[1:] != (hd // 2, 2)
-                                 or not rope.is_contiguous()):
-            raise ValueError(f"rope: contiguous float32 [positions, {hd // 2}, 2]")
-        b = self._batch(offsets, lengths, pages, rows)
-        _on_current_device(self.k, self.v, self.k_scale, self.v_scale, k, v, q, q_out, rope, offsets, lengths, pages)
-        check(lib().lmx_kv8_append(ctypes.addressof(self._c), ctypes.addressof(b), kind, k.data_ptr(), ks, v.data_ptr(), vs,
-                                   None if q is None else q.data_ptr(), qs, None if q is None else q_out.data_ptr(), os,
-                                   heads, None if rope is None else rope.data_ptr(), 0 if rope is None else rope.shape[0],
-                                   _stream_ptr(stream)))
+        positions = 0
+        if rope is not None:
+            if rope.dtype is not torch.float32 or rope.dim() != 3 or rope.shape[1:] != (hd // 2, 2) or not rope.is_contiguous():
+                _bad("rope", rope, f"contiguous float32 [positions, {hd // 2}, 2]")
+            rp, positions = rope.data_ptr(), rope.shape[0]
+        b = self._batch(offsets, lengths, pages, rows, k, v, q, q_out, rope)
+        check(lib().lmx_kv8_append(ctypes.byref(self._c), ctypes.byref(b), kind, k.data_ptr(), ks, v.data_ptr(), vs, qp, qs, op,
+                                   os, heads, rp, positions, _stream_ptr(stream)))
         return q_out
 
     def attend(self, q, offsets, lengths, pages, scale=None, out=None, workspace=None, stream=None):
@@ -120,31 +133,33 @@ class KvCache8:
         over the sequences' cached tokens; scale defaults to head_dim ** -0.5.
         workspace: a uint8 tensor of at least attend_workspace bytes that no
         overlapping call uses (default: torch allocates one for the call)."""
-        kind = _types().get(q.dtype)
+        dtype, hd = q.dtype, self.head_dim
+        kind = _types().get(dtype)
         if kind is None:
             raise LmxError(ERR_UNSUPPORTED_FORMAT, f"q is {q.dtype}: float32, float16 or bfloat16")
-        hd, rows = self.head_dim, q.shape[0]
-        qs = _rows("q", q, kind, 0, hd)
-        heads = q.shape[1]
+        rows, heads = q.shape[:2] if q.dim() == 3 else (0, 0)
+        qs = _rows("q", q, dtype, heads, hd, rows)
         if out is None:
-            # rows behind the last sequence are left as they are: of a new tensor, zeros
-            out = torch.empty(rows, heads, hd, dtype=q.dtype, device=q.device)
-        os = _rows("out", out, kind, heads, hd, rows)
-        b = self._batch(offsets, lengths, pages, rows)
-        need = ctypes.c_size_t()
-        check(lib().lmx_kv8_attention_workspace(ctypes.addressof(self._c), ctypes.addressof(b), heads, ctypes.byref(need)))
-        if workspace is None and need.value:
-            workspace = torch.empty(need.value, dtype=torch.uint8, device=q.device)
-        _on_current_device(self.k, self.v, self.k_scale, self.v_scale, q, out, offsets, lengths, pages, workspace)
-        check(lib().lmx_kv8_attention(ctypes.addressof(self._c), ctypes.addressof(b), kind, q.data_ptr(), qs, heads,
-                                      1.0 / math.sqrt(hd) if scale is None else scale, out.data_ptr(), os,
-                                      None if workspace is None else workspace.data_ptr(),
-                                      0 if workspace is None else workspace.numel() * workspace.element_size(),
+            out, os = torch.empty_like(q, memory_format=torch.contiguous_format), heads * hd
+        else:
+            os = _rows("out", out, dtype, heads, hd, rows)
+        b = self._batch(offsets, lengths, pages, rows, q, out, workspace)
+        c, b, size = ctypes.byref(self._c), ctypes.byref(b), ctypes.c_size_t()
+        if workspace is None:
+            check(lib().lmx_kv8_attention_workspace(c, b, kind, heads, ctypes.byref(size)))
+            size = size.value
+            if size:
+                workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+        else:
+            size = workspace.numel() * workspace.element_size()
+        check(lib().lmx_kv8_attention(c, b, kind, q.data_ptr(), qs, heads, hd ** -0.5 if scale is None else scale,
+                                      out.data_ptr(), os, None if workspace is None else workspace.data_ptr(), size,
                                       _stream_ptr(stream)))
         return out
 
-    def attend_workspace(self, rows, heads, n_seqs, max_pages):
+    def attend_workspace(self, dtype, rows, heads, n_seqs, max_pages):
         """Bytes of workspace of an attend call of these sizes."""
         b, n = Kv8BatchC(None, None, None, n_seqs, max_pages, rows), ctypes.c_size_t()
-        check(lib().lmx_kv8_attention_workspace(ctypes.addressof(self._c), ctypes.addressof(b), heads, ctypes.byref(n)))
+        check(lib().lmx_kv8_attention_workspace(ctypes.byref(self._c), ctypes.byref(b), _types()[dtype], heads,
+                                                ctypes.byref(n)))
         return n.value

@@ -97,12 +97,13 @@ class Cache:
         The bound, per row, with n tokens seen, weights p = exp(score - max), L = sum
         p: a score is off by at most d = scale * ||k||_1 * (half a step of the query's
         fixed point) plus fp32's rounding of it, which moves the output by at most
-        2 d max|v|; a weight p 2^e (e the exponent of its V scale) by half a step of
-        the largest such product, 2^-p_exp, times a code of at most 127; fp32 sums of
+        2 d max|v|; a weight p 2^e (e the exponent of its V scale, at most 60 below the
+        largest of the sequence) by half a step of
+        the largest such product, 2^-(p_exp + 1), times a code of at most 127; fp32 sums of
         one term a page (16 a page for L), joined over waves and parts; and the last
         rounding to the type."""
         f32 = dtype == "float32"
-        q_bits, p_exp = (22, 21.98) if f32 else (14, 14.98)
+        q_bits, p_exp = (22, 21.98) if f32 else (14, 10.98)
         out, most = np.full(q.shape, np.nan), np.zeros(q.shape)
         n_kv = self.k.shape[1]
         group = q.shape[1] // n_kv
@@ -132,7 +133,8 @@ class Cache:
                         # (join, scale, exponent and difference each round once, of values up to |score| + 200 in log2)
                         d += 6 * 2.0 ** -24 * (np.abs(sc).max() + 140)
                         a = np.abs(vv).max()
-                        step = 127 * 0.5 * (p * 2.0 ** np.frexp(ex)[1]).max() * 2.0 ** -p_exp * len(p) / p.sum()
+                        e2 = np.maximum(np.frexp(ex)[1], max(-100, np.frexp(vs[ok])[1].max() - 60))
+                        step = 127 * 0.5 * (p * 2.0 ** e2).max() * 2.0 ** -p_exp * len(p) / p.sum()
                         sums = (2 * (see / PAGE + 1) + 40) * 2.0 ** -24
                         most[r, g] = 2 * d * a + step + 2 * sums * a + np.abs(out[r, g]) * HALF_STEP[dtype] + \
                             (2.0 ** -24 if dtype == "float16" else 0.0)

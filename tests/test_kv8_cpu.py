@@ -79,14 +79,14 @@ def test_attention_workspace():
     """A long table splits: the call refuses a workspace that is short, missing or
     unaligned; a table of one page needs none."""
     n = ctypes.c_size_t()
-    size = lambda c, b, h: L.lib().lmx_kv8_attention_workspace(ctypes.addressof(c), ctypes.addressof(b), h, ctypes.byref(n))
+    size = lambda c, b, h: L.lib().lmx_kv8_attention_workspace(ctypes.addressof(c), ctypes.addressof(b), L.F32, h, ctypes.byref(n))
     assert size(cache(), batch(max_pages=1), 4) == L.OK and n.value == 0
     b = batch(max_pages=1024)
     assert size(cache(), b, 4) == L.OK and n.value > 0
     for kw in (dict(work=None), dict(size=n.value - 1), dict(work=A + 4)):
         assert attend(b=b, **kw) == L.ERR_INVALID_ARGUMENT
     assert size(cache(), b, 3) == L.ERR_INVALID_ARGUMENT
-    assert L.lib().lmx_kv8_attention_workspace(ctypes.addressof(cache()), ctypes.addressof(b), 4, None) == L.ERR_INVALID_ARGUMENT
+    assert L.lib().lmx_kv8_attention_workspace(ctypes.addressof(cache()), ctypes.addressof(b), L.F32, 4, None) == L.ERR_INVALID_ARGUMENT
 
 
 def linear(w=A, ws=128, sc=A, bias=None, x=A, y=A, kind=L.F32, rows=10, cols=100, n=3, work=A, size=1 << 30):
