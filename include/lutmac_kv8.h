@@ -94,12 +94,13 @@ int lmx_kv8_attention_workspace(const lmx_kv8_cache *cache,
  * positions: out = softmax(scale * q . k) v, query head h reading KV head
  * h / (n_heads / n_kv_heads).  A row that sees nothing gets zeros.  out
  * (out_stride; elements of `type`) may be q.
- * Queries become fixed point relative to a power of two at or above the
- * largest of their head (rounded to 2^-15 of it, for fp32 2^-23), weights of
- * the values rounded to 2^-12 (2^-22) of the largest or finer; products with the codes are exact, sums and
- * softmax statistics fp32.  V scales below 2^-60 of the largest in reach lose
- * bits like the small values of one block do.  A query head with an element that is not finite
- * gives NaN.
+ * Products with the codes are exact, sums and softmax statistics fp32.  Before
+ * the products queries are rounded to 2^-15 of a power of two at or above the
+ * largest of their head (fp32: 2^-23), the weights of the values to 2^-11 of
+ * themselves or 2^-15 of the largest (fp32: 2^-22 of the largest).  V scales
+ * lie between 2^-100 and 2^100; those below 2^-60 of the largest in reach lose
+ * bits like the small values of one block do.  A query head with an element
+ * that is not finite gives NaN.
  * workspace: lmx_kv8_attention_workspace bytes, 16-byte aligned, in any state;
  * calls that may overlap in time need workspaces of their own. */
 int lmx_kv8_attention(const lmx_kv8_cache *cache, const lmx_kv8_batch *batch,

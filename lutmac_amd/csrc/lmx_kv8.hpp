@@ -77,7 +77,8 @@ constexpr float kMagic = 12582912.0f;   // 1.5 * 2^23
 // The sums of weights carry 2^kSumExp, so that V scales from 2^-100 to 2^120
 // leave them in range (22 bits of weight, 2^24 tokens).
 constexpr int kSumExp = -24;
-__device__ __forceinline__ float inverse_sum(float l) { return l == 0.0f ? 0.0f : 0x1p-24f / l; }
+constexpr float kSumUnit = 0x1p-24f;
+__device__ __forceinline__ float inverse_sum(float l) { return l == 0.0f ? 0.0f : kSumUnit / l; }
 
 // ND digit sums (from kMagic) -> the fixed-point sum, rounded once.
 template <int ND>
@@ -135,7 +136,7 @@ __device__ __forceinline__ void query_digits(const float (&x)[16], float f, v4i 
 }
 
 // Many rows per sequence, 16-bit types (lmx_kv8_prompt.hip).
-constexpr int kPromptRows = 128;   // rows (query heads of tokens) per workgroup
+constexpr int kPromptRows = 256;   // rows (query heads of tokens) per workgroup
 int launch_prompt(const AttnArgs &a, int type, size_t hd, size_t units, hipStream_t st);
 
 }  // namespace lmx

@@ -99,11 +99,12 @@ class Cache:
         fixed point) plus fp32's rounding of it, which moves the output by at most
         2 d max|v|; a weight p 2^e (e the exponent of its V scale, at most 60 below the
         largest of the sequence) by half a step of
-        the largest such product, 2^-(p_exp + 1), times a code of at most 127; fp32 sums of
+        the largest such product, 2^-(p_exp + 1), times a code of at most 127, or (16-bit
+        types) by half a step of fp16, 2^-11 of itself; fp32 sums of
         one term a page (16 a page for L), joined over waves and parts; and the last
         rounding to the type."""
         f32 = dtype == "float32"
-        q_bits, p_exp = (22, 21.98) if f32 else (14, 10.98)
+        q_bits, p_exp = (22, 21.98) if f32 else (14, 14.98)
         out, most = np.full(q.shape, np.nan), np.zeros(q.shape)
         n_kv = self.k.shape[1]
         group = q.shape[1] // n_kv
@@ -135,6 +136,7 @@ class Cache:
                         a = np.abs(vv).max()
                         e2 = np.maximum(np.frexp(ex)[1], max(-100, np.frexp(vs[ok])[1].max() - 60))
                         step = 127 * 0.5 * (p * 2.0 ** e2).max() * 2.0 ** -p_exp * len(p) / p.sum()
+                        step += 0.0 if f32 else 2.0 ** -11 * (p @ np.abs(vv)).max() / p.sum()
                         sums = (2 * (see / PAGE + 1) + 40) * 2.0 ** -24
                         most[r, g] = 2 * d * a + step + 2 * sums * a + np.abs(out[r, g]) * HALF_STEP[dtype] + \
                             (2.0 ** -24 if dtype == "float16" else 0.0)

@@ -215,6 +215,31 @@ def test_unseen_scales(cuda):
     assert (out[3:7] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("hd,group", [(64, 3), (128, 8)])
+@pytest.mark.parametrize("new,old,width", [([300], [0], 5), ([97, 0, 260, 33], [64, 10, 31, 700], 12), ([150], [2000], 40)])
+def test_attend_prompts(cuda, dtype, hd, group, new, old, width):
+    """Prompts of 16-bit types take 256 rows a workgroup: whole and part tiles,
+    prefixes, tables with pages to spare (some outside the pool) and parts."""
+    s = Setup(dtype, hd, 2, group, new, old, seed=15, width=width)
+    s.cache.k_scale.mul_(4)   # scores that outgrow their first reference
+    s.check_attend()
+    s.pages[0, 1] = -1
+    s.where[2].copy_(torch.from_numpy(s.pages))
+    s.cache.v_scale[int(s.pages[0, 0]), 0, 2] = 0.0
+    s.check_attend()
+
+
+def test_prompt_reference_rises(cuda):
+    """Scores that grow page by page by more than a weight's range, and fall."""
+    for sign in (1.0, -1.0):
+        s = Setup("bfloat16", 128, 1, 2, [200], [400], seed=16)
+        rise = torch.linspace(0.001, 0.4, s.cache.n_pages * 4)
+        s.cache.k_scale.view(-1, 4)[torch.from_numpy(s.pages[0]).long().cuda()] = \
+            (rise if sign > 0 else rise.flip(0))[:s.pages.shape[1] * 4].view(-1, 4).cuda()
+        s.check_attend()
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_value_scales_far_apart(cuda, dtype):
     """V scales of 2^-99 to 2^100 in neighbouring blocks, K scales that leave scores
