@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "lmx_internal.hpp"
 #include "lmx_lanes.hpp"
@@ -26,97 +27,147 @@ struct I8Args {
   int rows, cols, batch, Kp;
   int8_t *codes;     // [batch][Kp]
   float *scales;     // [batch]
+  int splits;        // parts of k, each with sums of its own to join
+  int *sums;         // [splits][batch][rows]
 };
 
-// Codes of one row of x per workgroup: the largest magnitude, then
-// round(127 x / amax), exactly rounded (round_quotient), zeros up to Kp.
-// Up to K = 8192 the row stays in registers between the two.
+// Eight neighbouring elements of a row of x (zeros past its end); vec: the row
+// is 16-byte aligned.
 template <class T>
-__global__ __launch_bounds__(256) void i8_codes_kernel(I8Args a) {
-  constexpr int KEEP = 4, E = 8;   // rounds of 256 x 8 elements kept
-  __shared__ uint32_t tops[4];
-  const int lane = threadIdx.x & (kWave - 1), row = int(blockIdx.x);
-  const T *x = static_cast<const T *>(a.x) + size_t(row) * a.cols;
-  const bool vec = reinterpret_cast<size_t>(x) % 16 == 0;
-  const auto load = [&](int k, float (&v)[E]) {
-    if (vec && k + E <= a.cols) {
-      load_floats<E>(x + k, v);
-    } else {
+__device__ __forceinline__ void load8(const T *x, int k, int cols, bool vec, float (&v)[8]) {
+  if (vec && k + 8 <= cols) {
+    load_floats<8>(x + k, v);
+  } else {
 #pragma unroll
-      for (int i = 0; i < E; ++i) v[i] = k + i < a.cols ? float(x[k + i]) : 0.0f;
-    }
-  };
-  float keep[KEEP][E];
-  uint32_t top = 0;
-  const auto fold = [&top](const float (&v)[E]) {
+    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    if (k < cols)
 #pragma unroll
-    for (int i = 0; i < E; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-  };
-  const int k0 = int(threadIdx.x) * E;
-#pragma unroll
-  for (int j = 0; j < KEEP; ++j)
-    if (k0 + j * 256 * E < a.cols) {
-      load(k0 + j * 256 * E, keep[j]);
-      fold(keep[j]);
-    }
-  for (int k = k0 + KEEP * 256 * E; k < a.cols; k += 256 * E) {
-    float v[E];
-    load(k, v);
-    fold(v);
+      for (int i = 0; i < 8; ++i)
+        if (k + i < cols) v[i] = float(x[k + i]);
   }
+}
+__device__ __forceinline__ uint32_t top8(const float (&v)[8], uint32_t top) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+  return top;
+}
+__device__ __forceinline__ uint32_t wave_top(uint32_t top, int lane) {
   top = max(top, lane_xor_u32<32>(top, lane));
   top = max(top, lane_xor_u32<16>(top, lane));
   top = max(top, lane_xor_u32<8>(top, lane));
   top = max(top, lane_xor_u32<4>(top, lane));
   top = max(top, lane_xor_u32<2>(top, lane));
-  top = max(top, lane_xor_u32<1>(top, lane));
-  if (lane == 0) tops[threadIdx.x / kWave] = top;
-  __syncthreads();
-  top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
-  const float amax = __uint_as_float(top);
-  const bool some = top != 0 && top < 0x7F800000u;   // else the codes are zeros
-  const double d = amax, inv = 1.0 / d;
-  const auto store = [&](int k, const float (&v)[E]) {
+  return max(top, lane_xor_u32<1>(top, lane));
+}
+
+// round(127 v / amax), exactly rounded, of a row whose largest magnitude has the
+// bits `top`; zeros for a row of zeros or with a value that is not finite.
+struct Rounder {
+  float amax, finv;
+  bool some;
+  __device__ __forceinline__ explicit Rounder(uint32_t top)
+      : amax(__uint_as_float(top)), some(top != 0 && top < 0x7F800000u) {
+    finv = some ? 127.0f / amax : 0.0f;
+  }
+  __device__ __forceinline__ float scale() const { return amax < INFINITY ? amax / 127.0f : __builtin_nanf(""); }
+  // The quotient in fp32 is off by at most 127 * 3 * 2^-24, far less than kSure
+  // keeps it from a border between two codes; nearer ones, and those of an amax
+  // so small that 127 / amax overflows, are taken in 64 bits.
+  __device__ __forceinline__ uint2 codes(const float (&v)[8]) const {
+    constexpr float kSure = 0.4999f;
     uint32_t w[2] = {0, 0};
+    bool sure = finv < INFINITY;
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const int c = some ? int(round_quotient(double(v[i]) * 127.0, d, inv)) : 0;
-      w[i / 4] |= uint32_t(c & 0xFF) << (8 * (i % 4));
+    for (int i = 0; i < 8; ++i) {
+      const float q = v[i] * finv, n = rintf(q);
+      sure = sure && fabsf(q - n) < kSure;
+      w[i / 4] |= uint32_t(int(n) & 0xFF) << (8 * (i % 4));
     }
-    *reinterpret_cast<uint2 *>(a.codes + size_t(row) * a.Kp + k) = make_uint2(w[0], w[1]);
-  };
+    if (some && !sure) {
+      const double d = amax, inv = 1.0 / d;
+      w[0] = w[1] = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        w[i / 4] |= uint32_t(int(round_quotient(double(v[i]) * 127.0, d, inv)) & 0xFF) << (8 * (i % 4));
+    }
+    return some ? make_uint2(w[0], w[1]) : make_uint2(0, 0);
+  }
+};
+
+// The largest of a row's W / R waves.
+template <int W, int R>
+__device__ __forceinline__ uint32_t row_top(const uint32_t *tops, int m) {
+  uint32_t t = 0;
+#pragma unroll
+  for (int v = 0; v < W / R; ++v) t = max(t, tops[m * (W / R) + v]);
+  return t;
+}
+
+// Codes of x, zeros up to Kp: a workgroup a row, which up to K = 32 NT stays in
+// registers between its maximum and them (8192 rows of 2048 bf16: 21 us; a wave
+// a row took 24).
+template <class T, int NT>
+__global__ __launch_bounds__(NT) void i8_codes_kernel(I8Args a) {
+  constexpr int KEEP = 4, R = NT * 8;   // rounds of R elements kept
+  __shared__ uint32_t tops[NT / kWave];
+  const int lane = threadIdx.x & (kWave - 1), row = int(blockIdx.x);
+  const T *x = static_cast<const T *>(a.x) + size_t(row) * a.cols;
+  const bool vec = reinterpret_cast<size_t>(x) % 16 == 0;
+  float keep[KEEP][8];
+  uint32_t top = 0;
+  const int k0 = int(threadIdx.x) * 8;
 #pragma unroll
   for (int j = 0; j < KEEP; ++j) {
-    const int k = k0 + j * 256 * E;
-    if (k < a.Kp) {
-      if (k >= a.cols)
+    load8(x, k0 + j * R, a.cols, vec, keep[j]);
+    top = top8(keep[j], top);
+  }
+  for (int k = k0 + KEEP * R; k < a.cols; k += R) {
+    float v[8];
+    load8(x, k, a.cols, vec, v);
+    top = top8(v, top);
+  }
+  top = wave_top(top, lane);
+  if (lane == 0) tops[threadIdx.x / kWave] = top;
+  __syncthreads();
+  const Rounder r(row_top<NT / kWave, 1>(tops, 0));
+  int8_t *codes = a.codes + size_t(row) * a.Kp;
 #pragma unroll
-        for (int i = 0; i < E; ++i) keep[j][i] = 0.0f;
-      store(k, keep[j]);
-    }
+  for (int j = 0; j < KEEP; ++j)
+    if (k0 + j * R < a.Kp) *reinterpret_cast<uint2 *>(codes + k0 + j * R) = r.codes(keep[j]);
+  for (int k = k0 + KEEP * R; k < a.Kp; k += R) {
+    float v[8];
+    load8(x, k, a.cols, vec, v);
+    *reinterpret_cast<uint2 *>(codes + k) = r.codes(v);
   }
-  for (int k = k0 + KEEP * 256 * E; k < a.Kp; k += 256 * E) {
-    float v[E];
-    load(k, v);
-    store(k, v);
+  if (k0 == 0) a.scales[row] = r.scale();
+}
+
+// Scales and biases of four neighbouring weight rows (past the last: its own).
+struct Four { float scale[4], bias[4]; };
+template <class T>
+__device__ __forceinline__ Four row_factors(const I8Args &a, int n) {
+  Four f;
+  const T *b = static_cast<const T *>(a.bias);
+  int r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = min(n + i, a.rows - 1), f.scale[i] = a.w_scale[r[i]], f.bias[i] = 0.0f;
+  if (b) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f.bias[i] = float(b[r[i]]);
   }
-  if (threadIdx.x == 0) a.scales[row] = top < 0x7F800000u ? amax / 127.0f : __builtin_nanf("");
+  return f;
 }
 
 // Four neighbouring outputs y[m][n .. n + 3] from their integer sums; whole
 // groups go out in one store where y allows it (vec).
 template <class T>
-__device__ __forceinline__ void store4(const I8Args &a, int m, int n, const v4i s, float xs, bool vec) {
+__device__ __forceinline__ void store4(const I8Args &a, int m, int n, const v4i s, float xs, const Four &w, bool vec) {
   if (m >= a.batch || n >= a.rows) return;
   T *y = static_cast<T *>(a.y) + size_t(m) * a.rows + n;
-  const T *b = static_cast<const T *>(a.bias);
   float f[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = min(n + i, a.rows - 1);
-    f[i] = float(s[i]) * a.w_scale[r] * xs + (b ? float(b[r]) : 0.0f);
-  }
-  if (vec && n + 3 < a.rows) {
+  for (int i = 0; i < 4; ++i) f[i] = fmaf(float(s[i]) * w.scale[i], xs, w.bias[i]);
+  if (vec) {   // (then rows are whole groups)
     store_floats<4>(y, f);
   } else {
 #pragma unroll
@@ -146,87 +197,138 @@ __device__ __forceinline__ void buffer_to_lds(__amdgpu_buffer_rsrc_t buf, char *
 }
 
 // ---------------------------------------------------------------------------
-// Few rows of activations (up to 16 NT): a workgroup takes 16 weight rows, its
-// W waves the k-steps w, w + W, ...; every weight byte goes from memory to an
-// operand register once, the codes come from the caches.
+// One to four rows of activations, one launch: a workgroup takes 16 weight rows,
+// its W waves the k-steps w, w + W, ...; every weight byte goes from memory to
+// an operand register once, four steps of a wave in flight.  Every workgroup
+// makes the codes itself, in LDS while its first weights are on their way (R >=
+// batch rows, a power of two), which saves a launch and the trip through memory.
 //   A (weights): lane (i, g) holds bytes 16 g .. + 15 of a 64-byte step of row i;
 //   B (codes) the same of activation row j; C lane (j, g): weight rows 4 g .. + 3.
-template <class T, int NT, int W>
+template <class T, int W, int R>
 __global__ __launch_bounds__(W *kWave) void i8_rows_kernel(I8Args a) {
-  __shared__ v4i part[W > 1 ? W : 1][NT][kWave];
+  constexpr int U = 4;
+  __shared__ v4i part[W][kWave];
+  __shared__ uint32_t tops[W];
+  extern __shared__ __attribute__((aligned(16))) char codes[];   // [batch][Kp + 16]
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
   const int i = lane & 15, g = lane >> 4, row0 = int(blockIdx.x) * 16;
   const auto wbuf = weight_buffer(a, row0);
   const int wrow = min(i, a.rows - 1 - row0) * int(a.w_stride) + 16 * g;
-  const int8_t *xc[NT];
+  const int steps = a.Kp / kStep;
+  // (a step past the last reads nothing, and zeros)
+  const auto load_weights = [&](int s, v4i (&w)[U][2]) {
 #pragma unroll
-  for (int t = 0; t < NT; ++t) xc[t] = a.codes + size_t(min(16 * t + i, a.batch - 1)) * a.Kp + 16 * g;
-  v4i acc[NT];
+    for (int u = 0; u < U; ++u) {
+      const int at = s + u * W < steps ? (s + u * W) * kStep : 0x7F000000;
 #pragma unroll
-  for (int t = 0; t < NT; ++t) acc[t] = v4i{0, 0, 0, 0};
-  for (int k = wave * kStep; k < a.Kp; k += W * kStep) {
-    v4i w[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      w[h] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(wbuf, wrow + k + 64 * h, 0, 0));
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-        acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[h], *reinterpret_cast<const v4i *>(xc[t] + k + 64 * h), acc[t], 0, 0, 0);
+      for (int h = 0; h < 2; ++h) w[u][h] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(wbuf, wrow + 64 * h, at, 0));
+    }
+  };
+  v4i w[U][2], next[U][2];
+  load_weights(wave, w);
+  {
+    constexpr int TR = W * kWave / R;   // threads of an activation row
+    const int m = int(threadIdx.x) / TR, k0 = int(threadIdx.x) % TR * 8;
+    const T *x = static_cast<const T *>(a.x) + size_t(min(m, a.batch - 1)) * a.cols;
+    const bool vec = reinterpret_cast<size_t>(x) % 16 == 0;
+    uint32_t top = 0;
+    for (int k = k0; k < a.cols; k += TR * 8) {
+      float v[8];
+      load8(x, k, a.cols, vec, v);
+      top = top8(v, top);
+    }
+    top = wave_top(top, lane);
+    if (lane == 0) tops[wave] = top;
+    __syncthreads();
+    if (m < a.batch) {
+      const Rounder r(row_top<W, R>(tops, m));
+      for (int k = k0; k < a.Kp; k += TR * 8) {
+        float v[8];
+        load8(x, k, a.cols, vec, v);   // (from the cache)
+        *reinterpret_cast<uint2 *>(codes + m * (a.Kp + 16) + k) = r.codes(v);
+      }
+    }
+    __syncthreads();
   }
+  const int m = min(i, a.batch - 1);
+  const char *xc = codes + m * (a.Kp + 16) + 16 * g;
+  v4i acc = {0, 0, 0, 0};
+  for (int s = wave; s < steps; s += U * W) {
+    load_weights(s + U * W, next);
 #pragma unroll
-  for (int t = 0; t < NT; ++t) part[wave][t][lane] = acc[t];
+    for (int u = 0; u < U; ++u) {
+      const int k = min(s + u * W, steps - 1) * kStep;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u][h], *reinterpret_cast<const v4i *>(xc + k + 64 * h), acc, 0, 0, 0);
+        w[u][h] = next[u][h];
+      }
+    }
+  }
+  part[wave][lane] = acc;
+  const Four f = row_factors<T>(a, row0 + 4 * g);
   __syncthreads();
-  const bool vec = vector_rows<T>(a);
-  for (int t = wave; t < NT; t += W) {
-    v4i s = part[0][t][lane];
+  if (wave != 0) return;
 #pragma unroll
-    for (int w = 1; w < W; ++w) s += part[w][t][lane];
-    const int m = 16 * t + i;
-    store4<T>(a, m, row0 + 4 * g, s, a.scales[min(m, a.batch - 1)], vec);
-  }
+  for (int v = 1; v < W; ++v) acc += part[v][lane];
+  store4<T>(a, i, row0 + 4 * g, acc, Rounder(row_top<W, R>(tops, m)).scale(), f, vector_rows<T>(a));
 }
 
 // ---------------------------------------------------------------------------
 // Many rows of activations: BN weight rows x BM activation rows per workgroup,
-// WN x WM waves, k in steps of 128 bytes through two LDS buffers that are
-// filled straight from memory while the other is multiplied
-// (v_mfma_i32_32x32x32_i8).  A row's eight 16-byte pieces lie in LDS at p ^ (row
-// / 2) % 8, so that the 16 lanes of a read's phase touch all 64 banks once.
-template <class T, int BN, int BM, int WN, int WM>
-__global__ __launch_bounds__(WN *WM *kWave) void i8_tile_kernel(I8Args a) {
+// WN x WM waves, k in steps of BK bytes through S LDS buffers that are filled
+// straight from memory S - 1 steps ahead (v_mfma_i32_32x32x32_i8).  A row's
+// 16-byte pieces lie in LDS at p ^ swizzle(row), so that the 16 lanes of a
+// read's phase touch all 64 banks once.
+template <int N>
+__device__ __forceinline__ void wait_loads() {   // all but the wave's last N loads are there
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+//
+// PART: workgroup (tile, part) takes part blockIdx.y of k and leaves its integer
+// sums (T is int) for i8_join_kernel: where tiles are few and k is long.
+template <class T, int BN, int BM, int WN, int WM, int BK, int S>
+__global__ __launch_bounds__(WN *WM *kWave) __attribute__((amdgpu_waves_per_eu(BN *BM / (WN * WM) > 8192 ? 1 : 2))) void i8_tile_kernel(I8Args a) {
+  constexpr bool PART = std::is_same<T, int>::value;
   constexpr int W = WN * WM, TN = BN / WN / 32, TM = BM / WM / 32;
-  constexpr int RB = (BN + BM) * kStep;   // bytes of a buffer: weights, then codes
+  constexpr int RB = (BN + BM) * BK;   // bytes of a buffer: weights, then codes
+  constexpr int P = BK / 16;           // pieces of a row
   extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const auto swizzle = [](int row) { return BK == 128 ? (row >> 1) & 7 : (row >> 2) & 3; };
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
   const int wn = wave % WN, wm = wave / WN;
-  const int row0 = int(blockIdx.x) * BN, m0 = int(blockIdx.y) * BM;
+  // Workgroups go round the 8 XCDs, each with an L2 of its own: XCD x takes the
+  // x-th eighth of the tiles, in blocks of 4 weight tiles by all activation
+  // tiles, so that what its workgroups read at a time overlaps.
+  const int gn = (a.rows + BN - 1) / BN, gm = (a.batch + BM - 1) / BM, share = int(gridDim.x) / 8;
+  const int tile = int(blockIdx.x) % 8 * share + int(blockIdx.x) / 8;
+  if (tile >= gn * gm) return;
+  const int g0 = tile / (4 * gm) * 4, gw = min(4, gn - g0), in = tile - g0 * gm;
+  const int row0 = (g0 + in % gw) * BN, m0 = in / gw * BM;
   const auto wbuf = weight_buffer(a, row0);
   const auto xbuf = __builtin_amdgcn_make_buffer_rsrc(a.codes + size_t(m0) * a.Kp, 0,
                                                       int(min(size_t(a.batch - m0) * a.Kp, size_t(0x7FFFFFFF))), 0x00020000);
-  // One load instruction of a wave: 8 rows x 128 bytes.
-  const int lr = lane >> 3, lp = lane & 7;
-  constexpr int LN = BN / 8 / W, LM = BM / 8 / W;   // instructions per wave and buffer
-  static_assert(LN * 8 * W == BN && LM * 8 * W == BM, "whole instructions");
+  // One load instruction of a wave: 1 KB, 64 / P rows.
+  constexpr int LR = 64 / P, LN = BN / LR / W, LM = BM / LR / W;   // rows, instructions per wave and buffer
+  static_assert(LN * LR * W == BN && LM * LR * W == BM, "whole instructions");
+  const int lr = lane / P, lp = lane % P;
   int won[LN], wom[LM];
 #pragma unroll
   for (int j = 0; j < LN; ++j) {
-    const int r = (j * W + wave) * 8 + lr;
-    won[j] = min(r, a.rows - 1 - row0) * int(a.w_stride) + 16 * (lp ^ ((r >> 1) & 7));
+    const int r = (j * W + wave) * LR + lr;
+    won[j] = min(r, a.rows - 1 - row0) * int(a.w_stride) + 16 * (lp ^ swizzle(r));
   }
 #pragma unroll
   for (int j = 0; j < LM; ++j) {
-    const int r = (j * W + wave) * 8 + lr;
-    wom[j] = min(r, a.batch - 1 - m0) * a.Kp + 16 * (lp ^ ((r >> 1) & 7));
+    const int r = (j * W + wave) * LR + lr;
+    wom[j] = min(r, a.batch - 1 - m0) * a.Kp + 16 * (lp ^ swizzle(r));
   }
   const auto fill = [&](int buf, int k) {
 #pragma unroll
-    for (int j = 0; j < LN; ++j)
-      buffer_to_lds(wbuf, lds + buf * RB + (j * W + wave) * 1024, won[j], k);
+    for (int j = 0; j < LN; ++j) buffer_to_lds(wbuf, lds + buf * RB + (j * W + wave) * 1024, won[j], k);
 #pragma unroll
-    for (int j = 0; j < LM; ++j)
-      buffer_to_lds(xbuf, lds + buf * RB + BN * kStep + (j * W + wave) * 1024, wom[j], k);
+    for (int j = 0; j < LM; ++j) buffer_to_lds(xbuf, lds + buf * RB + BN * BK + (j * W + wave) * 1024, wom[j], k);
   };
   v16i acc[TN][TM];
 #pragma unroll
@@ -236,40 +338,118 @@ __global__ __launch_bounds__(WN *WM *kWave) void i8_tile_kernel(I8Args a) {
 #pragma unroll
       for (int v = 0; v < 16; ++v) acc[n][m][v] = 0;
   const int i = lane & 31, h = lane >> 5;
-  const int steps = a.Kp / kStep;
-  fill(0, 0);
-  for (int s = 0; s < steps; ++s) {
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    if (s + 1 < steps) fill((s + 1) & 1, (s + 1) * kStep);
-    const char *wl = lds + (s & 1) * RB + (wn * (BN / WN) + i) * kStep;
-    const char *xl = lds + (s & 1) * RB + BN * kStep + (wm * (BM / WM) + i) * kStep;
+  int steps = a.Kp / BK, k0 = 0;
+  if constexpr (PART) {
+    const int all = steps, part = int(blockIdx.y);
+    k0 = int(unsigned(all) * unsigned(part) / unsigned(a.splits));
+    steps = int(unsigned(all) * unsigned(part + 1) / unsigned(a.splits)) - k0;
+    k0 *= BK;
+  }
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int at = 16 * ((2 * q + h) ^ ((i >> 1) & 7));
+  for (int s = 0; s < S - 1; ++s)
+    if (s < steps) fill(s, k0 + s * BK);
+  int buf = 0;
+  for (int s = 0; s < steps; ++s) {
+    if (s + S - 1 <= steps) wait_loads<(S - 2) * (LN + LM)>();
+    else wait_loads<0>();
+    asm volatile("s_barrier" ::: "memory");   // (no wait for the loads of later steps, as __syncthreads makes)
+    if (s + S - 1 < steps) fill(buf == 0 ? S - 1 : buf - 1, k0 + (s + S - 1) * BK);
+    const char *wl = lds + buf * RB + (wn * (BN / WN) + i) * BK;
+    const char *xl = lds + buf * RB + BN * BK + (wm * (BM / WM) + i) * BK;
+#pragma unroll
+    for (int q = 0; q < BK / 32; ++q) {
+      const int at = 16 * ((2 * q + h) ^ swizzle(i));
       v4i wf[TN], xf[TM];
 #pragma unroll
-      for (int n = 0; n < TN; ++n) wf[n] = *reinterpret_cast<const v4i *>(wl + n * 32 * kStep + at);
+      for (int n = 0; n < TN; ++n) wf[n] = *reinterpret_cast<const v4i *>(wl + n * 32 * BK + at);
 #pragma unroll
-      for (int m = 0; m < TM; ++m) xf[m] = *reinterpret_cast<const v4i *>(xl + m * 32 * kStep + at);
+      for (int m = 0; m < TM; ++m) xf[m] = *reinterpret_cast<const v4i *>(xl + m * 32 * BK + at);
 #pragma unroll
       for (int n = 0; n < TN; ++n)
 #pragma unroll
         for (int m = 0; m < TM; ++m) acc[n][m] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[n], xf[m], acc[n][m], 0, 0, 0);
     }
+    buf = buf == S - 1 ? 0 : buf + 1;
   }
-  const bool vec = vector_rows<T>(a);
-#pragma unroll
-  for (int m = 0; m < TM; ++m) {
-    const int mr = m0 + wm * (BM / WM) + 32 * m + i;
-    const float xs = a.scales[min(mr, a.batch - 1)];
+  // The sums leave through LDS, 32 activation rows of the wave at a time, so
+  // that stores are whole lines of y (a lane's own four neighbours at a time
+  // take 2 to 4 times as long).
+  constexpr int NW = BN / WN, LD = NW * int(sizeof(T)) + 16;   // a row in LDS, apart by banks
+  static_assert(W * 32 * LD <= S * RB, "the rows fit in the buffers");
+  asm volatile("s_barrier" ::: "memory");   // every wave is done with the buffers
+  char *out = lds + wave * (32 * LD);
+  const int n0 = row0 + wn * NW;
+  Four w[TN][4];
+  if constexpr (!PART) {
 #pragma unroll
     for (int n = 0; n < TN; ++n)
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
-        store4<T>(a, mr, row0 + wn * (BN / WN) + 32 * n + 8 * b + 4 * h,
-                  v4i{acc[n][m][4 * b], acc[n][m][4 * b + 1], acc[n][m][4 * b + 2], acc[n][m][4 * b + 3]}, xs, vec);
+      for (int b = 0; b < 4; ++b) w[n][b] = row_factors<T>(a, min(n0 + 32 * n + 8 * b + 4 * h, a.rows - 1));
   }
+  constexpr int V = 16 / int(sizeof(T)), LPR = NW / V;   // elements of a store, lanes of a row
+  T *base = PART ? reinterpret_cast<T *>(a.sums) + size_t(blockIdx.y) * a.batch * a.rows : static_cast<T *>(a.y);
+  const bool vec = a.rows % V == 0 && reinterpret_cast<size_t>(base) % 16 == 0;
+#pragma unroll
+  for (int m = 0; m < TM; ++m) {
+    const int m1 = m0 + wm * (BM / WM) + 32 * m;
+    if (m1 >= a.batch) break;
+    const float xs = PART ? 0.0f : a.scales[min(m1 + i, a.batch - 1)];
+#pragma unroll
+    for (int n = 0; n < TN; ++n)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        T *at = reinterpret_cast<T *>(out + i * LD) + 32 * n + 8 * b + 4 * h;
+        if constexpr (PART) {
+          *reinterpret_cast<v4i *>(at) = v4i{acc[n][m][4 * b], acc[n][m][4 * b + 1], acc[n][m][4 * b + 2], acc[n][m][4 * b + 3]};
+        } else {
+          float f[4];
+#pragma unroll
+          for (int v = 0; v < 4; ++v) f[v] = fmaf(float(acc[n][m][4 * b + v]) * w[n][b].scale[v], xs, w[n][b].bias[v]);
+          store_floats<4>(at, f);
+        }
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    T *y = base + size_t(m1) * a.rows + n0;
+    if (vec) {
+      typedef T vecT __attribute__((ext_vector_type(V)));
+#pragma unroll
+      for (int q = 0; q < 32 * LPR / kWave; ++q) {
+        const int r = q * (kWave / LPR) + lane / LPR, n = lane % LPR * V;
+        if (m1 + r < a.batch && n0 + n < a.rows)
+          *reinterpret_cast<vecT *>(y + size_t(r) * a.rows + n) = *reinterpret_cast<const vecT *>(out + r * LD + n * sizeof(T));
+      }
+    } else {
+      for (int q = 0; q < 32 * NW / kWave; ++q) {
+        const int at = q * kWave + lane, r = at / NW, n = at % NW;
+        if (m1 + r < a.batch && n0 + n < a.rows) y[size_t(r) * a.rows + n] = *reinterpret_cast<const T *>(out + r * LD + n * sizeof(T));
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+}
+
+// y from the parts' sums, four weight rows of an activation row per thread.
+template <class T>
+__global__ __launch_bounds__(256) void i8_join_kernel(I8Args a) {
+  const int quads = (a.rows + 3) / 4;
+  const size_t at = size_t(blockIdx.x) * 256 + threadIdx.x;
+  if (at >= size_t(quads) * a.batch) return;
+  const int m = int(at / quads), n = int(at % quads) * 4;
+  const bool vec = vector_rows<T>(a);
+  const float xs = a.scales[m];
+  const Four w = row_factors<T>(a, n);
+  const int *p = a.sums + size_t(m) * a.rows + n;
+  v4i s = {0, 0, 0, 0};
+#pragma unroll 8
+  for (int q = 0; q < a.splits; ++q, p += size_t(a.batch) * a.rows) {
+    if (a.rows % 4 == 0) {
+      s += *reinterpret_cast<const v4i *>(p);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[i] += n + i < a.rows ? p[i] : 0;
+    }
+  }
+  store4<T>(a, m, n, s, xs, w, vec);
 }
 
 // ---- host side ----
@@ -279,47 +459,86 @@ int launch_err(const char *what) {
   return e == hipSuccess ? LMX_OK : fail(LMX_ERR_LAUNCH_FAILED, "%s launch: %s", what, hipGetErrorString(e));
 }
 
-template <class T, int NT>
-void launch_rows(const I8Args &a, hipStream_t st) {
-  const unsigned grid = unsigned((a.rows + 15) / 16);
-  // more waves share a row tile's k where the tiles alone leave CUs idle
-  if (grid < 512) i8_rows_kernel<T, NT, 8><<<grid, 8 * kWave, 0, st>>>(a);
-  else i8_rows_kernel<T, NT, 4><<<grid, 4 * kWave, 0, st>>>(a);
+size_t tile_count(size_t rows, size_t batch, size_t side) { return (rows + side - 1) / side * ((batch + side - 1) / side); }
+
+// Parts of k: as many as bring the 64 x 64 tiles to one per CU, of 8 steps at
+// least (us, in one part / in parts: 48 x 8960 -> 1536 in 8 28 / 16, 64 x 8192 ->
+// 8192 in 2 28 / 23, 48 x 2048 -> 2048 in 2 12.0 / 12.1).
+int split_count(size_t rows, size_t cols, size_t batch) {
+  const size_t tiles = tile_count(rows, batch, 64), steps = round_up(cols, kStep) / kStep;
+  return tiles ? int(std::max<size_t>(1, std::min<size_t>(256 / tiles, steps / 8))) : 1;
 }
 
-template <class T, int BN, int BM, int WN, int WM>
+// More waves share a row tile's k where the tiles alone leave CUs idle.
+int rows_waves(const I8Args &a) {
+  const int tiles = (a.rows + 15) / 16;
+  return tiles <= 256 ? 16 : tiles <= 768 ? 8 : 4;
+}
+
+template <class T, int R>
+void launch_rows(const I8Args &a, hipStream_t st) {
+  const unsigned grid = unsigned((a.rows + 15) / 16), lds = unsigned(a.batch * (a.Kp + 16));
+  switch (rows_waves(a)) {
+  case 16: i8_rows_kernel<T, 16, R><<<grid, 16 * kWave, lds, st>>>(a); break;
+  case 8: i8_rows_kernel<T, 8, R><<<grid, 8 * kWave, lds, st>>>(a); break;
+  default: i8_rows_kernel<T, 4, R><<<grid, 4 * kWave, lds, st>>>(a); break;
+  }
+}
+
+// Whether every workgroup makes the codes itself: up to 4 rows, as long as that
+// is two rounds of a workgroup's threads (us, itself / codes in a launch before:
+// 1 x 2048 -> 16384 9.2 / 12.1, 4 x 2048 -> 8192 9.7 / 11.1, 4 x 2048 -> 16384,
+// four rounds, 14.2 / 12.4).
+bool in_one_launch(const I8Args &a) {
+  return a.batch <= 4 && a.batch * a.Kp <= 1024 * rows_waves(a);
+}
+
+template <class T, int BN, int BM, int WN, int WM, int BK, int S>
 int launch_tile(const I8Args &a, hipStream_t st) {
-  constexpr size_t lds = 2 * (BN + BM) * kStep;
-  static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&i8_tile_kernel<T, BN, BM, WN, WM>),
+  constexpr size_t lds = S * (BN + BM) * BK;
+  static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&i8_tile_kernel<T, BN, BM, WN, WM, BK, S>),
                                                   hipFuncAttributeMaxDynamicSharedMemorySize, int(lds));
   if (e != hipSuccess) return fail(LMX_ERR_HIP, "LDS of the i8 tile kernel: %s", hipGetErrorString(e));
-  const dim3 grid(unsigned((a.rows + BN - 1) / BN), unsigned((a.batch + BM - 1) / BM));
-  i8_tile_kernel<T, BN, BM, WN, WM><<<grid, WN * WM * kWave, lds, st>>>(a);
+  const size_t tiles = size_t((a.rows + BN - 1) / BN) * size_t((a.batch + BM - 1) / BM);
+  if (tiles > (1u << 30)) return fail(LMX_ERR_INVALID_ARGUMENT, "%d x %d outputs", a.rows, a.batch);
+  i8_tile_kernel<T, BN, BM, WN, WM, BK, S><<<dim3(unsigned(round_up(tiles, 8)), unsigned(a.splits)), WN * WM * kWave, lds, st>>>(a);
   return LMX_OK;
 }
 
 template <class T>
 int launch_linear(const I8Args &a, hipStream_t st) {
-  i8_codes_kernel<T><<<unsigned(a.batch), 256, 0, st>>>(a);
+  if (in_one_launch(a)) {
+    if (a.batch == 1) launch_rows<T, 1>(a, st);
+    else if (a.batch == 2) launch_rows<T, 2>(a, st);
+    else launch_rows<T, 4>(a, st);
+    return launch_err("i8 linear");
+  }
+  // (few long rows: 1024 threads a row, 48 of 8960 in 4.3 us against 6.8)
+  if (a.Kp > 2048 && a.batch < 512) i8_codes_kernel<T, 1024><<<unsigned(a.batch), 1024, 0, st>>>(a);
+  else i8_codes_kernel<T, 256><<<unsigned(a.batch), 256, 0, st>>>(a);
   int r = launch_err("i8 codes");
   if (r) return r;
-  if (a.batch <= 64) {
-    switch ((a.batch + 15) / 16) {
-    case 1: launch_rows<T, 1>(a, st); break;
-    case 2: launch_rows<T, 2>(a, st); break;
-    case 3: launch_rows<T, 3>(a, st); break;
-    default: launch_rows<T, 4>(a, st); break;
-    }
-  } else {
-    const auto tiles = [&](int bn, int bm) { return size_t((a.rows + bn - 1) / bn) * size_t((a.batch + bm - 1) / bm); };
-    if (tiles(256, 256) >= 256) r = launch_tile<T, 256, 256, 4, 2>(a, st);
-    else r = launch_tile<T, 64, 64, 2, 2>(a, st);
+  if (a.splits > 1) {
+    if ((r = launch_tile<int, 64, 64, 2, 2, 128, 4>(a, st)) || (r = launch_err("i8 linear parts"))) return r;
+    i8_join_kernel<T><<<unsigned((size_t(a.batch) * ((a.rows + 3) / 4) + 255) / 256), 256, 0, st>>>(a);
+    return launch_err("i8 join");
   }
+  // The largest tiles that still fill most of the CUs, as larger ones read less
+  // from the L2s (us at K = 2048, 256 / 128 / 64: 2048 -> 8192 49 / 56 / 85, 1024
+  // -> 8192 39 / 32 / 44, 256 -> 16384 34 / 22 / 25, 100 -> 17920 32 / 21 / 21).
+  const size_t rows = a.rows, batch = a.batch;
+  if (tile_count(rows, batch, 256) >= 192) r = launch_tile<T, 256, 256, 4, 2, 128, 2>(a, st);
+  else if (tile_count(rows, batch, 128) >= 160) r = launch_tile<T, 128, 128, 2, 2, 128, 2>(a, st);
+  else r = launch_tile<T, 64, 64, 2, 2, 128, 4>(a, st);
   return r ? r : launch_err("i8 linear");
 }
 
-size_t i8_workspace(size_t cols, size_t batch) {
-  return round_up(batch * sizeof(float), 256) + batch * round_up(cols, kStep);
+// Scales, codes and, of a call that splits k, its parts' sums.
+size_t codes_at(size_t batch) { return round_up(batch * sizeof(float), 256); }
+size_t sums_at(size_t cols, size_t batch) { return codes_at(batch) + round_up(batch * round_up(cols, kStep), 256); }
+size_t i8_workspace(size_t rows, size_t cols, size_t batch) {
+  const int splits = split_count(rows, cols, batch);
+  return sums_at(cols, batch) + (splits > 1 ? size_t(splits) * batch * rows * sizeof(int) : 0);
 }
 
 // Codes of an 8-bit handle from its copy for the matrix cores: byte B of word t
@@ -347,7 +566,7 @@ int lmx_linear_i8_workspace(size_t rows, size_t cols, size_t batch, size_t *byte
   if (!bytes) return fail(LMX_ERR_INVALID_ARGUMENT, "bytes is NULL");
   if (rows == 0 || rows > (1u << 24) || cols == 0 || cols > 131072 || batch > (1u << 22))
     return fail(LMX_ERR_INVALID_ARGUMENT, "%zu x %zu, %zu vectors: rows 1..2^24, cols 1..131072, at most 2^22 vectors", rows, cols, batch);
-  *bytes = i8_workspace(cols, batch);
+  *bytes = i8_workspace(rows, cols, batch);
   return LMX_OK;
 }
 
@@ -373,7 +592,9 @@ int lmx_linear_i8(const int8_t *w, size_t w_stride, const float *w_scale, const 
   a.w = w, a.w_stride = w_stride, a.w_scale = w_scale, a.bias = bias, a.x = x, a.y = y;
   a.rows = int(rows), a.cols = int(cols), a.batch = int(batch), a.Kp = int(round_up(cols, kStep));
   a.scales = static_cast<float *>(workspace);
-  a.codes = static_cast<int8_t *>(workspace) + round_up(batch * sizeof(float), 256);
+  a.codes = static_cast<int8_t *>(workspace) + codes_at(batch);
+  a.splits = split_count(rows, cols, batch);
+  a.sums = reinterpret_cast<int *>(static_cast<char *>(workspace) + sums_at(cols, batch));
   hipStream_t st = static_cast<hipStream_t>(stream);
   switch (type) {
   case LMX_F32: return launch_linear<float>(a, st);

@@ -74,13 +74,10 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
   constexpr int E = HD / 32, VE = HD / 16;
   __shared__ __attribute__((aligned(16))) uint8_t cod[HD][kBlock];
   const int lane = threadIdx.x & (kWave - 1), tk = int(threadIdx.x) >> 4, part = int(threadIdx.x) & 15;
-  int first = 0;
-  const int seq = unit_sequence(a.c, int(blockIdx.x), 1, 2, lane, first);
-  if (seq < 0) return;
-  const SeqRows r(a.c, seq);
+  const SeqRows r = unit_rows(a.c, int(blockIdx.x), 1, 2, lane, kBlock);
   const int from = max(r.start, 0);   // rows before position 0 have no place
-  const int block = from / kBlock + (int(blockIdx.x) - first);
-  if (r.n == 0 || block >= (r.len + kBlock - 1) / kBlock) return;
+  const int block = from / kBlock + (int(blockIdx.x) - r.first);
+  if (r.seq < 0 || r.n == 0 || block >= (r.len + kBlock - 1) / kBlock) return;
   const int pos = block * kBlock + tk;
   const bool live = pos >= from && pos < r.len && (!a.rope || pos < a.rope_n);
   const size_t row = size_t(r.r0 + (live ? pos - r.start : from - r.start));
@@ -100,7 +97,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
   }
   const int pi = block / kPageBlocks, sub = block % kPageBlocks;
   if (pi >= a.c.max_pages) return;
-  const int page = a.c.pages[size_t(seq) * a.c.max_pages + pi];
+  const int page = a.c.pages[size_t(r.seq) * a.c.max_pages + pi];
   if (!page_ok(a.c, page)) return;
   const int kept = max(from - block * kBlock, 0);   // earlier tokens of the block
   const int last = min(r.len, a.rope ? a.rope_n : r.len) - block * kBlock;   // tokens of the block with the rows
@@ -196,20 +193,21 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
 //
 // The 4 waves take pages in turn, grid.z parts ("splits") a share of them;
 // (m, l, o) of the waves merge in LDS, of the parts in kv8_merge_kernel.
+// Bound by the cache's bytes where contexts are long, else by the chain of loads
+// (offsets, table, page, and each further page of a wave): table entries come 64
+// at a time, and a page's keys and values are requested as soon as the registers
+// of the page before are free of theirs.
 template <class T, int HD, int ND>
-__global__ __launch_bounds__(256) void kv8_rows_kernel(AttnArgs a) {
+__global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(ND == 3 && HD == 128 ? 2 : 3))) void kv8_rows_kernel(AttnArgs a) {
   constexpr int W = 4, M = HD / 64, H = HD / 16;
   __shared__ float os[W][16][HD + 4];
   __shared__ float ms[W][16], ls[W][16];
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
   const int j = lane & 15, g = lane >> 4;
   const int kvh = int(blockIdx.y), group = a.c.group;
-  int first = 0;
-  const int seq = unit_sequence(a.c, int(blockIdx.x), group, 1, lane, first);
-  if (seq < 0) return;
-  const SeqRows r(a.c, seq);
-  const int tile0 = (int(blockIdx.x) - first) * 16, rows = r.n * group;   // (< 2^31: checked by the host)
-  if (tile0 >= rows) return;
+  const SeqRows r = unit_rows(a.c, int(blockIdx.x), group, 1, lane, 16);
+  const int tile0 = (int(blockIdx.x) - r.first) * 16, rows = r.n * group;   // (< 2^31: checked by the host)
+  if (r.seq < 0 || tile0 >= rows) return;
   // row i of the sequence: query head kvh * group + i % group of token i / group
   const int i = tile0 + j;
   const int t = min(i, rows - 1) / group;
@@ -218,21 +216,67 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(AttnArgs a) {
   const int limit = min(r.start + t, see);
   const int n_pages = last_pos < 0 ? 0 : last_pos / kPage + 1;
   const int part = int(blockIdx.z);
-  const int p0 = int((long long)n_pages * part / a.splits), p1 = int((long long)n_pages * (part + 1) / a.splits);
+  const int p0 = part_begin(n_pages, part, a.splits), p1 = part_begin(n_pages, part + 1, a.splits);
 
-  // query digits, this lane's 16 dimensions of every 64-dimension step
+  float mref = -INFINITY, l = 0.0f;
+  int exmax = kLeastExp + kExpSpan;
+  float o[H][4];
+#pragma unroll
+  for (int h = 0; h < H; ++h)
+#pragma unroll
+    for (int v = 0; v < 4; ++v) o[h][v] = 0.0f;
+  const v4i zero = {__float_as_int(kMagic), __float_as_int(kMagic), __float_as_int(kMagic), __float_as_int(kMagic)};
+  const int *table = a.c.pages + size_t(r.seq) * a.c.max_pages;
+  int entries = 0;   // lane n: the table's entry of the wave's page n (of 64)
+  const auto read_entries = [&](int p) { entries = table[min(p + W * lane, p1 - 1)]; };
+  if (p0 + wave < p1) read_entries(p0 + wave);
+  // the row's query: this lane's 16 dimensions of every 64-dimension step
   const T *q = static_cast<const T *>(a.q) + size_t(r.r0 + t) * a.q_stride + size_t(kvh * group + min(i, rows - 1) % group) * HD;
+  float x[M][16];
+#pragma unroll
+  for (int m = 0; m < M; ++m) load_floats<16>(q + 64 * m + 16 * g, x[m]);
+  v4i kb[4][M], vb[H];
+  float ks = 0.0f, vs = 0.0f;   // the scales of the page whose keys were requested last
+  int page = -1;
+  // (through buffers of a page's size, or of none: then nothing is fetched, and
+  // no register waits behind a branch)
+  const auto buffer = [](const void *p, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, bytes, 0x00020000);
+  };
+  const int kat = (16 * (j >> 2) + (j & 3)) * HD + 16 * g, vat = j * kPage + 16 * g;
+  const auto request_keys = [&](int p, int n) {   // page p, the wave's n-th
+    page = p < p1 ? __builtin_amdgcn_readlane(entries, n & (kWave - 1)) : -1;
+    const bool ok = page_ok(a.c, page);
+    const size_t ph = size_t(ok ? page : 0) * a.c.n_kv + kvh;
+    const auto kbuf = buffer(a.c.k + ph * kPage * HD, ok ? kPage * HD : 0);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+        kb[u][m] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(kbuf, kat + 4 * u * HD + 64 * m, 0, 0));
+    ks = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(buffer(a.c.k_scale + ph * kPageBlocks, ok ? 16 : 0), 4 * g, 0, 0));
+    vs = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(buffer(a.c.v_scale + ph * kPageBlocks, ok ? 16 : 0), 4 * g, 0, 0));
+  };
+  const auto request_values = [&]() {
+    const bool ok = page_ok(a.c, page);
+    const auto vbuf = buffer(a.c.v + (size_t(ok ? page : 0) * a.c.n_kv + kvh) * (kPage * HD), ok ? kPage * HD : 0);
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+      vb[h] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(vbuf, vat + h * 16 * kPage, 0, 0));
+  };
+  if (p0 + wave < p1) {
+    request_keys(p0 + wave, 0);
+    request_values();
+  }
+  // (its digits are made while the first page is on its way)
   v4i qd[M][ND];
   float qs;
   {
-    float x[M][16];
     uint32_t top = 0;
 #pragma unroll
-    for (int m = 0; m < M; ++m) {
-      load_floats<16>(q + 64 * m + 16 * g, x[m]);
+    for (int m = 0; m < M; ++m)
 #pragma unroll
       for (int d = 0; d < 16; ++d) top = max(top, __float_as_uint(x[m][d]) & 0x7FFFFFFFu);
-    }
     top = max(top, lane_xor_u32<16>(top, lane));
     top = max(top, lane_xor_u32<32>(top, lane));
     const bool finite = top < 0x7F800000u;
@@ -247,38 +291,18 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(AttnArgs a) {
     qs = finite ? __builtin_amdgcn_ldexpf(a.scale, e - Digits<ND>::q_bits) : __builtin_nanf("");
   }
 
-  float mref = -INFINITY, l = 0.0f;
-  int exmax = kLeastExp + kExpSpan;
-  float o[H][4];
-#pragma unroll
-  for (int h = 0; h < H; ++h)
-#pragma unroll
-    for (int v = 0; v < 4; ++v) o[h][v] = 0.0f;
-  const v4i zero = {__float_as_int(kMagic), __float_as_int(kMagic), __float_as_int(kMagic), __float_as_int(kMagic)};
-  const int *table = a.c.pages + size_t(seq) * a.c.max_pages;
-  for (int p = p0 + wave; p < p1; p += W) {
-    const int page = __builtin_amdgcn_readfirstlane(table[p]);
-    if (!page_ok(a.c, page)) continue;
-    const size_t ph = size_t(page) * a.c.n_kv + kvh;
-    const int8_t *kp = a.c.k + ph * kPage * HD + (16 * (j >> 2) + (j & 3)) * HD + 16 * g;
-    const int8_t *vp = a.c.v + ph * HD * kPage + j * kPage + 16 * g;
-    v4i kb[4][M], vb[H];
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-#pragma unroll
-      for (int m = 0; m < M; ++m) kb[u][m] = *reinterpret_cast<const v4i *>(kp + 4 * u * HD + 64 * m);
-    float ks = a.c.k_scale[ph * kPageBlocks + g], vs = a.c.v_scale[ph * kPageBlocks + g];
-#pragma unroll
-    for (int h = 0; h < H; ++h) vb[h] = *reinterpret_cast<const v4i *>(vp + h * 16 * kPage);
+  for (int p = p0 + wave, n = 0; p < p1; p += W, ++n) {
+    const bool ok = page_ok(a.c, page);
+    float ksp = ks, vsp = vs;
+    if ((n & (kWave - 1)) == kWave - 1 && p + W < p1) read_entries(p + W);
     const int t0 = p * kPage + 16 * g;   // this lane's first token
-    if (t0 > last_pos) ks = 0.0f, vs = 0.0f;   // nothing of the block is seen: its scales may hold anything
-    int ex = value_exponent(vs);
+    if (t0 > last_pos || !ok) ksp = 0.0f, vsp = 0.0f;   // nothing of the block is seen: its scales may hold anything
+    int ex = value_exponent(vsp);
     exmax = max(exmax, max(ex, lane_xor_int<16>(ex, lane)));
     exmax = max(exmax, lane_xor_int<32>(exmax, lane));
     ex = max(ex, exmax - kExpSpan);
-    const float mant = __builtin_amdgcn_ldexpf(vs, -ex), fex = float(ex), c = qs * ks;
+    const float mant = __builtin_amdgcn_ldexpf(vsp, -ex), fex = float(ex), c = qs * ksp;
     float y[4][4], top = -INFINITY;
-    const bool masked = p * kPage + kPage - 1 > first_pos;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       v4i s[ND];
@@ -294,10 +318,17 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(AttnArgs a) {
 #pragma unroll
         for (int n = 0; n < ND; ++n) d[n] = __int_as_float(s[n][v]);
         y[u][v] = fmaf(join<ND>(d), c, fex);
-        if (masked && t0 + 4 * u + v > limit) y[u][v] = -INFINITY;
-        top = fmaxf(top, y[u][v]);
       }
     }
+    request_keys(p + W, n + 1);
+    __builtin_amdgcn_sched_barrier(0);
+    if (!ok || p * kPage + kPage - 1 > first_pos) {
+      const int lim = ok ? limit - t0 : -1;
+#pragma unroll
+      for (int v = 0; v < 16; ++v) y[v / 4][v % 4] = v > lim ? -INFINITY : y[v / 4][v % 4];
+    }
+#pragma unroll
+    for (int v = 0; v < 16; ++v) top = fmaxf(top, y[v / 4][v % 4]);
     top = fmaxf(top, lane_xor<16>(top, lane));
     top = fmaxf(top, lane_xor<32>(top, lane));
     const float mn = fmaxf(mref, top), base = mn == -INFINITY ? 0.0f : mn;
@@ -321,7 +352,7 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(AttnArgs a) {
       for (int d = 0; d < ND; ++d) pd[d][u] = int(dw[d]);
     }
     // (a block whose scale is not finite gives NaN to the rows that see it)
-    const float unit = vs - vs == 0.0f ? __builtin_amdgcn_ldexpf(1.0f, kSumExp - ex) : __builtin_nanf("");
+    const float unit = vsp - vsp == 0.0f ? __builtin_amdgcn_ldexpf(1.0f, kSumExp - ex) : __builtin_nanf("");
     l = l * root * root;   // (keep alone may underflow where l is large)
     if (sum != 0.0f) l = fmaf(sum, unit, l);
 #pragma unroll
@@ -337,6 +368,8 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(AttnArgs a) {
         o[h][v] = fmaf(o[h][v], keep, join<ND>(d));
       }
     }
+    request_values();
+    __builtin_amdgcn_sched_barrier(0);
   }
   l += lane_xor<16>(l, lane);
   l += lane_xor<32>(l, lane);
@@ -345,9 +378,9 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(AttnArgs a) {
   for (int h = 0; h < H; ++h)
     *reinterpret_cast<float4 *>(&os[wave][j][16 * h + 4 * g]) = make_float4(o[h][0], o[h][1], o[h][2], o[h][3]);
   __syncthreads();
-  // thread (row, 1/16 of the dimensions) merges the waves
-  constexpr int E = HD / 16;
-  const int row = int(threadIdx.x) >> 4, d0 = (int(threadIdx.x) & 15) * E;
+  // thread (row, its share of the dimensions) merges the waves
+  constexpr int TR = W * kWave / 16, E = HD / TR;   // threads of a row, dimensions of a thread
+  const int row = int(threadIdx.x) / TR, d0 = int(threadIdx.x) % TR * E;
   float mx = ms[0][row];
 #pragma unroll
   for (int w = 1; w < W; ++w) mx = fmaxf(mx, ms[w][row]);
@@ -364,7 +397,7 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(AttnArgs a) {
   }
   if (a.splits > 1) {
     const size_t at = ((size_t(blockIdx.x) * a.c.n_kv + kvh) * a.splits + part) * 16 + row;
-    if ((threadIdx.x & 15) == 0) a.part_ml[at] = make_float2(mx, sum);
+    if (int(threadIdx.x) % TR == 0) a.part_ml[at] = make_float2(mx, sum);
     store_floats<E>(a.part_o + at * HD + d0, acc);
     return;
   }
@@ -377,33 +410,51 @@ __global__ __launch_bounds__(256) void kv8_rows_kernel(AttnArgs a) {
   store_floats<E>(out, acc);
 }
 
-// The parts of a split unit: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.
+// The parts of a split unit: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s,
+// eight parts' loads at a time in flight.
 template <class T, int HD, int ROWS>
 __global__ __launch_bounds__(256) void kv8_merge_kernel(AttnArgs a) {
-  constexpr int E = HD / 16;
+  constexpr int E = HD / 16, S = 8;
   const int lane = threadIdx.x & (kWave - 1), kvh = int(blockIdx.y), group = a.c.group;
-  int first = 0;
-  const int seq = unit_sequence(a.c, int(blockIdx.x), group, 1, lane, first, ROWS);
-  if (seq < 0) return;
-  const SeqRows r(a.c, seq);
   const int row = int(blockIdx.z) * 16 + (int(threadIdx.x) >> 4), d0 = (int(threadIdx.x) & 15) * E;
-  const int i = (int(blockIdx.x) - first) * ROWS + row;
-  if (i >= r.n * group) return;
   const size_t at = (size_t(blockIdx.x) * a.c.n_kv + kvh) * a.splits * ROWS + row;
-  float mx = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) mx = fmaxf(mx, a.part_ml[at + size_t(s) * ROWS].x);
-  float sum = 0.0f, acc[E];
+  float mx = -INFINITY, sum = 0.0f, acc[E];
 #pragma unroll
   for (int d = 0; d < E; ++d) acc[d] = 0.0f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float2 ml = a.part_ml[at + size_t(s) * ROWS];
-    const float root = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(0.5f * (ml.x - mx)), f = root * root;
-    sum += ml.y * root * root;
-    float o[E];
-    load_floats<E>(a.part_o + (at + size_t(s) * ROWS) * HD + d0, o);
+  // (units and rows that no sequence has hold anything, and are dropped below)
+  for (int s0 = 0; s0 < a.splits; s0 += S) {
+    float2 ml[S];
+    float o[S][E];
 #pragma unroll
-    for (int d = 0; d < E; ++d) acc[d] = fmaf(f, o[d], acc[d]);
+    for (int s = 0; s < S; ++s) {
+      const size_t n = at + size_t(min(s0 + s, a.splits - 1)) * ROWS;
+      ml[s] = a.part_ml[n];
+      load_floats<E>(a.part_o + n * HD + d0, o[s]);
+    }
+    float now = mx;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      if (s0 + s >= a.splits) ml[s] = make_float2(-INFINITY, 0.0f);
+      now = fmaxf(now, ml[s].x);
+    }
+    // (1: a sum that is NaN stays so)
+    const float r0 = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(0.5f * (mx - now));
+    sum = sum * r0 * r0;
+#pragma unroll
+    for (int d = 0; d < E; ++d) acc[d] *= r0 * r0;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const float root = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(0.5f * (ml[s].x - now)), f = root * root;
+      sum += ml[s].y * root * root;
+#pragma unroll
+      for (int d = 0; d < E; ++d)
+        if (s0 + s < a.splits) acc[d] = fmaf(f, o[s][d], acc[d]);
+    }
+    mx = now;
   }
+  const SeqRows r = unit_rows(a.c, int(blockIdx.x), group, 1, lane, ROWS);
+  const int i = (int(blockIdx.x) - r.first) * ROWS + row;
+  if (r.seq < 0 || i >= r.n * group) return;
   const float inv = inverse_sum(sum);
 #pragma unroll
   for (int d = 0; d < E; ++d) acc[d] *= inv;
@@ -472,10 +523,14 @@ Plan plan(const lmx_kv8_cache *c, const lmx_kv8_batch *b, size_t n_heads, int ty
   Plan p{};
   p.rows = type != LMX_F32 && b->n_rows * group >= 64 * b->n_seqs ? kPromptRows : 16;
   p.units = b->n_rows * group / p.rows + b->n_seqs;
-  // As many parts as bring the grid to about three workgroups per CU (prompts:
-  // two), of four pages at least (one per wave; prompts: 8).
-  const size_t wgs = p.units * c->n_kv_heads, want = p.rows == 16 ? 768 : 512;
-  const size_t s = std::min<size_t>(want / wgs, b->max_pages / (p.rows == 16 ? 4 : 8));
+  // As many parts as fill the device once (three workgroups per CU; two of fp32
+  // with head_dim 128 and of prompts: a workgroup more runs a second round) if
+  // the sequences have equal shares of the rows, of four pages at least, one per
+  // wave (prompts: 8).
+  const size_t each = (b->n_rows + b->n_seqs - 1) / b->n_seqs;
+  const size_t wgs = b->n_seqs * ((each * group + p.rows - 1) / p.rows) * c->n_kv_heads;
+  const size_t room = p.rows > 16 || (type == LMX_F32 && c->head_dim == 128) ? 512 : 768;
+  const size_t s = std::min<size_t>(room / wgs, b->max_pages / (p.rows == 16 ? 4 : 8));
   p.splits = int(std::max<size_t>(1, std::min<size_t>(s, 64)));
   return p;
 }

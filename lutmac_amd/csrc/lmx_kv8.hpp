@@ -25,40 +25,44 @@ struct Kv8Args {
   int n_heads, group;
 };
 
-// The sequence that work unit u belongs to, where sequence s begins at unit
-// floor(offsets[s] * mul / size) + s * per (at least its units of `size` follow,
-// and at most `per` more): -1 past the last.  The wave looks at 64 sequences a
-// load.
-__device__ __forceinline__ int unit_sequence(const Kv8Args &a, int u, int mul, int per, int lane, int &first,
-                                             int size = 16) {
-  int lo = 0, n = a.n_seqs;
-  const auto begin = [&](int s) {
-    return min(max(a.offsets[s], 0), a.n_rows) * mul / size + s * per;   // (below 2^31: at most 2^24 rows, 64 heads)
-  };
-  while (true) {
-    const int step = (n + kWave - 1) / kWave, s = lo + lane * step;
-    const bool in = lane * step < n && begin(min(s, a.n_seqs - 1)) <= u;
-    const int c = __builtin_popcountll(__builtin_amdgcn_ballot_w64(in));
-    if (c == 0) return -1;
-    lo += (c - 1) * step;
-    n = min(step, n - (c - 1) * step);
-    if (step == 1) break;
-  }
-  first = begin(lo);
-  return lo;
-}
-
 // One sequence's rows of the call.
 struct SeqRows {
-  int r0, n;         // first row, count
-  int start, len;    // position of the first row (may be negative), tokens with the rows
-  __device__ __forceinline__ SeqRows(const Kv8Args &a, int s) {
-    r0 = min(max(a.offsets[s], 0), a.n_rows);
-    n = min(max(a.offsets[s + 1], r0), a.n_rows) - r0;
-    len = max(a.lengths[s], 0);
-    start = len - n;
-  }
+  int seq = -1;      // -1: none
+  int first = 0;     // its first work unit
+  int r0 = 0, n = 0;       // first row, count
+  int start = 0, len = 0;  // position of the first row (may be negative), tokens with the rows
 };
+
+// The sequence that work unit u belongs to, where sequence s begins at unit
+// floor(offsets[s] * mul / size) + s * per (at least its units of `size` follow,
+// and at most `per` more).  The wave looks at 64 sequences a load, with what
+// else it needs of them.
+__device__ __forceinline__ SeqRows unit_rows(const Kv8Args &a, int u, int mul, int per, int lane, int size) {
+  SeqRows r;
+  int lo = 0, n = a.n_seqs;
+  while (true) {
+    const int step = (n + kWave - 1) / kWave, s = min(lo + lane * step, a.n_seqs - 1);
+    const int o0 = min(max(a.offsets[s], 0), a.n_rows), o1 = min(a.offsets[s + 1], a.n_rows), len = a.lengths[s];
+    const int begin = o0 * mul / size + s * per;   // (below 2^31: at most 2^24 rows, 64 heads)
+    const int c = __builtin_popcountll(__builtin_amdgcn_ballot_w64(lane * step < n && begin <= u));
+    if (c == 0) return r;
+    if (step == 1) {
+      const auto pick = [c](int v) { return __builtin_amdgcn_readlane(v, c - 1); };
+      r.seq = lo + c - 1;
+      r.first = pick(begin);
+      r.r0 = pick(o0);
+      r.n = max(pick(o1), r.r0) - r.r0;
+      r.len = max(pick(len), 0);
+      r.start = r.len - r.n;
+      return r;
+    }
+    lo += (c - 1) * step;
+    n = min(step, n - (c - 1) * step);
+  }
+}
+
+// First of n pages (up to 2^24) that part `part` of `parts` (up to 64) takes.
+__device__ __forceinline__ int part_begin(int n, int part, int parts) { return int(unsigned(n) * unsigned(part) / unsigned(parts)); }
 
 __device__ __forceinline__ bool page_ok(const Kv8Args &a, int page) { return page >= 0 && page < a.n_pages; }
 

@@ -51,14 +51,11 @@ __global__ __launch_bounds__(kPromptWaves *kWave) __attribute__((amdgpu_waves_pe
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
   const int j = lane & 31, h = lane >> 5;
   const int kvh = int(blockIdx.y), group = a.c.group;
-  int first = 0;
   // the last tiles, which see the most, first
   const int unit = int(gridDim.x) - 1 - int(blockIdx.x);
-  const int seq = unit_sequence(a.c, unit, group, 1, lane, first, kPromptRows);
-  if (seq < 0) return;
-  const SeqRows r(a.c, seq);
-  const int tile0 = (unit - first) * kPromptRows, rows = r.n * group;
-  if (tile0 >= rows) return;
+  const SeqRows r = unit_rows(a.c, unit, group, 1, lane, kPromptRows);
+  const int tile0 = (unit - r.first) * kPromptRows, rows = r.n * group;
+  if (r.seq < 0 || tile0 >= rows) return;
   const int see = min(r.len, a.c.max_pages * kPage) - 1;
   const int i0 = tile0 + 32 * wave, i = min(i0 + j, rows - 1);
   const int first_pos = min(r.start + min(i0, rows - 1) / group, see);              // of the wave's rows
@@ -67,7 +64,7 @@ __global__ __launch_bounds__(kPromptWaves *kWave) __attribute__((amdgpu_waves_pe
   const int limit = min(r.start + i / group, see);
   const int n_pages = tile_last < 0 ? 0 : tile_last / kPage + 1;
   const int part = int(blockIdx.z);
-  const int p0 = int((long long)n_pages * part / a.splits), p1 = int((long long)n_pages * (part + 1) / a.splits);
+  const int p0 = part_begin(n_pages, part, a.splits), p1 = part_begin(n_pages, part + 1, a.splits);
 
   // the row's query: this lane's 8 dimensions of every 16-dimension step
   v8h qf[M];
@@ -120,7 +117,7 @@ __global__ __launch_bounds__(kPromptWaves *kWave) __attribute__((amdgpu_waves_pe
 #pragma unroll
   for (int t = 0; t < 4; ++t) voff[t] = j * 2 * kPage + 16 * ((4 * (t >> 1) + 2 * h + (t & 1)) ^ ((j >> 1) & 7));
 
-  const int *table = a.c.pages + size_t(seq) * a.c.max_pages;
+  const int *table = a.c.pages + size_t(r.seq) * a.c.max_pages;
   v16f acc[D];
 #pragma unroll
   for (int d = 0; d < D; ++d)
