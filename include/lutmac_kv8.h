@@ -72,9 +72,10 @@ typedef struct {
  * A block that receives rows gets the scale max(s, amax / 127, 2^-100), s its
  * present scale if it holds earlier tokens of the sequence, amax the largest
  * magnitude of the rows it receives; the codes of its earlier tokens are
- * rounded anew to a scale that has grown.  Rotation and quotients are computed
- * in 64 bits and rounded once (ties to even), so codes and scales do not
- * depend on the order of anything.  Where a value is not finite the block's
+ * rounded anew to a scale that has grown.  Scales and codes are those of the
+ * rotation and the quotients in 64 bits, rounded once (ties to even), so they
+ * do not depend on the order of anything; rotated queries are rounded once
+ * from 64 bits (fp32) or from fp32 (16-bit types).  Where a value is not finite the block's
  * scale becomes NaN (as does the attention of every row that sees the block)
  * until the block starts anew.  Blocks are read and written by one workgroup
  * each: two sequences of one call must not append to the same page. */

@@ -9,12 +9,18 @@ namespace lmx {
 namespace {
 
 // ---------------------------------------------------------------------------
-// Append.  A unit is one 16-token block of a sequence that receives rows; a
-// workgroup takes one unit of one KV head's keys, one KV head's values or one
-// query head, its 16 groups of 16 lanes a token each.  The block's scale needs
-// every value before any code, so the values wait in registers (in 64 bits: a
-// rotation or quotient next to a border between two codes has to fall on the
-// right side whatever the order of operations).
+// Append.  A unit is one page of a sequence that receives rows; a workgroup
+// takes one unit of one KV head's keys, of one KV head's values, or of kHeads
+// query heads.  Keys and values: a wave takes a 16-token block (4 lanes a
+// token), whose scale needs every value before any code, so the values wait in
+// registers.  Scales and codes are those of 64-bit arithmetic: what lies next to
+// a border between two codes falls on the right side whatever the order of
+// operations.  They are reached in fp32, which is off by far less than kSure
+// keeps a quotient from a border and kNear a value from the largest; the few
+// elements nearer than that, and blocks with a value that is not finite in fp32,
+// are done again in 64 bits (doing all of them so costs a third of the call).
+// Values are turned (4 x 4 bytes at a time, between lanes) into the page's order
+// and leave through LDS, whole rows of 64 tokens.
 struct AppendArgs {
   Kv8Args c;
   const void *k, *v, *q;
@@ -23,45 +29,43 @@ struct AppendArgs {
   const float2 *rope;
   int rope_n;
 };
+constexpr int kHeads = 8;
 
-// The rotated pairs (d0 + i, d0 + i + HD / 2) of a row.
-template <class T, int HD>
-__device__ __forceinline__ void rotated(const T *row, const float2 *rope, int pos, int d0, double (&x)[HD / 32],
-                                        double (&y)[HD / 32]) {
-  constexpr int E = HD / 32;
+// The pairs (d0 + i, d0 + i + HD / 2) of a row, rotated.
+template <int E, class T, int HD, class F>
+__device__ __forceinline__ void rotated(const T *row, const float2 *rope, int pos, int d0, F (&x)[E], F (&y)[E]) {
   float a[E], b[E];
   load_floats<E>(row + d0, a);
   load_floats<E>(row + d0 + HD / 2, b);
+  if (rope) {
+    const float2 *t = rope + size_t(pos) * (HD / 2) + d0;
 #pragma unroll
-  for (int i = 0; i < E; ++i) {
-    x[i] = a[i], y[i] = b[i];
-    if (rope) {
-      const float2 t = rope[size_t(pos) * (HD / 2) + d0 + i];
-      const double c = t.x, s = t.y;
-      x[i] = a[i] * c - b[i] * s;
-      y[i] = a[i] * s + b[i] * c;
+    for (int i = 0; i < E; ++i) {
+      const F c = t[i].x, s = t[i].y;
+      x[i] = F(a[i]) * c - F(b[i]) * s;
+      y[i] = F(a[i]) * s + F(b[i]) * c;
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i) x[i] = a[i], y[i] = b[i];
   }
 }
 
-__device__ __forceinline__ double wave_max(double v) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) v = fmax(v, __shfl_xor(v, d, kWave));
-  return v;
+// Element d (of the pair d, d + HD / 2: h) of a row, rotated, in 64 bits.
+template <class T, int HD>
+__device__ double exact_element(const T *row, const float2 *rope, int pos, int d, int h) {
+  double x[1], y[1];
+  rotated<1, T, HD>(row, rope, pos, d, x, y);
+  return h ? y[0] : x[0];
 }
 
-// The block's scale from its new values' largest magnitude and whether all of
-// them are finite; every thread of the workgroup calls it.
-__device__ __forceinline__ float block_scale(double top, bool finite, const float *scale, bool kept, float &was) {
-  __shared__ double tops[4];
-  was = *scale;   // (before the barrier: thread 0 writes it afterwards)
-  top = wave_max(top);
-  if ((threadIdx.x & (kWave - 1)) == 0) tops[threadIdx.x / kWave] = top;
-  const bool all = __syncthreads_and(finite);
-  top = fmax(fmax(tops[0], tops[1]), fmax(tops[2], tops[3]));
+__device__ __forceinline__ float wave_max(float v, int lane) { return lane_max<32>(v, lane); }
+
+// The block's scale from its new values' largest magnitude.
+__device__ __forceinline__ float block_scale(double top, bool finite, float was, bool kept) {
   float now = fmaxf(float(top / 127.0), 0x1p-100f);
   if (kept) now = was != was ? was : fmaxf(now, was);
-  return all && now < INFINITY ? now : __builtin_nanf("");
+  return finite && now < INFINITY ? now : __builtin_nanf("");
 }
 
 // (a NaN scale leaves the codes 0)
@@ -69,107 +73,206 @@ __device__ __forceinline__ int code_of(double x, double scale, double inverse) {
   return scale == scale ? int(round_quotient(x, scale, inverse)) : 0;
 }
 
+// Codes of four values, a byte each; false: one lies next to a border.
+constexpr float kSure = 0.4999f, kNear = 1.0f - 0x1p-18f;
+__device__ __forceinline__ bool sure_codes(const float *x, float inverse, uint32_t &w) {
+  bool sure = true;
+  w = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float q = x[j] * inverse, n = rintf(q);
+    sure = sure && fabsf(q - n) < kSure;
+    w |= uint32_t(int(n) & 0xFF) << (8 * j);
+  }
+  return sure;
+}
+
+// A block's part in a call: tokens [kept, last) of it are rows of the call,
+// those below kept the sequence's earlier ones.
+struct BlockRows { int kept, last; };
+
 template <class T, int HD>
 __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
-  constexpr int E = HD / 32, VE = HD / 16;
-  __shared__ __attribute__((aligned(16))) uint8_t cod[HD][kBlock];
-  const int lane = threadIdx.x & (kWave - 1), tk = int(threadIdx.x) >> 4, part = int(threadIdx.x) & 15;
-  const SeqRows r = unit_rows(a.c, int(blockIdx.x), 1, 2, lane, kBlock);
+  constexpr int E = HD / 8, VE = HD / 4, LD = kPage + 16;   // pairs and values of a lane; a value row in LDS
+  __shared__ __attribute__((aligned(16))) uint8_t cod[HD][LD];
+  __shared__ float scales[kPageBlocks][2];
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
+  const SeqRows r = unit_rows(a.c, int(blockIdx.x), 1, 2, lane, kPage);
   const int from = max(r.start, 0);   // rows before position 0 have no place
-  const int block = from / kBlock + (int(blockIdx.x) - r.first);
-  if (r.seq < 0 || r.n == 0 || block >= (r.len + kBlock - 1) / kBlock) return;
-  const int pos = block * kBlock + tk;
-  const bool live = pos >= from && pos < r.len && (!a.rope || pos < a.rope_n);
-  const size_t row = size_t(r.r0 + (live ? pos - r.start : from - r.start));
+  const int end = a.rope ? min(r.len, a.rope_n) : r.len;   // (rows past the rotation table are left out)
+  const int pi = from / kPage + (int(blockIdx.x) - r.first), t0 = pi * kPage;
+  if (r.seq < 0 || r.n == 0 || t0 >= end) return;
   const int role = int(blockIdx.y), n_kv = a.c.n_kv;
-  if (role >= 2 * n_kv) {   // a query head
-    if (!live) return;
-    const int head = role - 2 * n_kv;
-    double x[E], y[E];
-    rotated<T, HD>(static_cast<const T *>(a.q) + row * a.q_stride + size_t(head) * HD, a.rope, pos, part * E, x, y);
-    T *out = static_cast<T *>(a.q_out) + row * a.q_out_stride + size_t(head) * HD + part * E;
-    float f[E], g[E];
+  if (role >= 2 * n_kv) {   // query heads: 8 lanes a row and head
+    constexpr int QE = 8, QL = HD / 2 / QE, SLOTS = 256 / QL;
+    const int h0 = (role - 2 * n_kv) * kHeads, heads = min(kHeads, a.c.n_heads - h0);
+    const int first = max(from, t0), tokens = min(end, t0 + kPage) - first;
+    int tp = 1;   // tokens side by side, a power of two
+    while (tp < tokens && tp < SLOTS) tp *= 2;
+    const int slot = int(threadIdx.x) / QL, d0 = int(threadIdx.x) % QL * QE;
+    for (int t = slot % tp; t < tokens; t += tp) {
+      const int pos = first + t;
+      const size_t row = size_t(r.r0 + (pos - r.start));
+      const T *q = static_cast<const T *>(a.q) + row * a.q_stride + size_t(h0) * HD;
+      T *out = static_cast<T *>(a.q_out) + row * a.q_out_stride + size_t(h0) * HD;
+      for (int h = slot / tp; h < heads; h += SLOTS / tp) {
+        float f[QE], g[QE];
+        if constexpr (sizeof(T) == 4) {
+          double x[QE], y[QE];
+          rotated<QE, T, HD>(q + h * HD, a.rope, pos, d0, x, y);
 #pragma unroll
-    for (int i = 0; i < E; ++i) f[i] = narrow<T>(x[i]), g[i] = narrow<T>(y[i]);
-    store_floats<E>(out, f);
-    store_floats<E>(out + HD / 2, g);
+          for (int i = 0; i < QE; ++i) f[i] = float(x[i]), g[i] = float(y[i]);
+        } else {   // (rounded to 16 bits: fp32 leaves at most 2^-22 of the pair's larger)
+          rotated<QE, T, HD>(q + h * HD, a.rope, pos, d0, f, g);
+        }
+        store_floats<QE>(out + h * HD + d0, f);
+        store_floats<QE>(out + h * HD + d0 + HD / 2, g);
+      }
+    }
     return;
   }
-  const int pi = block / kPageBlocks, sub = block % kPageBlocks;
   if (pi >= a.c.max_pages) return;
   const int page = a.c.pages[size_t(r.seq) * a.c.max_pages + pi];
   if (!page_ok(a.c, page)) return;
-  const int kept = max(from - block * kBlock, 0);   // earlier tokens of the block
-  const int last = min(r.len, a.rope ? a.rope_n : r.len) - block * kBlock;   // tokens of the block with the rows
-  if (last <= kept) return;
-  double top = 0.0;
-  bool finite = true;
-  float was;
+  const int tk = lane >> 2, part = lane & 3;
+  const auto block_rows = [&](int b) {
+    return BlockRows{min(max(from - t0 - b * kBlock, 0), kBlock), min(max(end - t0 - b * kBlock, 0), kBlock)};
+  };
+  const BlockRows br = block_rows(wave);
+  const bool some = br.last > br.kept, live = tk >= br.kept && tk < br.last;
+  const int pos = t0 + wave * kBlock + tk;
+  const size_t row = size_t(r.r0 + ((live ? pos : from) - r.start));
   if (role < n_kv) {
+    if (!some) return;
     const size_t ph = size_t(page) * n_kv + role;
-    double x[E], y[E];
+    float *scale = a.c.k_scale + ph * kPageBlocks + wave;
+    const float was = *scale;
+    const T *src = static_cast<const T *>(a.k) + row * a.k_stride + size_t(role) * HD;
+    float x[2][E], most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) x[0][i] = x[1][i] = 0.0f;
+    if (live) rotated<E, T, HD>(src, a.rope, pos, part * E, x[0], x[1]);
+    bool in_range = true;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      most = fmaxf(most, fmaxf(fabsf(x[0][i]), fabsf(x[1][i])));
+      in_range = in_range && fabsf(x[0][i]) < INFINITY && fabsf(x[1][i]) < INFINITY;
+    }
+    most = wave_max(most, lane);
+    const bool fast = __builtin_amdgcn_ballot_w64(!in_range) == 0;
+    // the largest in 64 bits: of the elements that can be it (all, !fast)
+    double top = 0.0;
+    bool finite = true;
     if (live) {
-      rotated<T, HD>(static_cast<const T *>(a.k) + row * a.k_stride + size_t(role) * HD, a.rope, pos, part * E, x, y);
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        top = fmax(top, fmax(fabs(x[i]), fabs(y[i])));
-        finite = finite && fabs(x[i]) < INFINITY && fabs(y[i]) < INFINITY;
+        if (!fast || fmaxf(fabsf(x[0][i]), fabsf(x[1][i])) >= most * kNear) {
+          double u[1], v[1];
+          rotated<1, T, HD>(src, a.rope, pos, part * E + i, u, v);
+          top = fmax(top, fmax(fabs(u[0]), fabs(v[0])));
+          finite = finite && fabs(u[0]) < INFINITY && fabs(v[0]) < INFINITY;
+        }
       }
     }
-    float *scale = a.c.k_scale + ph * kPageBlocks + sub;
-    const float now = block_scale(top, finite, scale, kept > 0, was);
+#pragma unroll
+    for (int d = 32; d; d >>= 1) top = fmax(top, __shfl_xor(top, d, kWave));
+    const float now = block_scale(top, __builtin_amdgcn_ballot_w64(!finite) == 0, was, br.kept > 0);
     const double inv = 1.0 / double(now);
-    int8_t *dst = a.c.k + (ph * kPage + sub * kBlock + tk) * HD + part * E;
-    if (live || (tk < kept && now == now && now != was)) {
+    int8_t *dst = a.c.k + (ph * kPage + wave * kBlock + tk) * HD + part * E;
+    typedef uint32_t words __attribute__((ext_vector_type(E / 4)));
+    if (live) {
+      const float finv = float(inv);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        int8_t *p = dst + h * (HD / 2);
-        typedef int8_t bytes __attribute__((ext_vector_type(E)));
-        bytes c = *reinterpret_cast<bytes *>(p);
+        words c;
 #pragma unroll
-        for (int i = 0; i < E; ++i)
-          c[i] = int8_t(code_of(live ? (h ? y[i] : x[i]) : double(int(c[i])) * double(was), now, inv));
-        *reinterpret_cast<bytes *>(p) = c;
+        for (int i = 0; i < E / 4; ++i) {
+          uint32_t w;
+          if (!sure_codes(x[h] + 4 * i, finv, w) || !fast) {
+            w = 0;
+            for (int j = 0; j < 4; ++j)
+              w |= uint32_t(code_of(exact_element<T, HD>(src, a.rope, pos, part * E + 4 * i + j, h), now, inv) & 0xFF) << (8 * j);
+          }
+          c[i] = now == now ? w : 0u;
+        }
+        *reinterpret_cast<words *>(dst + h * (HD / 2)) = c;
+      }
+    } else if (tk < br.kept && now == now && now != was) {
+      typedef int8_t bytes __attribute__((ext_vector_type(E)));
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        bytes c = *reinterpret_cast<const bytes *>(dst + h * (HD / 2));
+#pragma unroll
+        for (int i = 0; i < E; ++i) c[i] = int8_t(code_of(double(int(c[i])) * double(was), now, inv));
+        *reinterpret_cast<bytes *>(dst + h * (HD / 2)) = c;
       }
     }
-    if (threadIdx.x == 0) *scale = now;
+    if (lane == 0) *scale = now;
     return;
   }
-  const int head = role - n_kv;
-  const size_t ph = size_t(page) * n_kv + head;
-  float x[VE];
-  if (live) {
-    load_floats<VE>(static_cast<const T *>(a.v) + row * a.v_stride + size_t(head) * HD + part * VE, x);
+  const size_t ph = size_t(page) * n_kv + (role - n_kv);
+  if (some) {
+    float *scale = a.c.v_scale + ph * kPageBlocks + wave;
+    const float was = *scale;
+    float x[VE], most = 0.0f;
+    bool finite = true;
+#pragma unroll
+    for (int i = 0; i < VE; ++i) x[i] = 0.0f;
+    if (live) load_floats<VE>(static_cast<const T *>(a.v) + row * a.v_stride + size_t(role - n_kv) * HD + part * VE, x);
 #pragma unroll
     for (int i = 0; i < VE; ++i) {
-      top = fmax(top, fabs(double(x[i])));
+      most = fmaxf(most, fabsf(x[i]));
       finite = finite && fabsf(x[i]) < INFINITY;
     }
-  }
-  float *scale = a.c.v_scale + ph * kPageBlocks + sub;
-  const float now = block_scale(top, finite, scale, kept > 0, was);
-  const double inv = 1.0 / double(now);
-  if (live) {
+    const float now = block_scale(wave_max(most, lane), __builtin_amdgcn_ballot_w64(!finite) == 0, was, br.kept > 0);
+    const double inv = 1.0 / double(now);
+    const float finv = float(inv);
+    // four dimensions of four tokens at a time: lane (token 4 n + q, part) ends
+    // with dimension 4 i + q of its part, the tokens 4 n .. 4 n + 3
+    const int q = tk & 3;
 #pragma unroll
-    for (int i = 0; i < VE; ++i) cod[part * VE + i][tk] = uint8_t(code_of(x[i], now, inv));
+    for (int i = 0; i < VE / 4; ++i) {
+      uint32_t w;
+      if (!sure_codes(x + 4 * i, finv, w)) {
+        w = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w |= uint32_t(code_of(x[4 * i + j], now, inv) & 0xFF) << (8 * j);
+      }
+      w = now == now ? w : 0u;
+      // the words of the lanes 4, 8 and 12 places on (row of 16 lanes = 4 tokens x 4 parts)
+      const uint32_t w1 = dpp_u32<0x12C>(w), w2 = dpp_u32<0x128>(w), w3 = dpp_u32<0x124>(w);
+      // byte q of each, tokens q, q + 1, q + 2, q + 3 (mod 4), turned to begin with token 0
+      const uint32_t b0 = w >> (8 * q) & 0xFF, b1 = w1 >> (8 * q) & 0xFF, b2 = w2 >> (8 * q) & 0xFF, b3 = w3 >> (8 * q) & 0xFF;
+      const uint32_t turned = b0 | b1 << 8 | b2 << 16 | b3 << 24;
+      const uint32_t out = q ? turned << (8 * q) | turned >> (32 - 8 * q) : turned;
+      *reinterpret_cast<uint32_t *>(&cod[part * VE + 4 * i + q][wave * kBlock + 4 * (tk >> 2)]) = out;
+    }
+    if (lane == 0) {
+      scales[wave][0] = was, scales[wave][1] = now;
+      *scale = now;
+    }
   }
   __syncthreads();
-  if (threadIdx.x < HD) {   // one dimension's 16 tokens: earlier ones rescaled, later ones left
-    int8_t *p = a.c.v + (ph * HD + threadIdx.x) * kPage + sub * kBlock;
+  for (int n = int(threadIdx.x); n < HD * kPageBlocks; n += 256) {   // a dimension's 16 tokens of a block
+    const int d = n / kPageBlocks, b = n % kPageBlocks;
+    const BlockRows w = block_rows(b);
+    if (w.last <= w.kept) continue;
+    int8_t *p = a.c.v + (ph * HD + d) * kPage + b * kBlock;
     typedef int8_t bytes __attribute__((ext_vector_type(16)));
-    bytes c = *reinterpret_cast<const bytes *>(cod[threadIdx.x]);
-    if (kept > 0 || last < kBlock) {
+    bytes c = *reinterpret_cast<const bytes *>(&cod[d][b * kBlock]);
+    if (w.kept > 0 || w.last < kBlock) {   // earlier tokens are rescaled, later places left
       const bytes old = *reinterpret_cast<const bytes *>(p);
+      const float was = scales[b][0], now = scales[b][1];
       const bool rescale = now == now && now != was;
+      const double inv = 1.0 / double(now);
 #pragma unroll
       for (int t = 0; t < kBlock; ++t) {
-        if (t < kept) c[t] = rescale ? int8_t(code_of(double(int(old[t])) * double(was), now, inv)) : old[t];
-        else if (t >= last) c[t] = old[t];
+        if (t < w.kept) c[t] = rescale ? int8_t(code_of(double(int(old[t])) * double(was), now, inv)) : old[t];
+        else if (t >= w.last) c[t] = old[t];
       }
     }
     *reinterpret_cast<bytes *>(p) = c;
   }
-  if (threadIdx.x == 0) *scale = now;
 }
 
 // ---------------------------------------------------------------------------
@@ -594,8 +697,9 @@ int lmx_kv8_append(const lmx_kv8_cache *cache, const lmx_kv8_batch *batch, int t
   a.k_stride = k_stride, a.v_stride = v_stride, a.q_stride = q_stride, a.q_out_stride = q_out_stride;
   a.rope = reinterpret_cast<const float2 *>(rope);
   a.rope_n = rope ? int(rope_positions) : 0;
-  // a sequence of n rows touches at most n / 16 + 2 blocks, rounded down
-  const dim3 grid(unsigned(rows / kBlock + 2 * batch->n_seqs), unsigned(2 * cache->n_kv_heads + (q ? n_heads : 0)));
+  // a sequence of n rows touches at most n / 64 + 2 pages, rounded down
+  const dim3 grid(unsigned(rows / kPage + 2 * batch->n_seqs),
+                  unsigned(2 * cache->n_kv_heads + (q ? (n_heads + kHeads - 1) / kHeads : 0)));
   hipStream_t st = static_cast<hipStream_t>(stream);
   switch (type) {
   case LMX_F32: return launch_append<float>(a, cache->head_dim, grid, st);

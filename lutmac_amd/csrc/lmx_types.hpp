@@ -41,21 +41,6 @@ __device__ __forceinline__ void store_floats(T *p, const float (&x)[N]) {
   }
 }
 
-// A 64-bit value as a float that rounds to a 16-bit type as the value itself
-// would (rounded to odd: nearest floats alone can land on a border between two
-// 16-bit values); fp32: the nearest.
-template <class T>
-__device__ __forceinline__ float narrow(double x) {
-  const float f = float(x);
-  if constexpr (sizeof(T) == 2) {
-    uint32_t u = __float_as_uint(f);
-    const double back = f;
-    if (back != x && (u & 1) == 0 && fabs(x) < INFINITY) u += fabs(x) > fabs(back) ? 1 : -1;
-    return __uint_as_float(u);
-  }
-  return f;
-}
-
 // a / d rounded to the nearest whole number, ties to even, for d > 0 and a
 // quotient of a few bits, with r near 1 / d: the remainder of the first guess
 // says whether it is the nearest.

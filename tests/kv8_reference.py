@@ -9,14 +9,19 @@ PAGE, BLOCK = 64, 16
 HALF_STEP = {"float32": 2.0 ** -24, "float16": 2.0 ** -11, "bfloat16": 2.0 ** -8}
 
 
-def rounded(x, dtype):
-    """float64 values rounded once, to the nearest (ties to even) of the type's, as float64."""
-    if dtype == "float16":
-        return x.astype(np.float16).astype(np.float64)
+def check_rotated(got, want, q, dtype):
+    """got (float64) against the rotation `want` in 64 bits of q: rounded once (fp32),
+    or to 16 bits after fp32's products and sum, off by at most 2^-22 of the pair's
+    larger magnitude."""
     if dtype == "float32":
-        return x.astype(np.float32).astype(np.float64)
-    m, e = np.frexp(x)   # normal bfloat16 values: 8 bits
-    return np.ldexp(np.round(m * 256), e - 8)
+        np.testing.assert_array_equal(got, want.astype(np.float32).astype(np.float64))
+        return
+    h = q.shape[-1] // 2
+    pair = np.maximum(np.abs(q[..., :h]), np.abs(q[..., h:]))
+    most = np.abs(want) * HALF_STEP[dtype] * (1 + 2.0 ** -10) + 2.0 ** -22 * np.concatenate([pair, pair], -1)
+    most += 2.0 ** -24 if dtype == "float16" else 0.0
+    ok = np.isfinite(want)
+    assert (np.abs(got - want)[ok] <= most[ok]).all() and not np.isfinite(got[~ok]).any()
 
 
 def rotate(x, rope, pos):

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import lutmac_amd as L
-from kv8_reference import PAGE, Cache, rounded
+from kv8_reference import PAGE, Cache, check_rotated
 from lutmac_amd.kv8 import KvCache8, rope_table
 
 pytestmark = pytest.mark.gpu
@@ -65,8 +65,9 @@ class Setup:
         out = torch.full((self.q.shape[0], self.heads, self.hd), 7.0, dtype=TYPES[self.dtype], device="cuda")
         self.cache.append(self.k, self.v, *self.where, rope=self.rope, q=self.q, q_out=out)
         self.same_cache(ref)
-        placed = ~np.isnan(want[:, 0, 0])
-        np.testing.assert_array_equal(f64(out), np.where(placed[:, None, None], rounded(want, self.dtype), 7.0))
+        placed = ~np.isnan(want).all((1, 2))
+        check_rotated(f64(out)[placed], want[placed], f64(self.q)[placed], self.dtype)
+        assert (f64(out)[~placed] == 7.0).all()
         return ref, out
 
     def check_attend(self, ref=None, q=None, scale=None, **kw):
@@ -138,10 +139,11 @@ def test_steps_together(cuda, dtype):
         # growing values, so that scales grow within their blocks
         s.qkv = ((1 + 0.1 * step) * torch.randn(int(s.offsets[-1]), 8, 64, generator=g)).to(TYPES[dtype]).cuda()
         s.q, s.k, s.v = s.qkv.split([4, 2, 2], 1)
-        want = ref.append(f64(s.k), f64(s.v), f64(s.q), s.offsets, s.lengths, s.pages, s.rope.cpu().numpy())
+        before = f64(s.q)
+        want = ref.append(f64(s.k), f64(s.v), before, s.offsets, s.lengths, s.pages, s.rope.cpu().numpy())
         q = s.cache.append(s.k, s.v, *s.where, rope=s.rope, q=s.q, q_out=s.q)
         assert q.data_ptr() == s.q.data_ptr()
-        np.testing.assert_array_equal(f64(q), rounded(want, dtype))
+        check_rotated(f64(q), want, before, dtype)
         s.same_cache(ref)
         s.check_attend(ref, q)
 
@@ -307,7 +309,7 @@ def test_graph_follows_lengths(cuda):
         want = ref.append(f64(s.k), f64(s.v), f64(s.q), s.offsets, s.lengths, s.pages, s.rope.cpu().numpy())
         s.same_cache(ref)
         n = int(s.offsets[-1])
-        np.testing.assert_array_equal(f64(q_out[:n]), rounded(want[:n], "float32"))
+        check_rotated(f64(q_out[:n]), want[:n], f64(s.q[:n]), "float32")
         assert torch.equal(out[:n], s.cache.attend(q_out, *s.where)[:n])
         s.check_attend(ref, q_out)
         s.lengths += 1
