@@ -20,7 +20,8 @@
  *   down     hidden x ffn
  *   head     vocab x hidden, also the embedding table (tied, model.cpp:667-689)
  * Numerics are fp32 throughout; KV cache fp32 [layer][pos][kv_head][hd]
- * (types.hpp:599-627 keeps the same per-layer layout).
+ * (types.hpp:599-627 keeps the same per-layer layout), or 8-bit pages
+ * (lutmac_kv8.h) on request.
  */
 #ifndef LUTMAC_DECODE_H
 #define LUTMAC_DECODE_H
@@ -72,6 +73,19 @@ int lmx_decoder_create(const lmx_decoder_config *cfg, lmx_decoder **out);
  * row-major and the logits of lmx_decoder_step [batch][vocab].  batch 1 is
  * lmx_decoder_create. */
 int lmx_decoder_create_batched(const lmx_decoder_config *cfg, size_t batch, lmx_decoder **out);
+/* A decoder of 1..64 sequences with the format of its KV cache chosen (the
+ * other two keep fp32).  LMX_KV_INT8: pages of lmx_kv8_append, a quarter of the
+ * memory; keys and values carry the rounding to 8 bits of their block of 16
+ * positions, and a block's codes are rounded anew when its scale grows, so
+ * logits depend a little on whether a prompt was read in passes or step by step
+ * (no counterpart in the reference, whose cache is fp32).  It pays where the
+ * cache is what a step reads: at the 1B width a layer's step takes 36 us against
+ * 29 with fp32 at 2048 positions of one sequence, 43 against 42 at 16384, 63
+ * against 74 at 4096 positions of 8 sequences and 79 against 107 at 2048 of 32;
+ * a prompt of 16000 tokens takes half the time. */
+#define LMX_KV_F32 0
+#define LMX_KV_INT8 1
+int lmx_decoder_create_kv(const lmx_decoder_config *cfg, size_t batch, int kv_format, lmx_decoder **out);
 int lmx_decoder_destroy(lmx_decoder *d);
 /* Layer weights (borrowed handles) and norm weights (host, copied);
  * qkv_bias (host, n_heads*hd + 2*n_kv*hd floats) may be NULL. */

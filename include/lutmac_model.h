@@ -41,6 +41,8 @@ typedef struct lmx_model lmx_model;
  * 2048, the capacity the reference's load_model gives its cache: it never
  * reads the file's max_position_embeddings back, types.hpp:558). */
 int lmx_model_load(const char *path, size_t max_seq, lmx_model **out);
+/* The same with the format of the KV cache chosen (lmx_decoder_create_kv). */
+int lmx_model_load_kv(const char *path, size_t max_seq, int kv_format, lmx_model **out);
 int lmx_model_destroy(lmx_model *m);
 /* The decoder config derived from the file, and the decoder itself (owned
  * by the model). */

@@ -40,13 +40,13 @@ EXPORTS = [
     "lmx_host_precompute_luts", "lmx_host_precompute_lut", "lmx_host_extract_indices", "lmx_host_forget",
     "lmx_host_cache_clear",
     # include/lutmac_decode.h
-    "lmx_decoder_create", "lmx_decoder_create_batched", "lmx_decoder_destroy", "lmx_decoder_set_layer", "lmx_decoder_set_head",
+    "lmx_decoder_create", "lmx_decoder_create_batched", "lmx_decoder_create_kv", "lmx_decoder_destroy", "lmx_decoder_set_layer", "lmx_decoder_set_head",
     "lmx_decoder_reset", "lmx_decoder_step", "lmx_decoder_tokens", "lmx_decoder_generate",
     "lmx_decoder_set_repetition_penalty",
     # include/lutmac_synth.h
     "lmx_quantize_int4", "lmx_quantize", "lmx_synth_int4_normal", "lmx_synth_normal",
     # include/lutmac_model.h
-    "lmx_model_load", "lmx_model_destroy", "lmx_model_config", "lmx_model_decoder", "lmx_model_weight_format",
+    "lmx_model_load", "lmx_model_load_kv", "lmx_model_destroy", "lmx_model_config", "lmx_model_decoder", "lmx_model_weight_format",
     # include/lutmac_kv8.h
     "lmx_kv8_append", "lmx_kv8_attention_workspace", "lmx_kv8_attention",
 ]
@@ -129,12 +129,14 @@ _SIGS = {
     "lmx_synth_int4_normal": ([ctypes.c_uint64, ctypes.c_uint64, _sz, _sz, ctypes.c_float, _sz, _p, _p], _i),
     "lmx_synth_normal": ([ctypes.c_uint64, ctypes.c_uint64, _sz, _sz, ctypes.c_float, _p], _i),
     "lmx_model_load": ([ctypes.c_char_p, _sz, ctypes.POINTER(_p)], _i),
+    "lmx_model_load_kv": ([ctypes.c_char_p, _sz, _i, ctypes.POINTER(_p)], _i),
     "lmx_model_destroy": ([_p], _i),
     "lmx_model_config": ([_p, ctypes.POINTER(DecoderConfigC)], _i),
     "lmx_model_decoder": ([_p], _p),
     "lmx_model_weight_format": ([_p, _i, _i, ctypes.POINTER(_i)], _i),
     "lmx_decoder_create": ([ctypes.POINTER(DecoderConfigC), ctypes.POINTER(_p)], _i),
     "lmx_decoder_create_batched": ([ctypes.POINTER(DecoderConfigC), _sz, ctypes.POINTER(_p)], _i),
+    "lmx_decoder_create_kv": ([ctypes.POINTER(DecoderConfigC), _sz, _i, ctypes.POINTER(_p)], _i),
     "lmx_decoder_destroy": ([_p], _i),
     "lmx_decoder_set_layer": ([_p, _sz, _p, _p, _p, _p, _p, _p, _p], _i),
     "lmx_decoder_set_head": ([_p, _p, _p, _p], _i),

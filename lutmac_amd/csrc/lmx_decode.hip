@@ -29,7 +29,9 @@
 // argmax_rows_kernel; their linears run on the digit kernels, as do those of
 // the passes that take many positions of a prompt at once, lmx_prefill.hpp.)
 // The position and the token sequence live in device memory, so the same
-// captured step replays for every position.
+// captured step replays for every position.  With an 8-bit KV cache the entry
+// points of lutmac_kv8.h take attn_kernel's place: the append (which rotates q
+// and k) and the attention over its pages.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -44,6 +46,7 @@
 #include "lmx_lanes.hpp"
 #include "lmx_prefill.hpp"
 #include "lutmac_decode.h"
+#include "lutmac_kv8.h"
 
 namespace lmx {
 namespace {
@@ -733,6 +736,18 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void a
                        __HIP_MEMORY_SCOPE_AGENT);
 }
 
+// 8-bit cache: the rows of a call, T of every sequence from position *pos, or
+// from p0 where pos is null.
+__global__ __launch_bounds__(64) void kv8_batch_kernel(const int *__restrict__ pos, int p0, int T, int batch,
+                                                       int *__restrict__ offsets, int *__restrict__ lengths) {
+  const int b = threadIdx.x;
+  if (b < batch) {
+    offsets[b] = b * T;
+    lengths[b] = (pos ? *pos : p0) + T;
+  }
+  if (b == 0) offsets[batch] = batch * T;
+}
+
 size_t attn_chunks(const lmx_decoder_config &c) { return (c.max_seq + kAttnChunk - 1) / kAttnChunk; }
 
 }  // namespace
@@ -762,6 +777,23 @@ struct lmx_decoder {
   unsigned long long *argmax_slots = nullptr;   // batch > 1: [batch][kArgmaxParts] keys
   unsigned *argmax_seq_tickets = nullptr;       // batch > 1: [batch] tickets, one 128-byte line each
   size_t kv_seq = 0;                         // floats of one sequence's K (or V) cache, all layers
+  // 8-bit cache (kv_format LMX_KV_INT8): each layer's pages one after another,
+  // sequence b's being b * kv8_pages .. of every layer's
+  int kv_format = LMX_KV_F32;
+  size_t kv8_pages = 0;                      // pages of a sequence
+  int8_t *k8 = nullptr, *v8 = nullptr;
+  float *k8_scale = nullptr, *v8_scale = nullptr;
+  int *kv8_table = nullptr, *kv8_offsets = nullptr, *kv8_lengths = nullptr;
+  void *kv8_work = nullptr;                  // workspace of a step's attention
+  size_t kv8_work_bytes = 0;
+  float *p_kv8_work = nullptr;               // and of a prompt pass's, with the pass's buffers
+  size_t p_kv8_work_bytes = 0;
+  lmx_kv8_cache kv8_layer(size_t l) const {
+    const size_t pages = batch * kv8_pages, heads = l * pages * cfg.n_kv_heads, codes = heads * LMX_KV8_PAGE * cfg.head_dim;
+    const size_t scales = heads * (LMX_KV8_PAGE / LMX_KV8_BLOCK);
+    return {k8 + codes, v8 + codes, k8_scale + scales, v8_scale + scales, pages, cfg.n_kv_heads, cfg.head_dim};
+  }
+  lmx_kv8_batch kv8_rows(size_t T) const { return {kv8_offsets, kv8_lengths, kv8_table, batch, kv8_pages, batch * T}; }
   unsigned long long *amax = nullptr;    // per-wave argmax keys of the head GEMV
   size_t amax_slots = 0;
   int *tokens = nullptr, *pos = nullptr;
@@ -914,8 +946,33 @@ int finish_embed(const lmx_decoder *d, hipStream_t st) {
   return launch_err("finish_embed");
 }
 
+// The rows of a step (T = 1, pos) or a prompt pass (T positions from p0) for
+// kv8_layer_rows; nothing to do with an fp32 cache.
+int kv8_batch(lmx_decoder *d, const int *pos, int p0, int T, hipStream_t st) {
+  if (d->kv_format != LMX_KV_INT8) return LMX_OK;
+  kv8_batch_kernel<<<dim3(1), dim3(64), 0, st>>>(pos, p0, T, int(d->batch), d->kv8_offsets, d->kv8_lengths);
+  return launch_err("kv8 batch");
+}
+
+// Append and (out not null) attention of T rows of every sequence, their q|k|v
+// in qkv (q is rotated in place).
+int kv8_layer_rows(lmx_decoder *d, size_t layer, float *qkv, size_t T, float *out, void *work, size_t work_bytes,
+                   hipStream_t st) {
+  const lmx_decoder_config &c = d->cfg;
+  const lmx_kv8_cache cache = d->kv8_layer(layer);
+  const lmx_kv8_batch rows = d->kv8_rows(T);
+  const size_t q = c.n_heads * c.head_dim, kv = c.n_kv_heads * c.head_dim, stride = q + 2 * kv;
+  const int r = lmx_kv8_append(&cache, &rows, LMX_F32, qkv + q, stride, qkv + q + kv, stride, out ? qkv : nullptr, stride, qkv,
+                               stride, c.n_heads, reinterpret_cast<const float *>(d->rope), c.max_seq, st);
+  if (r || !out) return r;
+  return lmx_kv8_attention(&cache, &rows, LMX_F32, qkv, stride, c.n_heads, 1.0f / std::sqrt(float(c.head_dim)), out, q, work,
+                           work_bytes, st);
+}
+
 int attention(lmx_decoder *d, size_t layer, hipStream_t st) {
   const lmx_decoder_config &c = d->cfg;
+  if (d->kv_format == LMX_KV_INT8)
+    return kv8_layer_rows(d, layer, d->qkv, 1, d->attn_out, d->kv8_work, d->kv8_work_bytes, st);
   const int group = int(c.n_heads / c.n_kv_heads);
   const int nch = int(attn_chunks(c));
   const int spec = min(nch, d->spec_chunks);
@@ -1015,14 +1072,19 @@ int prefill_pass(lmx_decoder *d, int p0, int T, hipStream_t st) {
   const size_t per_layer = attn_chunks(c) * kAttnChunk * c.n_kv_heads * c.head_dim;
   const float scale = 1.0f / std::sqrt(float(c.head_dim));
   int r = embed(d->embed, d->tokens, nullptr, d->p_hidden, d->batch, int(c.max_seq + 1), T, p0, st);
-  if (r) return r;
+  if (r || (r = kv8_batch(d, nullptr, p0, T, st))) return r;
+  const bool kv8 = d->kv_format == LMX_KV_INT8;
   const dim3 rope_grid(unsigned(((c.n_heads + 2 * c.n_kv_heads) * (c.head_dim / 2) + 255) / 256), unsigned(M));
   const dim3 attn_grid(unsigned((T * group + 15) / 16), unsigned(c.n_kv_heads), unsigned(d->batch));
   for (size_t l = 0; l < c.n_layers; ++l) {
     const lmx_decoder::Layer &L = d->layers[l];
     float *kc = d->kcache + l * per_layer, *vc = d->vcache + l * per_layer;
     if ((r = digit_rows(d, L.qkv, d->p_hidden, d->p_qkv, M, L.qkv_bias, nullptr, L.in_norm, kEpiStore, st))) return r;
-    if (hd == 64)
+    if (kv8) {
+      if ((r = kv8_layer_rows(d, l, d->p_qkv, size_t(T), l + 1 == c.n_layers ? nullptr : d->p_attn, d->p_kv8_work,
+                              d->p_kv8_work_bytes, st)))
+        return r;
+    } else if (hd == 64)
       prefill_rope_kernel<64><<<rope_grid, dim3(256), 0, st>>>(d->p_qkv, d->rope, kc, vc, int(c.n_heads),
                                                               int(c.n_kv_heads), T, p0, d->kv_seq);
     else
@@ -1030,7 +1092,8 @@ int prefill_pass(lmx_decoder *d, int p0, int T, hipStream_t st) {
                                                                int(c.n_kv_heads), T, p0, d->kv_seq);
     if ((r = launch_err("prefill_rope"))) return r;
     if (l + 1 == c.n_layers) break;
-    if (hd == 64)
+    if (kv8) {
+    } else if (hd == 64)
       prefill_attention_kernel<64><<<attn_grid, dim3(256), 0, st>>>(d->p_qkv, kc, vc, int(c.n_heads),
                                                                    int(c.n_kv_heads), T, p0, scale, d->kv_seq, d->p_attn);
     else
@@ -1061,12 +1124,24 @@ bool prefill_buffers(lmx_decoder *d, hipStream_t st) {
   // scratch holds 256 vectors of a small matrix: two launches, 25 us
   // against 19 for the 3072 x 2048 linear of 383 rows)
   const size_t dig = kDigitTicketBytes + digit_bytes(Kp, rows) + kDigitPartials;
+  // (a shorter pass may split its rows' pages into more parts)
+  size_t work = 0;
+  if (d->kv_format == LMX_KV_INT8) {
+    const lmx_kv8_cache cache = d->kv8_layer(0);
+    for (size_t T = 1; T <= rows / d->batch; ++T) {
+      const lmx_kv8_batch b = d->kv8_rows(T);
+      size_t n = 0;
+      if (lmx_kv8_attention_workspace(&cache, &b, LMX_F32, c.n_heads, &n)) return false;
+      work = std::max(work, n);
+    }
+  }
   struct { float **p; size_t floats; } want[] = {
       {&d->p_qkv, rows * (c.n_heads + 2 * c.n_kv_heads) * c.head_dim},
       {&d->p_attn, rows * c.n_heads * c.head_dim},
       {&d->p_gate_up, pairs ? 0 : rows * 2 * c.ffn},
       {&d->p_act, rows * c.ffn},
       {&d->p_digits, (dig + 3) / 4},
+      {&d->p_kv8_work, work / 4},
       {&d->p_hidden, rows * c.hidden}};
   const char *lim = std::getenv("LMX_PROMPT_BYTES");
   size_t left = lim ? size_t(std::strtoull(lim, nullptr, 10)) : SIZE_MAX;
@@ -1090,6 +1165,7 @@ bool prefill_buffers(lmx_decoder *d, hipStream_t st) {
     *want[i].p = static_cast<float *>(got[i]);
   }
   d->p_digit_bytes = dig;
+  d->p_kv8_work_bytes = work;
   return true;
 }
 
@@ -1114,7 +1190,7 @@ int step_batched(lmx_decoder *d, float *logits_out, hipStream_t st) {
   const size_t B = d->batch;
   float *lg = logits_out ? logits_out : d->logits;
   int r = embed(d->embed, d->tokens, d->pos, d->hidden, B, int(c.max_seq + 1), 1, 0, st);
-  if (r) return r;
+  if (r || (r = kv8_batch(d, d->pos, 0, 1, st))) return r;
   for (size_t l = 0; l < c.n_layers; ++l) {
     const lmx_decoder::Layer &L = d->layers[l];
     if ((r = digit_rows(d, L.qkv, d->hidden, d->qkv, B, L.qkv_bias, nullptr, L.in_norm, kEpiStore, st)) ||
@@ -1140,7 +1216,8 @@ int step_batched(lmx_decoder *d, float *logits_out, hipStream_t st) {
 int step(lmx_decoder *d, float *logits_out, hipStream_t st) {
   if (d->batch > 1) return step_batched(d, logits_out, st);
   const lmx_decoder_config &c = d->cfg;
-  int r = LMX_OK;
+  int r = kv8_batch(d, d->pos, 0, 1, st);
+  if (r) return r;
   for (size_t l = 0; l < c.n_layers; ++l) {
     const lmx_decoder::Layer &L = d->layers[l];
     if ((r = gemv(L.qkv, d->hidden, d->qkv, L.qkv_bias, kXModeRmsNorm, L.in_norm, c.rms_eps, st)) ||
@@ -1223,8 +1300,14 @@ int lmx_decoder_create(const lmx_decoder_config *cfg, lmx_decoder **out) {
 }
 
 int lmx_decoder_create_batched(const lmx_decoder_config *cfg, size_t batch, lmx_decoder **out) {
+  return lmx_decoder_create_kv(cfg, batch, LMX_KV_F32, out);
+}
+
+int lmx_decoder_create_kv(const lmx_decoder_config *cfg, size_t batch, int kv_format, lmx_decoder **out) {
   if (!cfg || !out) return fail(LMX_ERR_INVALID_ARGUMENT, "NULL argument");
   if (batch == 0 || batch > 64) return fail(LMX_ERR_INVALID_ARGUMENT, "batch %zu outside 1..64", batch);
+  if (kv_format != LMX_KV_F32 && kv_format != LMX_KV_INT8)
+    return fail(LMX_ERR_INVALID_ARGUMENT, "unknown KV cache format %d", kv_format);
   *out = nullptr;
   const lmx_decoder_config &c = *cfg;
   if (!c.hidden || !c.n_layers || !c.n_heads || !c.n_kv_heads || !c.ffn || !c.vocab || !c.max_seq)
@@ -1250,27 +1333,39 @@ int lmx_decoder_create_batched(const lmx_decoder_config *cfg, size_t batch, lmx_
   d->cfg = c;
   d->device = dev;
   d->batch = batch;
+  d->kv_format = kv_format;
   d->layers.resize(c.n_layers);
   d->pos_div = c.rope_mode == LMX_ROPE_REFERENCE ? c.rope_factor : 1.0f;
   if (const char *sp = std::getenv("LMX_ATTN_SPEC")) d->spec_chunks = std::max(1, std::atoi(sp));
   if (hipDeviceGetAttribute(&d->n_cu, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || d->n_cu < 1)
     d->n_cu = 256;
   const size_t qkv_rows = (c.n_heads + 2 * c.n_kv_heads) * c.head_dim;
-  const size_t kv = c.n_layers * attn_chunks(c) * kAttnChunk * c.n_kv_heads * c.head_dim;   // whole chunks
+  const bool kv8 = kv_format == LMX_KV_INT8;
+  const size_t kv = kv8 ? 0 : c.n_layers * attn_chunks(c) * kAttnChunk * c.n_kv_heads * c.head_dim;   // whole chunks
   d->kv_seq = kv;
   const size_t B = batch;
+  d->kv8_pages = (c.max_seq + LMX_KV8_PAGE - 1) / LMX_KV8_PAGE;
+  const size_t page_heads = kv8 ? c.n_layers * B * d->kv8_pages * c.n_kv_heads : 0;
+  const size_t page_codes = page_heads * LMX_KV8_PAGE * c.head_dim, page_scales = page_heads * (LMX_KV8_PAGE / LMX_KV8_BLOCK);
   const std::vector<float> fr = rope_freqs(c);
   int st;
   if ((st = d->alloc(reinterpret_cast<void **>(&d->hidden), B * c.hidden * 4)) ||
       (st = d->alloc(reinterpret_cast<void **>(&d->qkv), B * qkv_rows * 4)) ||
       (st = d->alloc(reinterpret_cast<void **>(&d->gate_up), B * 2 * c.ffn * 4)) ||
       (st = d->alloc(reinterpret_cast<void **>(&d->logits), B * c.vocab * 4)) ||
-      (st = d->alloc(reinterpret_cast<void **>(&d->kcache), B * kv * 4)) ||
-      (st = d->alloc(reinterpret_cast<void **>(&d->vcache), B * kv * 4)) ||
+      (!kv8 && (st = d->alloc(reinterpret_cast<void **>(&d->kcache), B * kv * 4))) ||
+      (!kv8 && (st = d->alloc(reinterpret_cast<void **>(&d->vcache), B * kv * 4))) ||
+      (kv8 && ((st = d->alloc(reinterpret_cast<void **>(&d->k8), page_codes)) ||
+               (st = d->alloc(reinterpret_cast<void **>(&d->v8), page_codes)) ||
+               (st = d->alloc(reinterpret_cast<void **>(&d->k8_scale), page_scales * 4)) ||
+               (st = d->alloc(reinterpret_cast<void **>(&d->v8_scale), page_scales * 4)) ||
+               (st = d->alloc(reinterpret_cast<void **>(&d->kv8_table), B * d->kv8_pages * 4)) ||
+               (st = d->alloc(reinterpret_cast<void **>(&d->kv8_offsets), (B + 1) * 4)) ||
+               (st = d->alloc(reinterpret_cast<void **>(&d->kv8_lengths), B * 4)))) ||
       (st = d->alloc(reinterpret_cast<void **>(&d->tokens), B * (c.max_seq + 1) * 4)) ||
       (st = d->alloc(reinterpret_cast<void **>(&d->pos), 4)) ||
-      (st = d->alloc(reinterpret_cast<void **>(&d->attn_part),
-                     B * c.n_heads * attn_chunks(c) * (c.head_dim + 4) * sizeof(float))) ||
+      (!kv8 && (st = d->alloc(reinterpret_cast<void **>(&d->attn_part),
+                              B * c.n_heads * attn_chunks(c) * (c.head_dim + 4) * sizeof(float)))) ||
       (st = d->alloc(reinterpret_cast<void **>(&d->attn_out), B * c.n_heads * c.head_dim * sizeof(float))) ||
       (st = d->alloc(reinterpret_cast<void **>(&d->attn_tickets),
                      B * c.n_kv_heads * kAttnMaxSplit * kTicketPad * sizeof(unsigned))) ||
@@ -1296,6 +1391,22 @@ int lmx_decoder_create_batched(const lmx_decoder_config *cfg, size_t batch, lmx_
     if (e != hipSuccess) {
       delete d;
       return hip_err(e, "rope table");
+    }
+  }
+  if (kv8) {   // pages in order, and the workspace of a step
+    const lmx_kv8_cache cache = d->kv8_layer(0);
+    const lmx_kv8_batch rows = d->kv8_rows(1);
+    std::vector<int> table(B * d->kv8_pages);
+    for (size_t i = 0; i < table.size(); ++i) table[i] = int(i);
+    if ((st = lmx_kv8_attention_workspace(&cache, &rows, LMX_F32, c.n_heads, &d->kv8_work_bytes)) ||
+        (d->kv8_work_bytes && (st = d->alloc(&d->kv8_work, d->kv8_work_bytes)))) {
+      delete d;
+      return st;
+    }
+    e = hipMemcpy(d->kv8_table, table.data(), table.size() * sizeof(int), hipMemcpyHostToDevice);
+    if (e != hipSuccess) {
+      delete d;
+      return hip_err(e, "kv8 page table");
     }
   }
   e = hipStreamCreateWithFlags(&d->stream, hipStreamNonBlocking);

@@ -357,6 +357,10 @@ bool has(const std::string &s, const char *needle) { return s.find(needle) != st
 extern "C" {
 
 int lmx_model_load(const char *path, size_t max_seq, lmx_model **out) {
+  return lmx_model_load_kv(path, max_seq, LMX_KV_F32, out);
+}
+
+int lmx_model_load_kv(const char *path, size_t max_seq, int kv_format, lmx_model **out) {
   if (!path || !out) return fail(LMX_ERR_INVALID_ARGUMENT, "NULL argument");
   *out = nullptr;
   File file;
@@ -493,7 +497,7 @@ int lmx_model_load(const char *path, size_t max_seq, lmx_model **out) {
   if (!m) return fail(LMX_ERR_OUT_OF_MEMORY, "model allocation");
   m->cfg = c;
   m->layers.resize(c.n_layers);
-  int st = lmx_decoder_create(&c, &m->dec);
+  int st = lmx_decoder_create_kv(&c, 1, kv_format, &m->dec);
   if (st) return st;
   const size_t qd = c.n_heads * c.head_dim, kvd = c.n_kv_heads * c.head_dim;
   std::vector<float> ones(c.hidden, 1.0f);   // Model::allocate() defaults (model.hpp:74-91)

@@ -20,6 +20,7 @@ from . import (FMT_INT4, DecoderConfigC, Weight, _np_ptr, _stream_ptr, check, li
 
 ROPE_REFERENCE = 0
 ROPE_LLAMA3 = 1
+KV_FORMATS = {"f32": 0, "int8": 1}   # LMX_KV_F32, LMX_KV_INT8 (any other name is refused by the library)
 
 
 @dataclass(frozen=True)
@@ -256,9 +257,10 @@ class _DecoderOps:
 
 class Decoder(_DecoderOps):
     """Device decoder over LUT-GEMV weight handles built from a SyntheticModel;
-    batch > 1 decodes that many sequences in lockstep."""
+    batch > 1 decodes that many sequences in lockstep; kv "int8" keeps their keys and
+    values in 8-bit pages (lmx_decoder_create_kv)."""
 
-    def __init__(self, model, batch=1):
+    def __init__(self, model, batch=1, kv="f32"):
         self.model, self.cfg = model, model.cfg
         self.batch = batch
         self._h = None
@@ -268,7 +270,7 @@ class Decoder(_DecoderOps):
         c = self.cfg
         h = ctypes.c_void_p()
         cs = c.c_struct()
-        check(lib().lmx_decoder_create_batched(ctypes.byref(cs), batch, ctypes.byref(h)))
+        check(lib().lmx_decoder_create_kv(ctypes.byref(cs), batch, KV_FORMATS.get(kv, -1), ctypes.byref(h)))
         self._h = h
         def weight(entry, rows, cols):
             # (planes, scales) of the model's 4-bit group, or (planes, scales, format, group)
@@ -299,11 +301,11 @@ class Decoder(_DecoderOps):
 
 class LutmacModel(_DecoderOps):
     """A .lutmac v1 file loaded onto the device decoder (lutmac_model.h): the
-    counterpart of load_model (src/model.cpp:576-701)."""
+    counterpart of load_model (src/model.cpp:576-701); kv as in Decoder."""
 
-    def __init__(self, path, max_seq=0):
+    def __init__(self, path, max_seq=0, kv="f32"):
         m = ctypes.c_void_p()
-        check(lib().lmx_model_load(str(path).encode(), max_seq, ctypes.byref(m)))
+        check(lib().lmx_model_load_kv(str(path).encode(), max_seq, KV_FORMATS.get(kv, -1), ctypes.byref(m)))
         self._m = m
         cs = DecoderConfigC()
         check(lib().lmx_model_config(self._m, ctypes.byref(cs)))

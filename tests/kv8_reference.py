@@ -40,6 +40,9 @@ class Cache:
     def __init__(self, k, v, k_scale, v_scale):
         self.k, self.v, self.k_scale, self.v_scale = (np.array(a) for a in (k, v, k_scale, v_scale))
 
+    def round(self, x):
+        return np.round(x).astype(np.int8)
+
     def append(self, k, v, q, offsets, lengths, pages, rope):
         """float64 row arrays; returns the rotated q (rows without a place: NaN)."""
         out = np.full(q.shape, np.nan) if q is not None else None
@@ -76,9 +79,9 @@ class Cache:
                         at = sub * BLOCK
                         if now == now and kept and now != was:
                             old = codes[at:at + kept].astype(np.float64) * np.float64(was)
-                            codes[at:at + kept] = np.round(old / np.float64(now)).astype(np.int8)
+                            codes[at:at + kept] = self.round(old / np.float64(now))
                         for (r, p), y in zip(rows, x):
-                            codes[p % PAGE] = np.round(y / np.float64(now)).astype(np.int8) if now == now else 0
+                            codes[p % PAGE] = self.round(y / np.float64(now)) if now == now else 0
         return out
 
     def tokens(self, pages, h, n):
