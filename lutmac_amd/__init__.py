@@ -7,6 +7,7 @@ shared library lutmac_amd/liblutmac_hip.so is built in-tree by
 nothing can silently fall back to a CPU path.
 """
 import ctypes
+import functools
 import os
 
 import numpy as np
@@ -505,6 +506,7 @@ def linear_i8(x, w, w_scale, bias=None, y=None, workspace=None, stream=None):
     return y
 
 
+@functools.lru_cache(maxsize=1024)   # (of sizes alone)
 def linear_i8_workspace(rows, cols, batch):
     """Bytes of workspace of a linear_i8 call."""
     n = ctypes.c_size_t()

@@ -187,83 +187,91 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t weight_buffer(const I8Args &a,
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t *>(a.w) + at, 0, int(min(end - at, size_t(0x7FFFFFFF))), 0x00020000);
 }
 
-// 16 bytes per lane from a buffer straight to LDS, lane l's at lds + 16 l (the
-// host pass, which emits no device code, rejects the builtin).
-__device__ __forceinline__ void buffer_to_lds(__amdgpu_buffer_rsrc_t buf, char *lds, int at, int base) {
-#ifdef __HIP_DEVICE_COMPILE__
-  typedef __attribute__((address_space(3))) void lds_void;
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(buf, (lds_void *)lds, 16, at, base, 0, 0);
-#endif
+__device__ __forceinline__ void lds_barrier() {   // no wait for loads on their way, as __syncthreads makes
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// 128-byte rows in LDS: piece p (16 bytes) of row r lies at p ^ (r / 2 mod 8), so
+// that the 16 lanes of a read's phase touch all 64 banks once.
+__device__ __forceinline__ int piece_place(int row, int piece) { return 16 * (piece ^ (row >> 1 & 7)); }
+// Where lane `lane` of a load of 8 rows reads row `row` (the last one past it).
+__device__ __forceinline__ int piece_offset(int row, int last, int stride, int lane) {
+  return min(row, last) * stride + piece_place(row, lane % 8);
 }
 
 // ---------------------------------------------------------------------------
 // One to four rows of activations, one launch: a workgroup takes 16 weight rows,
-// its W waves the k-steps w, w + W, ...; every weight byte goes from memory to
-// an operand register once, four steps of a wave in flight.  Every workgroup
-// makes the codes itself, in LDS while its first weights are on their way (R >=
-// batch rows, a power of two), which saves a launch and the trip through memory.
+// its W waves the k-steps w, w + W, ..., each through U LDS buffers of its own
+// (see i8_few_kernel).  Every workgroup makes the codes itself, in LDS while its
+// first weights are on their way (R >= batch rows, a power of two; at most 16
+// values a thread, which stay in registers), which saves a launch and the trip
+// through memory.
 //   A (weights): lane (i, g) holds bytes 16 g .. + 15 of a 64-byte step of row i;
 //   B (codes) the same of activation row j; C lane (j, g): weight rows 4 g .. + 3.
+constexpr int rows_buffers(int waves) { return waves == 16 ? 3 : 4; }
 template <class T, int W, int R>
 __global__ __launch_bounds__(W *kWave) void i8_rows_kernel(I8Args a) {
-  constexpr int U = 4;
+  constexpr int U = rows_buffers(W), RB = 16 * kStep;
   __shared__ v4i part[W][kWave];
   __shared__ uint32_t tops[W];
-  extern __shared__ __attribute__((aligned(16))) char codes[];   // [batch][Kp + 16]
+  extern __shared__ __attribute__((aligned(1024))) char lds[];   // the waves' buffers, then codes [batch][Kp + 16]
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
   const int i = lane & 15, g = lane >> 4, row0 = int(blockIdx.x) * 16;
-  const auto wbuf = weight_buffer(a, row0);
-  const int wrow = min(i, a.rows - 1 - row0) * int(a.w_stride) + 16 * g;
-  const int steps = a.Kp / kStep;
-  // (a step past the last reads nothing, and zeros)
-  const auto load_weights = [&](int s, v4i (&w)[U][2]) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int at = s + u * W < steps ? (s + u * W) * kStep : 0x7F000000;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) w[u][h] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(wbuf, wrow + 64 * h, at, 0));
-    }
-  };
-  v4i w[U][2], next[U][2];
-  load_weights(wave, w);
+  char *mine = lds + wave * (U * RB), *codes = lds + W * U * RB;
+  constexpr int KEEP = 2, TR = W * kWave / R;   // threads of an activation row
+  const int am = int(threadIdx.x) / TR, k0 = int(threadIdx.x) % TR * 8;
+  float v[KEEP][8];
   {
-    constexpr int TR = W * kWave / R;   // threads of an activation row
-    const int m = int(threadIdx.x) / TR, k0 = int(threadIdx.x) % TR * 8;
-    const T *x = static_cast<const T *>(a.x) + size_t(min(m, a.batch - 1)) * a.cols;
+    const T *x = static_cast<const T *>(a.x) + size_t(min(am, a.batch - 1)) * a.cols;
     const bool vec = reinterpret_cast<size_t>(x) % 16 == 0;
+#pragma unroll
+    for (int j = 0; j < KEEP; ++j) load8(x, k0 + j * TR * 8, a.cols, vec, v[j]);
+  }
+  const auto wbuf = weight_buffer(a, row0);
+  int won[2];
+#pragma unroll
+  for (int n = 0; n < 2; ++n) won[n] = piece_offset(8 * n + lane / 8, a.rows - 1 - row0, int(a.w_stride), lane);
+  const int steps = a.Kp / kStep, turns = wave < steps ? (steps - 1 - wave) / W + 1 : 0;
+  const auto fill = [&](int buf, int t) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n) buffer_to_lds(wbuf, mine + buf * RB + n * 1024, won[n], (wave + t * W) * kStep);
+  };
+#pragma unroll
+  for (int t = 0; t < U - 1; ++t)
+    if (t < turns) fill(t, t);
+  {
     uint32_t top = 0;
-    for (int k = k0; k < a.cols; k += TR * 8) {
-      float v[8];
-      load8(x, k, a.cols, vec, v);
-      top = top8(v, top);
-    }
+#pragma unroll
+    for (int j = 0; j < KEEP; ++j) top = top8(v[j], top);
     top = wave_top(top, lane);
     if (lane == 0) tops[wave] = top;
-    __syncthreads();
-    if (m < a.batch) {
-      const Rounder r(row_top<W, R>(tops, m));
-      for (int k = k0; k < a.Kp; k += TR * 8) {
-        float v[8];
-        load8(x, k, a.cols, vec, v);   // (from the cache)
-        *reinterpret_cast<uint2 *>(codes + m * (a.Kp + 16) + k) = r.codes(v);
-      }
+    lds_barrier();
+    if (am < a.batch) {
+      const Rounder r(row_top<W, R>(tops, am));
+#pragma unroll
+      for (int j = 0; j < KEEP; ++j)
+        if (k0 + j * TR * 8 < a.Kp) *reinterpret_cast<uint2 *>(codes + am * (a.Kp + 16) + k0 + j * TR * 8) = r.codes(v[j]);
     }
-    __syncthreads();
+    lds_barrier();
   }
   const int m = min(i, a.batch - 1);
   const char *xc = codes + m * (a.Kp + 16) + 16 * g;
   v4i acc = {0, 0, 0, 0};
-  for (int s = wave; s < steps; s += U * W) {
-    load_weights(s + U * W, next);
+  int buf = 0;
+  for (int t = 0; t < turns; ++t) {
+    if (t + U - 1 <= turns) wait_loads<(U - 2) * 2>();
+    else wait_loads<0>();
+    const char *at = mine + buf * RB + i * kStep;
+    v4i w[2], x[2];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int k = min(s + u * W, steps - 1) * kStep;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u][h], *reinterpret_cast<const v4i *>(xc + k + 64 * h), acc, 0, 0, 0);
-        w[u][h] = next[u][h];
-      }
+    for (int h = 0; h < 2; ++h) {
+      w[h] = *reinterpret_cast<const v4i *>(at + piece_place(i, 4 * h + g));
+      x[h] = *reinterpret_cast<const v4i *>(xc + (wave + t * W) * kStep + 64 * h);
     }
+    if (t + U - 1 < turns) fill(buf == 0 ? U - 1 : buf - 1, t + U - 1);   // (the buffer of the step before)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[h], x[h], acc, 0, 0, 0);
+    buf = buf == U - 1 ? 0 : buf + 1;
   }
   part[wave][lane] = acc;
   const Four f = row_factors<T>(a, row0 + 4 * g);
@@ -275,16 +283,89 @@ __global__ __launch_bounds__(W *kWave) void i8_rows_kernel(I8Args a) {
 }
 
 // ---------------------------------------------------------------------------
+// Some rows of activations (up to 16 G) and so few weight rows that tiles of
+// 64 x 64 leave CUs idle: 16 weight rows a workgroup, its W waves the k-steps w,
+// w + W, ..., each through U LDS buffers of its own that are filled straight from
+// memory U - 1 steps ahead, so that no wave waits for another before the end.
+// (Straight to registers a load instruction touches 64 lines instead of 8 and
+// takes as many cycles: 48 x 8960 -> 1536 24 us.)
+template <class T, int W, int R, int G, int U>
+__global__ __launch_bounds__(W *kWave) void i8_few_kernel(I8Args a) {
+  constexpr int RB = (R + G) * 16 * kStep;   // bytes of a buffer: weights, then codes
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
+  const int i = lane & 15, g = lane >> 4, row0 = int(blockIdx.x) * (16 * R);
+  const auto wbuf = weight_buffer(a, row0);
+  const auto xbuf = __builtin_amdgcn_make_buffer_rsrc(a.codes, 0, a.batch * a.Kp, 0x00020000);
+  int won[2 * R], xon[2 * G];   // (a load instruction: 8 rows)
+#pragma unroll
+  for (int n = 0; n < 2 * R; ++n) won[n] = piece_offset(8 * n + lane / 8, a.rows - 1 - row0, int(a.w_stride), lane);
+#pragma unroll
+  for (int n = 0; n < 2 * G; ++n) xon[n] = piece_offset(8 * n + lane / 8, a.batch - 1, a.Kp, lane);
+  char *mine = lds + wave * (U * RB);
+  const int steps = a.Kp / kStep, turns = wave < steps ? (steps - 1 - wave) / W + 1 : 0;
+  const auto fill = [&](int buf, int t) {
+    const int k = (wave + t * W) * kStep;
+#pragma unroll
+    for (int n = 0; n < 2 * R; ++n) buffer_to_lds(wbuf, mine + buf * RB + n * 1024, won[n], k);
+#pragma unroll
+    for (int n = 0; n < 2 * G; ++n) buffer_to_lds(xbuf, mine + buf * RB + (2 * R + n) * 1024, xon[n], k);
+  };
+#pragma unroll
+  for (int t = 0; t < U - 1; ++t)
+    if (t < turns) fill(t, t);
+  v4i acc[R][G];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int n = 0; n < G; ++n) acc[r][n] = v4i{0, 0, 0, 0};
+  int buf = 0;
+  for (int t = 0; t < turns; ++t) {
+    if (t + U - 1 <= turns) wait_loads<(U - 2) * 2 * (R + G)>();
+    else wait_loads<0>();
+    const char *at = mine + buf * RB + i * kStep;
+    v4i w[R][2], x[G][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int piece = piece_place(i, 4 * h + g);
+#pragma unroll
+      for (int r = 0; r < R; ++r) w[r][h] = *reinterpret_cast<const v4i *>(at + r * 16 * kStep + piece);
+#pragma unroll
+      for (int n = 0; n < G; ++n) x[n][h] = *reinterpret_cast<const v4i *>(at + (R + n) * 16 * kStep + piece);
+    }
+    if (t + U - 1 < turns) fill(buf == 0 ? U - 1 : buf - 1, t + U - 1);   // (the buffer of the step before)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int n = 0; n < G; ++n) acc[r][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[r][h], x[n][h], acc[r][n], 0, 0, 0);
+    buf = buf == U - 1 ? 0 : buf + 1;
+  }
+  __syncthreads();   // every wave is done with its buffers
+  v4i(*part)[R * G][kWave] = reinterpret_cast<v4i(*)[R * G][kWave]>(lds);
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int n = 0; n < G; ++n) part[wave][r * G + n][lane] = acc[r][n];
+  __syncthreads();
+  for (int q = wave; q < R * G; q += W) {
+    const int r = q / G, m = 16 * (q % G) + i, row = row0 + 16 * r + 4 * g;
+    const Four f = row_factors<T>(a, row);
+    const float xs = a.scales[min(m, a.batch - 1)];
+    v4i sum = {0, 0, 0, 0};
+#pragma unroll
+    for (int v = 0; v < W; ++v) sum += part[v][q][lane];
+    store4<T>(a, m, row, sum, xs, f, vector_rows<T>(a));
+  }
+}
+
+// ---------------------------------------------------------------------------
 // Many rows of activations: BN weight rows x BM activation rows per workgroup,
 // WN x WM waves, k in steps of BK bytes through S LDS buffers that are filled
 // straight from memory S - 1 steps ahead (v_mfma_i32_32x32x32_i8).  A row's
 // 16-byte pieces lie in LDS at p ^ swizzle(row), so that the 16 lanes of a
 // read's phase touch all 64 banks once.
-template <int N>
-__device__ __forceinline__ void wait_loads() {   // all but the wave's last N loads are there
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
-
 //
 // PART: workgroup (tile, part) takes part blockIdx.y of k and leaves its integer
 // sums (T is int) for i8_join_kernel: where tiles are few and k is long.
@@ -459,14 +540,36 @@ int launch_err(const char *what) {
   return e == hipSuccess ? LMX_OK : fail(LMX_ERR_LAUNCH_FAILED, "%s launch: %s", what, hipGetErrorString(e));
 }
 
+// (per device: asked before each launch, 0.2 us)
+int allow_lds(const void *kernel, size_t bytes) {
+  const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+  return e == hipSuccess ? LMX_OK : fail(LMX_ERR_HIP, "LDS of an i8 kernel: %s", hipGetErrorString(e));
+}
+
 size_t tile_count(size_t rows, size_t batch, size_t side) { return (rows + side - 1) / side * ((batch + side - 1) / side); }
 
-// Parts of k: as many as bring the 64 x 64 tiles to one per CU, of 8 steps at
-// least (us, in one part / in parts: 48 x 8960 -> 1536 in 8 28 / 16, 64 x 8192 ->
-// 8192 in 2 28 / 23, 48 x 2048 -> 2048 in 2 12.0 / 12.1).
+// Up to 64 activation rows go to i8_few_kernel, unless tiles of 64 x 64 are just
+// one round of the CUs (us, tiles / 16 weight rows and 4 waves a workgroup / 32 and
+// 4 / 64 and 2: 16 x 2048 -> 2048 11.8 / 7.4 / 7.7 / 8.8, 48 x 8960 -> 1536 16.4 /
+// 13.6 / 15.1 / 22, 48 x 2048 -> 8192 13.3 / 11.5 / 10.3 / 12.0, 48 x 2048 -> 16384
+// 13.1 / 18.4 / 15.1 / 14.1, 48 x 8192 -> 24576 55 / 53 / 52 / 43): more weight rows
+// a workgroup read the codes less often.
+enum class FewShape { none, rows16, rows32, rows64 };
+FewShape few_shape(size_t rows, size_t batch) {
+  const size_t tiles = tile_count(rows, batch, 64);
+  if (batch > 64 || (batch > 16 && tiles >= 192 && tiles <= 256)) return FewShape::none;
+  if (batch > 16 && rows > 16384) return FewShape::rows64;
+  return batch > 32 && rows > 4096 ? FewShape::rows32 : FewShape::rows16;
+}
+
+// Parts of k for other calls of few tiles: as many as bring the 64 x 64 tiles to
+// one per CU, of 8 steps at least, if they are three (us, in one part / in parts:
+// 100 x 8960 -> 1536 in 5 28.8 / 17.8, 100 x 2048 -> 2048 in 2 11.5 / 12.1).
 int split_count(size_t rows, size_t cols, size_t batch) {
+  if (few_shape(rows, batch) != FewShape::none) return 1;
   const size_t tiles = tile_count(rows, batch, 64), steps = round_up(cols, kStep) / kStep;
-  return tiles ? int(std::max<size_t>(1, std::min<size_t>(256 / tiles, steps / 8))) : 1;
+  const size_t parts = tiles ? std::min<size_t>(256 / tiles, steps / 8) : 1;
+  return parts < 3 ? 1 : int(parts);
 }
 
 // More waves share a row tile's k where the tiles alone leave CUs idle.
@@ -475,49 +578,75 @@ int rows_waves(const I8Args &a) {
   return tiles <= 256 ? 16 : tiles <= 768 ? 8 : 4;
 }
 
+template <class T, int W, int R>
+int launch_rows(const I8Args &a, hipStream_t st) {
+  constexpr size_t ring = W * rows_buffers(W) * 16 * kStep, most = ring + 1024 * W + 16 * R;
+  if (const int r = allow_lds(reinterpret_cast<const void *>(&i8_rows_kernel<T, W, R>), most)) return r;
+  i8_rows_kernel<T, W, R><<<unsigned((a.rows + 15) / 16), W * kWave, ring + size_t(a.batch) * (a.Kp + 16), st>>>(a);
+  return launch_err("i8 linear");
+}
 template <class T, int R>
-void launch_rows(const I8Args &a, hipStream_t st) {
-  const unsigned grid = unsigned((a.rows + 15) / 16), lds = unsigned(a.batch * (a.Kp + 16));
+int launch_rows(const I8Args &a, hipStream_t st) {
   switch (rows_waves(a)) {
-  case 16: i8_rows_kernel<T, 16, R><<<grid, 16 * kWave, lds, st>>>(a); break;
-  case 8: i8_rows_kernel<T, 8, R><<<grid, 8 * kWave, lds, st>>>(a); break;
-  default: i8_rows_kernel<T, 4, R><<<grid, 4 * kWave, lds, st>>>(a); break;
+  case 16: return launch_rows<T, 16, R>(a, st);
+  case 8: return launch_rows<T, 8, R>(a, st);
+  default: return launch_rows<T, 4, R>(a, st);
   }
 }
 
 // Whether every workgroup makes the codes itself: up to 4 rows, as long as that
-// is two rounds of a workgroup's threads (us, itself / codes in a launch before:
-// 1 x 2048 -> 16384 9.2 / 12.1, 4 x 2048 -> 8192 9.7 / 11.1, 4 x 2048 -> 16384,
-// four rounds, 14.2 / 12.4).
+// is two rounds of a workgroup's threads, and not too often for nothing (us,
+// itself / codes in a launch before: 1 x 2048 -> 16384 8.6 / 11.4, 4 x 2048 -> 8192
+// 8.5 / 8.7, 2 x 2048 -> 16384 9.9 / 11.7, 2 x 2048 -> 65536 28 / 26).
+int row_slots(const I8Args &a) { return a.batch <= 2 ? a.batch : 4; }
 bool in_one_launch(const I8Args &a) {
-  return a.batch <= 4 && a.batch * a.Kp <= 1024 * rows_waves(a);
+  return a.batch <= 4 && row_slots(a) * a.Kp <= 1024 * rows_waves(a) && (a.batch == 1 || a.rows <= 32768);
 }
 
 template <class T, int BN, int BM, int WN, int WM, int BK, int S>
 int launch_tile(const I8Args &a, hipStream_t st) {
   constexpr size_t lds = S * (BN + BM) * BK;
-  static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&i8_tile_kernel<T, BN, BM, WN, WM, BK, S>),
-                                                  hipFuncAttributeMaxDynamicSharedMemorySize, int(lds));
-  if (e != hipSuccess) return fail(LMX_ERR_HIP, "LDS of the i8 tile kernel: %s", hipGetErrorString(e));
+  if (const int r = allow_lds(reinterpret_cast<const void *>(&i8_tile_kernel<T, BN, BM, WN, WM, BK, S>), lds)) return r;
   const size_t tiles = size_t((a.rows + BN - 1) / BN) * size_t((a.batch + BM - 1) / BM);
   if (tiles > (1u << 30)) return fail(LMX_ERR_INVALID_ARGUMENT, "%d x %d outputs", a.rows, a.batch);
   i8_tile_kernel<T, BN, BM, WN, WM, BK, S><<<dim3(unsigned(round_up(tiles, 8)), unsigned(a.splits)), WN * WM * kWave, lds, st>>>(a);
   return LMX_OK;
 }
 
+template <class T, int W, int R, int G>
+int launch_few(const I8Args &a, hipStream_t st) {
+  constexpr size_t lds = W * 3 * (R + G) * 16 * kStep;
+  if (const int r = allow_lds(reinterpret_cast<const void *>(&i8_few_kernel<T, W, R, G, 3>), lds)) return r;
+  i8_few_kernel<T, W, R, G, 3><<<unsigned((a.rows + 16 * R - 1) / (16 * R)), W * kWave, lds, st>>>(a);
+  return launch_err("i8 linear");
+}
+template <class T>
+int launch_few(const I8Args &a, hipStream_t st) {
+  const int G = (a.batch + 15) / 16;
+  switch (few_shape(a.rows, a.batch)) {
+  case FewShape::rows64: return G == 2 ? launch_few<T, 2, 4, 2>(a, st) : G == 3 ? launch_few<T, 2, 4, 3>(a, st) : launch_few<T, 2, 4, 4>(a, st);
+  case FewShape::rows32: return G == 3 ? launch_few<T, 4, 2, 3>(a, st) : launch_few<T, 4, 2, 4>(a, st);
+  default:
+    return G == 1 ? launch_few<T, 4, 1, 1>(a, st) : G == 2 ? launch_few<T, 4, 1, 2>(a, st) : G == 3 ? launch_few<T, 4, 1, 3>(a, st)
+                                                                                      : launch_few<T, 4, 1, 4>(a, st);
+  }
+}
+
 template <class T>
 int launch_linear(const I8Args &a, hipStream_t st) {
   if (in_one_launch(a)) {
-    if (a.batch == 1) launch_rows<T, 1>(a, st);
-    else if (a.batch == 2) launch_rows<T, 2>(a, st);
-    else launch_rows<T, 4>(a, st);
-    return launch_err("i8 linear");
+    switch (row_slots(a)) {
+    case 1: return launch_rows<T, 1>(a, st);
+    case 2: return launch_rows<T, 2>(a, st);
+    default: return launch_rows<T, 4>(a, st);
+    }
   }
   // (few long rows: 1024 threads a row, 48 of 8960 in 4.3 us against 6.8)
   if (a.Kp > 2048 && a.batch < 512) i8_codes_kernel<T, 1024><<<unsigned(a.batch), 1024, 0, st>>>(a);
   else i8_codes_kernel<T, 256><<<unsigned(a.batch), 256, 0, st>>>(a);
   int r = launch_err("i8 codes");
   if (r) return r;
+  if (few_shape(a.rows, a.batch) != FewShape::none) return launch_few<T>(a, st);
   if (a.splits > 1) {
     if ((r = launch_tile<int, 64, 64, 2, 2, 128, 4>(a, st)) || (r = launch_err("i8 linear parts"))) return r;
     i8_join_kernel<T><<<unsigned((size_t(a.batch) * ((a.rows + 3) / 4) + 255) / 256), 256, 0, st>>>(a);

@@ -335,7 +335,7 @@ __global__ __launch_bounds__(kPromptWaves *kWave) __attribute__((amdgpu_waves_pe
 template <class T, int HD>
 int launch(const AttnArgs &a, dim3 grid, hipStream_t st) {
   constexpr int lds = 5 * kPage * HD * 2;
-  static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&kv8_prompt_kernel<T, HD>),
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&kv8_prompt_kernel<T, HD>),
                                                   hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   if (e != hipSuccess) return fail(LMX_ERR_LAUNCH_FAILED, "hipFuncSetAttribute: %s", hipGetErrorString(e));
   kv8_prompt_kernel<T, HD><<<grid, dim3(kPromptWaves * kWave), lds, st>>>(a);

@@ -110,6 +110,19 @@ __device__ __forceinline__ unsigned long long wave_max_key(unsigned long long ke
   else return key;
 }
 
+// 16 bytes per lane from a buffer straight to LDS, lane l's at lds + 16 l (the
+// host pass, which emits no device code, rejects the builtin).
+__device__ __forceinline__ void buffer_to_lds(__amdgpu_buffer_rsrc_t buf, char *lds, int at, int base) {
+#ifdef __HIP_DEVICE_COMPILE__
+  typedef __attribute__((address_space(3))) void lds_void;
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(buf, (lds_void *)lds, 16, at, base, 0, 0);
+#endif
+}
+template <int N>
+__device__ __forceinline__ void wait_loads() {   // all but the wave's last N loads are there
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
 }  // namespace lmx
 
 #endif  // LMX_LANES_HPP

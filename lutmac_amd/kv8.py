@@ -14,6 +14,7 @@ offsets, lengths and pages are int32 and read when the work runs, so a captured
 call follows what they hold at each replay.
 """
 import ctypes
+import functools
 
 import torch
 
@@ -37,14 +38,21 @@ def _bad(name, t, want):
 
 def _rows(name, t, dtype, heads, head_dim, rows):
     """Checks a row tensor [rows, heads, head_dim], rows any stride apart; returns its row stride."""
-    # (written for speed: every call checks four of them)
-    if t.dtype is not dtype or t.dim() != 3:
-        _bad(name, t, f"{dtype} [rows, heads, {head_dim}]")
-    n, h, d = t.shape
+    # (written for speed: every call checks up to four of them)
+    if t.dtype is not dtype or t.shape != (rows, heads, head_dim):
+        _bad(name, t, f"{dtype} [{rows}, {heads}, {head_dim}]")
     row, head, one = t.stride()
-    if n != rows or h != heads or d != head_dim or (n and (one != 1 or (h > 1 and head != head_dim))):
-        _bad(name, t, f"[{rows}, {heads}, {head_dim}] with a row's heads side by side")
-    return row if n > 1 else h * d   # (a single row's stride says nothing)
+    if (one != 1 or (head != head_dim and heads > 1)) and rows:
+        _bad(name, t, "a row's heads side by side")
+    return row if rows > 1 else heads * head_dim   # (a single row's stride says nothing)
+
+
+@functools.lru_cache(maxsize=1024)   # (of sizes alone)
+def _workspace(n_pages, n_kv_heads, head_dim, kind, rows, heads, n_seqs, max_pages):
+    c = Kv8CacheC(None, None, None, None, n_pages, n_kv_heads, head_dim)
+    b, n = Kv8BatchC(None, None, None, n_seqs, max_pages, rows), ctypes.c_size_t()
+    check(lib().lmx_kv8_attention_workspace(ctypes.byref(c), ctypes.byref(b), kind, heads, ctypes.byref(n)))
+    return n.value
 
 
 class KvCache8:
@@ -53,14 +61,16 @@ class KvCache8:
     v_scale fp32 [pages, kv_heads, 4]; value = code * scale."""
 
     def __init__(self, k, v, k_scale, v_scale):
-        if k.dim() != 4 or k.dtype is not torch.int8 or not k.is_contiguous() or k.shape[2] != PAGE or k.shape[3] not in (64, 128):
+        pages, heads, page, hd = k.shape if k.dim() == 4 else (0, 0, 0, 0)
+        if page != PAGE or (hd != 64 and hd != 128) or k.dtype is not torch.int8 or not k.is_contiguous():
             _bad("k", k, f"contiguous int8 [pages, kv_heads, {PAGE}, 64 or 128]")
-        pages, heads, _, hd = k.shape
         if v.dtype is not torch.int8 or v.shape != (pages, heads, hd, PAGE) or not v.is_contiguous():
             _bad("v", v, f"contiguous int8 {(pages, heads, hd, PAGE)}")
-        for s in (k_scale, v_scale):
-            if s.dtype is not torch.float32 or s.shape != (pages, heads, PAGE // BLOCK) or not s.is_contiguous():
-                _bad("scales", s, f"contiguous float32 {(pages, heads, PAGE // BLOCK)}")
+        shape = (pages, heads, PAGE // BLOCK)
+        if k_scale.dtype is not torch.float32 or k_scale.shape != shape or not k_scale.is_contiguous():
+            _bad("k_scale", k_scale, f"contiguous float32 {shape}")
+        if v_scale.dtype is not torch.float32 or v_scale.shape != shape or not v_scale.is_contiguous():
+            _bad("v_scale", v_scale, f"contiguous float32 {shape}")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.n_pages, self.n_kv_heads, self.head_dim = pages, heads, hd
         self._device = k.get_device()
@@ -78,18 +88,16 @@ class KvCache8:
 
     def _batch(self, offsets, lengths, pages, rows, *others):
         """The call's batch, after checking that all its tensors are on the current device."""
-        if offsets.dtype is not torch.int32 or lengths.dtype is not torch.int32 or pages.dtype is not torch.int32 or \
-                offsets.dim() != 1 or lengths.dim() != 1 or pages.dim() != 2 or \
-                not (offsets.is_contiguous() and lengths.is_contiguous() and pages.is_contiguous()):
-            for name, t, dim in (("offsets", offsets, 1), ("lengths", lengths, 1), ("pages", pages, 2)):
-                if t.dtype is not torch.int32 or t.dim() != dim or not t.is_contiguous():
-                    _bad(name, t, f"contiguous int32 of {dim} dimension(s)")
-        n = lengths.shape[0]
-        listed, width = pages.shape
-        if offsets.shape[0] != n + 1 or listed != n:
-            raise ValueError(f"{n} lengths need {n + 1} offsets and {n} page table rows")
+        int32 = torch.int32
+        if pages.dtype is not int32 or pages.dim() != 2 or not pages.is_contiguous():
+            _bad("pages", pages, "contiguous int32 of 2 dimensions")
+        n, width = pages.shape
+        if offsets.dtype is not int32 or offsets.shape != (n + 1,) or not offsets.is_contiguous():
+            _bad("offsets", offsets, f"contiguous int32 [{n + 1}] beside {n} page table rows")
+        if lengths.dtype is not int32 or lengths.shape != (n,) or not lengths.is_contiguous():
+            _bad("lengths", lengths, f"contiguous int32 [{n}] beside {n} page table rows")
         device = self._device
-        for t in (offsets, lengths, pages) + others:
+        for t in (offsets, lengths, pages, *others):
             if t is not None and t.get_device() != device:
                 raise ValueError(f"expected tensors on the cache's device, got one on {t.device}")
         if device < 0 or device != _current_device():
@@ -105,7 +113,8 @@ class KvCache8:
         kind = _types().get(dtype)
         if kind is None:
             raise LmxError(ERR_UNSUPPORTED_FORMAT, f"k is {k.dtype}: float32, float16 or bfloat16")
-        ks, vs = _rows("k", k, dtype, self.n_kv_heads, hd, rows), _rows("v", v, dtype, self.n_kv_heads, hd, rows)
+        ks = _rows("k", k, dtype, self.n_kv_heads, hd, rows)
+        vs = _rows("v", v, dtype, self.n_kv_heads, hd, rows)
         heads = qs = os = 0
         qp = op = rp = None
         if q is not None:
@@ -120,9 +129,10 @@ class KvCache8:
             raise ValueError("q_out without q")
         positions = 0
         if rope is not None:
-            if rope.dtype is not torch.float32 or rope.dim() != 3 or rope.shape[1:] != (hd // 2, 2) or not rope.is_contiguous():
+            positions = rope.shape[0] if rope.dim() else 0
+            if rope.dtype is not torch.float32 or rope.shape != (positions, hd // 2, 2) or not rope.is_contiguous():
                 _bad("rope", rope, f"contiguous float32 [positions, {hd // 2}, 2]")
-            rp, positions = rope.data_ptr(), rope.shape[0]
+            rp = rope.data_ptr()
         b = self._batch(offsets, lengths, pages, rows, k, v, q, q_out, rope)
         check(lib().lmx_kv8_append(ctypes.byref(self._c), ctypes.byref(b), kind, k.data_ptr(), ks, v.data_ptr(), vs, qp, qs, op,
                                    os, heads, rp, positions, _stream_ptr(stream)))
@@ -144,22 +154,18 @@ class KvCache8:
         else:
             os = _rows("out", out, dtype, heads, hd, rows)
         b = self._batch(offsets, lengths, pages, rows, q, out, workspace)
-        c, b, size = ctypes.byref(self._c), ctypes.byref(b), ctypes.c_size_t()
+        c = ctypes.byref(self._c)
         if workspace is None:
-            check(lib().lmx_kv8_attention_workspace(c, b, kind, heads, ctypes.byref(size)))
-            size = size.value
+            size = _workspace(self.n_pages, self.n_kv_heads, hd, kind, rows, heads, b.n_seqs, b.max_pages)
             if size:
                 workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
         else:
             size = workspace.numel() * workspace.element_size()
-        check(lib().lmx_kv8_attention(c, b, kind, q.data_ptr(), qs, heads, hd ** -0.5 if scale is None else scale,
+        check(lib().lmx_kv8_attention(c, ctypes.byref(b), kind, q.data_ptr(), qs, heads, hd ** -0.5 if scale is None else scale,
                                       out.data_ptr(), os, None if workspace is None else workspace.data_ptr(), size,
                                       _stream_ptr(stream)))
         return out
 
     def attend_workspace(self, dtype, rows, heads, n_seqs, max_pages):
         """Bytes of workspace of an attend call of these sizes."""
-        b, n = Kv8BatchC(None, None, None, n_seqs, max_pages, rows), ctypes.c_size_t()
-        check(lib().lmx_kv8_attention_workspace(ctypes.byref(self._c), ctypes.byref(b), _types()[dtype], heads,
-                                                ctypes.byref(n)))
-        return n.value
+        return _workspace(self.n_pages, self.n_kv_heads, self.head_dim, _types()[dtype], rows, heads, n_seqs, max_pages)

@@ -54,6 +54,14 @@ def test_linear_i8(cuda, dtype, rows, cols, batch):
     check(*a, L.linear_i8(a[0], a[1], a[2], bias=a[3]))
 
 
+# workgroups of 16, 32 and 64 weight rows, the last one in part; tiles of just one round of the CUs
+@pytest.mark.parametrize("rows,cols", [(4101, 700), (7001, 2048), (14000, 128), (20003, 300), (33000, 256)])
+@pytest.mark.parametrize("batch", [2, 4, 20, 37, 64])
+def test_linear_i8_many_weight_rows(cuda, rows, cols, batch):
+    a = make(rows, cols, batch, torch.bfloat16, rows + batch)
+    check(*a, L.linear_i8(a[0], a[1], a[2], bias=a[3]))
+
+
 @pytest.mark.parametrize("rows,cols,batch", [(4096, 512, 4100), (4100, 260, 4097), (8190, 1400, 2200), (16384, 128, 1100)])
 def test_linear_i8_large(cuda, rows, cols, batch):
     a = make(rows, cols, batch, torch.bfloat16, 7)
