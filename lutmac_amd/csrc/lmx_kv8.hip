@@ -2,6 +2,7 @@
 // append, and attention of a few rows per sequence over it.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "lmx_kv8.hpp"
 
@@ -300,8 +301,8 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
 // (offsets, table, page, and each further page of a wave): table entries come 64
 // at a time, and a page's keys and values are requested as soon as the registers
 // of the page before are free of theirs.
-template <class T, int HD, int ND>
-__global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(ND == 3 && HD == 128 ? 2 : 3))) void kv8_rows_kernel(AttnArgs a) {
+template <class T, int HD, int ND, int PD>
+__global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(PD == 3 && HD == 128 ? 2 : 3))) void kv8_rows_kernel(AttnArgs a) {
   constexpr int W = 4, M = HD / 64, H = HD / 16;
   __shared__ float os[W][16][HD + 4];
   __shared__ float ms[W][16], ls[W][16];
@@ -436,23 +437,23 @@ __global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(ND ==
     top = fmaxf(top, lane_xor<32>(top, lane));
     const float mn = fmaxf(mref, top), base = mn == -INFINITY ? 0.0f : mn;
     const float root = __builtin_amdgcn_exp2f(0.5f * (mref - base)), keep = root * root;
-    const float off = Digits<ND>::p_exp - base;
+    const float off = Digits<PD>::p_exp - base;
     mref = mn;
-    v4i pd[ND];
+    v4i pd[PD];
     float sum = 0.0f;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      uint32_t w[4], dw[ND];
+      uint32_t w[4], dw[PD];
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         const float e = __builtin_amdgcn_exp2f(y[u][v] + off);
         sum += e;
-        w[v] = __float_as_uint(fmaf(e, mant, kMagic + float(Digits<ND>::carry)));
+        w[v] = __float_as_uint(fmaf(e, mant, kMagic + float(Digits<PD>::carry)));
       }
-      digit_words<ND>(w, dw);
-      if constexpr (ND == 3) dw[2] ^= 0x40404040u;   // (kMagic's own bit 22)
+      digit_words<PD>(w, dw);
+      if constexpr (PD == 3) dw[2] ^= 0x40404040u;   // (kMagic's own bit 22)
 #pragma unroll
-      for (int d = 0; d < ND; ++d) pd[d][u] = int(dw[d]);
+      for (int d = 0; d < PD; ++d) pd[d][u] = int(dw[d]);
     }
     // (a block whose scale is not finite gives NaN to the rows that see it)
     const float unit = vsp - vsp == 0.0f ? __builtin_amdgcn_ldexpf(1.0f, kSumExp - ex) : __builtin_nanf("");
@@ -460,15 +461,15 @@ __global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(ND ==
     if (sum != 0.0f) l = fmaf(sum, unit, l);
 #pragma unroll
     for (int h = 0; h < H; ++h) {
-      v4i s[ND];
+      v4i s[PD];
 #pragma unroll
-      for (int d = 0; d < ND; ++d) s[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vb[h], pd[d], zero, 0, 0, 0);
+      for (int d = 0; d < PD; ++d) s[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vb[h], pd[d], zero, 0, 0, 0);
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
-        float d[ND];
+        float d[PD];
 #pragma unroll
-        for (int n = 0; n < ND; ++n) d[n] = __int_as_float(s[n][v]);
-        o[h][v] = fmaf(o[h][v], keep, join<ND>(d));
+        for (int n = 0; n < PD; ++n) d[n] = __int_as_float(s[n][v]);
+        o[h][v] = fmaf(o[h][v], keep, join<PD>(d));
       }
     }
     request_values();
@@ -627,12 +628,12 @@ Plan plan(const lmx_kv8_cache *c, const lmx_kv8_batch *b, size_t n_heads, int ty
   p.rows = type != LMX_F32 && b->n_rows * group >= 64 * b->n_seqs ? kPromptRows : 16;
   p.units = b->n_rows * group / p.rows + b->n_seqs;
   // As many parts as fill the device once (three workgroups per CU; two of fp32
-  // with head_dim 128 and of prompts: a workgroup more runs a second round) if
+  // and fp16 with head_dim 128 and of prompts: a workgroup more runs a second round) if
   // the sequences have equal shares of the rows, of four pages at least, one per
   // wave (prompts: 8).
   const size_t each = (b->n_rows + b->n_seqs - 1) / b->n_seqs;
   const size_t wgs = b->n_seqs * ((each * group + p.rows - 1) / p.rows) * c->n_kv_heads;
-  const size_t room = p.rows > 16 || (type == LMX_F32 && c->head_dim == 128) ? 512 : 768;
+  const size_t room = p.rows > 16 || (type != LMX_BF16 && c->head_dim == 128) ? 512 : 768;
   const size_t s = std::min<size_t>(room / wgs, b->max_pages / (p.rows == 16 ? 4 : 8));
   p.splits = int(std::max<size_t>(1, std::min<size_t>(s, 64)));
   return p;
@@ -647,11 +648,13 @@ size_t workspace_bytes(const lmx_kv8_cache *c, const lmx_kv8_batch *b, size_t n_
 
 template <class T, int HD>
 int launch_attention(const AttnArgs &a, int type, const Plan &p, hipStream_t st) {
-  constexpr int ND = sizeof(T) == 4 ? 3 : 2;
+  // (weights of 14 bits below the largest are less than the rounding of bf16 where
+  // contexts are some 10 000 tokens long, but not than that of fp16)
+  constexpr int ND = sizeof(T) == 4 ? 3 : 2, PD = std::is_same<T, bf16>::value ? 2 : 3;
   const dim3 grid(unsigned(p.units), unsigned(a.c.n_kv), unsigned(a.splits));
   int r;
   if (p.rows == 16) {
-    kv8_rows_kernel<T, HD, ND><<<grid, dim3(256), 0, st>>>(a);
+    kv8_rows_kernel<T, HD, ND, PD><<<grid, dim3(256), 0, st>>>(a);
     r = launch_err("kv8 attention");
   } else {
     r = launch_prompt(a, type, HD, p.units, st);
