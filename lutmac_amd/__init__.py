@@ -7,7 +7,6 @@ shared library lutmac_amd/liblutmac_hip.so is built in-tree by
 nothing can silently fall back to a CPU path.
 """
 import ctypes
-import functools
 import os
 
 import numpy as np
@@ -227,32 +226,6 @@ def _stream_ptr(stream):
     return _current_stream() if stream is None else stream.cuda_stream
 
 
-_TYPES = None
-
-
-def _types():
-    global _TYPES
-    if _TYPES is None:
-        import torch
-        _TYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
-    return _TYPES
-
-
-_CURRENT_DEVICE = None
-
-
-def _current_device():
-    """Index of torch's current device, where the calls launch; -1 without a GPU."""
-    global _CURRENT_DEVICE
-    if _CURRENT_DEVICE is None:
-        import torch
-        if not torch.cuda.is_available():
-            return -1
-        torch.cuda.init()
-        _CURRENT_DEVICE = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
-    return _CURRENT_DEVICE()
-
-
 # ---- host-only helpers -----------------------------------------------------
 
 def blocks_to_planes(fmt, blocks, rows, cols):
@@ -461,52 +434,30 @@ class Weight:
             pass
 
 
+_TORCH = None
+
+
+def torch_module():
+    """The module of the operators on torch tensors (csrc/lmx_torch.cpp)."""
+    global _TORCH
+    if _TORCH is None:
+        lib()   # (loads torch and the library, which the module needs)
+        from . import _torch
+        _torch.set_error(LmxError)
+        _TORCH = _torch
+    return _TORCH
+
+
 def linear_i8(x, w, w_scale, bias=None, y=None, workspace=None, stream=None):
     """Linear layer in 8-bit integers (lmx_linear_i8): x [..., cols] fp32, fp16 or
     bf16, w [rows, cols] int8 whose rows start on multiples of 16 bytes (any row
     stride that is one), w_scale [rows] fp32, bias [rows] of x's type.  Returns
     [..., rows] of x's type.  workspace: a uint8 tensor of at least
     linear_i8_workspace bytes that no overlapping call uses (default: torch
-    allocates one for the call)."""
-    import torch
-    dtype = x.dtype
-    kind = _types().get(dtype)
-    if kind is None:
-        raise LmxError(ERR_UNSUPPORTED_FORMAT, f"x is {dtype}: float32, float16 or bfloat16")
-    if w.dim() != 2 or w.dtype is not torch.int8 or w.stride(1) != 1:
-        raise ValueError("w: int8 [rows, cols] with neighbouring columns side by side")
-    rows, cols = w.shape
-    if x.dim() == 0 or x.shape[-1] != cols or not x.is_contiguous():
-        raise ValueError(f"x {tuple(x.shape)}: contiguous, {cols} values a row")
-    if w_scale.dtype is not torch.float32 or w_scale.shape != (rows,) or not w_scale.is_contiguous():
-        raise ValueError(f"w_scale: contiguous float32 [{rows}]")
-    bp = None
-    if bias is not None:
-        if bias.dtype is not dtype or bias.shape != (rows,) or not bias.is_contiguous():
-            raise ValueError(f"bias: contiguous {dtype} [{rows}]")
-        bp = bias.data_ptr()
-    batch = x.numel() // cols if cols else 0
-    if y is None:
-        y = x.new_empty((batch, rows) if x.dim() == 2 else (*x.shape[:-1], rows))
-    elif y.dtype is not dtype or y.numel() != batch * rows or not y.is_contiguous():
-        raise ValueError(f"y: contiguous {dtype}, {batch} x {rows}")
-    if workspace is None:
-        size = linear_i8_workspace(rows, cols, batch)
-        workspace = torch.empty(size, dtype=torch.uint8, device=x.device)
-    else:
-        size = workspace.numel() * workspace.element_size()
-    here = _current_device()
-    for t in (x, w, w_scale, bias, y, workspace):
-        if t is not None and (t.get_device() != here or here < 0):
-            raise ValueError(f"expected tensors on the current device, got one on {t.device}")
-    # (the stride of a single row says nothing)
-    check(lib().lmx_linear_i8(w.data_ptr(), w.stride(0) if rows > 1 else -(-cols // 16) * 16, w_scale.data_ptr(), bp,
-                              x.data_ptr(), y.data_ptr(), kind, rows, cols, batch, workspace.data_ptr(), size,
-                              _stream_ptr(stream)))
-    return y
+    allocates one for the call, on its current stream)."""
+    return torch_module().linear_i8(x, w, w_scale, bias, y, workspace, stream)
 
 
-@functools.lru_cache(maxsize=1024)   # (of sizes alone)
 def linear_i8_workspace(rows, cols, batch):
     """Bytes of workspace of a linear_i8 call."""
     n = ctypes.c_size_t()

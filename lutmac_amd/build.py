@@ -1,4 +1,5 @@
-"""Build the in-tree HIP library (lutmac_amd/liblutmac_hip.so) for gfx950.
+"""Build the in-tree HIP library (lutmac_amd/liblutmac_hip.so) for gfx950, and
+the Python module over torch's tensors that calls it (lutmac_amd/_torch.so).
 
 Run as ``python -m lutmac_amd.build``.  Object files go to lutmac_amd/_build/
 (git-ignored); the shared library lands next to this file so it travels with
@@ -14,6 +15,7 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "liblutmac_hip.so")
+TORCH_LIB = os.path.join(HERE, "_torch.so")
 ARCH = os.environ.get("LMX_OFFLOAD_ARCH", "gfx950")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -51,6 +53,21 @@ def _run(cmd, verbose):
     subprocess.run(cmd, check=True)
 
 
+def torch_command():
+    """The compile of the Python module over torch's tensors (host code only; torch
+    itself is not imported, its libraries are found loaded when the module is)."""
+    import importlib.util
+    import sysconfig
+    torch = os.path.dirname(importlib.util.find_spec("torch").origin)
+    include = [sysconfig.get_paths()["include"], os.path.join(torch, "include"),
+               os.path.join(torch, "include", "torch", "csrc", "api", "include"), "/opt/rocm/include"]
+    libs = ["torch_python", "torch", "torch_cpu", "torch_hip", "c10", "c10_hip"]
+    return (["g++", "-O2", "-std=c++17", "-fPIC", "-Wall", "-shared", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+             "-I", os.path.join(ROOT, "include")] + [f for i in include for f in ("-isystem", i)] +
+            [os.path.join(CSRC, "lmx_torch.cpp"), "-o", TORCH_LIB, "-L", HERE, "-llutmac_hip", "-Wl,-rpath,$ORIGIN",
+             "-L", os.path.join(torch, "lib")] + [f"-l{l}" for l in libs])
+
+
 def build(verbose=True):
     """Compiles every translation unit (in parallel, one hipcc per file) and
     links the library."""
@@ -73,6 +90,7 @@ def build(verbose=True):
     tmp = LIB + ".tmp"
     _run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp] + objs, verbose)
     os.replace(tmp, LIB)
+    _run(torch_command(), verbose)
     # C++ drop-in check program (run by tests/test_gpu_compat.py)
     smoke = os.path.join(ROOT, "tests", "cpp", "compat_smoke")
     _run([HIPCC, "-O2", "-std=c++17", "-I", os.path.join(ROOT, "include"),

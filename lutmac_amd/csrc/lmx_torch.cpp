@@ -1,0 +1,349 @@
+// lmx_torch.cpp -- the 8-bit serving operators on torch tensors: what
+// lutmac_amd.kv8 and lutmac_amd.linear_i8 check of their arguments, the outputs
+// and workspaces that they allocate, and their calls into the C ABI.
+//
+// A serving loop calls them eagerly many times a step, and in Python the checks
+// of a call take longer than the kernels of a small one: an append of 64 rows
+// 12.4 us against 7.2, the attention of one row 11.1 against 6.0.
+#define PY_SSIZE_T_CLEAN
+#include <Python.h>
+
+#include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
+#include <c10/hip/HIPFunctions.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <cmath>
+#include <string>
+
+#include "lutmac_hip.h"
+#include "lutmac_kv8.h"
+
+namespace {
+
+struct PyError {};   // a Python exception is set
+
+PyObject *g_lmx_error = nullptr;   // lutmac_amd.LmxError
+
+[[noreturn]] void raise_lmx(int status, const std::string &message) {
+  PyObject *e = PyObject_CallFunction(g_lmx_error, "is", status, message.c_str());
+  if (e) {
+    PyErr_SetObject(g_lmx_error, e);
+    Py_DECREF(e);
+  }
+  throw PyError{};
+}
+void check(int status) {
+  if (status != LMX_OK) raise_lmx(status, lmx_last_error());
+}
+
+std::string text(const at::Tensor &t) {
+  std::string s = std::string(c10::toString(t.scalar_type())) + " [";
+  for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.size(i));
+  s += "] with strides (";
+  for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.stride(i));
+  return s + ") on " + t.device().str();
+}
+[[noreturn]] void raise_value(const std::string &message) {
+  PyErr_SetString(PyExc_ValueError, message.c_str());
+  throw PyError{};
+}
+[[noreturn]] void bad(const char *name, const at::Tensor &t, const std::string &want) {
+  raise_value(std::string(name) + ": " + text(t) + ", expected " + want);
+}
+
+const at::Tensor &tensor(const char *name, PyObject *o) {
+  if (!THPVariable_Check(o)) {
+    PyErr_Format(PyExc_TypeError, "%s: expected a tensor, got %s", name, Py_TYPE(o)->tp_name);
+    throw PyError{};
+  }
+  return THPVariable_Unpack(o);
+}
+
+int type_of(const char *name, const at::Tensor &t) {
+  switch (t.scalar_type()) {
+  case at::kFloat: return LMX_F32;
+  case at::kHalf: return LMX_F16;
+  case at::kBFloat16: return LMX_BF16;
+  default: raise_lmx(LMX_ERR_UNSUPPORTED_FORMAT, std::string(name) + " is " + c10::toString(t.scalar_type()) + ": float32, float16 or bfloat16");
+  }
+}
+
+bool has_sizes(const at::Tensor &t, at::IntArrayRef sizes) { return t.sizes().equals(sizes); }
+
+// Every tensor of a call lies on the current device, where it launches.
+void check_device(const at::Tensor &t, int device) {
+  if (t.get_device() != device) raise_value("expected tensors on one device, the current one, got one on " + t.device().str());
+}
+int current_device_of(const at::Tensor &t) {
+  const int device = t.is_cuda() ? int(t.get_device()) : -1;
+  if (device < 0 || device != int(c10::hip::current_device()))
+    raise_value("expected tensors on the current device, got one on " + t.device().str());
+  return device;
+}
+void *stream_of(PyObject *stream, int device) {
+  if (stream == Py_None) return c10::hip::getCurrentHIPStream(c10::DeviceIndex(device)).stream();
+  PyObject *raw = PyObject_GetAttrString(stream, "cuda_stream");
+  if (!raw) throw PyError{};
+  void *p = PyLong_AsVoidPtr(raw);
+  Py_DECREF(raw);
+  if (PyErr_Occurred()) throw PyError{};
+  return p;
+}
+
+// Runs f() -> new reference; C++ exceptions become Python's.
+template <class F>
+PyObject *guarded(F f) {
+  HANDLE_TH_ERRORS
+  try {
+    return f();
+  } catch (const PyError &) {
+    return nullptr;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
+bool arguments(const char *name, Py_ssize_t got, Py_ssize_t want) {
+  if (got != want) PyErr_Format(PyExc_TypeError, "%s: %zd arguments, expected %zd", name, got, want);
+  return got == want;
+}
+
+// ---- cache ----
+
+struct Cache {
+  lmx_kv8_cache c;
+  int device;
+};
+constexpr const char *kCache = "lutmac_amd.kv8_cache";
+const Cache &cache_of(PyObject *o) {
+  const Cache *c = static_cast<const Cache *>(PyCapsule_GetPointer(o, kCache));
+  if (!c) throw PyError{};
+  return *c;
+}
+
+// (k, v, k_scale, v_scale) -> the cache's sizes and pointers, checked; the
+// caller keeps the tensors.
+PyObject *kv8_cache(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject * {
+    if (!arguments("kv8_cache", n, 4)) throw PyError{};
+    const at::Tensor &k = tensor("k", args[0]), &v = tensor("v", args[1]);
+    if (k.dim() != 4 || k.size(2) != LMX_KV8_PAGE || (k.size(3) != 64 && k.size(3) != 128) || k.scalar_type() != at::kChar ||
+        !k.is_contiguous())
+      bad("k", k, "contiguous int8 [pages, kv_heads, 64, 64 or 128]");
+    const int64_t pages = k.size(0), heads = k.size(1), hd = k.size(3);
+    if (v.scalar_type() != at::kChar || !has_sizes(v, {pages, heads, hd, LMX_KV8_PAGE}) || !v.is_contiguous())
+      bad("v", v, "contiguous int8 [pages, kv_heads, head_dim, 64], as k has them");
+    float *scales[2];
+    const char *names[2] = {"k_scale", "v_scale"};
+    if (v.device() != k.device()) raise_value("the cache's tensors must be on one device");
+    for (int i = 0; i < 2; ++i) {
+      const at::Tensor &s = tensor(names[i], args[2 + i]);
+      if (s.scalar_type() != at::kFloat || !has_sizes(s, {pages, heads, LMX_KV8_PAGE / LMX_KV8_BLOCK}) || !s.is_contiguous())
+        bad(names[i], s, "contiguous float32 [pages, kv_heads, 4], as k has them");
+      if (s.device() != k.device()) raise_value("the cache's tensors must be on one device");
+      scales[i] = static_cast<float *>(s.data_ptr());
+    }
+    Cache *c = new Cache{{static_cast<int8_t *>(k.data_ptr()), static_cast<int8_t *>(v.data_ptr()), scales[0], scales[1],
+                          size_t(pages), size_t(heads), size_t(hd)},
+                         k.is_cuda() ? int(k.get_device()) : -1};
+    PyObject *o = PyCapsule_New(c, kCache, [](PyObject *o) { delete static_cast<Cache *>(PyCapsule_GetPointer(o, kCache)); });
+    if (!o) {
+      delete c;
+      throw PyError{};
+    }
+    return o;
+  });
+}
+
+// A row tensor [rows, heads, head_dim], rows any stride apart: its row stride.
+size_t row_stride(const char *name, const at::Tensor &t, at::ScalarType type, int64_t rows, int64_t heads, int64_t hd) {
+  if (t.scalar_type() != type || !has_sizes(t, {rows, heads, hd}))
+    bad(name, t, std::string(c10::toString(type)) + " [" + std::to_string(rows) + ", " + std::to_string(heads) + ", " +
+                     std::to_string(hd) + "]");
+  if (rows && (t.stride(2) != 1 || (heads > 1 && t.stride(1) != hd))) bad(name, t, "a row's heads side by side");
+  return size_t(rows > 1 ? t.stride(0) : heads * hd);   // (a single row's stride says nothing)
+}
+
+// The call's batch; its tensors lie on the cache's device, which is the current one.
+lmx_kv8_batch batch_of(const Cache &c, PyObject *const *args, int64_t rows) {
+  const at::Tensor &offsets = tensor("offsets", args[0]), &lengths = tensor("lengths", args[1]), &pages = tensor("pages", args[2]);
+  if (pages.scalar_type() != at::kInt || pages.dim() != 2 || !pages.is_contiguous()) bad("pages", pages, "contiguous int32 of 2 dimensions");
+  const int64_t n = pages.size(0);
+  if (offsets.scalar_type() != at::kInt || !has_sizes(offsets, {n + 1}) || !offsets.is_contiguous())
+    bad("offsets", offsets, "contiguous int32 [" + std::to_string(n + 1) + "] beside " + std::to_string(n) + " page table rows");
+  if (lengths.scalar_type() != at::kInt || !has_sizes(lengths, {n}) || !lengths.is_contiguous())
+    bad("lengths", lengths, "contiguous int32 [" + std::to_string(n) + "] beside " + std::to_string(n) + " page table rows");
+  if (c.device < 0) raise_value("expected tensors on the current device, the cache is on the CPU");
+  for (const at::Tensor *t : {&offsets, &lengths, &pages}) check_device(*t, c.device);
+  if (current_device_of(pages) != c.device) raise_value("expected tensors on the cache's device");
+  return {static_cast<const int32_t *>(offsets.data_ptr()), static_cast<const int32_t *>(lengths.data_ptr()),
+          static_cast<const int32_t *>(pages.data_ptr()), size_t(n), size_t(pages.size(1)), size_t(rows)};
+}
+
+// (cache, k, v, offsets, lengths, pages, rope, q, q_out, stream) -> q_out
+PyObject *kv8_append(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject * {
+    if (!arguments("kv8_append", n, 10)) throw PyError{};
+    const Cache &c = cache_of(args[0]);
+    const at::Tensor &k = tensor("k", args[1]), &v = tensor("v", args[2]);
+    const int type = type_of("k", k);
+    const at::ScalarType st = k.scalar_type();
+    const int64_t kv = int64_t(c.c.n_kv_heads), hd = int64_t(c.c.head_dim), rows = k.dim() ? k.size(0) : 0;
+    const size_t ks = row_stride("k", k, st, rows, kv, hd), vs = row_stride("v", v, st, rows, kv, hd);
+    const lmx_kv8_batch b = batch_of(c, args + 3, rows);
+    check_device(k, c.device);
+    check_device(v, c.device);
+    const float *rope = nullptr;
+    int64_t positions = 0;
+    if (args[6] != Py_None) {
+      const at::Tensor &r = tensor("rope", args[6]);
+      positions = r.dim() ? r.size(0) : 0;
+      if (r.scalar_type() != at::kFloat || !has_sizes(r, {positions, hd / 2, 2}) || !r.is_contiguous())
+        bad("rope", r, "contiguous float32 [positions, " + std::to_string(hd / 2) + ", 2]");
+      check_device(r, c.device);
+      rope = static_cast<const float *>(r.data_ptr());
+    }
+    const void *qp = nullptr;
+    at::Tensor out;
+    int64_t heads = 0;
+    size_t qs = 0, os = 0;
+    if (args[7] != Py_None) {
+      const at::Tensor &q = tensor("q", args[7]);
+      heads = q.dim() == 3 ? q.size(1) : 0;
+      qs = row_stride("q", q, st, rows, heads, hd);
+      check_device(q, c.device);
+      if (args[8] == Py_None) {
+        out = at::empty({rows, heads, hd}, q.options());
+      } else {
+        out = tensor("q_out", args[8]);
+        check_device(out, c.device);
+      }
+      os = row_stride("q_out", out, st, rows, heads, hd);
+      qp = q.data_ptr();
+    } else if (args[8] != Py_None) {
+      raise_value("q_out without q");
+    }
+    check(lmx_kv8_append(&c.c, &b, type, k.data_ptr(), ks, v.data_ptr(), vs, qp, qs, qp ? out.data_ptr() : nullptr, os, size_t(heads),
+                         rope, size_t(positions), stream_of(args[9], c.device)));
+    if (!out.defined()) Py_RETURN_NONE;
+    if (args[8] != Py_None) return Py_NewRef(args[8]);
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
+// Workspace of a call: the caller's, or one that torch allocates (for the
+// current stream, as its empty() does).
+at::Tensor workspace_of(PyObject *given, size_t need, int device, void *&p, size_t &bytes) {
+  at::Tensor t;
+  p = nullptr;
+  if (given != Py_None) {
+    t = tensor("workspace", given);
+    check_device(t, device);
+    if (!t.is_contiguous()) bad("workspace", t, "a contiguous tensor");
+    bytes = t.nbytes();
+  } else {
+    bytes = need;
+    if (!need) return t;
+    t = at::empty({int64_t(need)}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, c10::DeviceIndex(device)));
+  }
+  p = t.data_ptr();
+  return t;
+}
+
+// (cache, q, offsets, lengths, pages, scale, out, workspace, stream) -> out
+PyObject *kv8_attend(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject * {
+    if (!arguments("kv8_attend", n, 9)) throw PyError{};
+    const Cache &c = cache_of(args[0]);
+    const at::Tensor &q = tensor("q", args[1]);
+    const int type = type_of("q", q);
+    const int64_t hd = int64_t(c.c.head_dim), rows = q.dim() == 3 ? q.size(0) : 0, heads = q.dim() == 3 ? q.size(1) : 0;
+    const size_t qs = row_stride("q", q, q.scalar_type(), rows, heads, hd);
+    const lmx_kv8_batch b = batch_of(c, args + 2, rows);
+    check_device(q, c.device);
+    double scale = 1.0 / std::sqrt(double(hd));
+    if (args[5] != Py_None && (scale = PyFloat_AsDouble(args[5])) == -1.0 && PyErr_Occurred()) throw PyError{};
+    at::Tensor out;
+    if (args[6] == Py_None) {
+      out = at::empty({rows, heads, hd}, q.options());
+    } else {
+      out = tensor("out", args[6]);
+      check_device(out, c.device);
+    }
+    const size_t os = row_stride("out", out, q.scalar_type(), rows, heads, hd);
+    size_t need = 0, bytes = 0;
+    check(lmx_kv8_attention_workspace(&c.c, &b, type, size_t(heads), &need));
+    void *work;
+    const at::Tensor w = workspace_of(args[7], need, c.device, work, bytes);
+    check(lmx_kv8_attention(&c.c, &b, type, q.data_ptr(), qs, size_t(heads), float(scale), out.data_ptr(), os, work, bytes,
+                            stream_of(args[8], c.device)));
+    if (args[6] != Py_None) return Py_NewRef(args[6]);
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
+// (x, w, w_scale, bias, y, workspace, stream) -> y
+PyObject *linear_i8(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject * {
+    if (!arguments("linear_i8", n, 7)) throw PyError{};
+    const at::Tensor &x = tensor("x", args[0]), &w = tensor("w", args[1]), &scale = tensor("w_scale", args[2]);
+    const int type = type_of("x", x);
+    if (w.dim() != 2 || w.scalar_type() != at::kChar || w.stride(1) != 1) bad("w", w, "int8 [rows, cols] with neighbouring columns side by side");
+    const int64_t rows = w.size(0), cols = w.size(1);
+    if (x.dim() == 0 || x.size(-1) != cols || !x.is_contiguous()) bad("x", x, "contiguous, " + std::to_string(cols) + " values a row");
+    if (scale.scalar_type() != at::kFloat || !has_sizes(scale, {rows}) || !scale.is_contiguous())
+      bad("w_scale", scale, "contiguous float32 [" + std::to_string(rows) + "]");
+    const int device = current_device_of(x);
+    check_device(w, device);
+    check_device(scale, device);
+    const void *bias = nullptr;
+    if (args[3] != Py_None) {
+      const at::Tensor &b = tensor("bias", args[3]);
+      if (b.scalar_type() != x.scalar_type() || !has_sizes(b, {rows}) || !b.is_contiguous())
+        bad("bias", b, std::string("contiguous ") + c10::toString(x.scalar_type()) + " [" + std::to_string(rows) + "]");
+      check_device(b, device);
+      bias = b.data_ptr();
+    }
+    const int64_t batch = cols ? x.numel() / cols : 0;
+    size_t need = 0, bytes = 0;
+    check(lmx_linear_i8_workspace(size_t(rows), size_t(cols), size_t(batch), &need));
+    at::Tensor y;
+    if (args[4] == Py_None) {
+      auto sizes = x.sizes().vec();
+      sizes.back() = rows;
+      y = at::empty(sizes, x.options());
+    } else {
+      y = tensor("y", args[4]);
+      if (y.scalar_type() != x.scalar_type() || y.numel() != batch * rows || !y.is_contiguous())
+        bad("y", y, "contiguous, of x's type, " + std::to_string(batch) + " x " + std::to_string(rows));
+      check_device(y, device);
+    }
+    void *work;
+    const at::Tensor ws = workspace_of(args[5], need, device, work, bytes);
+    // (the stride of a single row says nothing)
+    check(lmx_linear_i8(static_cast<const int8_t *>(w.data_ptr()), size_t(rows > 1 ? w.stride(0) : (cols + 15) / 16 * 16),
+                        static_cast<const float *>(scale.data_ptr()), bias, x.data_ptr(), y.data_ptr(), type, size_t(rows),
+                        size_t(cols), size_t(batch), work, bytes, stream_of(args[6], device)));
+    if (args[4] != Py_None) return Py_NewRef(args[4]);
+    return THPVariable_Wrap(std::move(y));
+  });
+}
+
+// (LmxError): set once by the package.
+PyObject *set_error(PyObject *, PyObject *o) {
+  Py_XDECREF(g_lmx_error);
+  g_lmx_error = Py_NewRef(o);
+  Py_RETURN_NONE;
+}
+
+#define LMX_FAST(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
+PyMethodDef g_methods[] = {LMX_FAST(kv8_cache), LMX_FAST(kv8_append), LMX_FAST(kv8_attend), LMX_FAST(linear_i8),
+                           {"set_error", set_error, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
+PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_torch", "The 8-bit serving operators on torch tensors.", -1, g_methods,
+                        nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__torch() { return PyModule_Create(&g_module); }
