@@ -32,12 +32,10 @@ struct AppendArgs {
 };
 constexpr int kHeads = 8;
 
-// The pairs (d0 + i, d0 + i + HD / 2) of a row, rotated.
-template <int E, class T, int HD, class F>
-__device__ __forceinline__ void rotated(const T *row, const float2 *rope, int pos, int d0, F (&x)[E], F (&y)[E]) {
-  float a[E], b[E];
-  load_floats<E>(row + d0, a);
-  load_floats<E>(row + d0 + HD / 2, b);
+// The pairs (a[i], b[i]) of elements d0 + i and d0 + i + HD / 2, rotated.
+template <int E, int HD, class F>
+__device__ __forceinline__ void turned(const float (&a)[E], const float (&b)[E], const float2 *rope, int pos, int d0, F (&x)[E],
+                                       F (&y)[E]) {
   if (rope) {
     const float2 *t = rope + size_t(pos) * (HD / 2) + d0;
 #pragma unroll
@@ -50,6 +48,13 @@ __device__ __forceinline__ void rotated(const T *row, const float2 *rope, int po
 #pragma unroll
     for (int i = 0; i < E; ++i) x[i] = a[i], y[i] = b[i];
   }
+}
+template <int E, class T, int HD, class F>
+__device__ __forceinline__ void rotated(const T *row, const float2 *rope, int pos, int d0, F (&x)[E], F (&y)[E]) {
+  float a[E], b[E];
+  load_floats<E>(row + d0, a);
+  load_floats<E>(row + d0 + HD / 2, b);
+  turned<E, HD>(a, b, rope, pos, d0, x, y);
 }
 
 // Element d (of the pair d, d + HD / 2: h) of a row, rotated, in 64 bits.
@@ -107,27 +112,42 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
   if (role >= 2 * n_kv) {   // query heads: 8 lanes a row and head
     constexpr int QE = 8, QL = HD / 2 / QE, SLOTS = 256 / QL;
     const int h0 = (role - 2 * n_kv) * kHeads, heads = min(kHeads, a.c.n_heads - h0);
-    const int first = max(from, t0), tokens = min(end, t0 + kPage) - first;
-    int tp = 1;   // tokens side by side, a power of two
-    while (tp < tokens && tp < SLOTS) tp *= 2;
+    const int first = max(from, t0), items = (min(end, t0 + kPage) - first) * heads;
     const int slot = int(threadIdx.x) / QL, d0 = int(threadIdx.x) % QL * QE;
-    for (int t = slot % tp; t < tokens; t += tp) {
-      const int pos = first + t;
-      const size_t row = size_t(r.r0 + (pos - r.start));
-      const T *q = static_cast<const T *>(a.q) + row * a.q_stride + size_t(h0) * HD;
-      T *out = static_cast<T *>(a.q_out) + row * a.q_out_stride + size_t(h0) * HD;
-      for (int h = slot / tp; h < heads; h += SLOTS / tp) {
-        float f[QE], g[QE];
+    const int inverse = 65536 / heads + 1;   // (item / heads, exactly for the up to 512)
+    constexpr int U = sizeof(T) == 4 ? 1 : 4;   // rows of a lane on their way
+    for (int n = slot; n < items; n += U * SLOTS) {
+      float f[U][QE], g[U][QE];
+      const T *q[U];
+      size_t to[U];
+      int pos[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int item = min(n + u * SLOTS, items - 1), t = item * inverse >> 16, h = h0 + item - t * heads;
+        pos[u] = first + t;
+        const size_t row = size_t(r.r0 + (pos[u] - r.start));
+        q[u] = static_cast<const T *>(a.q) + row * a.q_stride + size_t(h) * HD;
+        to[u] = row * a.q_out_stride + size_t(h) * HD + d0;
+        load_floats<QE>(q[u] + d0, f[u]);
+        load_floats<QE>(q[u] + d0 + HD / 2, g[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (n + u * SLOTS >= items) break;
         if constexpr (sizeof(T) == 4) {
           double x[QE], y[QE];
-          rotated<QE, T, HD>(q + h * HD, a.rope, pos, d0, x, y);
+          turned<QE, HD>(f[u], g[u], a.rope, pos[u], d0, x, y);
 #pragma unroll
-          for (int i = 0; i < QE; ++i) f[i] = float(x[i]), g[i] = float(y[i]);
+          for (int i = 0; i < QE; ++i) f[u][i] = float(x[i]), g[u][i] = float(y[i]);
         } else {   // (rounded to 16 bits: fp32 leaves at most 2^-22 of the pair's larger)
-          rotated<QE, T, HD>(q + h * HD, a.rope, pos, d0, f, g);
+          float x[QE], y[QE];
+          turned<QE, HD>(f[u], g[u], a.rope, pos[u], d0, x, y);
+#pragma unroll
+          for (int i = 0; i < QE; ++i) f[u][i] = x[i], g[u][i] = y[i];
         }
-        store_floats<QE>(out + h * HD + d0, f);
-        store_floats<QE>(out + h * HD + d0 + HD / 2, g);
+        T *out = static_cast<T *>(a.q_out) + to[u];
+        store_floats<QE>(out, f[u]);
+        store_floats<QE>(out + HD / 2, g[u]);
       }
     }
     return;
