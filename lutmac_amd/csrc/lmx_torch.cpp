@@ -16,6 +16,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
+#include <initializer_list>
 #include <string>
 
 #include "lutmac_hip.h"
@@ -73,14 +74,18 @@ int type_of(const char *name, const at::Tensor &t) {
 
 bool has_sizes(const at::Tensor &t, at::IntArrayRef sizes) { return t.sizes().equals(sizes); }
 
-// Every tensor of a call lies on the current device, where it launches.
+// Every tensor of a call lies on one device, the current one, where it launches.
 void check_device(const at::Tensor &t, int device) {
-  if (t.get_device() != device) raise_value("expected tensors on one device, the current one, got one on " + t.device().str());
-}
-int current_device_of(const at::Tensor &t) {
-  const int device = t.is_cuda() ? int(t.get_device()) : -1;
-  if (device < 0 || device != int(c10::hip::current_device()))
+  if (!t.is_cuda() || t.get_device() != device)
     raise_value("expected tensors on the current device, got one on " + t.device().str());
+}
+int check_devices(std::initializer_list<const at::Tensor *> tensors) {   // (null: an argument left out)
+  const at::Tensor &first = **tensors.begin();
+  const int device = first.is_cuda() ? int(first.get_device()) : -1;
+  for (const at::Tensor *t : tensors)
+    if (t) check_device(*t, device);
+  if (device != int(c10::hip::current_device()))
+    raise_value("expected tensors on the current device, got " + first.device().str());
   return device;
 }
 void *stream_of(PyObject *stream, int device) {
@@ -166,7 +171,7 @@ size_t row_stride(const char *name, const at::Tensor &t, at::ScalarType type, in
   return size_t(rows > 1 ? t.stride(0) : heads * hd);   // (a single row's stride says nothing)
 }
 
-// The call's batch; its tensors lie on the cache's device, which is the current one.
+// The call's batch, but for its tensors' device.
 lmx_kv8_batch batch_of(const Cache &c, PyObject *const *args, int64_t rows) {
   const at::Tensor &offsets = tensor("offsets", args[0]), &lengths = tensor("lengths", args[1]), &pages = tensor("pages", args[2]);
   if (pages.scalar_type() != at::kInt || pages.dim() != 2 || !pages.is_contiguous()) bad("pages", pages, "contiguous int32 of 2 dimensions");
@@ -175,11 +180,14 @@ lmx_kv8_batch batch_of(const Cache &c, PyObject *const *args, int64_t rows) {
     bad("offsets", offsets, "contiguous int32 [" + std::to_string(n + 1) + "] beside " + std::to_string(n) + " page table rows");
   if (lengths.scalar_type() != at::kInt || !has_sizes(lengths, {n}) || !lengths.is_contiguous())
     bad("lengths", lengths, "contiguous int32 [" + std::to_string(n) + "] beside " + std::to_string(n) + " page table rows");
-  if (c.device < 0) raise_value("expected tensors on the current device, the cache is on the CPU");
-  for (const at::Tensor *t : {&offsets, &lengths, &pages}) check_device(*t, c.device);
-  if (current_device_of(pages) != c.device) raise_value("expected tensors on the cache's device");
   return {static_cast<const int32_t *>(offsets.data_ptr()), static_cast<const int32_t *>(lengths.data_ptr()),
           static_cast<const int32_t *>(pages.data_ptr()), size_t(n), size_t(pages.size(1)), size_t(rows)};
+}
+
+int check_call(const Cache &c, std::initializer_list<const at::Tensor *> tensors) {
+  const int device = check_devices(tensors);
+  if (device != c.device) raise_value("expected tensors on the cache's device");
+  return device;
 }
 
 // (cache, k, v, offsets, lengths, pages, rope, q, q_out, stream) -> q_out
@@ -193,40 +201,22 @@ PyObject *kv8_append(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const int64_t kv = int64_t(c.c.n_kv_heads), hd = int64_t(c.c.head_dim), rows = k.dim() ? k.size(0) : 0;
     const size_t ks = row_stride("k", k, st, rows, kv, hd), vs = row_stride("v", v, st, rows, kv, hd);
     const lmx_kv8_batch b = batch_of(c, args + 3, rows);
-    check_device(k, c.device);
-    check_device(v, c.device);
-    const float *rope = nullptr;
-    int64_t positions = 0;
-    if (args[6] != Py_None) {
-      const at::Tensor &r = tensor("rope", args[6]);
-      positions = r.dim() ? r.size(0) : 0;
-      if (r.scalar_type() != at::kFloat || !has_sizes(r, {positions, hd / 2, 2}) || !r.is_contiguous())
-        bad("rope", r, "contiguous float32 [positions, " + std::to_string(hd / 2) + ", 2]");
-      check_device(r, c.device);
-      rope = static_cast<const float *>(r.data_ptr());
-    }
-    const void *qp = nullptr;
+    const at::Tensor *rope = args[6] != Py_None ? &tensor("rope", args[6]) : nullptr;
+    const int64_t positions = rope && rope->dim() ? rope->size(0) : 0;
+    if (rope && (rope->scalar_type() != at::kFloat || !has_sizes(*rope, {positions, hd / 2, 2}) || !rope->is_contiguous()))
+      bad("rope", *rope, "contiguous float32 [positions, " + std::to_string(hd / 2) + ", 2]");
+    const at::Tensor *q = args[7] != Py_None ? &tensor("q", args[7]) : nullptr;
+    const at::Tensor *given = args[8] != Py_None ? &tensor("q_out", args[8]) : nullptr;
+    if (given && !q) raise_value("q_out without q");
+    const int64_t heads = q && q->dim() == 3 ? q->size(1) : 0;
+    const size_t qs = q ? row_stride("q", *q, st, rows, heads, hd) : 0;
+    const size_t os = given ? row_stride("q_out", *given, st, rows, heads, hd) : size_t(heads * hd);
+    const int device = check_call(c, {&k, &v, &THPVariable_Unpack(args[3]), &THPVariable_Unpack(args[4]), &THPVariable_Unpack(args[5]), rope, q, given});
     at::Tensor out;
-    int64_t heads = 0;
-    size_t qs = 0, os = 0;
-    if (args[7] != Py_None) {
-      const at::Tensor &q = tensor("q", args[7]);
-      heads = q.dim() == 3 ? q.size(1) : 0;
-      qs = row_stride("q", q, st, rows, heads, hd);
-      check_device(q, c.device);
-      if (args[8] == Py_None) {
-        out = at::empty({rows, heads, hd}, q.options());
-      } else {
-        out = tensor("q_out", args[8]);
-        check_device(out, c.device);
-      }
-      os = row_stride("q_out", out, st, rows, heads, hd);
-      qp = q.data_ptr();
-    } else if (args[8] != Py_None) {
-      raise_value("q_out without q");
-    }
-    check(lmx_kv8_append(&c.c, &b, type, k.data_ptr(), ks, v.data_ptr(), vs, qp, qs, qp ? out.data_ptr() : nullptr, os, size_t(heads),
-                         rope, size_t(positions), stream_of(args[9], c.device)));
+    if (q) out = given ? *given : at::empty({rows, heads, hd}, q->options());
+    check(lmx_kv8_append(&c.c, &b, type, k.data_ptr(), ks, v.data_ptr(), vs, q ? q->data_ptr() : nullptr, qs,
+                         q ? out.data_ptr() : nullptr, os, size_t(heads), rope ? static_cast<const float *>(rope->data_ptr()) : nullptr,
+                         size_t(positions), stream_of(args[9], device)));
     if (!out.defined()) Py_RETURN_NONE;
     if (args[8] != Py_None) return Py_NewRef(args[8]);
     return THPVariable_Wrap(std::move(out));
@@ -262,23 +252,18 @@ PyObject *kv8_attend(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const int64_t hd = int64_t(c.c.head_dim), rows = q.dim() == 3 ? q.size(0) : 0, heads = q.dim() == 3 ? q.size(1) : 0;
     const size_t qs = row_stride("q", q, q.scalar_type(), rows, heads, hd);
     const lmx_kv8_batch b = batch_of(c, args + 2, rows);
-    check_device(q, c.device);
     double scale = 1.0 / std::sqrt(double(hd));
     if (args[5] != Py_None && (scale = PyFloat_AsDouble(args[5])) == -1.0 && PyErr_Occurred()) throw PyError{};
-    at::Tensor out;
-    if (args[6] == Py_None) {
-      out = at::empty({rows, heads, hd}, q.options());
-    } else {
-      out = tensor("out", args[6]);
-      check_device(out, c.device);
-    }
-    const size_t os = row_stride("out", out, q.scalar_type(), rows, heads, hd);
+    const at::Tensor *given = args[6] != Py_None ? &tensor("out", args[6]) : nullptr;
+    const size_t os = given ? row_stride("out", *given, q.scalar_type(), rows, heads, hd) : size_t(heads * hd);
+    const int device = check_call(c, {&q, &THPVariable_Unpack(args[2]), &THPVariable_Unpack(args[3]), &THPVariable_Unpack(args[4]), given});
+    at::Tensor out = given ? *given : at::empty({rows, heads, hd}, q.options());
     size_t need = 0, bytes = 0;
     check(lmx_kv8_attention_workspace(&c.c, &b, type, size_t(heads), &need));
     void *work;
-    const at::Tensor w = workspace_of(args[7], need, c.device, work, bytes);
+    const at::Tensor w = workspace_of(args[7], need, device, work, bytes);
     check(lmx_kv8_attention(&c.c, &b, type, q.data_ptr(), qs, size_t(heads), float(scale), out.data_ptr(), os, work, bytes,
-                            stream_of(args[8], c.device)));
+                            stream_of(args[8], device)));
     if (args[6] != Py_None) return Py_NewRef(args[6]);
     return THPVariable_Wrap(std::move(out));
   });
@@ -295,36 +280,29 @@ PyObject *linear_i8(PyObject *, PyObject *const *args, Py_ssize_t n) {
     if (x.dim() == 0 || x.size(-1) != cols || !x.is_contiguous()) bad("x", x, "contiguous, " + std::to_string(cols) + " values a row");
     if (scale.scalar_type() != at::kFloat || !has_sizes(scale, {rows}) || !scale.is_contiguous())
       bad("w_scale", scale, "contiguous float32 [" + std::to_string(rows) + "]");
-    const int device = current_device_of(x);
-    check_device(w, device);
-    check_device(scale, device);
-    const void *bias = nullptr;
-    if (args[3] != Py_None) {
-      const at::Tensor &b = tensor("bias", args[3]);
-      if (b.scalar_type() != x.scalar_type() || !has_sizes(b, {rows}) || !b.is_contiguous())
-        bad("bias", b, std::string("contiguous ") + c10::toString(x.scalar_type()) + " [" + std::to_string(rows) + "]");
-      check_device(b, device);
-      bias = b.data_ptr();
-    }
+    const at::Tensor *bias = args[3] != Py_None ? &tensor("bias", args[3]) : nullptr;
+    if (bias && (bias->scalar_type() != x.scalar_type() || !has_sizes(*bias, {rows}) || !bias->is_contiguous()))
+      bad("bias", *bias, std::string("contiguous ") + c10::toString(x.scalar_type()) + " [" + std::to_string(rows) + "]");
     const int64_t batch = cols ? x.numel() / cols : 0;
+    const at::Tensor *given = args[4] != Py_None ? &tensor("y", args[4]) : nullptr;
+    if (given && (given->scalar_type() != x.scalar_type() || given->numel() != batch * rows || !given->is_contiguous()))
+      bad("y", *given, "contiguous, of x's type, " + std::to_string(batch) + " x " + std::to_string(rows));
+    const int device = check_devices({&x, &w, &scale, bias, given});
     size_t need = 0, bytes = 0;
     check(lmx_linear_i8_workspace(size_t(rows), size_t(cols), size_t(batch), &need));
     at::Tensor y;
-    if (args[4] == Py_None) {
+    if (given) {
+      y = *given;
+    } else {
       auto sizes = x.sizes().vec();
       sizes.back() = rows;
       y = at::empty(sizes, x.options());
-    } else {
-      y = tensor("y", args[4]);
-      if (y.scalar_type() != x.scalar_type() || y.numel() != batch * rows || !y.is_contiguous())
-        bad("y", y, "contiguous, of x's type, " + std::to_string(batch) + " x " + std::to_string(rows));
-      check_device(y, device);
     }
     void *work;
     const at::Tensor ws = workspace_of(args[5], need, device, work, bytes);
     // (the stride of a single row says nothing)
     check(lmx_linear_i8(static_cast<const int8_t *>(w.data_ptr()), size_t(rows > 1 ? w.stride(0) : (cols + 15) / 16 * 16),
-                        static_cast<const float *>(scale.data_ptr()), bias, x.data_ptr(), y.data_ptr(), type, size_t(rows),
+                        static_cast<const float *>(scale.data_ptr()), bias ? bias->data_ptr() : nullptr, x.data_ptr(), y.data_ptr(), type, size_t(rows),
                         size_t(cols), size_t(batch), work, bytes, stream_of(args[6], device)));
     if (args[4] != Py_None) return Py_NewRef(args[4]);
     return THPVariable_Wrap(std::move(y));

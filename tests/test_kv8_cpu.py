@@ -121,16 +121,25 @@ def test_python_checks():
     k = z(3, 1, 64, dtype=f)
     i32 = lambda *s: z(*s, dtype=torch.int32)
     ok = dict(offsets=i32(2), lengths=i32(1), pages=i32(1, 2))
-    for bad in [dict(offsets=i32(3)), dict(lengths=z(1, dtype=torch.int64)), dict(pages=i32(2, 2)), dict(pages=i32(2, 1).t()[:, ::2]),
+    for bad in [dict(offsets=i32(3)), dict(lengths=z(1, dtype=torch.int64)), dict(pages=i32(2, 2)), dict(pages=i32(1, 4)[:, ::2]),
                 dict(offsets=i32(4)[::2])]:
-        with pytest.raises(ValueError):
+        with pytest.raises(ValueError, match="offsets:|lengths:|pages:"):
             c.append(k, k, **{**ok, **bad})
-        with pytest.raises(ValueError):
+        with pytest.raises(ValueError, match="offsets:|lengths:|pages:"):
             c.attend(k, **{**ok, **bad})
     for bad in [dict(v=z(2, 1, 64, dtype=f)), dict(v=k.half()), dict(k=z(3, 2, 64, dtype=f)), dict(q=z(3, 2, 32, dtype=f)),
                 dict(q_out=k), dict(rope=z(5, 32, dtype=f)), dict(q=z(3, 64, 2, dtype=f).transpose(1, 2))]:
-        with pytest.raises(ValueError):
+        with pytest.raises(ValueError, match="^(k|v|q|rope): |^q_out without q"):
             c.append(**{**dict(k=k, v=k), **bad}, **ok)
+    with pytest.raises(ValueError, match="^q_out: "):
+        c.append(k, k, q=k, q_out=k[:2], **ok)
+    with pytest.raises(ValueError, match="^out: "):
+        c.attend(k, out=k.half(), **ok)
+    for bad in [lambda: c.append(k, k, **ok), lambda: c.append(k, k, q=k, rope=z(5, 32, 2, dtype=f), **ok), lambda: c.attend(k, **ok)]:
+        with pytest.raises(ValueError, match="current device"):   # (all is well but for the device)
+            bad()
+    with pytest.raises(TypeError, match="expected a tensor"):
+        c.attend(k.numpy(), **ok)
     with pytest.raises(L.LmxError):
         c.append(k.double(), k.double(), **ok)
     with pytest.raises(L.LmxError):
@@ -138,8 +147,10 @@ def test_python_checks():
     x, w, s = z(2, 20, dtype=f), z(5, 32)[:, :20], z(5, dtype=f)
     for bad in [dict(x=x[:, :19]), dict(x=x.t()), dict(w=w.float()), dict(w=z(20, 5).t()), dict(w_scale=s[:4]), dict(bias=s.half()),
                 dict(y=z(2, 4, dtype=f))]:
-        with pytest.raises(ValueError):
+        with pytest.raises(ValueError, match=f"^{next(iter(bad))}: "):
             L.linear_i8(**{**dict(x=x, w=w, w_scale=s), **bad})
+    with pytest.raises(ValueError, match="current device"):
+        L.linear_i8(x, w, s)
     with pytest.raises(L.LmxError):
         L.linear_i8(x.double(), w, s)
 
