@@ -78,7 +78,7 @@ typedef struct {
  * from 64 bits (fp32) or from fp32 (16-bit types).  Where a value is not finite the block's
  * scale becomes NaN (as does the attention of every row that sees the block)
  * until the block starts anew.  Blocks are read and written by one workgroup
- * each: two sequences of one call must not append to the same page. */
+ * each: the pages that receive rows in one call differ from each other. */
 int lmx_kv8_append(const lmx_kv8_cache *cache, const lmx_kv8_batch *batch,
                    int type, const void *k, size_t k_stride, const void *v,
                    size_t v_stride, const void *q, size_t q_stride, void *q_out,

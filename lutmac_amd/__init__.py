@@ -448,14 +448,24 @@ def torch_module():
     return _TORCH
 
 
+def on_stream(stream, f, *args):
+    """f(*args) on torch's current stream or, if one is given, with that as the
+    current one: the call's work, and the memory of what it allocates."""
+    if stream is None:
+        return f(*args)
+    import torch
+    with torch.cuda.stream(stream):
+        return f(*args)
+
+
 def linear_i8(x, w, w_scale, bias=None, y=None, workspace=None, stream=None):
     """Linear layer in 8-bit integers (lmx_linear_i8): x [..., cols] fp32, fp16 or
     bf16, w [rows, cols] int8 whose rows start on multiples of 16 bytes (any row
     stride that is one), w_scale [rows] fp32, bias [rows] of x's type.  Returns
     [..., rows] of x's type.  workspace: a uint8 tensor of at least
     linear_i8_workspace bytes that no overlapping call uses (default: torch
-    allocates one for the call, on its current stream)."""
-    return torch_module().linear_i8(x, w, w_scale, bias, y, workspace, stream)
+    allocates one for the call)."""
+    return on_stream(stream, torch_module().linear_i8, x, w, w_scale, bias, y, workspace)
 
 
 def linear_i8_workspace(rows, cols, batch):

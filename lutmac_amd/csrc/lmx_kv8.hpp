@@ -50,6 +50,7 @@ __device__ __forceinline__ SeqRows unit_rows(const Kv8Args &a, int u, int mul, i
       const auto pick = [c](int v) { return __builtin_amdgcn_readlane(v, c - 1); };
       r.seq = lo + c - 1;
       r.first = pick(begin);
+      if (r.first > u) r.seq = -1;   // (offsets that decrease)
       r.r0 = pick(o0);
       r.n = max(pick(o1), r.r0) - r.r0;
       r.len = max(pick(len), 0);

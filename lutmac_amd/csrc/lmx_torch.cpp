@@ -89,15 +89,8 @@ int check_devices(std::initializer_list<const at::Tensor *> tensors) {   // (nul
     raise_value("expected tensors on the current device, got " + first.device().str());
   return device;
 }
-void *stream_of(PyObject *stream, int device) {
-  if (stream == Py_None) return c10::hip::getCurrentHIPStream(c10::DeviceIndex(device)).stream();
-  PyObject *raw = PyObject_GetAttrString(stream, "cuda_stream");
-  if (!raw) throw PyError{};
-  void *p = PyLong_AsVoidPtr(raw);
-  Py_DECREF(raw);
-  if (PyErr_Occurred()) throw PyError{};
-  return p;
-}
+// Work runs on torch's current stream, whose memory new outputs and workspaces are.
+void *stream_on(int device) { return c10::hip::getCurrentHIPStream(c10::DeviceIndex(device)).stream(); }
 
 // Runs f() -> new reference; C++ exceptions become Python's.
 template <class F>
@@ -191,10 +184,10 @@ int check_call(const Cache &c, std::initializer_list<const at::Tensor *> tensors
   return device;
 }
 
-// (cache, k, v, offsets, lengths, pages, rope, q, q_out, stream) -> q_out
+// (cache, k, v, offsets, lengths, pages, rope, q, q_out) -> q_out
 PyObject *kv8_append(PyObject *, PyObject *const *args, Py_ssize_t n) {
   return guarded([&]() -> PyObject * {
-    if (!arguments("kv8_append", n, 10)) throw PyError{};
+    if (!arguments("kv8_append", n, 9)) throw PyError{};
     const Cache &c = cache_of(args[0]);
     const at::Tensor &k = tensor("k", args[1]), &v = tensor("v", args[2]);
     const int type = type_of("k", k);
@@ -217,15 +210,14 @@ PyObject *kv8_append(PyObject *, PyObject *const *args, Py_ssize_t n) {
     if (q) out = given ? *given : at::empty({rows, heads, hd}, q->options());
     check(lmx_kv8_append(&c.c, &b, type, k.data_ptr(), ks, v.data_ptr(), vs, q ? q->data_ptr() : nullptr, qs,
                          q ? out.data_ptr() : nullptr, os, size_t(heads), rope ? static_cast<const float *>(rope->data_ptr()) : nullptr,
-                         size_t(positions), stream_of(args[9], device)));
+                         size_t(positions), stream_on(device)));
     if (!out.defined()) Py_RETURN_NONE;
     if (args[8] != Py_None) return Py_NewRef(args[8]);
     return THPVariable_Wrap(std::move(out));
   });
 }
 
-// Workspace of a call: the caller's, or one that torch allocates (for the
-// current stream, as its empty() does).
+// Workspace of a call: the caller's, or one that torch allocates.
 at::Tensor workspace_of(PyObject *given, size_t need, int device, void *&p, size_t &bytes) {
   at::Tensor t;
   p = nullptr;
@@ -243,10 +235,10 @@ at::Tensor workspace_of(PyObject *given, size_t need, int device, void *&p, size
   return t;
 }
 
-// (cache, q, offsets, lengths, pages, scale, out, workspace, stream) -> out
+// (cache, q, offsets, lengths, pages, scale, out, workspace) -> out
 PyObject *kv8_attend(PyObject *, PyObject *const *args, Py_ssize_t n) {
   return guarded([&]() -> PyObject * {
-    if (!arguments("kv8_attend", n, 9)) throw PyError{};
+    if (!arguments("kv8_attend", n, 8)) throw PyError{};
     const Cache &c = cache_of(args[0]);
     const at::Tensor &q = tensor("q", args[1]);
     const int type = type_of("q", q);
@@ -264,16 +256,16 @@ PyObject *kv8_attend(PyObject *, PyObject *const *args, Py_ssize_t n) {
     void *work;
     const at::Tensor w = workspace_of(args[7], need, device, work, bytes);
     check(lmx_kv8_attention(&c.c, &b, type, q.data_ptr(), qs, size_t(heads), float(scale), out.data_ptr(), os, work, bytes,
-                            stream_of(args[8], device)));
+                            stream_on(device)));
     if (args[6] != Py_None) return Py_NewRef(args[6]);
     return THPVariable_Wrap(std::move(out));
   });
 }
 
-// (x, w, w_scale, bias, y, workspace, stream) -> y
+// (x, w, w_scale, bias, y, workspace) -> y
 PyObject *linear_i8(PyObject *, PyObject *const *args, Py_ssize_t n) {
   return guarded([&]() -> PyObject * {
-    if (!arguments("linear_i8", n, 7)) throw PyError{};
+    if (!arguments("linear_i8", n, 6)) throw PyError{};
     const at::Tensor &x = tensor("x", args[0]), &w = tensor("w", args[1]), &scale = tensor("w_scale", args[2]);
     const int type = type_of("x", x);
     if (w.dim() != 2 || w.scalar_type() != at::kChar || w.stride(1) != 1) bad("w", w, "int8 [rows, cols] with neighbouring columns side by side");
@@ -304,7 +296,7 @@ PyObject *linear_i8(PyObject *, PyObject *const *args, Py_ssize_t n) {
     // (the stride of a single row says nothing)
     check(lmx_linear_i8(static_cast<const int8_t *>(w.data_ptr()), size_t(rows > 1 ? w.stride(0) : (cols + 15) / 16 * 16),
                         static_cast<const float *>(scale.data_ptr()), bias ? bias->data_ptr() : nullptr, x.data_ptr(), y.data_ptr(), type, size_t(rows),
-                        size_t(cols), size_t(batch), work, bytes, stream_of(args[6], device)));
+                        size_t(cols), size_t(batch), work, bytes, stream_on(device)));
     if (args[4] != Py_None) return Py_NewRef(args[4]);
     return THPVariable_Wrap(std::move(y));
   });

@@ -17,7 +17,7 @@ import ctypes
 
 import torch
 
-from . import BF16, F16, F32, Kv8BatchC, Kv8CacheC, check, lib, torch_module
+from . import BF16, F16, F32, Kv8BatchC, Kv8CacheC, check, lib, on_stream, torch_module
 
 PAGE, BLOCK = 64, 16
 
@@ -59,15 +59,14 @@ class KvCache8:
         (which may be q; default a new tensor), or None without q.  rope: fp32
         [positions, head_dim // 2, 2] (rope_table), or None.  Rows may lie any stride
         apart."""
-        return self._ops.kv8_append(self._c, k, v, offsets, lengths, pages, rope, q, q_out, stream)
+        return on_stream(stream, self._ops.kv8_append, self._c, k, v, offsets, lengths, pages, rope, q, q_out)
 
     def attend(self, q, offsets, lengths, pages, scale=None, out=None, workspace=None, stream=None):
         """lmx_kv8_attention: causal attention of q [rows, heads, head_dim] (rotated)
         over the sequences' cached tokens; scale defaults to head_dim ** -0.5.
         workspace: a uint8 tensor of at least attend_workspace bytes that no
-        overlapping call uses (default: torch allocates one for the call, on its
-        current stream)."""
-        return self._ops.kv8_attend(self._c, q, offsets, lengths, pages, scale, out, workspace, stream)
+        overlapping call uses (default: torch allocates one for the call)."""
+        return on_stream(stream, self._ops.kv8_attend, self._c, q, offsets, lengths, pages, scale, out, workspace)
 
     def attend_workspace(self, dtype, rows, heads, n_seqs, max_pages):
         """Bytes of workspace of an attend call of these sizes."""

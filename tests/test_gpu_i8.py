@@ -119,7 +119,7 @@ def test_linear_i8_views(cuda):
 
 
 def test_linear_i8_graph_and_stream(cuda):
-    for batch in (3, 130):
+    for batch in (3, 40, 130):
         x, w, scale, b = make(200, 500, batch, torch.bfloat16, 11)
         y = torch.empty(batch, 200, dtype=x.dtype, device="cuda")
         work = torch.empty(L.linear_i8_workspace(200, 500, batch), dtype=torch.uint8, device="cuda")

@@ -329,3 +329,22 @@ def test_streams_and_repeats(cuda):
     n = int(s.offsets[-1])
     for o in outs + [explicit]:
         assert torch.equal(o[:n], first[:n])
+
+
+def test_given_stream_owns_what_it_writes(cuda):
+    """A call on a given stream takes its output and workspace from that stream's
+    memory: what is freed on another stream while its work is under way is not
+    written over."""
+    s = Setup("bfloat16", 128, 2, 4, [1, 1, 30], [1000, 3, 200], seed=15, width=40)
+    first, n = s.cache.attend(s.q, *s.where).clone(), int(s.offsets[-1])
+    other = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    marks, outs = [], []
+    for i in range(10):
+        x = torch.full(first.shape, float(i), dtype=first.dtype, device="cuda")
+        marks.append((x * 2).sum(dtype=torch.float64))   # (frees x * 2 on the current stream)
+        outs.append(s.cache.attend(s.q, *s.where, stream=other))
+        del x
+    torch.cuda.synchronize()
+    for i, (m, o) in enumerate(zip(marks, outs)):
+        assert m.item() == 2.0 * i * first.numel() and torch.equal(o[:n], first[:n])
