@@ -51,9 +51,10 @@ __global__ __launch_bounds__(kPromptWaves *kWave) __attribute__((amdgpu_waves_pe
   extern __shared__ __attribute__((aligned(1024))) char buf[];    // keys of two pages, values of three
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
   const int j = lane & 31, h = lane >> 5;
-  const int kvh = int(blockIdx.y), group = a.c.group;
-  // the last tiles, which see the most, first
-  const int unit = int(gridDim.x) - 1 - int(blockIdx.x);
+  const int kvh = int(blockIdx.x) % a.c.n_kv, group = a.c.group;
+  // the last tiles, which see the most, first, of all heads: what is left at the
+  // end is short (heads one after another left CUs idle for a sixth of the time)
+  const int unit = int(gridDim.x - 1 - blockIdx.x) / a.c.n_kv;
   const SeqRows r = unit_rows(a.c, unit, group, 1, lane, kPromptRows);
   const int tile0 = (unit - r.first) * kPromptRows, rows = r.n * group;
   if (r.seq < 0 || tile0 >= rows) return;
@@ -346,7 +347,8 @@ int launch(const AttnArgs &a, dim3 grid, hipStream_t st) {
 }  // namespace
 
 int launch_prompt(const AttnArgs &a, int type, size_t hd, size_t units, hipStream_t st) {
-  const dim3 grid(unsigned(units), unsigned(a.c.n_kv), unsigned(a.splits));
+  if (units * a.c.n_kv >= (1u << 31)) return fail(LMX_ERR_INVALID_ARGUMENT, "%zu tiles of rows for %d KV heads", units, a.c.n_kv);
+  const dim3 grid(unsigned(units * a.c.n_kv), 1, unsigned(a.splits));
   int r;
   if (type == LMX_F16) r = hd == 64 ? launch<f16, 64>(a, grid, st) : launch<f16, 128>(a, grid, st);
   else r = hd == 64 ? launch<bf16, 64>(a, grid, st) : launch<bf16, 128>(a, grid, st);
