@@ -474,10 +474,9 @@ __global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(PD ==
       for (int v = 0; v < 4; ++v) {
         const float e = __builtin_amdgcn_exp2f(y[u][v] + off);
         sum += e;
-        w[v] = __float_as_uint(fmaf(e, mant, kMagic + float(Digits<PD>::carry)));
+        w[v] = __float_as_uint(fmaf(e, mant, Digits<PD>::p_base + float(Digits<PD>::carry)));
       }
       digit_words<PD>(w, dw);
-      if constexpr (PD == 3) dw[2] ^= 0x40404040u;   // (kMagic's own bit 22)
 #pragma unroll
       for (int d = 0; d < PD; ++d) pd[d][u] = int(dw[d]);
     }

@@ -80,7 +80,7 @@ struct AttnArgs {
 
 constexpr float kMagic = 12582912.0f;   // 1.5 * 2^23
 // The sums of weights carry 2^kSumExp, so that V scales from 2^-100 to 2^120
-// leave them in range (22 bits of weight, 2^24 tokens).
+// leave them in range (23 bits of weight, 2^24 tokens).
 constexpr int kSumExp = -24;
 constexpr float kSumUnit = 0x1p-24f;
 __device__ __forceinline__ float inverse_sum(float l) { return l == 0.0f ? 0.0f : kSumUnit / l; }
@@ -120,10 +120,16 @@ __device__ __forceinline__ int lane_xor_int(int v, int lane) { return int(lane_x
 
 template <int ND> struct Digits;
 // carry: 128 for every digit below the top; q_bits: |q| <= 2^q_bits; p_exp: the
-// largest weight is 2^p_exp, so that weight + carry stays below 2^22 (three
-// digits: below the window of kMagic) or 2^15 (two)
-template <> struct Digits<2> { static constexpr int carry = 0x80, q_bits = 14; static constexpr float p_exp = 14.98f; };
-template <> struct Digits<3> { static constexpr int carry = 0x8080, q_bits = 22; static constexpr float p_exp = 21.98f; };
+// largest weight is 2^p_exp, so that weight + carry stays below 2^15 or, of three
+// digits, 2^23: added to p_base it is then the low bits of the float
+template <> struct Digits<2> {
+  static constexpr int carry = 0x80, q_bits = 14;
+  static constexpr float p_exp = 14.98f, p_base = kMagic;
+};
+template <> struct Digits<3> {
+  static constexpr int carry = 0x8080, q_bits = 22;
+  static constexpr float p_exp = 22.98f, p_base = 0x1p23f;
+};
 
 // A row's 16 contiguous elements of step m -> its digit words; f: the power of
 // two of the fixed point.
