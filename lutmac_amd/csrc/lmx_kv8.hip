@@ -431,7 +431,7 @@ __global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(PD ==
     exmax = max(exmax, max(ex, lane_xor_int<16>(ex, lane)));
     exmax = max(exmax, lane_xor_int<32>(exmax, lane));
     ex = max(ex, exmax - kExpSpan);
-    const float mant = __builtin_amdgcn_ldexpf(vsp, -ex), fex = float(ex), c = qs * ksp;
+    const float mant = __builtin_amdgcn_ldexpf(vsp, -ex) * Digits<PD>::p_unit, fex = float(ex), c = qs * ksp;
     float y[4][4], top = -INFINITY;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -463,7 +463,6 @@ __global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(PD ==
     top = fmaxf(top, lane_xor<32>(top, lane));
     const float mn = fmaxf(mref, top), base = mn == -INFINITY ? 0.0f : mn;
     const float root = __builtin_amdgcn_exp2f(0.5f * (mref - base)), keep = root * root;
-    const float off = Digits<PD>::p_exp - base;
     mref = mn;
     v4i pd[PD];
     float sum = 0.0f;
@@ -472,7 +471,7 @@ __global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(PD ==
       uint32_t w[4], dw[PD];
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
-        const float e = __builtin_amdgcn_exp2f(y[u][v] + off);
+        const float e = __builtin_amdgcn_exp2f(y[u][v] - base);
         sum += e;
         w[v] = __float_as_uint(fmaf(e, mant, Digits<PD>::p_base + float(Digits<PD>::carry)));
       }
@@ -481,7 +480,7 @@ __global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(PD ==
       for (int d = 0; d < PD; ++d) pd[d][u] = int(dw[d]);
     }
     // (a block whose scale is not finite gives NaN to the rows that see it)
-    const float unit = vsp - vsp == 0.0f ? __builtin_amdgcn_ldexpf(1.0f, kSumExp - ex) : __builtin_nanf("");
+    const float unit = vsp - vsp == 0.0f ? __builtin_amdgcn_ldexpf(Digits<PD>::p_unit, kSumExp - ex) : __builtin_nanf("");
     l = l * root * root;   // (keep alone may underflow where l is large)
     if (sum != 0.0f) l = fmaf(sum, unit, l);
 #pragma unroll

@@ -112,7 +112,7 @@ class Cache:
         one term a page (16 a page for L), joined over waves and parts; and the last
         rounding to the type."""
         f32 = dtype == "float32"
-        q_bits, p_exp = 22 if f32 else 14, 14.98 if dtype == "bfloat16" else 22.98
+        q_bits, p_exp = 22 if f32 else 14, np.log2(32560 if dtype == "bfloat16" else 8350000)
         out, most = np.full(q.shape, np.nan), np.zeros(q.shape)
         n_kv = self.k.shape[1]
         group = q.shape[1] // n_kv
