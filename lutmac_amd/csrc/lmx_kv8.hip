@@ -78,8 +78,8 @@ __device__ __forceinline__ float block_scale(double top, bool finite, float was,
 }
 
 // (a NaN scale leaves the codes 0)
-__device__ __forceinline__ int code_of(double x, double scale, double inverse) {
-  return scale == scale ? int(round_quotient(x, scale, inverse)) : 0;
+__device__ __forceinline__ int code_of(double x, double scale) {
+  return scale == scale ? int(round_quotient(x, scale, 1.0 / scale)) : 0;
 }
 
 // Codes of four values, a byte each; false: one lies next to a border.
@@ -95,6 +95,21 @@ __device__ __forceinline__ bool sure_codes(const float *x, float inverse, uint32
   }
   return sure;
 }
+
+// Four codes of a block whose scale grew.
+__device__ __forceinline__ uint32_t rescaled(uint32_t old, float was, float now) {
+  const auto code = [old](int j) { return int(old << (24 - 8 * j)) >> 24; };
+  const float x[4] = {float(code(0)), float(code(1)), float(code(2)), float(code(3))};
+  uint32_t w;
+  if (!sure_codes(x, was / now, w)) {
+    w = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w |= uint32_t(code_of(double(code(j)) * double(was), now) & 0xFF) << (8 * j);
+  }
+  return w;
+}
+// A word's first n bytes (none below 1, all from 4 on).
+__device__ __forceinline__ uint32_t low_bytes(int n) { return n <= 0 ? 0u : n >= 4 ? ~0u : (1u << (8 * n)) - 1; }
 
 // A block's part in a call: tokens [kept, last) of it are rows of the call,
 // those below kept the sequence's earlier ones.
@@ -172,6 +187,13 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
     float *scale = a.c.k_scale + ph * kPageBlocks + wave;
     const float was = *scale;
     const T *src = static_cast<const T *>(a.k) + row * a.k_stride + size_t(role) * HD;
+    int8_t *dst = a.c.k + (ph * kPage + wave * kBlock + tk) * HD + part * E;
+    typedef uint32_t words __attribute__((ext_vector_type(E / 4)));
+    words old[2] = {};   // (fetched before they are known to be needed)
+    if (tk < br.kept) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) old[h] = *reinterpret_cast<const words *>(dst + h * (HD / 2));
+    }
     float x[2][E], most = 0.0f;
 #pragma unroll
     for (int i = 0; i < E; ++i) x[0][i] = x[1][i] = 0.0f;
@@ -198,14 +220,11 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
         }
       }
     }
-#pragma unroll
-    for (int d = 32; d; d >>= 1) top = fmax(top, __shfl_xor(top, d, kWave));
+    // (of numbers >= 0 the largest has the largest bits; what is not finite goes by itself)
+    top = __longlong_as_double(static_cast<long long>(wave_max_key(static_cast<unsigned long long>(__double_as_longlong(top)), lane)));
     const float now = block_scale(top, __builtin_amdgcn_ballot_w64(!finite) == 0, was, br.kept > 0);
-    const double inv = 1.0 / double(now);
-    int8_t *dst = a.c.k + (ph * kPage + wave * kBlock + tk) * HD + part * E;
-    typedef uint32_t words __attribute__((ext_vector_type(E / 4)));
     if (live) {
-      const float finv = float(inv);
+      const float finv = 1.0f / now;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         words c;
@@ -215,26 +234,37 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
           if (!sure_codes(x[h] + 4 * i, finv, w) || !fast) {
             w = 0;
             for (int j = 0; j < 4; ++j)
-              w |= uint32_t(code_of(exact_element<T, HD>(src, a.rope, pos, part * E + 4 * i + j, h), now, inv) & 0xFF) << (8 * j);
+              w |= uint32_t(code_of(exact_element<T, HD>(src, a.rope, pos, part * E + 4 * i + j, h), now) & 0xFF) << (8 * j);
           }
           c[i] = now == now ? w : 0u;
         }
         *reinterpret_cast<words *>(dst + h * (HD / 2)) = c;
       }
     } else if (tk < br.kept && now == now && now != was) {
-      typedef int8_t bytes __attribute__((ext_vector_type(E)));
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        bytes c = *reinterpret_cast<const bytes *>(dst + h * (HD / 2));
+        words c;
 #pragma unroll
-        for (int i = 0; i < E; ++i) c[i] = int8_t(code_of(double(int(c[i])) * double(was), now, inv));
-        *reinterpret_cast<bytes *>(dst + h * (HD / 2)) = c;
+        for (int i = 0; i < E / 4; ++i) c[i] = rescaled(old[h][i], was, now);
+        *reinterpret_cast<words *>(dst + h * (HD / 2)) = c;
       }
     }
     if (lane == 0) *scale = now;
     return;
   }
   const size_t ph = size_t(page) * n_kv + (role - n_kv);
+  // a thread's dimension and block (two of head_dim 128), of which it writes the
+  // row of 16 tokens in the end; what is there now, for blocks not written whole
+  typedef uint32_t words __attribute__((ext_vector_type(kBlock / 4)));
+  constexpr int ROUNDS = HD * kPageBlocks / 256;
+  words old[ROUNDS] = {};
+#pragma unroll
+  for (int n = 0; n < ROUNDS; ++n) {
+    const int d = (n * 256 + int(threadIdx.x)) / kPageBlocks, b = int(threadIdx.x) % kPageBlocks;
+    const BlockRows w = block_rows(b);
+    if (w.last > w.kept && (w.kept > 0 || w.last < kBlock))
+      old[n] = *reinterpret_cast<const words *>(a.c.v + (ph * HD + d) * kPage + b * kBlock);
+  }
   if (some) {
     float *scale = a.c.v_scale + ph * kPageBlocks + wave;
     const float was = *scale;
@@ -249,8 +279,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
       finite = finite && fabsf(x[i]) < INFINITY;
     }
     const float now = block_scale(wave_max(most, lane), __builtin_amdgcn_ballot_w64(!finite) == 0, was, br.kept > 0);
-    const double inv = 1.0 / double(now);
-    const float finv = float(inv);
+    const float finv = 1.0f / now;
     // four dimensions of four tokens at a time: lane (token 4 n + q, part) ends
     // with dimension 4 i + q of its part, the tokens 4 n .. 4 n + 3
     const int q = tk & 3;
@@ -260,7 +289,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
       if (!sure_codes(x + 4 * i, finv, w)) {
         w = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w |= uint32_t(code_of(x[4 * i + j], now, inv) & 0xFF) << (8 * j);
+        for (int j = 0; j < 4; ++j) w |= uint32_t(code_of(x[4 * i + j], now) & 0xFF) << (8 * j);
       }
       w = now == now ? w : 0u;
       // the words of the lanes 4, 8 and 12 places on (row of 16 lanes = 4 tokens x 4 parts)
@@ -277,25 +306,22 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
     }
   }
   __syncthreads();
-  for (int n = int(threadIdx.x); n < HD * kPageBlocks; n += 256) {   // a dimension's 16 tokens of a block
-    const int d = n / kPageBlocks, b = n % kPageBlocks;
+#pragma unroll
+  for (int n = 0; n < ROUNDS; ++n) {
+    const int d = (n * 256 + int(threadIdx.x)) / kPageBlocks, b = int(threadIdx.x) % kPageBlocks;
     const BlockRows w = block_rows(b);
     if (w.last <= w.kept) continue;
-    int8_t *p = a.c.v + (ph * HD + d) * kPage + b * kBlock;
-    typedef int8_t bytes __attribute__((ext_vector_type(16)));
-    bytes c = *reinterpret_cast<const bytes *>(&cod[d][b * kBlock]);
+    words c = *reinterpret_cast<const words *>(&cod[d][b * kBlock]);
     if (w.kept > 0 || w.last < kBlock) {   // earlier tokens are rescaled, later places left
-      const bytes old = *reinterpret_cast<const bytes *>(p);
       const float was = scales[b][0], now = scales[b][1];
       const bool rescale = now == now && now != was;
-      const double inv = 1.0 / double(now);
 #pragma unroll
-      for (int t = 0; t < kBlock; ++t) {
-        if (t < w.kept) c[t] = rescale ? int8_t(code_of(double(int(old[t])) * double(was), now, inv)) : old[t];
-        else if (t >= w.last) c[t] = old[t];
+      for (int i = 0; i < kBlock / 4; ++i) {
+        const uint32_t kept = low_bytes(w.kept - 4 * i), rows = low_bytes(w.last - 4 * i) & ~kept;
+        c[i] = (c[i] & rows) | (old[n][i] & ~(rows | kept)) | ((rescale && kept ? rescaled(old[n][i], was, now) : old[n][i]) & kept);
       }
     }
-    *reinterpret_cast<bytes *>(p) = c;
+    *reinterpret_cast<words *>(a.c.v + (ph * HD + d) * kPage + b * kBlock) = c;
   }
 }
 
