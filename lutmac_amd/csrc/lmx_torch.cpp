@@ -4,7 +4,7 @@
 //
 // A serving loop calls them eagerly many times a step, and in Python a call's
 // checks took longer than the kernels of a small one (host time of an append of 64
-// rows 12.4 us, here 5.0, on the GPU 7.2; of the attention of one row 11.1, 5.0
+// rows 12.4 us, here 5.0, on the GPU 6.7; of the attention of one row 11.1, 5.0
 // and 6.0).
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
