@@ -349,8 +349,9 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
 // Bound by the cache's bytes where contexts are long (32 sequences of 20 to 33
 // thousand tokens, 8 KV heads of 128: 346 us, 5.0 TB/s, what a copy reaches),
 // else by the chain of loads (offsets, table, page, and each further page of a
-// wave; one row of 320 tokens: 6.0 us) and some 600 vector instructions a page
-// (64 sequences of up to 2048 tokens: 14.7 us and 4 for the merge): table entries
+// wave; one row of 320 tokens: 5.9 us) and some 320 vector and 48 matrix
+// instructions a page of head_dim 128 (64 sequences of up to 2048 tokens, fp32: 14.7
+// us and 4 for the merge): table entries
 // come 64 at a time, and a page's keys and values are requested as soon as the
 // registers of the page before are free of theirs.
 template <class T, int HD, int ND, int PD>
@@ -439,11 +440,7 @@ __global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(PD ==
     const int e = max(int(top >> 23), 29) - 126;   // |x| < 2^e
     const float f = finite ? __builtin_amdgcn_ldexpf(1.0f, Digits<ND>::q_bits - e) : 0.0f;
 #pragma unroll
-    for (int m = 0; m < M; ++m) {
-#pragma unroll
-      for (int d = 0; d < 16; ++d) x[m][d] = finite ? x[m][d] : 0.0f;
-      query_digits<ND>(x[m], f, qd[m]);
-    }
+    for (int m = 0; m < M; ++m) query_digits<ND>(x[m], f, qd[m]);   // (anything where not finite: qs is NaN then)
     qs = finite ? __builtin_amdgcn_ldexpf(a.scale, e - Digits<ND>::q_bits) : __builtin_nanf("");
   }
 
@@ -519,7 +516,10 @@ __global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(PD ==
         float d[PD];
 #pragma unroll
         for (int n = 0; n < PD; ++n) d[n] = __int_as_float(s[n][v]);
-        o[h][v] = fmaf(o[h][v], keep, join<PD>(d));
+        // (in place: as a plain fma the compiler makes another register of it and
+        // copies all of them back, a tenth of the loop)
+        const float sum = join<PD>(d);
+        asm("v_fma_f32 %0, %0, %1, %2" : "+v"(o[h][v]) : "v"(keep), "v"(sum));
       }
     }
     request_values();

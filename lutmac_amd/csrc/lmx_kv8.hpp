@@ -139,7 +139,8 @@ __device__ __forceinline__ void query_digits(const float (&x)[16], float f, v4i 
   for (int b = 0; b < 4; ++b) {
     uint32_t u[4], d[ND];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = uint32_t(__float2int_rn(x[4 * b + i] * f) + Digits<ND>::carry);
+    for (int i = 0; i < 4; ++i)   // (the float's low bits are the rounded product, up to 2^22 on either side)
+      u[i] = __float_as_uint(fmaf(x[4 * b + i], f, kMagic)) + (uint32_t(Digits<ND>::carry) - 0x4B400000u);
     digit_words<ND>(u, d);
 #pragma unroll
     for (int j = 0; j < ND; ++j) w[j][b] = int(d[j]);
