@@ -103,6 +103,10 @@ int lmx_kv8_attention_workspace(const lmx_kv8_cache *cache,
  * lie between 2^-100 and 2^100; those below 2^-60 of the largest in reach lose
  * bits like the small values of one block do.  A query head with an element
  * that is not finite gives NaN.
+ * The work is split by the call's sizes alone, as if its sequences had equal
+ * shares of the rows: long prompts and single tokens after long contexts are
+ * faster in calls of their own (4096 rows of one sequence and single ones of 63
+ * after 8000, 32 + 8 heads of 128, bf16: 714 us together, 163 + 211 apart).
  * workspace: lmx_kv8_attention_workspace bytes, 16-byte aligned, in any state;
  * calls that may overlap in time need workspaces of their own. */
 int lmx_kv8_attention(const lmx_kv8_cache *cache, const lmx_kv8_batch *batch,

@@ -571,11 +571,13 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(AttnArgs a) {
   constexpr int E = HD / 16, S = 8;
   const int lane = threadIdx.x & (kWave - 1), kvh = int(blockIdx.y), group = a.c.group;
   const int row = int(blockIdx.z) * 16 + (int(threadIdx.x) >> 4), d0 = (int(threadIdx.x) & 15) * E;
+  const SeqRows r = unit_rows(a.c, int(blockIdx.x), group, 1, lane, ROWS);
+  const int i = (int(blockIdx.x) - r.first) * ROWS + row;
+  if (r.seq < 0 || i >= r.n * group) return;
   const size_t at = (size_t(blockIdx.x) * a.c.n_kv + kvh) * a.splits * ROWS + row;
   float mx = -INFINITY, sum = 0.0f, acc[E];
 #pragma unroll
   for (int d = 0; d < E; ++d) acc[d] = 0.0f;
-  // (units and rows that no sequence has hold anything, and are dropped below)
   for (int s0 = 0; s0 < a.splits; s0 += S) {
     float2 ml[S];
     float o[S][E];
@@ -606,9 +608,6 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(AttnArgs a) {
     }
     mx = now;
   }
-  const SeqRows r = unit_rows(a.c, int(blockIdx.x), group, 1, lane, ROWS);
-  const int i = (int(blockIdx.x) - r.first) * ROWS + row;
-  if (r.seq < 0 || i >= r.n * group) return;
   const float inv = inverse_sum(sum);
 #pragma unroll
   for (int d = 0; d < E; ++d) acc[d] *= inv;
