@@ -2,7 +2,6 @@
 // append, and attention of a few rows per sequence over it.
 #include <algorithm>
 #include <cmath>
-#include <type_traits>
 
 #include "lmx_kv8.hpp"
 
@@ -340,9 +339,15 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
 //     tokens 16 g + 4 t + 0..3 -- over the four tiles the 16 tokens of block g,
 //     in order: one K and one V scale per lane, and P^T's operand in place.
 //   V operand: lane (i, g) holds tokens 16 g .. + 15 of dimension 16 h + i.
-// Weights are relative to the running maximum of score + log2 of the V scale's
-// power of two (what bounds the fixed point); the rest of the scale is
-// multiplied in as the digits are made (see value_exponent).
+// Weights are relative to their page's largest score + log2 of the V scale's
+// power of two (what bounds the fixed point), so that a heavy token takes bits
+// from its own page alone; the page's sums are brought to the running reference
+// as they are added.  The rest of the scale is multiplied in as the digits are
+// made (see value_exponent).  (Relative to the running reference, weights far
+// below a heavy first token counted in their sum and not in the values': a tenth
+// of the output lost with 15 bits, 1e-4 with 23.  Two digits instead of three
+// would save up to 7 % of a step, and leave the other tokens of a page whose
+// heaviest has 0.99 of the weight some 5 steps each.)
 //
 // The 4 waves take pages in turn, grid.z parts ("splits") a share of them;
 // (m, l, o) of the waves merge in LDS, of the parts in kv8_merge_kernel.
@@ -354,9 +359,9 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
 // us and 4 for the merge): table entries
 // come 64 at a time, and a page's keys and values are requested as soon as the
 // registers of the page before are free of theirs.
-template <class T, int HD, int ND, int PD>
-__global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(PD == 3 && HD == 128 ? 2 : 3))) void kv8_rows_kernel(AttnArgs a) {
-  constexpr int W = 4, M = HD / 64, H = HD / 16;
+template <class T, int HD, int ND>
+__global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(HD == 128 ? 2 : 3))) void kv8_rows_kernel(AttnArgs a) {
+  constexpr int W = 4, M = HD / 64, H = HD / 16, PD = 3;   // PD: digits of a weight
   __shared__ float os[W][16][HD + 4];
   __shared__ float ms[W][16], ls[W][16];
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
@@ -454,7 +459,7 @@ __global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(PD ==
     exmax = max(exmax, max(ex, lane_xor_int<16>(ex, lane)));
     exmax = max(exmax, lane_xor_int<32>(exmax, lane));
     ex = max(ex, exmax - kExpSpan);
-    const float mant = __builtin_amdgcn_ldexpf(vsp, -ex) * Digits<PD>::p_unit, fex = float(ex), c = qs * ksp;
+    const float mant = __builtin_amdgcn_ldexpf(vsp, -ex) * kWeightUnit, fex = float(ex), c = qs * ksp;
     float y[4][4], top = -INFINITY;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -484,9 +489,19 @@ __global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(PD ==
     for (int v = 0; v < 16; ++v) top = fmaxf(top, y[v / 4][v % 4]);
     top = fmaxf(top, lane_xor<16>(top, lane));
     top = fmaxf(top, lane_xor<32>(top, lane));
-    const float mn = fmaxf(mref, top), base = mn == -INFINITY ? 0.0f : mn;
-    const float root = __builtin_amdgcn_exp2f(0.5f * (mref - base)), keep = root * root;
-    mref = mn;
+    // weights relative to the page's largest; `share` brings its sums to the
+    // running reference, and where that rises the sums so far follow it
+    const float base = top == -INFINITY ? 0.0f : top, was = mref;
+    mref = fmaxf(mref, top);
+    if (n > 0 && __builtin_amdgcn_ballot_w64(mref > was) != 0) {
+      const float root = mref > was ? __builtin_amdgcn_exp2f(0.5f * (was - mref)) : 1.0f, keep = root * root;
+      l = l * root * root;   // (keep alone may underflow where l is large)
+#pragma unroll
+      for (int h = 0; h < H; ++h)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) asm("v_mul_f32 %0, %0, %1" : "+v"(o[h][v]) : "v"(keep));
+    }
+    const float root = __builtin_amdgcn_exp2f(0.5f * (top - (mref == -INFINITY ? 0.0f : mref))), share = root * root;
     v4i pd[PD];
     float sum = 0.0f;
 #pragma unroll
@@ -496,16 +511,15 @@ __global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(PD ==
       for (int v = 0; v < 4; ++v) {
         const float e = __builtin_amdgcn_exp2f(y[u][v] - base);
         sum += e;
-        w[v] = __float_as_uint(fmaf(e, mant, Digits<PD>::p_base + float(Digits<PD>::carry)));
+        w[v] = __float_as_uint(fmaf(e, mant, 0x1p23f + float(Digits<PD>::carry)));
       }
       digit_words<PD>(w, dw);
 #pragma unroll
       for (int d = 0; d < PD; ++d) pd[d][u] = int(dw[d]);
     }
     // (a block whose scale is not finite gives NaN to the rows that see it)
-    const float unit = vsp - vsp == 0.0f ? __builtin_amdgcn_ldexpf(Digits<PD>::p_unit, kSumExp - ex) : __builtin_nanf("");
-    l = l * root * root;   // (keep alone may underflow where l is large)
-    if (sum != 0.0f) l = fmaf(sum, unit, l);
+    const float unit = vsp - vsp == 0.0f ? __builtin_amdgcn_ldexpf(kWeightUnit, kSumExp - ex) : __builtin_nanf("");
+    if (sum != 0.0f) l = fmaf(sum * root, unit * root, l);
 #pragma unroll
     for (int h = 0; h < H; ++h) {
       v4i s[PD];
@@ -519,7 +533,7 @@ __global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(PD ==
         // (in place: as a plain fma the compiler makes another register of it and
         // copies all of them back, a tenth of the loop)
         const float sum = join<PD>(d);
-        asm("v_fma_f32 %0, %0, %1, %2" : "+v"(o[h][v]) : "v"(keep), "v"(sum));
+        asm("v_fma_f32 %0, %1, %2, %0" : "+v"(o[h][v]) : "v"(sum), "v"(share));
       }
     }
     request_values();
@@ -676,13 +690,13 @@ Plan plan(const lmx_kv8_cache *c, const lmx_kv8_batch *b, size_t n_heads, int ty
   Plan p{};
   p.rows = type != LMX_F32 && b->n_rows * group >= 64 * b->n_seqs ? kPromptRows : 16;
   p.units = b->n_rows * group / p.rows + b->n_seqs;
-  // As many parts as fill the device once (three workgroups per CU; two of fp32
-  // and fp16 with head_dim 128 and of prompts: a workgroup more runs a second round) if
+  // As many parts as fill the device once (three workgroups per CU; two with
+  // head_dim 128 and of prompts: a workgroup more runs a second round) if
   // the sequences have equal shares of the rows, of four pages at least, one per
   // wave (prompts: 8).
   const size_t each = (b->n_rows + b->n_seqs - 1) / b->n_seqs;
   const size_t wgs = b->n_seqs * ((each * group + p.rows - 1) / p.rows) * c->n_kv_heads;
-  const size_t room = p.rows > 16 || (type != LMX_BF16 && c->head_dim == 128) ? 512 : 768;
+  const size_t room = p.rows > 16 || c->head_dim == 128 ? 512 : 768;
   const size_t s = std::min<size_t>(room / wgs, b->max_pages / (p.rows == 16 ? 4 : 8));
   p.splits = int(std::max<size_t>(1, std::min<size_t>(s, 64)));
   return p;
@@ -697,13 +711,11 @@ size_t workspace_bytes(const lmx_kv8_cache *c, const lmx_kv8_batch *b, size_t n_
 
 template <class T, int HD>
 int launch_attention(const AttnArgs &a, int type, const Plan &p, hipStream_t st) {
-  // (weights of 14 bits below the largest are less than the rounding of bf16 where
-  // contexts are some 10 000 tokens long, but not than that of fp16)
-  constexpr int ND = sizeof(T) == 4 ? 3 : 2, PD = std::is_same<T, bf16>::value ? 2 : 3;
+  constexpr int ND = sizeof(T) == 4 ? 3 : 2;
   const dim3 grid(unsigned(p.units), unsigned(a.c.n_kv), unsigned(a.splits));
   int r;
   if (p.rows == 16) {
-    kv8_rows_kernel<T, HD, ND, PD><<<grid, dim3(256), 0, st>>>(a);
+    kv8_rows_kernel<T, HD, ND><<<grid, dim3(256), 0, st>>>(a);
     r = launch_err("kv8 attention");
   } else {
     r = launch_prompt(a, type, HD, p.units, st);

@@ -119,17 +119,16 @@ template <int D>
 __device__ __forceinline__ int lane_xor_int(int v, int lane) { return int(lane_xor_u32<D>(uint32_t(v), lane)); }
 
 template <int ND> struct Digits;
-// carry: 128 for every digit below the top; q_bits: |q| <= 2^q_bits; p_unit: the
-// largest weight, such that weight + carry stays below 2^15 or, of three digits,
-// 2^23: added to p_base it is then the low bits of the float
+// carry: 128 for every digit below the top; q_bits: |q| <= 2^q_bits
 template <> struct Digits<2> {
   static constexpr int carry = 0x80, q_bits = 14;
-  static constexpr float p_unit = 32560.0f, p_base = kMagic;
 };
 template <> struct Digits<3> {
   static constexpr int carry = 0x8080, q_bits = 22;
-  static constexpr float p_unit = 8350000.0f, p_base = 0x1p23f;
 };
+// The largest weight, of three digits: weight + carry stays below 2^23, so that
+// added to 2^23 it is the low bits of the float.
+constexpr float kWeightUnit = 8350000.0f;
 
 // A row's 16 contiguous elements of step m -> its digit words; f: the power of
 // two of the fixed point.

@@ -1,0 +1,68 @@
+"""Attention over the paged 8-bit cache (lutmac_kv8.h) where the bound of
+kv8_bounds.py says more than that of kv8_reference.py: rows whose weight lies in a
+few tokens."""
+import numpy as np
+import pytest
+import torch
+
+import kv8_bounds
+from test_gpu_kv8 import TYPES, Setup, f64
+
+pytestmark = pytest.mark.gpu
+
+
+def check(s, q=None, ref=None):
+    """The attention of a Setup's rows, held to the bound."""
+    q = s.q if q is None else q
+    out = s.cache.attend(q, *s.where)
+    want, most = kv8_bounds.attend(ref or s.reference(), f64(q), s.offsets, s.lengths, s.pages, s.hd ** -0.5, s.dtype)
+    n = int(s.offsets[-1])
+    got, want, most = f64(out)[:n], want[:n], most[:n]
+    nan = np.isnan(want)
+    np.testing.assert_array_equal(np.isnan(got), nan)
+    over = (np.abs(got - want) / most)[~nan]
+    assert over.size == 0 or over.max() <= 1, f"{over.max():.3g} times the bound, off by {np.abs(got - want)[~nan].max():.3g}"
+    return got, nan
+
+
+def peaked(dtype, hd, group, n, share, one_part, zeros, new=2, seed=40):
+    """Sequence 0: a first token with about `share` of each row's weight before n others
+    of scores of spread 0.5 and values around 1, its page's values zero or not; with a
+    second hundred of sequences of one token each, so that no row's pages are split."""
+    seqs = 200 if one_part else 1
+    s = Setup(dtype, hd, 2, group, [new] + [1] * (seqs - 1), [n] + [0] * (seqs - 1), seed=seed, behind=0)
+    g = torch.Generator().manual_seed(seed)
+    q = torch.randint(-2, 3, s.q.shape, generator=g).float()   # (whole numbers: exact in any fixed point)
+    q[..., 5] = 4
+    s.q.copy_(q)
+    c, first = s.cache, int(s.pages[0, 0])
+    c.k[..., 5] = 0
+    c.k_scale.fill_(0.5 / (2 ** 0.5 * 40))   # spread of scores: codes of 40, queries of sqrt 2, hd ** 0.5 cancels
+    c.v.copy_((torch.randn(c.v.shape, generator=g) * 30 + 40).round().clamp(-127, 127))
+    c.v_scale.fill_(0.025)
+    c.k[first, :, :16] = 0
+    c.k[first, :, 0, 5] = 127
+    c.k_scale[first, :, 0] = (np.log(share / (1 - share) * n) + 0.125) / (4 * 127 * hd ** -0.5)
+    if zeros:
+        c.v[first] = 0
+    return s
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("hd,group", [(64, 4), (128, 2)])
+@pytest.mark.parametrize("n,share", [(300, 0.9), (4000, 0.5), (4000, 0.9), (30000, 0.5), (30000, 0.8), (30000, 0.9)])
+@pytest.mark.parametrize("one_part", [True, False])
+@pytest.mark.parametrize("zeros", [True, False])
+def test_tail_behind_a_heavy_first_token(cuda, dtype, hd, group, n, share, one_part, zeros):
+    check(peaked(dtype, hd, group, n, share, one_part, zeros))
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("hd,group", [(64, 4), (128, 2)])
+@pytest.mark.parametrize("n,share", [(300, 0.9), (8000, 0.5), (8000, 0.9)])
+@pytest.mark.parametrize("zeros", [True, False])
+def test_tail_behind_a_heavy_first_token_in_prompts(cuda, dtype, hd, group, n, share, zeros):
+    """Rows enough for the kernel of prompts, in one part and several (of long tables)."""
+    s = peaked(dtype, hd, group, n, share, False, zeros, new=70)
+    assert kv8_bounds.tiled(dtype, f64(s.q), s.offsets, group)
+    check(s)
