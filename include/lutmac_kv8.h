@@ -96,9 +96,9 @@ int lmx_kv8_attention_workspace(const lmx_kv8_cache *cache,
  * h / (n_heads / n_kv_heads).  A row that sees nothing gets zeros.  out
  * (out_stride; elements of `type`) may be q.
  * Products with the codes are exact, sums and softmax statistics fp32.  Before
- * the products queries are rounded to 2^-15 of a power of two at or above the
- * largest of their head (fp32: 2^-23), the weights of the values to 2^-23 of the
- * largest of their page or, of 64 rows and more a sequence in the 16-bit types,
+ * the products queries are rounded to 2^-23 of a power of two above the largest
+ * of their head, the weights of the values to 2^-23 of the largest of their page
+ * or, of 64 rows and more a sequence in the 16-bit types,
  * to 2^-11 of themselves.  V scales
  * lie between 2^-100 and 2^100; those below 2^-60 of the largest in reach lose
  * bits like the small values of one block do.  A query head with an element

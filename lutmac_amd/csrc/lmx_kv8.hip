@@ -328,7 +328,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
 // Attention of up to 16 rows (a row: one query head of one token) of one KV
 // head per workgroup, on the 8-bit matrix cores with exact products.
 //
-// A query row becomes fixed point of ND signed-byte digits relative to a power
+// A query row becomes fixed point of three signed-byte digits relative to a power
 // of two; S^T = K Q^T digit by digit (v_mfma_i32_16x16x64_i8, sums from the bits
 // of 1.5 * 2^23, so the sum is a float that differs from it by the sum); the
 // weights p become fixed point the same way, and O^T = V^T P^T.  No code is
@@ -359,9 +359,9 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
 // us and 4 for the merge): table entries
 // come 64 at a time, and a page's keys and values are requested as soon as the
 // registers of the page before are free of theirs.
-template <class T, int HD, int ND>
+template <class T, int HD>
 __global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(HD == 128 ? 2 : 3))) void kv8_rows_kernel(AttnArgs a) {
-  constexpr int W = 4, M = HD / 64, H = HD / 16, PD = 3;   // PD: digits of a weight
+  constexpr int W = 4, M = HD / 64, H = HD / 16;
   __shared__ float os[W][16][HD + 4];
   __shared__ float ms[W][16], ls[W][16];
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
@@ -431,7 +431,7 @@ __global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(HD ==
     request_values();
   }
   // (its digits are made while the first page is on its way)
-  v4i qd[M][ND];
+  v4i qd[M][kDigits];
   float qs;
   {
     uint32_t top = 0;
@@ -443,10 +443,10 @@ __global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(HD ==
     top = max(top, lane_xor_u32<32>(top, lane));
     const bool finite = top < 0x7F800000u;
     const int e = max(int(top >> 23), 29) - 126;   // |x| < 2^e
-    const float f = finite ? __builtin_amdgcn_ldexpf(1.0f, Digits<ND>::q_bits - e) : 0.0f;
+    const float f = finite ? __builtin_amdgcn_ldexpf(1.0f, kQueryBits - e) : 0.0f;
 #pragma unroll
-    for (int m = 0; m < M; ++m) query_digits<ND>(x[m], f, qd[m]);   // (anything where not finite: qs is NaN then)
-    qs = finite ? __builtin_amdgcn_ldexpf(a.scale, e - Digits<ND>::q_bits) : __builtin_nanf("");
+    for (int m = 0; m < M; ++m) query_digits(x[m], f, qd[m]);   // (anything where not finite: qs is NaN then)
+    qs = finite ? __builtin_amdgcn_ldexpf(a.scale, e - kQueryBits) : __builtin_nanf("");
   }
 
   for (int p = p0 + wave, n = 0; p < p1; p += W, ++n) {
@@ -463,19 +463,19 @@ __global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(HD ==
     float y[4][4], top = -INFINITY;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      v4i s[ND];
+      v4i s[kDigits];
 #pragma unroll
-      for (int d = 0; d < ND; ++d) {
+      for (int d = 0; d < kDigits; ++d) {
         s[d] = zero;
 #pragma unroll
         for (int m = 0; m < M; ++m) s[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kb[u][m], qd[m][d], s[d], 0, 0, 0);
       }
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
-        float d[ND];
+        float d[kDigits];
 #pragma unroll
-        for (int n = 0; n < ND; ++n) d[n] = __int_as_float(s[n][v]);
-        y[u][v] = fmaf(join<ND>(d), c, fex);
+        for (int n = 0; n < kDigits; ++n) d[n] = __int_as_float(s[n][v]);
+        y[u][v] = fmaf(join(d), c, fex);
       }
     }
     request_keys(p + W, n + 1);
@@ -502,37 +502,37 @@ __global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(HD ==
         for (int v = 0; v < 4; ++v) asm("v_mul_f32 %0, %0, %1" : "+v"(o[h][v]) : "v"(keep));
     }
     const float root = __builtin_amdgcn_exp2f(0.5f * (top - (mref == -INFINITY ? 0.0f : mref))), share = root * root;
-    v4i pd[PD];
+    v4i pd[kDigits];
     float sum = 0.0f;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      uint32_t w[4], dw[PD];
+      uint32_t w[4], dw[kDigits];
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         const float e = __builtin_amdgcn_exp2f(y[u][v] - base);
         sum += e;
-        w[v] = __float_as_uint(fmaf(e, mant, 0x1p23f + float(Digits<PD>::carry)));
+        w[v] = __float_as_uint(fmaf(e, mant, 0x1p23f + float(kCarry)));
       }
-      digit_words<PD>(w, dw);
+      digit_words(w, dw);
 #pragma unroll
-      for (int d = 0; d < PD; ++d) pd[d][u] = int(dw[d]);
+      for (int d = 0; d < kDigits; ++d) pd[d][u] = int(dw[d]);
     }
     // (a block whose scale is not finite gives NaN to the rows that see it)
     const float unit = vsp - vsp == 0.0f ? __builtin_amdgcn_ldexpf(kWeightUnit, kSumExp - ex) : __builtin_nanf("");
     if (sum != 0.0f) l = fmaf(sum * root, unit * root, l);
 #pragma unroll
     for (int h = 0; h < H; ++h) {
-      v4i s[PD];
+      v4i s[kDigits];
 #pragma unroll
-      for (int d = 0; d < PD; ++d) s[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vb[h], pd[d], zero, 0, 0, 0);
+      for (int d = 0; d < kDigits; ++d) s[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vb[h], pd[d], zero, 0, 0, 0);
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
-        float d[PD];
+        float d[kDigits];
 #pragma unroll
-        for (int n = 0; n < PD; ++n) d[n] = __int_as_float(s[n][v]);
+        for (int n = 0; n < kDigits; ++n) d[n] = __int_as_float(s[n][v]);
         // (in place: as a plain fma the compiler makes another register of it and
         // copies all of them back, a tenth of the loop)
-        const float sum = join<PD>(d);
+        const float sum = join(d);
         asm("v_fma_f32 %0, %1, %2, %0" : "+v"(o[h][v]) : "v"(sum), "v"(share));
       }
     }
@@ -711,11 +711,10 @@ size_t workspace_bytes(const lmx_kv8_cache *c, const lmx_kv8_batch *b, size_t n_
 
 template <class T, int HD>
 int launch_attention(const AttnArgs &a, int type, const Plan &p, hipStream_t st) {
-  constexpr int ND = sizeof(T) == 4 ? 3 : 2;
   const dim3 grid(unsigned(p.units), unsigned(a.c.n_kv), unsigned(a.splits));
   int r;
   if (p.rows == 16) {
-    kv8_rows_kernel<T, HD, ND><<<grid, dim3(256), 0, st>>>(a);
+    kv8_rows_kernel<T, HD><<<grid, dim3(256), 0, st>>>(a);
     r = launch_err("kv8 attention");
   } else {
     r = launch_prompt(a, type, HD, p.units, st);

@@ -85,26 +85,21 @@ constexpr int kSumExp = -24;
 constexpr float kSumUnit = 0x1p-24f;
 __device__ __forceinline__ float inverse_sum(float l) { return l == 0.0f ? 0.0f : kSumUnit / l; }
 
-// ND digit sums (from kMagic) -> the fixed-point sum, rounded once.
-template <int ND>
-__device__ __forceinline__ float join(const float (&d)[ND]) {
-  const float lo = fmaf(d[1], 256.0f, -257.0f * kMagic) + d[0];
-  if constexpr (ND == 2) return lo;
-  else return fmaf(d[2] - kMagic, 65536.0f, lo);
+constexpr int kDigits = 3;   // signed bytes of the fixed point of queries and weights
+// Digit sums (from kMagic) -> the fixed-point sum, rounded once.
+__device__ __forceinline__ float join(const float (&d)[kDigits]) {
+  return fmaf(d[2] - kMagic, 65536.0f, fmaf(d[1], 256.0f, -257.0f * kMagic) + d[0]);
 }
 
-// Four fixed-point values, each in the low bits of a word, 128 added to every
-// digit but the top one -> dword d of the result: their digits d.
-template <int ND>
-__device__ __forceinline__ void digit_words(const uint32_t (&u)[4], uint32_t (&w)[ND]) {
+// Four fixed-point values, each in the low bits of a word with kCarry added ->
+// dword d of the result: their digits d.
+constexpr int kCarry = 0x8080;   // 128 for every digit below the top
+__device__ __forceinline__ void digit_words(const uint32_t (&u)[4], uint32_t (&w)[kDigits]) {
   const uint32_t a = __builtin_amdgcn_perm(u[1], u[0], 0x05010400u), c = __builtin_amdgcn_perm(u[3], u[2], 0x05010400u);
+  const uint32_t b = __builtin_amdgcn_perm(u[1], u[0], 0x0C0C0602u), e = __builtin_amdgcn_perm(u[3], u[2], 0x0C0C0602u);
   w[0] = __builtin_amdgcn_perm(c, a, 0x05040100u) ^ 0x80808080u;
-  w[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
-  if constexpr (ND == 3) {
-    w[1] ^= 0x80808080u;
-    const uint32_t b = __builtin_amdgcn_perm(u[1], u[0], 0x0C0C0602u), e = __builtin_amdgcn_perm(u[3], u[2], 0x0C0C0602u);
-    w[2] = __builtin_amdgcn_perm(e, b, 0x05040100u);
-  }
+  w[1] = __builtin_amdgcn_perm(c, a, 0x07060302u) ^ 0x80808080u;
+  w[2] = __builtin_amdgcn_perm(e, b, 0x05040100u);
 }
 
 // A weight enters the fixed point as p 2^ex with ex its V scale's power of two,
@@ -118,31 +113,27 @@ __device__ __forceinline__ int value_exponent(float scale) {
 template <int D>
 __device__ __forceinline__ int lane_xor_int(int v, int lane) { return int(lane_xor_u32<D>(uint32_t(v), lane)); }
 
-template <int ND> struct Digits;
-// carry: 128 for every digit below the top; q_bits: |q| <= 2^q_bits
-template <> struct Digits<2> {
-  static constexpr int carry = 0x80, q_bits = 14;
-};
-template <> struct Digits<3> {
-  static constexpr int carry = 0x8080, q_bits = 22;
-};
+// Queries: |q| <= 2^kQueryBits.  Of two digits (14 bits) a head's loud channel would
+// leave the others fewer bits than a 16-bit type holds (64 times as loud 8), for 1 to
+// 5 % of a step.  (fp32's too lose what lies below 2^-23 of the loud one, about
+// what a sum of products in fp32 loses beside it.)
+constexpr int kQueryBits = 22;
 // The largest weight, of three digits: weight + carry stays below 2^23, so that
 // added to 2^23 it is the low bits of the float.
 constexpr float kWeightUnit = 8350000.0f;
 
 // A row's 16 contiguous elements of step m -> its digit words; f: the power of
 // two of the fixed point.
-template <int ND>
-__device__ __forceinline__ void query_digits(const float (&x)[16], float f, v4i (&w)[ND]) {
+__device__ __forceinline__ void query_digits(const float (&x)[16], float f, v4i (&w)[kDigits]) {
 #pragma unroll
   for (int b = 0; b < 4; ++b) {
-    uint32_t u[4], d[ND];
+    uint32_t u[4], d[kDigits];
 #pragma unroll
     for (int i = 0; i < 4; ++i)   // (the float's low bits are the rounded product, up to 2^22 on either side)
-      u[i] = __float_as_uint(fmaf(x[4 * b + i], f, kMagic)) + (uint32_t(Digits<ND>::carry) - 0x4B400000u);
-    digit_words<ND>(u, d);
+      u[i] = __float_as_uint(fmaf(x[4 * b + i], f, kMagic)) + (uint32_t(kCarry) - 0x4B400000u);
+    digit_words(u, d);
 #pragma unroll
-    for (int j = 0; j < ND; ++j) w[j][b] = int(d[j]);
+    for (int j = 0; j < kDigits; ++j) w[j][b] = int(d[j]);
   }
 }
 

@@ -1,6 +1,6 @@
 """Attention over the paged 8-bit cache (lutmac_kv8.h) where the bound of
 kv8_bounds.py says more than that of kv8_reference.py: rows whose weight lies in a
-few tokens."""
+few tokens, and queries with far channels."""
 import numpy as np
 import pytest
 import torch
@@ -66,3 +66,16 @@ def test_tail_behind_a_heavy_first_token_in_prompts(cuda, dtype, hd, group, n, s
     s = peaked(dtype, hd, group, n, share, False, zeros, new=70)
     assert kv8_bounds.tiled(dtype, f64(s.q), s.offsets, group)
     check(s)
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("hd,group", [(64, 3), (128, 1)])
+@pytest.mark.parametrize("loud", [60, 700])
+def test_queries_with_a_far_channel(cuda, dtype, hd, group, loud):
+    """One channel far louder than the others, which decide where the weight goes (its
+    keys are zero): they keep the bits that their type holds, in steps and in prompts."""
+    for new, old in (([1, 2], [40, 300]), ([70, 66], [0, 200])):
+        s = Setup(dtype, hd, 2, group, new, old, seed=50 + loud, behind=0)
+        s.q[..., 17] = loud
+        s.cache.k[..., 17] = 0
+        check(s)
