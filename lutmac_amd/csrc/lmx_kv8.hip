@@ -455,6 +455,10 @@ __global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(HD ==
     if ((n & (kWave - 1)) == kWave - 1 && p + W < p1) read_entries(p + W);
     const int t0 = p * kPage + 16 * g;   // this lane's first token
     if (t0 > last_pos || !ok) ksp = 0.0f, vsp = 0.0f;   // nothing of the block is seen: its scales may hold anything
+    // (of a block whose scale is not finite nothing is summed: rows that see it get
+    // NaN below, the tile's others are not to find its scale in their digits)
+    const bool finite = vsp - vsp == 0.0f;
+    if (!finite) vsp = 0.0f;
     int ex = value_exponent(vsp);
     exmax = max(exmax, max(ex, lane_xor_int<16>(ex, lane)));
     exmax = max(exmax, lane_xor_int<32>(exmax, lane));
@@ -517,9 +521,8 @@ __global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(HD ==
 #pragma unroll
       for (int d = 0; d < kDigits; ++d) pd[d][u] = int(dw[d]);
     }
-    // (a block whose scale is not finite gives NaN to the rows that see it)
-    const float unit = vsp - vsp == 0.0f ? __builtin_amdgcn_ldexpf(kWeightUnit, kSumExp - ex) : __builtin_nanf("");
-    if (sum != 0.0f) l = fmaf(sum * root, unit * root, l);
+    l = fmaf(sum * root, __builtin_amdgcn_ldexpf(kWeightUnit, kSumExp - ex) * root, l);
+    if (!finite && t0 <= limit) l = __builtin_nanf("");
 #pragma unroll
     for (int h = 0; h < H; ++h) {
       v4i s[kDigits];

@@ -1,6 +1,7 @@
 """Attention over the paged 8-bit cache (lutmac_kv8.h) where the bound of
 kv8_bounds.py says more than that of kv8_reference.py: rows whose weight lies in a
-few tokens, and queries with far channels."""
+few tokens, queries with far channels, and values that are not finite beside finite
+ones."""
 import numpy as np
 import pytest
 import torch
@@ -79,3 +80,34 @@ def test_queries_with_a_far_channel(cuda, dtype, hd, group, loud):
         s.q[..., 17] = loud
         s.cache.k[..., 17] = 0
         check(s)
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("hd,group", [(64, 2), (128, 4), (128, 1)])
+@pytest.mark.parametrize("new,old,bad", [(8, 12, 5), (3, 14, 2), (1, 63, 0), (10, 60, 4), (100, 30, 50)])
+def test_value_not_finite_beside_rows_before_it(cuda, dtype, hd, group, new, old, bad):
+    """A tile whose later rows see a block with a value that is not finite, its earlier
+    ones not; the places behind the last row hold the codes of whoever had the page
+    before."""
+    for value in (float("nan"), float("inf")):
+        s = Setup(dtype, hd, 2, group, [new, 1], [old, 5], seed=20 + bad, behind=0)
+        s.v[bad, 0, 7] = value
+        ref, q = s.check_append()
+        _, nan = check(s, q, ref)
+        sees = old + np.arange(new) >= (old + bad) // 16 * 16   # (rows from the block's first token on)
+        assert (nan[:new, :group] == sees[:, None, None]).all() and not nan[:, group:].any() and not nan[new:].any()
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("hd", [64, 128])
+def test_value_not_finite_of_little_weight(cuda, dtype, hd):
+    """A block that is not finite gives NaN to the rows that see it though their weights
+    of it are zero."""
+    s = Setup(dtype, hd, 1, 2, [1, 4], [200, 70], seed=31, behind=0)
+    s.q.copy_(torch.ones_like(s.q))
+    page = int(s.pages[0, 1])
+    s.cache.k_scale[page, 0, 2] = 1.0
+    s.cache.k[page, 0, 32:48] = -127   # scores some 1000 below the others
+    s.cache.v_scale[page, 0, 2] = float("nan")
+    _, nan = check(s)
+    assert nan[0].all() and not nan[1:].any()
