@@ -18,6 +18,7 @@
 
 #include <cmath>
 #include <initializer_list>
+#include <memory>
 #include <string>
 
 #include "lutmac_hip.h"
@@ -111,9 +112,29 @@ bool arguments(const char *name, Py_ssize_t got, Py_ssize_t want) {
 
 // ---- cache ----
 
+// The tensors of a cache: held, and looked at anew in every call, so that a call
+// writes what they are then and nothing that they gave up.
 struct Cache {
-  lmx_kv8_cache c;
-  int device;
+  at::Tensor k, v, scale[2];
+
+  // Their sizes and pointers, checked.
+  lmx_kv8_cache now() const {
+    if (k.dim() != 4 || k.size(2) != LMX_KV8_PAGE || (k.size(3) != 64 && k.size(3) != 128) || k.scalar_type() != at::kChar ||
+        !k.is_contiguous())
+      bad("k", k, "contiguous int8 [pages, kv_heads, 64, 64 or 128]");
+    const int64_t pages = k.size(0), heads = k.size(1), hd = k.size(3);
+    if (v.scalar_type() != at::kChar || !has_sizes(v, {pages, heads, hd, LMX_KV8_PAGE}) || !v.is_contiguous())
+      bad("v", v, "contiguous int8 [pages, kv_heads, head_dim, 64], as k has them");
+    if (v.device() != k.device()) raise_value("the cache's tensors must be on one device");
+    for (int i = 0; i < 2; ++i) {
+      const at::Tensor &s = scale[i];
+      if (s.scalar_type() != at::kFloat || !has_sizes(s, {pages, heads, LMX_KV8_PAGE / LMX_KV8_BLOCK}) || !s.is_contiguous())
+        bad(i ? "v_scale" : "k_scale", s, "contiguous float32 [pages, kv_heads, 4], as k has them");
+      if (s.device() != k.device()) raise_value("the cache's tensors must be on one device");
+    }
+    return {static_cast<int8_t *>(k.data_ptr()), static_cast<int8_t *>(v.data_ptr()), static_cast<float *>(scale[0].data_ptr()),
+            static_cast<float *>(scale[1].data_ptr()), size_t(pages), size_t(heads), size_t(hd)};
+  }
 };
 constexpr const char *kCache = "lutmac_amd.kv8_cache";
 const Cache &cache_of(PyObject *o) {
@@ -122,36 +143,15 @@ const Cache &cache_of(PyObject *o) {
   return *c;
 }
 
-// (k, v, k_scale, v_scale) -> the cache's sizes and pointers, checked; the
-// caller keeps the tensors.
+// (k, v, k_scale, v_scale) -> what the calls take.
 PyObject *kv8_cache(PyObject *, PyObject *const *args, Py_ssize_t n) {
   return guarded([&]() -> PyObject * {
     if (!arguments("kv8_cache", n, 4)) throw PyError{};
-    const at::Tensor &k = tensor("k", args[0]), &v = tensor("v", args[1]);
-    if (k.dim() != 4 || k.size(2) != LMX_KV8_PAGE || (k.size(3) != 64 && k.size(3) != 128) || k.scalar_type() != at::kChar ||
-        !k.is_contiguous())
-      bad("k", k, "contiguous int8 [pages, kv_heads, 64, 64 or 128]");
-    const int64_t pages = k.size(0), heads = k.size(1), hd = k.size(3);
-    if (v.scalar_type() != at::kChar || !has_sizes(v, {pages, heads, hd, LMX_KV8_PAGE}) || !v.is_contiguous())
-      bad("v", v, "contiguous int8 [pages, kv_heads, head_dim, 64], as k has them");
-    float *scales[2];
-    const char *names[2] = {"k_scale", "v_scale"};
-    if (v.device() != k.device()) raise_value("the cache's tensors must be on one device");
-    for (int i = 0; i < 2; ++i) {
-      const at::Tensor &s = tensor(names[i], args[2 + i]);
-      if (s.scalar_type() != at::kFloat || !has_sizes(s, {pages, heads, LMX_KV8_PAGE / LMX_KV8_BLOCK}) || !s.is_contiguous())
-        bad(names[i], s, "contiguous float32 [pages, kv_heads, 4], as k has them");
-      if (s.device() != k.device()) raise_value("the cache's tensors must be on one device");
-      scales[i] = static_cast<float *>(s.data_ptr());
-    }
-    Cache *c = new Cache{{static_cast<int8_t *>(k.data_ptr()), static_cast<int8_t *>(v.data_ptr()), scales[0], scales[1],
-                          size_t(pages), size_t(heads), size_t(hd)},
-                         k.is_cuda() ? int(k.get_device()) : -1};
-    PyObject *o = PyCapsule_New(c, kCache, [](PyObject *o) { delete static_cast<Cache *>(PyCapsule_GetPointer(o, kCache)); });
-    if (!o) {
-      delete c;
-      throw PyError{};
-    }
+    std::unique_ptr<Cache> c(new Cache{tensor("k", args[0]), tensor("v", args[1]), {tensor("k_scale", args[2]), tensor("v_scale", args[3])}});
+    c->now();
+    PyObject *o = PyCapsule_New(c.get(), kCache, [](PyObject *o) { delete static_cast<Cache *>(PyCapsule_GetPointer(o, kCache)); });
+    if (!o) throw PyError{};
+    c.release();
     return o;
   });
 }
@@ -166,7 +166,7 @@ size_t row_stride(const char *name, const at::Tensor &t, at::ScalarType type, in
 }
 
 // The call's batch, but for its tensors' device.
-lmx_kv8_batch batch_of(const Cache &c, PyObject *const *args, int64_t rows) {
+lmx_kv8_batch batch_of(PyObject *const *args, int64_t rows) {
   const at::Tensor &offsets = tensor("offsets", args[0]), &lengths = tensor("lengths", args[1]), &pages = tensor("pages", args[2]);
   if (pages.scalar_type() != at::kInt || pages.dim() != 2 || !pages.is_contiguous()) bad("pages", pages, "contiguous int32 of 2 dimensions");
   const int64_t n = pages.size(0);
@@ -180,7 +180,7 @@ lmx_kv8_batch batch_of(const Cache &c, PyObject *const *args, int64_t rows) {
 
 int check_call(const Cache &c, std::initializer_list<const at::Tensor *> tensors) {
   const int device = check_devices(tensors);
-  if (device != c.device) raise_value("expected tensors on the cache's device");
+  if (c.k.device() != (*tensors.begin())->device()) raise_value("expected tensors on the cache's device");
   return device;
 }
 
@@ -188,13 +188,14 @@ int check_call(const Cache &c, std::initializer_list<const at::Tensor *> tensors
 PyObject *kv8_append(PyObject *, PyObject *const *args, Py_ssize_t n) {
   return guarded([&]() -> PyObject * {
     if (!arguments("kv8_append", n, 9)) throw PyError{};
-    const Cache &c = cache_of(args[0]);
+    const Cache &held = cache_of(args[0]);
+    const lmx_kv8_cache c = held.now();
     const at::Tensor &k = tensor("k", args[1]), &v = tensor("v", args[2]);
     const int type = type_of("k", k);
     const at::ScalarType st = k.scalar_type();
-    const int64_t kv = int64_t(c.c.n_kv_heads), hd = int64_t(c.c.head_dim), rows = k.dim() ? k.size(0) : 0;
+    const int64_t kv = int64_t(c.n_kv_heads), hd = int64_t(c.head_dim), rows = k.dim() ? k.size(0) : 0;
     const size_t ks = row_stride("k", k, st, rows, kv, hd), vs = row_stride("v", v, st, rows, kv, hd);
-    const lmx_kv8_batch b = batch_of(c, args + 3, rows);
+    const lmx_kv8_batch b = batch_of(args + 3, rows);
     const at::Tensor *rope = args[6] != Py_None ? &tensor("rope", args[6]) : nullptr;
     const int64_t positions = rope && rope->dim() ? rope->size(0) : 0;
     if (rope && (rope->scalar_type() != at::kFloat || !has_sizes(*rope, {positions, hd / 2, 2}) || !rope->is_contiguous()))
@@ -205,10 +206,10 @@ PyObject *kv8_append(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const int64_t heads = q && q->dim() == 3 ? q->size(1) : 0;
     const size_t qs = q ? row_stride("q", *q, st, rows, heads, hd) : 0;
     const size_t os = given ? row_stride("q_out", *given, st, rows, heads, hd) : size_t(heads * hd);
-    const int device = check_call(c, {&k, &v, &THPVariable_Unpack(args[3]), &THPVariable_Unpack(args[4]), &THPVariable_Unpack(args[5]), rope, q, given});
+    const int device = check_call(held, {&k, &v, &THPVariable_Unpack(args[3]), &THPVariable_Unpack(args[4]), &THPVariable_Unpack(args[5]), rope, q, given});
     at::Tensor out;
     if (q) out = given ? *given : at::empty({rows, heads, hd}, q->options());
-    check(lmx_kv8_append(&c.c, &b, type, k.data_ptr(), ks, v.data_ptr(), vs, q ? q->data_ptr() : nullptr, qs,
+    check(lmx_kv8_append(&c, &b, type, k.data_ptr(), ks, v.data_ptr(), vs, q ? q->data_ptr() : nullptr, qs,
                          q ? out.data_ptr() : nullptr, os, size_t(heads), rope ? static_cast<const float *>(rope->data_ptr()) : nullptr,
                          size_t(positions), stream_on(device)));
     if (!out.defined()) Py_RETURN_NONE;
@@ -239,23 +240,24 @@ at::Tensor workspace_of(PyObject *given, size_t need, int device, void *&p, size
 PyObject *kv8_attend(PyObject *, PyObject *const *args, Py_ssize_t n) {
   return guarded([&]() -> PyObject * {
     if (!arguments("kv8_attend", n, 8)) throw PyError{};
-    const Cache &c = cache_of(args[0]);
+    const Cache &held = cache_of(args[0]);
+    const lmx_kv8_cache c = held.now();
     const at::Tensor &q = tensor("q", args[1]);
     const int type = type_of("q", q);
-    const int64_t hd = int64_t(c.c.head_dim), rows = q.dim() == 3 ? q.size(0) : 0, heads = q.dim() == 3 ? q.size(1) : 0;
+    const int64_t hd = int64_t(c.head_dim), rows = q.dim() == 3 ? q.size(0) : 0, heads = q.dim() == 3 ? q.size(1) : 0;
     const size_t qs = row_stride("q", q, q.scalar_type(), rows, heads, hd);
-    const lmx_kv8_batch b = batch_of(c, args + 2, rows);
+    const lmx_kv8_batch b = batch_of(args + 2, rows);
     double scale = 1.0 / std::sqrt(double(hd));
     if (args[5] != Py_None && (scale = PyFloat_AsDouble(args[5])) == -1.0 && PyErr_Occurred()) throw PyError{};
     const at::Tensor *given = args[6] != Py_None ? &tensor("out", args[6]) : nullptr;
     const size_t os = given ? row_stride("out", *given, q.scalar_type(), rows, heads, hd) : size_t(heads * hd);
-    const int device = check_call(c, {&q, &THPVariable_Unpack(args[2]), &THPVariable_Unpack(args[3]), &THPVariable_Unpack(args[4]), given});
+    const int device = check_call(held, {&q, &THPVariable_Unpack(args[2]), &THPVariable_Unpack(args[3]), &THPVariable_Unpack(args[4]), given});
     at::Tensor out = given ? *given : at::empty({rows, heads, hd}, q.options());
     size_t need = 0, bytes = 0;
-    check(lmx_kv8_attention_workspace(&c.c, &b, type, size_t(heads), &need));
+    check(lmx_kv8_attention_workspace(&c, &b, type, size_t(heads), &need));
     void *work;
     const at::Tensor w = workspace_of(args[7], need, device, work, bytes);
-    check(lmx_kv8_attention(&c.c, &b, type, q.data_ptr(), qs, size_t(heads), float(scale), out.data_ptr(), os, work, bytes,
+    check(lmx_kv8_attention(&c, &b, type, q.data_ptr(), qs, size_t(heads), float(scale), out.data_ptr(), os, work, bytes,
                             stream_on(device)));
     if (args[6] != Py_None) return Py_NewRef(args[6]);
     return THPVariable_Wrap(std::move(out));

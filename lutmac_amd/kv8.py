@@ -34,13 +34,18 @@ def rope_table(positions, head_dim, theta=10000.0, factor=1.0, device="cuda"):
 class KvCache8:
     """One layer's cache on tensors that the caller may hold too: k int8 [pages,
     kv_heads, 64, head_dim], v int8 [pages, kv_heads, head_dim, 64], k_scale and
-    v_scale fp32 [pages, kv_heads, 4]; value = code * scale."""
+    v_scale fp32 [pages, kv_heads, 4]; value = code * scale.  The cache holds its
+    tensors, which are not replaced (another cache costs little to make)."""
 
     def __init__(self, k, v, k_scale, v_scale):
         self._ops = torch_module()
         self._c = self._ops.kv8_cache(k, v, k_scale, v_scale)   # (checks them)
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._tensors = k, v, k_scale, v_scale
 
+    k = property(lambda self: self._tensors[0])
+    v = property(lambda self: self._tensors[1])
+    k_scale = property(lambda self: self._tensors[2])
+    v_scale = property(lambda self: self._tensors[3])
     n_pages = property(lambda self: self.k.shape[0])
     n_kv_heads = property(lambda self: self.k.shape[1])
     head_dim = property(lambda self: self.k.shape[3])
