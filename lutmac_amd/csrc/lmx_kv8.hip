@@ -2,6 +2,7 @@
 // append, and attention of a few rows per sequence over it.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "lmx_kv8.hpp"
 
@@ -359,8 +360,14 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
 // us and 4 for the merge): table entries
 // come 64 at a time, and a page's keys and values are requested as soon as the
 // registers of the page before are free of theirs.
+//
+// With head_dim 128 the registers are those of two workgroups a CU for fp32 and
+// fp16, of three for bf16 (us, two / three: 64 sequences of up to 2048 tokens 18.4 /
+// 19.8, 16 of 4000 32.4 / 30.3, 32 of 20 to 33 thousand 380 / 354).
+template <class T>
+constexpr bool kThree = std::is_same<T, bf16>::value;
 template <class T, int HD>
-__global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(HD == 128 ? 2 : 3))) void kv8_rows_kernel(AttnArgs a) {
+__global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(HD == 128 && !kThree<T> ? 2 : 3))) void kv8_rows_kernel(AttnArgs a) {
   constexpr int W = 4, M = HD / 64, H = HD / 16;
   __shared__ float os[W][16][HD + 4];
   __shared__ float ms[W][16], ls[W][16];
@@ -693,13 +700,13 @@ Plan plan(const lmx_kv8_cache *c, const lmx_kv8_batch *b, size_t n_heads, int ty
   Plan p{};
   p.rows = type != LMX_F32 && b->n_rows * group >= 64 * b->n_seqs ? kPromptRows : 16;
   p.units = b->n_rows * group / p.rows + b->n_seqs;
-  // As many parts as fill the device once (three workgroups per CU; two with
-  // head_dim 128 and of prompts: a workgroup more runs a second round) if
+  // As many parts as fill the device once (three workgroups per CU; two of fp32
+  // and fp16 with head_dim 128 and of prompts: a workgroup more runs a second round) if
   // the sequences have equal shares of the rows, of four pages at least, one per
   // wave (prompts: 8).
   const size_t each = (b->n_rows + b->n_seqs - 1) / b->n_seqs;
   const size_t wgs = b->n_seqs * ((each * group + p.rows - 1) / p.rows) * c->n_kv_heads;
-  const size_t room = p.rows > 16 || c->head_dim == 128 ? 512 : 768;
+  const size_t room = p.rows > 16 || (type != LMX_BF16 && c->head_dim == 128) ? 512 : 768;
   const size_t s = std::min<size_t>(room / wgs, b->max_pages / (p.rows == 16 ? 4 : 8));
   p.splits = int(std::max<size_t>(1, std::min<size_t>(s, 64)));
   return p;
