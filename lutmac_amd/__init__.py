@@ -415,12 +415,14 @@ class Weight:
     def codes_i8(self, stream=None):
         """(codes [rows, cols] int8, scales [rows] fp32) of an 8-bit handle with one
         scale per row, on the device, as linear_i8 takes them."""
-        import torch
-        width = -(-self.cols // 16) * 16
-        codes = torch.empty(self.rows, width, dtype=torch.int8, device="cuda")
-        scales = torch.empty(self.rows, dtype=torch.float32, device="cuda")
-        check(lib().lmx_weight_codes_i8(self._h, codes.data_ptr(), width, scales.data_ptr(), _stream_ptr(stream)))
-        return codes[:, :self.cols], scales
+        def call():
+            import torch
+            width = -(-self.cols // 16) * 16
+            codes = torch.empty(self.rows, width, dtype=torch.int8, device="cuda")
+            scales = torch.empty(self.rows, dtype=torch.float32, device="cuda")
+            check(lib().lmx_weight_codes_i8(self._h, codes.data_ptr(), width, scales.data_ptr(), _stream_ptr(None)))
+            return codes[:, :self.cols], scales
+        return on_stream(stream, call)
 
     def close(self):
         if self._h:
