@@ -124,13 +124,14 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
   const SeqRows r = unit_rows(a.c, int(blockIdx.x), 1, 2, lane, kPage);
   const int from = max(r.start, 0);   // rows before position 0 have no place
   const int end = a.rope ? min(r.len, a.rope_n) : r.len;   // (rows past the rotation table are left out)
-  const int pi = from / kPage + (int(blockIdx.x) - r.first), t0 = pi * kPage;
-  if (r.seq < 0 || r.n == 0 || t0 >= end) return;
+  const int pi = from / kPage + (int(blockIdx.x) - r.first);
+  if (r.seq < 0 || end <= from || pi > (end - 1) / kPage) return;
+  const int t0 = pi * kPage;   // (at most 2^31 - kPage, whatever the length: t0 + kPage may be past int)
   const int role = int(blockIdx.y), n_kv = a.c.n_kv;
   if (role >= 2 * n_kv) {   // query heads: 8 lanes a row and head
     constexpr int QE = 8, QL = HD / 2 / QE, SLOTS = 256 / QL;
     const int h0 = (role - 2 * n_kv) * kHeads, heads = min(kHeads, a.c.n_heads - h0);
-    const int first = max(from, t0), items = (min(end, t0 + kPage) - first) * heads;
+    const int first = max(from, t0), items = (min(end - t0, kPage) - (first - t0)) * heads;
     const int slot = int(threadIdx.x) / QL, d0 = int(threadIdx.x) % QL * QE;
     const int inverse = 65536 / heads + 1;   // (item / heads, exactly for the up to 512)
     constexpr int U = sizeof(T) == 4 ? 1 : 4;   // rows of a lane on their way
