@@ -97,16 +97,18 @@ int lmx_kv8_attention_workspace(const lmx_kv8_cache *cache,
  * (out_stride; elements of `type`) may be q.
  * Products with the codes are exact, sums and softmax statistics fp32.  Before
  * the products queries are rounded to 2^-23 of a power of two above the largest
- * of their head, the weights of the values to 2^-23 of the largest of their page
- * or, of 64 rows and more a sequence in the 16-bit types,
- * to 2^-11 of themselves.  V scales
+ * of their head, the weights of the values to 2^-23 of the largest of their page.
+ * Large calls of prompts in the 16-bit types hold queries to 2^-39 and weights to
+ * 2^-11 of themselves: those where each = ceil(n_rows / n_seqs) * n_heads /
+ * n_kv_heads is 96 or more and n_seqs * n_kv_heads * ceil(each / 16) 1024 or more,
+ * so that the last bits of a row depend on the call that it is in.  V scales
  * lie between 2^-100 and 2^100; those below 2^-60 of the largest in reach lose
  * bits like the small values of one block do.  A query head with an element
  * that is not finite gives NaN.
  * The work is split by the call's sizes alone, as if its sequences had equal
  * shares of the rows: long prompts and single tokens after long contexts are
  * faster in calls of their own (4096 rows of one sequence and single ones of 63
- * after 8000, 32 + 8 heads of 128, bf16: 714 us together, 163 + 211 apart).
+ * after 8000, 32 + 8 heads of 128, bf16: 722 us together, 164 + 209 apart).
  * workspace: lmx_kv8_attention_workspace bytes, 16-byte aligned, in any state;
  * calls that may overlap in time need workspaces of their own. */
 int lmx_kv8_attention(const lmx_kv8_cache *cache, const lmx_kv8_batch *batch,

@@ -698,17 +698,25 @@ struct Plan {
 
 Plan plan(const lmx_kv8_cache *c, const lmx_kv8_batch *b, size_t n_heads, int type) {
   const size_t group = n_heads / c->n_kv_heads;
+  const size_t each = (b->n_rows + b->n_seqs - 1) / b->n_seqs * group;   // rows of a sequence, if they have equal shares
+  const auto tiles = [&](size_t rows) { return b->n_seqs * ((each + rows - 1) / rows) * c->n_kv_heads; };
+  // 256 rows a workgroup, of 16-bit types, where their tiles are not mostly empty
+  // and tiles of 16 would be four a CU and more, each of them with the pages to read
+  // (us, 16 / 256 rows a workgroup, bf16, KV heads: 16 tokens x 4 heads after 500, 8
+  // of 128, 13 / 25; 606 x 4 after 300, 8 of 64, 21 / 28; 64 sequences of 16 x 4 after
+  // 4000, 8 of 64, 160 / 201, of 24 x 4 after 0 22 / 20; 8 of 130 x 2 after 300, 8 of 128,
+  // 25 / 26; 27 of 54 x 2, 8 of 128, 18 / 13; 43 of 68 x 4 after 6000, 4 of 128, 450 / 394.
+  // It is wrong for fewer tiles of long contexts: 8 of 28 x 8 after 6000, 8 of 128,
+  // 181 / 116.  Over 108 calls of 1 to 91 sequences this rule's times are 3 % above
+  // the better kernel's; those of 256 rows from 64 a sequence on were 20 %.)
   Plan p{};
-  p.rows = type != LMX_F32 && b->n_rows * group >= 64 * b->n_seqs ? kPromptRows : 16;
+  p.rows = type != LMX_F32 && each >= 96 && tiles(16) >= 1024 ? kPromptRows : 16;
   p.units = b->n_rows * group / p.rows + b->n_seqs;
   // As many parts as fill the device once (three workgroups per CU; two of fp32
-  // and fp16 with head_dim 128 and of prompts: a workgroup more runs a second round) if
-  // the sequences have equal shares of the rows, of four pages at least, one per
-  // wave (prompts: 8).
-  const size_t each = (b->n_rows + b->n_seqs - 1) / b->n_seqs;
-  const size_t wgs = b->n_seqs * ((each * group + p.rows - 1) / p.rows) * c->n_kv_heads;
+  // and fp16 with head_dim 128 and of prompts: a workgroup more runs a second round),
+  // of four pages at least, one per wave (prompts: 8).
   const size_t room = p.rows > 16 || (type != LMX_BF16 && c->head_dim == 128) ? 512 : 768;
-  const size_t s = std::min<size_t>(room / wgs, b->max_pages / (p.rows == 16 ? 4 : 8));
+  const size_t s = std::min<size_t>(room / tiles(p.rows), b->max_pages / (p.rows == 16 ? 4 : 8));
   p.splits = int(std::max<size_t>(1, std::min<size_t>(s, 64)));
   return p;
 }
