@@ -1080,27 +1080,29 @@ int prefill_pass(lmx_decoder *d, int p0, int T, hipStream_t st) {
     const lmx_decoder::Layer &L = d->layers[l];
     float *kc = d->kcache + l * per_layer, *vc = d->vcache + l * per_layer;
     if ((r = digit_rows(d, L.qkv, d->p_hidden, d->p_qkv, M, L.qkv_bias, nullptr, L.in_norm, kEpiStore, st))) return r;
+    const bool last = l + 1 == c.n_layers;   // (of the last layer only keys and values are needed)
     if (kv8) {
-      if ((r = kv8_layer_rows(d, l, d->p_qkv, size_t(T), l + 1 == c.n_layers ? nullptr : d->p_attn, d->p_kv8_work,
-                              d->p_kv8_work_bytes, st)))
+      if ((r = kv8_layer_rows(d, l, d->p_qkv, size_t(T), last ? nullptr : d->p_attn, d->p_kv8_work, d->p_kv8_work_bytes, st)))
         return r;
-    } else if (hd == 64)
-      prefill_rope_kernel<64><<<rope_grid, dim3(256), 0, st>>>(d->p_qkv, d->rope, kc, vc, int(c.n_heads),
-                                                              int(c.n_kv_heads), T, p0, d->kv_seq);
-    else
-      prefill_rope_kernel<128><<<rope_grid, dim3(256), 0, st>>>(d->p_qkv, d->rope, kc, vc, int(c.n_heads),
-                                                               int(c.n_kv_heads), T, p0, d->kv_seq);
-    if ((r = launch_err("prefill_rope"))) return r;
-    if (l + 1 == c.n_layers) break;
-    if (kv8) {
-    } else if (hd == 64)
-      prefill_attention_kernel<64><<<attn_grid, dim3(256), 0, st>>>(d->p_qkv, kc, vc, int(c.n_heads),
-                                                                   int(c.n_kv_heads), T, p0, scale, d->kv_seq, d->p_attn);
-    else
-      prefill_attention_kernel<128><<<attn_grid, dim3(256), 0, st>>>(
-          d->p_qkv, kc, vc, int(c.n_heads), int(c.n_kv_heads), T, p0, scale, d->kv_seq, d->p_attn);
-    if ((r = launch_err("prefill_attention")) ||
-        (r = digit_rows(d, L.o, d->p_attn, d->p_hidden, M, nullptr, d->p_hidden, nullptr, kEpiStore, st)) ||
+      if (last) break;
+    } else {
+      if (hd == 64)
+        prefill_rope_kernel<64><<<rope_grid, dim3(256), 0, st>>>(d->p_qkv, d->rope, kc, vc, int(c.n_heads),
+                                                                int(c.n_kv_heads), T, p0, d->kv_seq);
+      else
+        prefill_rope_kernel<128><<<rope_grid, dim3(256), 0, st>>>(d->p_qkv, d->rope, kc, vc, int(c.n_heads),
+                                                                 int(c.n_kv_heads), T, p0, d->kv_seq);
+      if ((r = launch_err("prefill_rope"))) return r;
+      if (last) break;
+      if (hd == 64)
+        prefill_attention_kernel<64><<<attn_grid, dim3(256), 0, st>>>(
+            d->p_qkv, kc, vc, int(c.n_heads), int(c.n_kv_heads), T, p0, scale, d->kv_seq, d->p_attn);
+      else
+        prefill_attention_kernel<128><<<attn_grid, dim3(256), 0, st>>>(
+            d->p_qkv, kc, vc, int(c.n_heads), int(c.n_kv_heads), T, p0, scale, d->kv_seq, d->p_attn);
+      if ((r = launch_err("prefill_attention"))) return r;
+    }
+    if ((r = digit_rows(d, L.o, d->p_attn, d->p_hidden, M, nullptr, d->p_hidden, nullptr, kEpiStore, st)) ||
         (r = digit_mlp(d, L, d->p_hidden, d->p_gate_up, d->p_act, M, st)))
       return r;
   }
