@@ -79,9 +79,9 @@ int lmx_decoder_create_batched(const lmx_decoder_config *cfg, size_t batch, lmx_
  * positions, and a block's codes are rounded anew when its scale grows, so
  * logits depend a little on whether a prompt was read in passes or step by step
  * (no counterpart in the reference, whose cache is fp32).  It pays where the
- * cache is what a step reads: at the 1B width a layer's step takes 36 us against
- * 29 with fp32 at 2048 positions of one sequence, 43 against 42 at 16384, 63
- * against 74 at 4096 positions of 8 sequences and 79 against 107 at 2048 of 32;
+ * cache is what a step reads: at the 1B width a layer's step takes 35 us against
+ * 29 with fp32 at 2048 positions of one sequence, 41 against 42 at 16384, 62
+ * against 74 at 4096 positions of 8 sequences and 79 against 106 at 2048 of 32;
  * a prompt of 16000 tokens takes half the time. */
 #define LMX_KV_F32 0
 #define LMX_KV_INT8 1

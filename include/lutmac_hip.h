@@ -186,8 +186,8 @@ int lmx_linear(const lmx_weight *w, const float *bias, const float *x,
  * round(127 x / amax) of its largest magnitude amax (ties to even, exactly), and
  *   y[b][r] = (sum_k c[b][k] w[r][k]) * (amax[b] / 127) * w_scale[r] + bias[r],
  * the sum exact, the rest fp32, rounded once to y's type.  w: signed bytes, row
- * r at w + r * w_stride (w and w_stride multiples of 16; cols any number up to
- * 131072; the bytes between cols and w_stride are not used); x, bias (or NULL)
+ * r at w + r * w_stride (w and w_stride multiples of 16, the stride at most
+ * 262144; cols any number up to 131072; the bytes between cols and w_stride are not used); x, bias (or NULL)
  * and y [batch][rows] have elements of `type` (lmx_type) and their own alignment
  * only.  A row of x with an element that is not finite gives NaN.  y does not
  * overlap x.  workspace: lmx_linear_i8_workspace bytes, 16-byte aligned, in any

@@ -40,7 +40,7 @@ typedef struct {
   float *k_scale;    /* [n_pages][n_kv_heads][4] */
   float *v_scale;    /* [n_pages][n_kv_heads][4] */
   size_t n_pages;    /* < 2^31 */
-  size_t n_kv_heads;
+  size_t n_kv_heads; /* 1 .. 512; query heads: 1 .. 64 times as many */
   size_t head_dim;   /* 64 or 128 */
 } lmx_kv8_cache;
 
@@ -48,17 +48,17 @@ typedef struct {
  * offsets[s] .. offsets[s + 1] - 1 are the last of the lengths[s] tokens that
  * sequence s has with them, in order (none: the sequence has no row in this
  * call).  Token j of sequence s lies in page pages[s * max_pages + j / 64].
- * offsets do not decrease; rows from offsets[n_seqs] on belong to no sequence
- * and are neither read nor written.  A row whose position is negative (more
+ * offsets do not decrease; rows below offsets[0] and from offsets[n_seqs] on belong
+ * to no sequence and are neither read nor written.  A row whose position is negative (more
  * rows than lengths[s]) or past the table has no place in the cache and sees
  * nothing there; nor has one whose page is outside 0 .. n_pages - 1. */
 typedef struct {
   const int32_t *offsets;  /* [n_seqs + 1] */
   const int32_t *lengths;  /* [n_seqs] */
   const int32_t *pages;    /* [n_seqs][max_pages] */
-  size_t n_seqs;
-  size_t max_pages;
-  size_t n_rows;           /* rows that the row arrays hold, >= offsets[n_seqs] */
+  size_t n_seqs;           /* <= 2^20 */
+  size_t max_pages;        /* <= 2^24 */
+  size_t n_rows;           /* rows that the row arrays hold, >= offsets[n_seqs]; <= 2^24 */
 } lmx_kv8_batch;
 
 /* Rotates and appends: for every row, its keys k and values v (row r at
@@ -86,14 +86,15 @@ int lmx_kv8_append(const lmx_kv8_cache *cache, const lmx_kv8_batch *batch,
                    size_t rope_positions, void *stream);
 
 /* Bytes of workspace that lmx_kv8_attention needs for a call of these sizes
- * (pointers are not looked at; 0 is possible). */
+ * (pointers are not looked at; 0 is possible).  Fewer rows can need more: their
+ * pages are split over workgroups. */
 int lmx_kv8_attention_workspace(const lmx_kv8_cache *cache,
                                 const lmx_kv8_batch *batch, int type,
                                 size_t n_heads, size_t *bytes);
 /* Attention of the rows' queries (row r at q + r * q_stride, [n_heads]
  * [head_dim], rotated) over their sequences' cached tokens up to their own
  * positions: out = softmax(scale * q . k) v, query head h reading KV head
- * h / (n_heads / n_kv_heads).  A row that sees nothing gets zeros.  out
+ * h / (n_heads / n_kv_heads), scale positive.  A row that sees nothing gets zeros.  out
  * (out_stride; elements of `type`) may be q.
  * Products with the codes are exact, sums and softmax statistics fp32.  Before
  * the products queries are rounded to 2^-23 of a power of two above the largest

@@ -354,10 +354,10 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
 // The 4 waves take pages in turn, grid.z parts ("splits") a share of them;
 // (m, l, o) of the waves merge in LDS, of the parts in kv8_merge_kernel.
 // Bound by the cache's bytes where contexts are long (32 sequences of 20 to 33
-// thousand tokens, 8 KV heads of 128: 346 us, 5.0 TB/s, what a copy reaches),
+// thousand tokens, 8 KV heads of 128, bf16: 349 us, 5.0 TB/s, what a copy reaches),
 // else by the chain of loads (offsets, table, page, and each further page of a
-// wave; one row of 320 tokens: 5.9 us) and some 320 vector and 48 matrix
-// instructions a page of head_dim 128 (64 sequences of up to 2048 tokens, fp32: 14.7
+// wave; one row of 320 tokens: 5.9 us) and some 450 vector and 48 matrix
+// instructions a page of head_dim 128 (64 sequences of up to 2048 tokens, fp32: 14.5
 // us and 4 for the merge): table entries
 // come 64 at a time, and a page's keys and values are requested as soon as the
 // registers of the page before are free of theirs.

@@ -8,7 +8,9 @@
 //   S^T = K Q^T: key row i = 8 b + 4 h' + r of a 32-token tile is its token 16 h'
 //     + 4 b + r, so lane (row j, h) ends with the 16 tokens of block h in order:
 //     one K and one V scale per lane, and P^T's operand in place;
-//   O^T = V^T P^T with weights p 2^E in fp16 (11 bits each).
+//   O^T = V^T P^T with weights p 2^E in fp16: 11 bits each, which moves an fp16
+//     output by about its own rounding and a bf16 one by an eighth of that (with
+//     byte digits, as steps have them, the kernel took 1052 us).
 // p is relative to a running reference of score + log2(V scale), raised only
 // when a row outgrows it by 2^kRoom: then, seldom, the sums are scaled down.
 //
@@ -17,8 +19,9 @@
 // flight: while the matrix cores sum the values of the tile before, the scores
 // of this one are scaled, and while they make the scores of the next, its
 // weights.  Two sequences of 4096 rows after 4096, 32 query and 8 KV heads of 128:
-// 862 us, 950 TFLOP/s (vector unit busy two thirds of the time, matrix cores 0.42;
-// operands read three or four steps ahead instead of two change nothing).
+// 863 to 882 us by card, 930 to 950 TFLOP/s (CUs busy 0.95 of the time, of that the
+// vector unit 0.62 and the matrix cores 0.45; operands read three or four steps
+// ahead instead of two change nothing).
 #include "lmx_kv8.hpp"
 
 namespace lmx {
