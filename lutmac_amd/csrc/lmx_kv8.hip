@@ -707,7 +707,7 @@ Plan plan(const lmx_kv8_cache *c, const lmx_kv8_batch *b, size_t n_heads, int ty
   // 4000, 8 of 64, 160 / 201, of 24 x 4 after 0 22 / 20; 8 of 130 x 2 after 300, 8 of 128,
   // 25 / 26; 27 of 54 x 2, 8 of 128, 18 / 13; 43 of 68 x 4 after 6000, 4 of 128, 450 / 394.
   // It is wrong for fewer tiles of long contexts: 8 of 28 x 8 after 6000, 8 of 128,
-  // 181 / 116.  Over 108 calls of 1 to 91 sequences this rule's times are 3 % above
+  // 181 / 116.  Over 110 calls of 1 to 91 sequences this rule's times are 3 % above
   // the better kernel's; those of 256 rows from 64 a sequence on were 20 %.)
   Plan p{};
   p.rows = type != LMX_F32 && each >= 96 && tiles(16) >= 1024 ? kPromptRows : 16;
