@@ -228,6 +228,11 @@ def run(s):
 
 # ---- the plain forms -------------------------------------------------------
 
+def power_of_two(e):
+    """2^e in fp32, exactly (a power function may be off in its last bit)."""
+    return ((e + 127) << 23).view(torch.float32)
+
+
 def plain_linear(s):
     x, w, scale = s["x"].float(), s["w"].float(), s["w_scale"]
     m, k, n = x.shape[0], x.shape[1], w.shape[0]
@@ -236,9 +241,9 @@ def plain_linear(s):
     top = x.abs().amax(-1, keepdim=True)
     half, e = torch.frexp(top)                       # top = half * 2^e, half in [0.5, 1)
     e = (e - 9 + (half > E4M3_MOST / 512).int()).clamp_min(LEAST_EXPONENT)   # the least with top <= 448 * 2^e
-    e = torch.where(top > 0, e, LEAST_EXPONENT)
-    code = torch.ldexp(x, -e).to(torch.float8_e4m3fn).float()
-    x = torch.ldexp(code, e).view(m, blocks * BLOCK)[:, :k]
+    e = torch.where(top > 0, e, LEAST_EXPONENT).int()
+    code = (x * power_of_two(-e)).to(torch.float8_e4m3fn).float()
+    x = (code * power_of_two(e)).view(m, blocks * BLOCK)[:, :k]
     w = w * scale.repeat_interleave(BLOCK, 0)[:n].repeat_interleave(BLOCK, 1)[:, :k]
     y = x @ w.t()
     if s["bias"] is not None:
@@ -355,6 +360,10 @@ def exact(case, seed):
     return {"linear": exact_linear, "verify": exact_verify, "pages": lambda s: None, "rotary": exact_rotary}[case["op"]](s)
 
 
+def exact_power(e):
+    return (e + 1023 << 52).view(torch.float64)
+
+
 def exact_linear(s):
     x, w, scale = s["x"].double(), s["w"].float().double(), s["w_scale"].double()
     out = []
@@ -363,12 +372,15 @@ def exact_linear(s):
         for b in range(scale.shape[1]):
             cols = slice(b * BLOCK, min((b + 1) * BLOCK, x.shape[1]))
             block = part[:, cols]
-            least = torch.ceil(torch.log2(block.abs().max(1).values / E4M3_MOST).clamp(LEAST_EXPONENT, 200))
-            # (log2 of a number next to a power of two may round across it)
-            least = torch.where(torch.exp2(least - 1) * E4M3_MOST >= block.abs().max(1).values, least - 1, least).clamp_min(LEAST_EXPONENT)
-            unit = torch.exp2(least)[:, None]
+            top = block.abs().max(1).values
+            least = torch.full_like(top, LEAST_EXPONENT, dtype=torch.int64)
+            for e in range(LEAST_EXPONENT, 120):
+                least += (top > E4M3_MOST * 2.0 ** e).long()
+            unit = exact_power(least)[:, None]
             value = block / unit
-            step = torch.exp2(torch.floor(torch.log2(value.abs().clamp_min(2.0 ** -6))) - 3)   # e4m3: 4 bits, 2^-9 at least
+            # e4m3: 4 bits from the first on, down to 2^-9
+            bits = value.abs().clamp_min(2.0 ** -6).view(torch.int64) >> 52
+            step = exact_power(bits - 1023 - 3)
             value = torch.round(value / step) * step * unit
             rows = scale[:, b].repeat_interleave(BLOCK)[: w.shape[0]]
             y += torch.matmul(value, w[:, cols].T.contiguous()) * rows
