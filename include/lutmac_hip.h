@@ -203,6 +203,31 @@ int lmx_linear_i8(const int8_t *w, size_t w_stride, const float *w_scale,
  * w_scale [rows], device buffers of the caller. */
 int lmx_weight_codes_i8(const lmx_weight *w, int8_t *codes, size_t w_stride,
                         float *scales, void *stream);
+/* A linear layer in 8-bit floating point (e4m3: 4 exponent bits, 3 of mantissa,
+ * largest 448; no counterpart in the reference) for weights that come with a
+ * scale per block of 128 x 128: value of w[r][k] = code * w_scale[r / 128][k / 128].
+ * Every 128 columns of a row of x share a scale too, the smallest power of two s
+ * with amax <= 448 s (at least 2^-126), so that x / s is exact; c = x / s rounded
+ * to e4m3 (ties to even), and
+ *   y[b][r] = sum_j s[b][j] w_scale[r / 128][j] (sum of c w over k of block j) + bias[r],
+ * rounded once to y's type.  Sums are fp32, for fp32 x with every product exact;
+ * for the 16-bit types the products of 64 or 128 k that one matrix instruction
+ * takes lose what lies below 2^-13 of their largest (about 2^-16 of y; half a
+ * step of fp16 is 2^-11).
+ * w: codes, row r at w + r * w_stride (w and w_stride multiples of 16, the
+ * stride at most 262144; cols any number up to 131072; the bytes between cols and
+ * w_stride are not used); w_scale contiguous, [ceil(rows / 128)][ceil(cols / 128)];
+ * x, bias (or NULL) and y [batch][rows] have elements of `type` (lmx_type) and
+ * their own alignment only.  128 columns of x with an element that is not finite
+ * give NaN in their row of y.  y does not overlap x.  workspace:
+ * lmx_linear_f8_workspace bytes, 16-byte aligned, in any state; calls that may
+ * overlap in time need workspaces of their own.  Nothing is allocated: calls can
+ * be captured into a HIP graph. */
+int lmx_linear_f8_workspace(size_t rows, size_t cols, size_t batch, int type, size_t *bytes);
+int lmx_linear_f8(const uint8_t *w, size_t w_stride, const float *w_scale,
+                  const void *bias, const void *x, void *y, int type,
+                  size_t rows, size_t cols, size_t batch, void *workspace,
+                  size_t workspace_bytes, void *stream);
 /* In-place blockwise FWHT-256 (transform.hpp:19 apply_hadamard_rotation);
  * n a multiple of 256 (whole chunks only, as the reference). */
 int lmx_fwht256(float *x, size_t n, void *stream);

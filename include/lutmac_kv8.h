@@ -117,6 +117,62 @@ int lmx_kv8_attention(const lmx_kv8_cache *cache, const lmx_kv8_batch *batch,
                       float scale, void *out, size_t out_stride,
                       void *workspace, size_t workspace_bytes, void *stream);
 
+/* Whose pages are whose: a page table as lmx_kv8_batch has it, the sequences'
+ * lengths and a stack of free pages, all on the device, so that a step is planned
+ * without the host.  Pages of a table row belong to its sequence alone. */
+typedef struct {
+  int32_t *pages;      /* [n_seqs][max_pages] */
+  int32_t *lengths;    /* [n_seqs] */
+  int32_t *free_pages; /* [n_pages], the stack: the last of the first n_free[0] is on top */
+  int32_t *n_free;     /* [1] */
+  size_t n_seqs;       /* <= 2^20 */
+  size_t max_pages;    /* <= 2^24 */
+  size_t n_pages;      /* < 2^31 */
+} lmx_kv8_pages;
+
+/* Makes room for new_tokens[s] tokens of every sequence s (none where it is 0 or
+ * less) and says where they go.  A sequence gets all of its tokens or none
+ * (granted[s]): none where they would pass the end of its table row or of 2^31 - 1
+ * tokens; where the tokens of those asked for up to and with s are more than
+ * n_rows; and, if it needs pages, where the pages needed up to and with s are more
+ * than are free.  (Those left out for their table row count for nothing, the others
+ * whether granted or not.)  Then
+ *   offsets [n_seqs + 1]: the rows of the granted tokens, as lmx_kv8_batch has them;
+ *   lengths: grown by granted;
+ *   pages: the new pages, taken from the top of the stack in the order of sequences
+ *   and tokens;
+ *   positions [n_rows], slots [n_rows] (or NULL): each row's position in its
+ *   sequence, and page * 64 + position % 64 (-1 where the row's page is negative).
+ *   Rows from offsets[n_seqs] on stay as they are. */
+int lmx_kv8_extend(const lmx_kv8_pages *pages, const int32_t *new_tokens, size_t n_rows,
+                   int32_t *offsets, int32_t *granted, int32_t *positions,
+                   int64_t *slots, void *stream);
+/* Takes the last drop[s] tokens (all, where it has fewer; none below 0) from every
+ * sequence s: drafts that were rejected, or a sequence that has ended.  Pages that
+ * hold none of its tokens any more go back to the stack (their table entries
+ * become -1), those of the first sequence on top and of each sequence the earliest, so
+ * that taking back what one lmx_kv8_extend granted restores the stack. */
+int lmx_kv8_trim(const lmx_kv8_pages *pages, const int32_t *drop, void *stream);
+
+/* Rotates rows to their positions: for row r and each head of q ([n_heads]
+ * [head_dim], row r at q + r * q_stride) and of k ([n_kv_heads][head_dim]; NULL:
+ * q only), the first rotary_dim elements are turned in pairs, (a, b) -> (a c - b s,
+ * a s + b c) with (c, s) = rope[positions[r]][pair]; the rest is copied.
+ * rope [rope_positions][rotary_dim / 2] pairs, 8-byte aligned.  interleaved 0: the
+ * pairs are (d, d + rotary_dim / 2), as the reference's apply_rope has them
+ * (embedding.cpp:36-75); 1: (2 d, 2 d + 1).  inverse 1: by -s, which undoes it and
+ * is its gradient.  Rows whose position is negative or not below rope_positions are
+ * left out: neither read nor written.  q_out may be q, k_out k (with the same
+ * stride); else they do not overlap.  Computed in fp32 and rounded once.  At most 1024 heads each, head_dim at most 1024,
+ * rotary_dim even and at most head_dim; strides count elements and are at least a row's (rows <= 1: any);
+ * alignment that of the elements (16 bytes, and sizes that are whole groups of 16
+ * bytes, are faster). */
+int lmx_rotary(int type, const void *q, size_t q_stride, void *q_out, size_t q_out_stride,
+               size_t n_heads, const void *k, size_t k_stride, void *k_out,
+               size_t k_out_stride, size_t n_kv_heads, size_t head_dim,
+               size_t rotary_dim, int interleaved, int inverse, const int32_t *positions,
+               size_t rows, const float *rope, size_t rope_positions, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

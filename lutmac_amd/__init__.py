@@ -35,6 +35,7 @@ EXPORTS = [
     "lmx_weight_kernel_config", "lmx_weight_read_tiles", "lmx_gemv", "lmx_linear", "lmx_fwht256",
     "lmx_precompute_luts", "lmx_extract_indices", "lmx_hbm_read_probe", "lmx_hbm_read_probe_shape",
     "lmx_hbm_read_probe_tiles", "lmx_linear_i8_workspace", "lmx_linear_i8", "lmx_weight_codes_i8",
+    "lmx_linear_f8_workspace", "lmx_linear_f8",
     # include/lutmac_hip_compat.h
     "lmx_host_gemv", "lmx_host_lut_linear", "lmx_host_apply_hadamard_rotation",
     "lmx_host_precompute_luts", "lmx_host_precompute_lut", "lmx_host_extract_indices", "lmx_host_forget",
@@ -48,7 +49,9 @@ EXPORTS = [
     # include/lutmac_model.h
     "lmx_model_load", "lmx_model_load_kv", "lmx_model_destroy", "lmx_model_config", "lmx_model_decoder", "lmx_model_weight_format",
     # include/lutmac_kv8.h
-    "lmx_kv8_append", "lmx_kv8_attention_workspace", "lmx_kv8_attention",
+    "lmx_kv8_append", "lmx_kv8_attention_workspace", "lmx_kv8_attention", "lmx_kv8_extend", "lmx_kv8_trim", "lmx_rotary",
+    # include/lutmac_verify.h
+    "lmx_verify_drafts_workspace", "lmx_verify_drafts",
 ]
 
 # lmx_type (include/lutmac_hip.h): activations of the calls that take more than fp32
@@ -76,6 +79,20 @@ class Kv8BatchC(ctypes.Structure):
     """lmx_kv8_batch (include/lutmac_kv8.h)."""
     _fields_ = [("offsets", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("pages", ctypes.c_void_p),
                 ("n_seqs", ctypes.c_size_t), ("max_pages", ctypes.c_size_t), ("n_rows", ctypes.c_size_t)]
+
+
+class Kv8PagesC(ctypes.Structure):
+    """lmx_kv8_pages (include/lutmac_kv8.h)."""
+    _fields_ = [("pages", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("free_pages", ctypes.c_void_p),
+                ("n_free", ctypes.c_void_p), ("n_seqs", ctypes.c_size_t), ("max_pages", ctypes.c_size_t),
+                ("n_pages", ctypes.c_size_t)]
+
+
+class DraftsC(ctypes.Structure):
+    """lmx_drafts (include/lutmac_verify.h)."""
+    _fields_ = [("offsets", ctypes.c_void_p), ("drafts", ctypes.c_void_p), ("uniforms", ctypes.c_void_p),
+                ("temperature", ctypes.c_void_p), ("n_seqs", ctypes.c_size_t), ("n_rows", ctypes.c_size_t),
+                ("vocab", ctypes.c_size_t)]
 
 
 class LmxError(RuntimeError):
@@ -152,6 +169,13 @@ _SIGS = {
     "lmx_linear_i8_workspace": ([_sz, _sz, _sz, ctypes.POINTER(_sz)], _i),
     "lmx_linear_i8": ([_p, _sz, _p, _p, _p, _p, _i, _sz, _sz, _sz, _p, _sz, _p], _i),
     "lmx_weight_codes_i8": ([_p, _p, _sz, _p, _p], _i),
+    "lmx_linear_f8_workspace": ([_sz, _sz, _sz, _i, ctypes.POINTER(_sz)], _i),
+    "lmx_linear_f8": ([_p, _sz, _p, _p, _p, _p, _i, _sz, _sz, _sz, _p, _sz, _p], _i),
+    "lmx_kv8_extend": ([_p, _p, _sz, _p, _p, _p, _p, _p], _i),
+    "lmx_kv8_trim": ([_p, _p, _p], _i),
+    "lmx_rotary": ([_i, _p, _sz, _p, _sz, _sz, _p, _sz, _p, _sz, _sz, _sz, _sz, _i, _i, _p, _sz, _p, _sz, _p], _i),
+    "lmx_verify_drafts_workspace": ([_p, _i, ctypes.POINTER(_sz)], _i),
+    "lmx_verify_drafts": ([_p, _i, _p, _sz, _p, _sz, _p, _p, _p, _sz, _p], _i),
     "lmx_kv8_append": ([_p, _p, _i, _p, _sz, _p, _sz, _p, _sz, _p, _sz, _sz, _p, _sz, _p], _i),
     "lmx_kv8_attention_workspace": ([_p, _p, _i, _sz, ctypes.POINTER(_sz)], _i),
     "lmx_kv8_attention": ([_p, _p, _i, _p, _sz, _sz, ctypes.c_float, _p, _sz, _p, _sz, _p], _i),
@@ -474,6 +498,67 @@ def linear_i8_workspace(rows, cols, batch):
     """Bytes of workspace of a linear_i8 call."""
     n = ctypes.c_size_t()
     check(lib().lmx_linear_i8_workspace(rows, cols, batch, ctypes.byref(n)))
+    return n.value
+
+
+def blocks_f8(w):
+    """Weights [rows, cols] (a torch tensor) -> (codes float8_e4m3fn [rows, cols] whose
+    rows start on multiples of 16 bytes, w_scale fp32 [ceil(rows / 128), ceil(cols /
+    128)]) as linear_f8 takes them: value = code * scale of its 128 x 128 block, scale
+    = amax / 448 of the block (1 for a block of zeros)."""
+    import torch
+    rows, cols = w.shape
+    n, k = -(-rows // 128), -(-cols // 128)
+    full = torch.nn.functional.pad(w.detach().float(), (0, k * 128 - cols, 0, n * 128 - rows)).view(n, 128, k, 128)
+    scale = full.abs().amax((1, 3)) / 448.0
+    scale = torch.where(scale > 0, scale, 1.0)
+    codes = (full / scale[:, None, :, None]).clamp_(-448.0, 448.0).to(torch.float8_e4m3fn).view(n * 128, k * 128)
+    return codes[:rows, :cols], scale
+
+
+def linear_f8(x, w, w_scale, bias=None, y=None, workspace=None, stream=None):
+    """Linear layer in 8-bit floating point (lmx_linear_f8): x [..., cols] fp32, fp16 or
+    bf16, w [rows, cols] float8_e4m3fn whose rows start on multiples of 16 bytes (any
+    row stride that is one), w_scale fp32 [ceil(rows / 128), ceil(cols / 128)], bias
+    [rows] of x's type.  x is rounded to e4m3 too, with a power of two per row and 128
+    columns.  Returns [..., rows] of x's type.  workspace: a uint8 tensor of at least
+    linear_f8_workspace bytes that no overlapping call uses (default: torch
+    allocates one for the call)."""
+    return on_stream(stream, torch_module().linear_f8, x, w, w_scale, bias, y, workspace)
+
+
+def _type_of(dtype):
+    import torch
+    return {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}[dtype]
+
+
+def linear_f8_workspace(rows, cols, batch, dtype):
+    """Bytes of workspace of a linear_f8 call."""
+    n = ctypes.c_size_t()
+    check(lib().lmx_linear_f8_workspace(rows, cols, batch, _type_of(dtype), ctypes.byref(n)))
+    return n.value
+
+
+def verify_drafts(logits, drafts, offsets, uniforms, probs=None, temperature=None, accepted=None, tokens=None,
+                  workspace=None, stream=None):
+    """Which drafted tokens a step keeps, and the token that follows (lmx_verify_drafts).
+
+    Rows offsets[s] .. offsets[s + 1] - 1 are sequence s's, one more than it has
+    drafted tokens: logits [rows, vocab] fp32, fp16 or bf16 of the target (rows any
+    stride apart), drafts int32 [rows] (the entry of a sequence's last row is not
+    looked at), uniforms fp32 [rows, 2] in [0, 1), probs fp32 [rows, vocab] the
+    draft's probabilities (None: the drafted token had 1), temperature fp32
+    [sequences] (None: 1; 0: greedy).  Returns (accepted int32 [sequences], tokens
+    int32 [rows]): row by row the accepted tokens, the token sampled after them, then
+    -1.  Rows of no sequence stay as they are in `tokens` (in a new tensor, anything)."""
+    return on_stream(stream, torch_module().verify_drafts, logits, drafts, offsets, uniforms, probs, temperature, accepted,
+                     tokens, workspace)
+
+
+def verify_drafts_workspace(n_seqs, rows, vocab, dtype):
+    """Bytes of workspace of a verify_drafts call."""
+    d, n = DraftsC(None, None, None, None, n_seqs, rows, vocab), ctypes.c_size_t()
+    check(lib().lmx_verify_drafts_workspace(ctypes.byref(d), _type_of(dtype), ctypes.byref(n)))
     return n.value
 
 

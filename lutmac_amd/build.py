@@ -39,6 +39,10 @@ SOURCES = [
     ("lmx_kv8.hip", True),
     ("lmx_kv8_prompt.hip", True),
     ("lmx_i8.hip", True),
+    ("lmx_f8.hip", True),
+    ("lmx_rotary.hip", True),
+    ("lmx_pages.hip", True),
+    ("lmx_verify.hip", True),
     ("lmx_capi.cpp", False),
     ("lmx_repack.cpp", False),
     ("lut_gemm_compat.cpp", False),
@@ -105,7 +109,7 @@ def build(verbose=True):
         _run(command, verbose)
     else:
         print(f"torch's headers are not installed: {os.path.basename(TORCH_LIB)} is left out "
-              "(lutmac_amd.kv8 and lutmac_amd.linear_i8 need it, the C interface does not)", flush=True)
+              "(lutmac_amd.kv8, linear_i8, linear_f8 and verify_drafts need it, the C interface does not)", flush=True)
     return LIB
 
 

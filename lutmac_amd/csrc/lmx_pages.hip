@@ -1,0 +1,259 @@
+// lmx_pages.hip -- the page table of the 8-bit cache kept on the device
+// (lmx_kv8_extend, lmx_kv8_trim): which sequences get their tokens, where each
+// row goes, and the stack of free pages.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "lmx_internal.hpp"
+#include "lutmac_kv8.h"
+
+namespace lmx {
+namespace {
+
+constexpr int kPage = LMX_KV8_PAGE, kThreads = 1024, kWaves = kThreads / kWave;
+
+struct PagesArgs {
+  int *pages, *lengths, *free_pages, *n_free;
+  int n_seqs, n_pages;
+  size_t max_pages;
+  const int *count;   // new or dropped tokens
+  int n_rows;
+  int *offsets, *granted, *positions;
+  long long *slots;
+};
+
+// Sums that stop at 2^32 - 1, past every limit that they are compared with: in
+// any order they come out the same.
+__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
+
+// Inclusive sums over the workgroup's threads of N numbers each on top of
+// base[N], which grows by all of them.
+template <int N>
+__device__ __forceinline__ void block_sums(uint32_t (&v)[N], uint32_t (&base)[N], uint32_t (*waves)[kWaves]) {
+  const int lane = threadIdx.x & (kWave - 1), wave = int(threadIdx.x) / kWave;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+      const uint32_t o = __shfl_up(v[n], d);
+      if (lane >= d) v[n] = add_sat(v[n], o);
+    }
+    if (lane == kWave - 1) waves[n][wave] = v[n];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    uint32_t before = base[n], all = base[n];
+    for (int w = 0; w < kWaves; ++w) {
+      const uint32_t o = waves[n][w];
+      if (w < wave) before = add_sat(before, o);
+      all = add_sat(all, o);
+    }
+    v[n] = add_sat(v[n], before);
+    base[n] = all;
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ uint32_t pages_of(uint32_t tokens) { return (tokens + kPage - 1) / kPage; }
+
+// n pages between a table row (from its entry `first` on) and the stack (from its
+// place `top` down): f(table entry, stack place) for each, by the thread itself
+// or, of many, by its wave.
+template <class F>
+__device__ __forceinline__ void each_page(uint32_t n, size_t first, uint32_t top, F f) {
+  if (n <= kWave)
+    for (uint32_t j = 0; j < n; ++j) f(first + j, top - j);
+  uint64_t many = __builtin_amdgcn_ballot_w64(n > kWave);
+  while (many) {
+    const int from = __builtin_ctzll(many);
+    many &= many - 1;
+    const auto pick = [from](uint32_t v) { return uint32_t(__builtin_amdgcn_readlane(int(v), from)); };
+    const uint32_t all = pick(n), t = pick(top);
+    const size_t e = size_t(pick(uint32_t(first >> 32))) << 32 | pick(uint32_t(first));
+    for (uint32_t j = threadIdx.x & (kWave - 1); j < all; j += kWave) f(e + j, t - j);
+  }
+}
+
+// Row r is the token at `pos` of sequence s.
+__device__ __forceinline__ void place_row(const PagesArgs &a, int r, int s, int pos) {
+  a.positions[r] = pos;
+  if (!a.slots) return;
+  const int page = a.pages[size_t(s) * a.max_pages + pos / kPage];
+  a.slots[r] = page < 0 ? -1 : (long long)page * kPage + pos % kPage;
+}
+
+// The last of n ascending numbers (the first of which is at most r) that is at
+// most r.
+__device__ __forceinline__ int last_at_most(const int *v, int n, int r) {
+  int lo = 0;
+  while (n > 1) {
+    const int half = n / 2;
+    const bool up = v[lo + half] <= r;
+    lo = up ? lo + half : lo;
+    n = up ? n - half : half;
+  }
+  return lo;
+}
+
+// One workgroup over all sequences, a thread each, kThreads of them at a time:
+// the sums of new tokens, pages and granted tokens are all that couples them.
+// ROWS: places the rows as well.
+template <bool ROWS>
+__global__ __launch_bounds__(kThreads) void extend_kernel(PagesArgs a) {
+  __shared__ uint32_t waves[2][kWaves], used;
+  __shared__ int begin[kThreads], start[kThreads];
+  const uint32_t have = uint32_t(min(max(*a.n_free, 0), a.n_pages));
+  uint32_t asked[2] = {0, 0}, rows[1] = {0};
+  if (threadIdx.x == 0) used = 0, a.offsets[0] = 0;
+  for (int s0 = 0; s0 < a.n_seqs; s0 += kThreads) {
+    const int s = s0 + int(threadIdx.x);
+    const bool live = s < a.n_seqs;
+    const uint32_t old = live ? uint32_t(max(a.lengths[s], 0)) : 0;
+    uint32_t add = live ? uint32_t(max(a.count[s], 0)) : 0;
+    if (size_t(old) + add > min(a.max_pages * kPage, size_t(0x7FFFFFFF))) add = 0;
+    const uint32_t first = pages_of(old), need = add ? pages_of(old + add) - first : 0;
+    uint32_t v[2] = {add, need};
+    block_sums<2>(v, asked, waves);
+    const bool yes = add && v[0] <= uint32_t(a.n_rows) && (need == 0 || v[1] <= have);
+    const uint32_t before = rows[0];
+    uint32_t g[1] = {yes ? add : 0};
+    block_sums<1>(g, rows, waves);
+    if (live) {
+      a.granted[s] = yes ? int(add) : 0;
+      a.offsets[s + 1] = int(g[0]);
+      if (yes) a.lengths[s] = int(old + add);
+    }
+    // (a sequence that gets pages is behind none that needed some and got none)
+    const uint32_t take = yes ? need : 0;
+    if (take) atomicMax(&used, v[1]);
+    each_page(take, size_t(s) * a.max_pages + first, have - 1 - (v[1] - need),
+              [&](size_t entry, uint32_t place) { a.pages[entry] = a.free_pages[place]; });
+    if constexpr (ROWS) {
+      begin[threadIdx.x] = int(g[0]) - (yes ? int(add) : 0);
+      start[threadIdx.x] = int(old);
+      __syncthreads();
+      const int n = min(kThreads, a.n_seqs - s0);
+      for (int r = int(before + threadIdx.x); r < int(rows[0]); r += kThreads) {
+        const int i = last_at_most(begin, n, r);
+        place_row(a, r, s0 + i, start[i] + r - begin[i]);
+      }
+    }
+    __syncthreads();
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) *a.n_free = int(have - used);
+}
+
+// The rows of the call, where they are many.
+__global__ __launch_bounds__(256) void rows_kernel(PagesArgs a) {
+  const int r = int(blockIdx.x * 256 + threadIdx.x);
+  if (r >= a.offsets[a.n_seqs]) return;
+  const int s = last_at_most(a.offsets, a.n_seqs, r);
+  place_row(a, r, s, a.lengths[s] - a.offsets[s + 1] + r);
+}
+
+__global__ __launch_bounds__(kThreads) void trim_kernel(PagesArgs a) {
+  __shared__ uint32_t waves[1][kWaves];
+  const uint32_t have = uint32_t(min(max(*a.n_free, 0), a.n_pages));
+  struct Cut { uint32_t keep, kept, gone; bool live; };
+  const auto cut = [&](int s) {
+    Cut c{};
+    c.live = s < a.n_seqs;
+    if (!c.live) return c;
+    const uint32_t old = uint32_t(max(a.lengths[s], 0)), drop = uint32_t(max(a.count[s], 0));
+    c.keep = old - min(old, drop);
+    c.kept = uint32_t(min(size_t(pages_of(c.keep)), a.max_pages));
+    c.gone = uint32_t(min(size_t(pages_of(old)), a.max_pages)) - c.kept;
+    return c;
+  };
+  uint32_t all[1] = {0};   // pages of the whole call
+  for (int s0 = 0; s0 < a.n_seqs; s0 += kThreads) {
+    uint32_t v[1] = {cut(s0 + int(threadIdx.x)).gone};
+    block_sums<1>(v, all, waves);
+  }
+  uint32_t before[1] = {0};
+  for (int s0 = 0; s0 < a.n_seqs; s0 += kThreads) {
+    const int s = s0 + int(threadIdx.x);
+    const Cut c = cut(s);
+    uint32_t v[1] = {c.gone};
+    block_sums<1>(v, before, waves);
+    each_page(c.gone, size_t(s) * a.max_pages + c.kept, have + all[0] - 1 - (v[0] - c.gone), [&](size_t entry, uint32_t place) {
+      if (place < uint32_t(a.n_pages)) a.free_pages[place] = a.pages[entry];   // (pages freed twice may be more than there are)
+      a.pages[entry] = -1;
+    });
+    if (c.live) a.lengths[s] = int(c.keep);
+  }
+  if (threadIdx.x == 0) *a.n_free = int(min(add_sat(have, all[0]), uint32_t(a.n_pages)));
+}
+
+int launch_err(const char *what) {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? LMX_OK : fail(LMX_ERR_LAUNCH_FAILED, "%s launch: %s", what, hipGetErrorString(e));
+}
+
+int check_pages(const lmx_kv8_pages *p) {
+  if (!p) return fail(LMX_ERR_INVALID_ARGUMENT, "NULL pointer");
+  if (p->n_seqs > (1u << 20) || p->max_pages > (1u << 24) || p->n_pages >= (1u << 31))
+    return fail(LMX_ERR_INVALID_ARGUMENT, "%zu sequences of %zu pages, %zu pages: at most 2^20, 2^24 and 2^31 - 1", p->n_seqs, p->max_pages, p->n_pages);
+  return LMX_OK;
+}
+int check_pointers(const lmx_kv8_pages *p, const int32_t *count) {
+  if (!p->n_free || (p->n_seqs && (!p->lengths || !count)) || (p->n_seqs && p->max_pages && !p->pages) || (p->n_pages && !p->free_pages))
+    return fail(LMX_ERR_INVALID_ARGUMENT, "NULL pointer");
+  if ((reinterpret_cast<size_t>(p->lengths) | reinterpret_cast<size_t>(p->n_free) | reinterpret_cast<size_t>(p->pages) |
+       reinterpret_cast<size_t>(p->free_pages) | reinterpret_cast<size_t>(count)) % 4)
+    return fail(LMX_ERR_INVALID_ARGUMENT, "pointers must be aligned to their elements");
+  return LMX_OK;
+}
+PagesArgs pages_args(const lmx_kv8_pages *p, const int32_t *count) {
+  PagesArgs a{};
+  a.pages = p->pages, a.lengths = p->lengths, a.free_pages = p->free_pages, a.n_free = p->n_free;
+  a.n_seqs = int(p->n_seqs), a.n_pages = int(p->n_pages), a.max_pages = p->max_pages, a.count = count;
+  return a;
+}
+
+// Rows that the one workgroup places itself.
+constexpr size_t kFewRows = 8192;
+
+}  // namespace
+}  // namespace lmx
+
+using namespace lmx;
+
+extern "C" {
+
+int lmx_kv8_extend(const lmx_kv8_pages *pages, const int32_t *new_tokens, size_t n_rows, int32_t *offsets, int32_t *granted,
+                   int32_t *positions, int64_t *slots, void *stream) {
+  int r = check_pages(pages);
+  if (r) return r;
+  if (n_rows > (1u << 24)) return fail(LMX_ERR_INVALID_ARGUMENT, "%zu rows: at most 2^24", n_rows);
+  if (!offsets || (pages->n_seqs && !granted) || (n_rows && !positions)) return fail(LMX_ERR_INVALID_ARGUMENT, "NULL pointer");
+  if ((reinterpret_cast<size_t>(offsets) | reinterpret_cast<size_t>(granted) | reinterpret_cast<size_t>(positions)) % 4 ||
+      reinterpret_cast<size_t>(slots) % 8)
+    return fail(LMX_ERR_INVALID_ARGUMENT, "pointers must be aligned to their elements");
+  if ((r = check_pointers(pages, new_tokens))) return r;
+  PagesArgs a = pages_args(pages, new_tokens);
+  a.n_rows = int(n_rows);
+  a.offsets = offsets, a.granted = granted, a.positions = positions, a.slots = reinterpret_cast<long long *>(slots);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (n_rows <= kFewRows) {
+    extend_kernel<true><<<1, kThreads, 0, st>>>(a);
+    return launch_err("kv8 extend");
+  }
+  extend_kernel<false><<<1, kThreads, 0, st>>>(a);
+  if ((r = launch_err("kv8 extend"))) return r;
+  rows_kernel<<<unsigned((n_rows + 255) / 256), 256, 0, st>>>(a);
+  return launch_err("kv8 extend rows");
+}
+
+int lmx_kv8_trim(const lmx_kv8_pages *pages, const int32_t *drop, void *stream) {
+  int r = check_pages(pages);
+  if (r || pages->n_seqs == 0) return r;
+  if ((r = check_pointers(pages, drop))) return r;
+  trim_kernel<<<1, kThreads, 0, static_cast<hipStream_t>(stream)>>>(pages_args(pages, drop));
+  return launch_err("kv8 trim");
+}
+
+}  // extern "C"

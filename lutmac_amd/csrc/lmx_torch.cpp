@@ -1,6 +1,6 @@
-// lmx_torch.cpp -- the 8-bit serving operators on torch tensors: what
-// lutmac_amd.kv8 and lutmac_amd.linear_i8 check of their arguments, the outputs
-// and workspaces that they allocate, and their calls into the C ABI.
+// lmx_torch.cpp -- the serving operators on torch tensors: what lutmac_amd.kv8,
+// linear_i8, linear_f8 and verify_drafts check of their arguments, the outputs and
+// workspaces that they allocate, and their calls into the C ABI.
 //
 // A serving loop calls them eagerly many times a step, and in Python a call's
 // checks took longer than the kernels of a small one (host time of an append of 64
@@ -23,6 +23,7 @@
 
 #include "lutmac_hip.h"
 #include "lutmac_kv8.h"
+#include "lutmac_verify.h"
 
 namespace {
 
@@ -264,43 +265,232 @@ PyObject *kv8_attend(PyObject *, PyObject *const *args, Py_ssize_t n) {
   });
 }
 
+// What the two linear layers' arguments have in common: their sizes, the output.
+struct Linear {
+  const at::Tensor &x, &w, &scale;
+  const at::Tensor *bias, *given;
+  int type;
+  int64_t rows, cols, batch;
+
+  Linear(PyObject *const *args, at::ScalarType codes)
+      : x(tensor("x", args[0])), w(tensor("w", args[1])), scale(tensor("w_scale", args[2])),
+        bias(args[3] != Py_None ? &tensor("bias", args[3]) : nullptr), given(args[4] != Py_None ? &tensor("y", args[4]) : nullptr),
+        type(type_of("x", x)) {
+    if (w.dim() != 2 || w.scalar_type() != codes || w.stride(1) != 1)
+      bad("w", w, std::string(c10::toString(codes)) + " [rows, cols] with neighbouring columns side by side");
+    rows = w.size(0), cols = w.size(1);
+    if (x.dim() == 0 || x.size(-1) != cols || !x.is_contiguous()) bad("x", x, "contiguous, " + std::to_string(cols) + " values a row");
+  }
+  void check_scale(at::IntArrayRef sizes) const {
+    if (scale.scalar_type() != at::kFloat || !has_sizes(scale, sizes) || !scale.is_contiguous()) {
+      std::string s;
+      for (const int64_t n : sizes) s += (s.empty() ? "" : ", ") + std::to_string(n);
+      bad("w_scale", scale, "contiguous float32 [" + s + "]");
+    }
+  }
+  int check_rest() {   // -> the device
+    if (bias && (bias->scalar_type() != x.scalar_type() || !has_sizes(*bias, {rows}) || !bias->is_contiguous()))
+      bad("bias", *bias, std::string("contiguous ") + c10::toString(x.scalar_type()) + " [" + std::to_string(rows) + "]");
+    batch = cols ? x.numel() / cols : 0;
+    if (given && (given->scalar_type() != x.scalar_type() || given->numel() != batch * rows || !given->is_contiguous()))
+      bad("y", *given, "contiguous, of x's type, " + std::to_string(batch) + " x " + std::to_string(rows));
+    return check_devices({&x, &w, &scale, bias, given});
+  }
+  at::Tensor output() const {
+    if (given) return *given;
+    auto sizes = x.sizes().vec();
+    sizes.back() = rows;
+    return at::empty(sizes, x.options());
+  }
+  size_t stride() const { return size_t(rows > 1 ? w.stride(0) : (cols + 15) / 16 * 16); }   // (that of a single row says nothing)
+  const float *scales() const { return static_cast<const float *>(scale.data_ptr()); }
+  void *bias_pointer() const { return bias ? bias->data_ptr() : nullptr; }
+};
+
 // (x, w, w_scale, bias, y, workspace) -> y
 PyObject *linear_i8(PyObject *, PyObject *const *args, Py_ssize_t n) {
   return guarded([&]() -> PyObject * {
     if (!arguments("linear_i8", n, 6)) throw PyError{};
-    const at::Tensor &x = tensor("x", args[0]), &w = tensor("w", args[1]), &scale = tensor("w_scale", args[2]);
-    const int type = type_of("x", x);
-    if (w.dim() != 2 || w.scalar_type() != at::kChar || w.stride(1) != 1) bad("w", w, "int8 [rows, cols] with neighbouring columns side by side");
-    const int64_t rows = w.size(0), cols = w.size(1);
-    if (x.dim() == 0 || x.size(-1) != cols || !x.is_contiguous()) bad("x", x, "contiguous, " + std::to_string(cols) + " values a row");
-    if (scale.scalar_type() != at::kFloat || !has_sizes(scale, {rows}) || !scale.is_contiguous())
-      bad("w_scale", scale, "contiguous float32 [" + std::to_string(rows) + "]");
-    const at::Tensor *bias = args[3] != Py_None ? &tensor("bias", args[3]) : nullptr;
-    if (bias && (bias->scalar_type() != x.scalar_type() || !has_sizes(*bias, {rows}) || !bias->is_contiguous()))
-      bad("bias", *bias, std::string("contiguous ") + c10::toString(x.scalar_type()) + " [" + std::to_string(rows) + "]");
-    const int64_t batch = cols ? x.numel() / cols : 0;
-    const at::Tensor *given = args[4] != Py_None ? &tensor("y", args[4]) : nullptr;
-    if (given && (given->scalar_type() != x.scalar_type() || given->numel() != batch * rows || !given->is_contiguous()))
-      bad("y", *given, "contiguous, of x's type, " + std::to_string(batch) + " x " + std::to_string(rows));
-    const int device = check_devices({&x, &w, &scale, bias, given});
+    Linear l(args, at::kChar);
+    l.check_scale({l.rows});
+    const int device = l.check_rest();
     size_t need = 0, bytes = 0;
-    check(lmx_linear_i8_workspace(size_t(rows), size_t(cols), size_t(batch), &need));
-    at::Tensor y;
-    if (given) {
-      y = *given;
-    } else {
-      auto sizes = x.sizes().vec();
-      sizes.back() = rows;
-      y = at::empty(sizes, x.options());
-    }
+    check(lmx_linear_i8_workspace(size_t(l.rows), size_t(l.cols), size_t(l.batch), &need));
+    at::Tensor y = l.output();
     void *work;
     const at::Tensor ws = workspace_of(args[5], need, device, work, bytes);
-    // (the stride of a single row says nothing)
-    check(lmx_linear_i8(static_cast<const int8_t *>(w.data_ptr()), size_t(rows > 1 ? w.stride(0) : (cols + 15) / 16 * 16),
-                        static_cast<const float *>(scale.data_ptr()), bias ? bias->data_ptr() : nullptr, x.data_ptr(), y.data_ptr(), type, size_t(rows),
-                        size_t(cols), size_t(batch), work, bytes, stream_on(device)));
-    if (args[4] != Py_None) return Py_NewRef(args[4]);
+    check(lmx_linear_i8(static_cast<const int8_t *>(l.w.data_ptr()), l.stride(), l.scales(), l.bias_pointer(), l.x.data_ptr(), y.data_ptr(),
+                        l.type, size_t(l.rows), size_t(l.cols), size_t(l.batch), work, bytes, stream_on(device)));
+    if (l.given) return Py_NewRef(args[4]);
     return THPVariable_Wrap(std::move(y));
+  });
+}
+
+// (x, w, w_scale, bias, y, workspace) -> y
+PyObject *linear_f8(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject * {
+    if (!arguments("linear_f8", n, 6)) throw PyError{};
+    Linear l(args, at::kFloat8_e4m3fn);
+    l.check_scale({(l.rows + 127) / 128, (l.cols + 127) / 128});
+    const int device = l.check_rest();
+    size_t need = 0, bytes = 0;
+    check(lmx_linear_f8_workspace(size_t(l.rows), size_t(l.cols), size_t(l.batch), l.type, &need));
+    at::Tensor y = l.output();
+    void *work;
+    const at::Tensor ws = workspace_of(args[5], need, device, work, bytes);
+    check(lmx_linear_f8(static_cast<const uint8_t *>(l.w.data_ptr()), l.stride(), l.scales(), l.bias_pointer(), l.x.data_ptr(), y.data_ptr(),
+                        l.type, size_t(l.rows), size_t(l.cols), size_t(l.batch), work, bytes, stream_on(device)));
+    if (l.given) return Py_NewRef(args[4]);
+    return THPVariable_Wrap(std::move(y));
+  });
+}
+
+// ---- pages, rotation, verification ----
+
+// A contiguous tensor of whole numbers.
+const at::Tensor &whole(const char *name, PyObject *o, at::ScalarType type, at::IntArrayRef sizes) {
+  const at::Tensor &t = tensor(name, o);
+  if (t.scalar_type() != type || !has_sizes(t, sizes) || !t.is_contiguous()) {
+    std::string s;
+    for (const int64_t n : sizes) s += (s.empty() ? "" : ", ") + std::to_string(n);
+    bad(name, t, std::string("contiguous ") + c10::toString(type) + " [" + s + "]");
+  }
+  return t;
+}
+template <class I>
+I *pointer(const at::Tensor &t) { return static_cast<I *>(t.data_ptr()); }
+at::Tensor int_tensor(int64_t n, int device) {
+  return at::empty({n}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, c10::DeviceIndex(device)));
+}
+
+// (pages, lengths, free, n_free), checked but for their device.
+lmx_kv8_pages pages_of(PyObject *const *args) {
+  const at::Tensor &pages = tensor("pages", args[0]);
+  if (pages.scalar_type() != at::kInt || pages.dim() != 2 || !pages.is_contiguous()) bad("pages", pages, "contiguous int32 of 2 dimensions");
+  const at::Tensor &lengths = whole("lengths", args[1], at::kInt, {pages.size(0)});
+  const at::Tensor &free = tensor("free", args[2]);
+  if (free.scalar_type() != at::kInt || free.dim() != 1 || !free.is_contiguous()) bad("free", free, "contiguous int32 of 1 dimension");
+  const at::Tensor &n_free = whole("n_free", args[3], at::kInt, {1});
+  return {pointer<int32_t>(pages), pointer<int32_t>(lengths), pointer<int32_t>(free), pointer<int32_t>(n_free), size_t(pages.size(0)),
+          size_t(pages.size(1)), size_t(free.size(0))};
+}
+
+// (pages, lengths, free, n_free): checked.
+PyObject *kv8_pages(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject * {
+    if (!arguments("kv8_pages", n, 4)) throw PyError{};
+    pages_of(args);
+    for (int i = 1; i < 4; ++i)
+      if (THPVariable_Unpack(args[i]).device() != THPVariable_Unpack(args[0]).device()) raise_value("the tensors of the pages must be on one device");
+    Py_RETURN_NONE;
+  });
+}
+
+// (pages, lengths, free, n_free, new, positions, slots, offsets, granted) -> (offsets, granted)
+PyObject *kv8_extend(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject * {
+    if (!arguments("kv8_extend", n, 9)) throw PyError{};
+    const lmx_kv8_pages p = pages_of(args);
+    const int64_t seqs = int64_t(p.n_seqs);
+    const at::Tensor &fresh = whole("new", args[4], at::kInt, {seqs});
+    const at::Tensor &positions = tensor("positions", args[5]);
+    if (positions.scalar_type() != at::kInt || positions.dim() != 1 || !positions.is_contiguous())
+      bad("positions", positions, "contiguous int32 of 1 dimension");
+    const at::Tensor *slots = args[6] != Py_None ? &whole("slots", args[6], at::kLong, {positions.size(0)}) : nullptr;
+    const at::Tensor *off = args[7] != Py_None ? &whole("offsets", args[7], at::kInt, {seqs + 1}) : nullptr;
+    const at::Tensor *yes = args[8] != Py_None ? &whole("granted", args[8], at::kInt, {seqs}) : nullptr;
+    const int device = check_devices({&THPVariable_Unpack(args[0]), &THPVariable_Unpack(args[1]), &THPVariable_Unpack(args[2]),
+                                      &THPVariable_Unpack(args[3]), &fresh, &positions, slots, off, yes});
+    const at::Tensor offsets = off ? *off : int_tensor(seqs + 1, device), granted = yes ? *yes : int_tensor(seqs, device);
+    check(lmx_kv8_extend(&p, pointer<int32_t>(fresh), size_t(positions.size(0)), pointer<int32_t>(offsets), pointer<int32_t>(granted),
+                         pointer<int32_t>(positions), slots ? pointer<int64_t>(*slots) : nullptr, stream_on(device)));
+    return Py_BuildValue("(NN)", off ? Py_NewRef(args[7]) : THPVariable_Wrap(offsets), yes ? Py_NewRef(args[8]) : THPVariable_Wrap(granted));
+  });
+}
+
+// (pages, lengths, free, n_free, drop)
+PyObject *kv8_trim(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject * {
+    if (!arguments("kv8_trim", n, 5)) throw PyError{};
+    const lmx_kv8_pages p = pages_of(args);
+    const at::Tensor &drop = whole("drop", args[4], at::kInt, {int64_t(p.n_seqs)});
+    const int device = check_devices({&THPVariable_Unpack(args[0]), &THPVariable_Unpack(args[1]), &THPVariable_Unpack(args[2]),
+                                      &THPVariable_Unpack(args[3]), &drop});
+    check(lmx_kv8_trim(&p, pointer<int32_t>(drop), stream_on(device)));
+    Py_RETURN_NONE;
+  });
+}
+
+// (q, k, positions, rope, interleaved, inverse, q_out, k_out) -> (q_out, k_out)
+PyObject *rotate(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject * {
+    if (!arguments("rotate", n, 8)) throw PyError{};
+    const at::Tensor &q = tensor("q", args[0]);
+    const int type = type_of("q", q);
+    if (q.dim() != 3) bad("q", q, "[rows, heads, head_dim]");
+    const at::ScalarType st = q.scalar_type();
+    const int64_t rows = q.size(0), heads = q.size(1), hd = q.size(2);
+    const at::Tensor *k = args[1] != Py_None ? &tensor("k", args[1]) : nullptr;
+    const int64_t kv = k && k->dim() == 3 ? k->size(1) : 0;
+    const size_t qs = row_stride("q", q, st, rows, heads, hd), ks = k ? row_stride("k", *k, st, rows, kv, hd) : 0;
+    const at::Tensor &positions = whole("positions", args[2], at::kInt, {rows}), &rope = tensor("rope", args[3]);
+    if (rope.scalar_type() != at::kFloat || rope.dim() != 3 || rope.size(2) != 2 || rope.size(1) < 1 || 2 * rope.size(1) > hd || !rope.is_contiguous())
+      bad("rope", rope, "contiguous float32 [positions, 1.." + std::to_string(hd / 2) + ", 2]");
+    const int interleaved = PyObject_IsTrue(args[4]), inverse = PyObject_IsTrue(args[5]);
+    if (interleaved < 0 || inverse < 0) throw PyError{};
+    const at::Tensor *qg = args[6] != Py_None ? &tensor("q_out", args[6]) : nullptr, *kg = args[7] != Py_None ? &tensor("k_out", args[7]) : nullptr;
+    if (kg && !k) raise_value("k_out without k");
+    const size_t qos = qg ? row_stride("q_out", *qg, st, rows, heads, hd) : size_t(heads * hd);
+    const size_t kos = kg ? row_stride("k_out", *kg, st, rows, kv, hd) : size_t(kv * hd);
+    const int device = check_devices({&q, k, &positions, &rope, qg, kg});
+    const at::Tensor qo = qg ? *qg : at::empty({rows, heads, hd}, q.options());
+    const at::Tensor ko = kg ? *kg : k ? at::empty({rows, kv, hd}, q.options()) : at::Tensor();
+    check(lmx_rotary(type, q.data_ptr(), qs, qo.data_ptr(), qos, size_t(heads), k ? k->data_ptr() : nullptr, ks,
+                     k ? ko.data_ptr() : nullptr, kos, size_t(kv), size_t(hd), size_t(2 * rope.size(1)), interleaved, inverse,
+                     pointer<int32_t>(positions), size_t(rows), pointer<float>(rope), size_t(rope.size(0)), stream_on(device)));
+    return Py_BuildValue("(NN)", qg ? Py_NewRef(args[6]) : THPVariable_Wrap(qo),
+                         kg ? Py_NewRef(args[7]) : k ? THPVariable_Wrap(ko) : Py_NewRef(Py_None));
+  });
+}
+
+// A matrix of `rows` rows of neighbouring elements: its row stride.
+size_t matrix_stride(const char *name, const at::Tensor &t, int64_t rows, int64_t width) {
+  if (!has_sizes(t, {rows, width})) bad(name, t, "[" + std::to_string(rows) + ", " + std::to_string(width) + "]");
+  if (rows && width > 1 && t.stride(1) != 1) bad(name, t, "a row's elements side by side");
+  return size_t(rows > 1 ? t.stride(0) : width);
+}
+
+// (logits, drafts, offsets, uniforms, probs, temperature, accepted, tokens, workspace) -> (accepted, tokens)
+PyObject *verify_drafts(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject * {
+    if (!arguments("verify_drafts", n, 9)) throw PyError{};
+    const at::Tensor &logits = tensor("logits", args[0]);
+    const int type = type_of("logits", logits);
+    if (logits.dim() != 2) bad("logits", logits, "[rows, vocab]");
+    const int64_t rows = logits.size(0), vocab = logits.size(1);
+    const size_t stride = matrix_stride("logits", logits, rows, vocab);
+    const at::Tensor &drafts = whole("drafts", args[1], at::kInt, {rows}), &offsets = tensor("offsets", args[2]);
+    if (offsets.scalar_type() != at::kInt || offsets.dim() != 1 || offsets.size(0) < 1 || !offsets.is_contiguous())
+      bad("offsets", offsets, "contiguous int32 [sequences + 1]");
+    const int64_t seqs = offsets.size(0) - 1;
+    const at::Tensor &uniforms = whole("uniforms", args[3], at::kFloat, {rows, 2});
+    const at::Tensor *probs = args[4] != Py_None ? &tensor("probs", args[4]) : nullptr;
+    if (probs && probs->scalar_type() != at::kFloat) bad("probs", *probs, "float32");
+    const size_t ps = probs ? matrix_stride("probs", *probs, rows, vocab) : 0;
+    const at::Tensor *t = args[5] != Py_None ? &whole("temperature", args[5], at::kFloat, {seqs}) : nullptr;
+    const at::Tensor *ag = args[6] != Py_None ? &whole("accepted", args[6], at::kInt, {seqs}) : nullptr;
+    const at::Tensor *tg = args[7] != Py_None ? &whole("tokens", args[7], at::kInt, {rows}) : nullptr;
+    const int device = check_devices({&logits, &drafts, &offsets, &uniforms, probs, t, ag, tg});
+    const lmx_drafts d = {pointer<int32_t>(offsets), pointer<int32_t>(drafts), pointer<float>(uniforms), t ? pointer<float>(*t) : nullptr,
+                          size_t(seqs), size_t(rows), size_t(vocab)};
+    size_t need = 0, bytes = 0;
+    check(lmx_verify_drafts_workspace(&d, type, &need));
+    const at::Tensor accepted = ag ? *ag : int_tensor(seqs, device), tokens = tg ? *tg : int_tensor(rows, device);
+    void *work;
+    const at::Tensor ws = workspace_of(args[8], need, device, work, bytes);
+    check(lmx_verify_drafts(&d, type, logits.data_ptr(), stride, probs ? pointer<float>(*probs) : nullptr, ps, pointer<int32_t>(accepted),
+                            pointer<int32_t>(tokens), work, bytes, stream_on(device)));
+    return Py_BuildValue("(NN)", ag ? Py_NewRef(args[6]) : THPVariable_Wrap(accepted), tg ? Py_NewRef(args[7]) : THPVariable_Wrap(tokens));
   });
 }
 
@@ -312,9 +502,10 @@ PyObject *set_error(PyObject *, PyObject *o) {
 }
 
 #define LMX_FAST(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
-PyMethodDef g_methods[] = {LMX_FAST(kv8_cache), LMX_FAST(kv8_append), LMX_FAST(kv8_attend), LMX_FAST(linear_i8),
+PyMethodDef g_methods[] = {LMX_FAST(kv8_cache), LMX_FAST(kv8_append), LMX_FAST(kv8_attend), LMX_FAST(kv8_pages), LMX_FAST(kv8_extend),
+                           LMX_FAST(kv8_trim), LMX_FAST(rotate), LMX_FAST(linear_i8), LMX_FAST(linear_f8), LMX_FAST(verify_drafts),
                            {"set_error", set_error, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
-PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_torch", "The 8-bit serving operators on torch tensors.", -1, g_methods,
+PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_torch", "The serving operators on torch tensors.", -1, g_methods,
                         nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
