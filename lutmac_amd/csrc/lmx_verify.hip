@@ -41,35 +41,42 @@ struct VerifyArgs {
 
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
 
-// 2^y for y <= 0: 2^k times the series of 2^f, |f| <= 1/2, to the 10th power (the
-// next term is below 2^-42).  Far below, and for NaN (-inf - -inf), 0.
-__device__ __forceinline__ double exp2_neg(double y) {
-  y = fmax(y, -1100.0);
-  const double k = rint(y), f = y - k;
-  double p = 7.054911620801123e-09;   // log(2)^n / n!
-  p = fma(p, f, 1.0178086009239699e-07);
-  p = fma(p, f, 1.321548679014431e-06);
-  p = fma(p, f, 1.525273380405984e-05);
-  p = fma(p, f, 1.5403530393381608e-04);
-  p = fma(p, f, 1.3333558146428443e-03);
-  p = fma(p, f, 9.618129107628477e-03);
-  p = fma(p, f, 5.550410866482158e-02);
-  p = fma(p, f, 2.402265069591007e-01);
-  p = fma(p, f, 6.931471805599453e-01);
-  p = fma(p, f, 1.0);
-  return ldexp(p, int(k));
+// Sums over a wave, the same bits in every lane, and inclusive sums over its lanes
+// (without LDS: a shuffle of 64 bits takes two trips through it).
+template <int D = kWave / 2>
+__device__ __forceinline__ double wave_sum(double v, int lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint64_t o = uint64_t(lane_xor_u32<D>(uint32_t(u >> 32), lane)) << 32 | lane_xor_u32<D>(uint32_t(u), lane);
+  v += __builtin_bit_cast(double, o);
+  if constexpr (D > 1) return wave_sum<D / 2>(v, lane);
+  else return v;
 }
-constexpr double kLog2e = 1.4426950408889634074;
-
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int d = kWave / 2; d; d /= 2) v += __shfl_xor(v, d);
-  return v;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_add(double v) {   // v plus that of another lane, where there is one
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(u)), CTRL, ROWS, 0xF, false));
+  const uint32_t hi = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(u >> 32)), CTRL, ROWS, 0xF, false));
+  return v + __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
 }
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int d = kWave / 2; d; d /= 2) v = fmaxf(v, __shfl_xor(v, d));
-  return v;
+__device__ __forceinline__ double wave_scan(double v) {
+  v = dpp_add<0x111, 0xF>(v);   // the lane 1, 2, 4, 8 below in a row of 16
+  v = dpp_add<0x112, 0xF>(v);
+  v = dpp_add<0x114, 0xF>(v);
+  v = dpp_add<0x118, 0xF>(v);
+  v = dpp_add<0x142, 0xA>(v);   // rows 0 and 2 to the next
+  return dpp_add<0x143, 0xC>(v);   // the lower half to the upper
+}
+__device__ __forceinline__ double lane_value(double v, int from) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(u)), from)), hi = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(u >> 32)), from));
+  return __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
+}
+__device__ __forceinline__ float wave_max(float v, int lane) { return lane_max<kWave / 2>(v, lane); }
+template <int D = kWave / 2>
+__device__ __forceinline__ int wave_min(int v, int lane) {
+  v = min(v, int(lane_xor_u32<D>(uint32_t(v), lane)));
+  if constexpr (D > 1) return wave_min<D / 2>(v, lane);
+  else return v;
 }
 
 // The last sequence whose first row is at most r (-1: none), by a wave.
@@ -86,17 +93,38 @@ __device__ __forceinline__ int sequence_of(const int *offsets, int n, int r, int
   return -1;
 }
 
-// A sequence's temperature and what logits' differences are multiplied by: (0, 0)
-// for a greedy one.
+// A sequence's temperature (0: greedy) and what a difference of logits is
+// multiplied by to become a power of two; `least`: the difference that gives 2^-1100.
 struct Heat {
   float t;
-  double by;
+  double by, least;
 };
 __device__ __forceinline__ Heat heat_of(const VerifyArgs &a, int s) {
   const float t = a.temperature ? a.temperature[s] : 1.0f;
-  return t > 0.0f ? Heat{t, kLog2e / double(t)} : Heat{0.0f, 0.0};
+  const double by = fmax(1.4426950408889634074 / double(t), 1e-300);
+  return t > 0.0f ? Heat{t, by, -1100.0 / by} : Heat{0.0f, 0.0, 0.0};
 }
-__device__ __forceinline__ double weight_of(float l, float top, double by) { return exp2_neg((double(l) - double(top)) * by); }
+// e^((l - top) / t): with y = (l - top) by, 2^k times 1 + f P(f), f = y - k within
+// 1/2 and P of degree 8 the interpolation of (2^f - 1) / f at Chebyshev's points (2^f is off by 2^-44.6 at
+// most).  Adding 1.5 * 2^52 leaves k in the low word.  -inf, or a part of only such
+// (-inf - -inf), weighs nothing.  15 operations in 64 bits, which cost as much as in
+// 32 here.
+__device__ __forceinline__ double weight_of(float l, float top, const Heat &h) {
+  constexpr double kRound = 6755399441055744.0;
+  const double d = fmax(double(l) - double(top), h.least);
+  const double n = fma(d, h.by, kRound), f = fma(d, h.by, kRound - n);
+  double p = 1.0203121138901363e-07;
+  p = fma(p, f, 1.325522487892511e-06);
+  p = fma(p, f, 1.525268684597521e-05);
+  p = fma(p, f, 1.5403455852451678e-04);
+  p = fma(p, f, 1.3333558179043376e-03);
+  p = fma(p, f, 9.618129159402562e-03);
+  p = fma(p, f, 5.5504108664760424e-02);
+  p = fma(p, f, 0.2402265069581299);
+  p = fma(p, f, 0.6931471805599453);
+  p = fma(p, f, 1.0);
+  return ldexp(p, int(uint32_t(__builtin_bit_cast(uint64_t, n))));
+}
 
 // A row's elements in pieces of 16 bytes: piece c holds elements c E - lead .. + E - 1,
 // so that pieces are aligned wherever the row begins.
@@ -150,7 +178,7 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(VerifyArgs a) {
       nan |= v[j][e] != v[j][e];
       top = fmaxf(top, v[j][e]);
     }
-  top = wave_max(top);
+  top = wave_max(top, lane);
   if (lane == 0) tops[wave] = top;
   __syncthreads();
 #pragma unroll
@@ -161,18 +189,17 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(VerifyArgs a) {
 #pragma unroll
     for (int j = 0; j < J; ++j)
 #pragma unroll
-      for (int e = 0; e < E; ++e) sum += weight_of(v[j][e], top, h.by);
+      for (int e = 0; e < E; ++e) sum += weight_of(v[j][e], top, h);
   } else {
 #pragma unroll
     for (int j = 0; j < J; ++j)
 #pragma unroll
       for (int e = 0; e < E; ++e)
         if (v[j][e] == top) first = min(first, (c0 + j * kThreads) * E - r.lead + e);
-#pragma unroll
-    for (int d = kWave / 2; d; d /= 2) first = min(first, __shfl_xor(first, d));
+    first = wave_min(first, lane);
   }
   if (nan || top == INFINITY) sum = __builtin_nan("");
-  sum = wave_sum(sum);
+  sum = wave_sum(sum, lane);
   if (lane == 0) sums[wave] = sum, firsts[wave] = first;
   __syncthreads();
   if (threadIdx.x != 0) return;
@@ -187,34 +214,71 @@ struct Row {
   float top;
   int best;
 };
-// By a wave.
-__device__ __forceinline__ Row row_of(const VerifyArgs &a, int row, const Heat &h, int lane) {
-  const Part *p = a.parts + size_t(row) * a.n_parts;
-  Row r{0.0, -INFINITY, 0x7FFFFFFF};
-  for (int i = lane; i < a.n_parts; i += kWave) r.top = fmaxf(r.top, p[i].top);
-  r.top = wave_max(r.top);
-  for (int i = lane; i < a.n_parts; i += kWave) {
-    const Part q = p[i];
-    r.total += h.t > 0.0f || q.sum != q.sum ? q.sum * weight_of(q.top, r.top, h.by) : 0.0;
+// A part's weights in a row's units.
+__device__ __forceinline__ double part_weight(const Part &p, const Row &r, const Heat &h) { return p.sum * weight_of(p.top, r.top, h); }
+// By a wave, each lane with its first part (of lane `lane`) in `first`.
+__device__ __forceinline__ Row row_of(const Part *p, int n, const Part &first, const Heat &h, int lane) {
+  Row r{0.0, first.top, 0x7FFFFFFF};
+  for (int i = lane + kWave; i < n; i += kWave) r.top = fmaxf(r.top, p[i].top);
+  r.top = wave_max(r.top, lane);
+  const auto add = [&](const Part &q) {
+    r.total += h.t > 0.0f || q.sum != q.sum ? q.sum * weight_of(q.top, r.top, h) : 0.0;
     if (q.top == r.top) r.best = min(r.best, q.best);
+  };
+  add(first);
+  for (int i = lane + kWave; i < n; i += kWave) add(p[i]);
+  r.total = wave_sum(r.total, lane);
+  if (h.t == 0.0f) {
+    r.best = wave_min(r.best, lane);
+    if (r.total == 0.0) r.total = 1.0;
   }
-  r.total = wave_sum(r.total);
-#pragma unroll
-  for (int d = kWave / 2; d; d /= 2) r.best = min(r.best, __shfl_xor(r.best, d));
-  if (h.t == 0.0f && r.total == 0.0) r.total = 1.0;
   if (r.top == -INFINITY || !(r.total > 0.0)) r.total = 0.0;
   return r;
 }
 
-// Inclusive sums over a wave's lanes.
-__device__ __forceinline__ double wave_scan(double v, int lane) {
+// The weights of a row's pieces: OVER: what p has over q, times the total, else p's,
+// but for `skip`.
+template <class T>
+struct Piece : RowOf<T> {
+  using RowOf<T>::E, RowOf<T>::lead, RowOf<T>::vocab;
+  const Row &r;
+  const Heat &h;
+  const float *q;
+  bool q_aligned;
+  __device__ __forceinline__ Piece(const VerifyArgs &a, int row, const Row &r, const Heat &h)
+      : RowOf<T>(a, row), r(r), h(h), q(a.probs + size_t(row) * a.probs_stride), q_aligned(lead == 0 && reinterpret_cast<size_t>(q) % 16 == 0) {}
+  template <bool OVER>
+  __device__ __forceinline__ void weights(int c, int skip, double (&w)[E]) const {
+    float v[E], u[E];
+    const int i0 = c * E - lead;
+    if constexpr (OVER) {
+      if (q_aligned && i0 + E <= vocab) {
+        load_floats<E>(q + i0, u);
+      } else {
 #pragma unroll
-  for (int d = 1; d < kWave; d *= 2) {
-    const double o = __shfl_up(v, d);
-    if (lane >= d) v += o;
+        for (int e = 0; e < E; ++e) u[e] = i0 + e >= 0 && i0 + e < vocab ? q[i0 + e] : 0.0f;
+      }
+    }
+    this->load(c, v);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      w[e] = weight_of(v[e], r.top, h);
+      if constexpr (OVER) w[e] = fmax(fma(double(u[e]), -r.total, w[e]), 0.0);
+      else if (i0 + e == skip) w[e] = 0.0;
+    }
   }
-  return v;
-}
+  template <bool OVER, int J>
+  __device__ __forceinline__ void sums(int part, int skip, double (&mine)[J]) const {
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      double w[E];
+      weights<OVER>((part * J + j) * kThreads + int(threadIdx.x), skip, w);
+      mine[j] = 0.0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) mine[j] += w[e];
+    }
+  }
+};
 
 // A workgroup a sequence, or one for each part where q may be needed: each finds
 // the row that the sequence stops at, four rows at a time.  The token there: parts'
@@ -222,35 +286,39 @@ __device__ __forceinline__ double wave_scan(double v, int lane) {
 // finds the part that the threshold falls into, then the element in it.
 template <class T, int J>
 __global__ __launch_bounds__(kThreads) void pick_kernel(VerifyArgs a) {
-  constexpr int E = RowOf<T>::E;
+  constexpr int E = RowOf<T>::E, PART = J * kThreads;   // pieces of a part
   __shared__ Row rows[kWaves];
   __shared__ int stops[kWaves];
   __shared__ double scan[J][kWaves];
-  __shared__ double chosen_sum;
+  __shared__ double chosen_target;
   __shared__ int chosen, at, last, joins;
   const int s = int(blockIdx.x), part = int(blockIdx.y), lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
   const int begin = max(a.offsets[s], 0), end = min(a.offsets[s + 1], a.n_rows);
+  const Heat h = heat_of(a, s);
   if (begin >= end) {
     if (part == 0 && threadIdx.x == 0) a.accepted[s] = 0;
     return;
   }
-  const Heat h = heat_of(a, s);
   int row = begin;
   Row r;
   for (;; row += kWaves) {
     const int mine = row + wave;
     if (mine < end) {
+      // (parts and token on their way at once, then the token's logit and share)
+      const Part *parts = a.parts + size_t(mine) * a.n_parts;
+      const Part first = lane < a.n_parts ? parts[lane] : Part{0.0, -INFINITY, 0x7FFFFFFF};
       const int token = a.drafts[mine];
+      const double u = a.uniforms[mine].x;
       const bool drafted = mine != end - 1 && token >= 0 && token < a.vocab;
       float l = 0.0f, q = 1.0f;
       if (drafted) {
         l = float((static_cast<const T *>(a.logits) + size_t(mine) * a.stride)[token]);
         if (a.probs) q = a.probs[size_t(mine) * a.probs_stride + token];
       }
-      const Row x = row_of(a, mine, h, lane);
-      const double w = h.t > 0.0f ? weight_of(l, x.top, h.by) : token == x.best ? 1.0 : 0.0;
-      const bool go = drafted && x.total > 0.0 && double(a.uniforms[mine].x) * double(q) * x.total < w;
+      const Row x = row_of(parts, a.n_parts, first, h, lane);
+      const double w = h.t > 0.0f ? weight_of(l, x.top, h) : token == x.best ? 1.0 : 0.0;
+      const bool go = drafted && x.total > 0.0 && u * double(q) * x.total < w;
       if (lane == 0) rows[wave] = x, stops[wave] = !go;
     } else if (lane == 0) {
       stops[wave] = 1;
@@ -274,47 +342,24 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(VerifyArgs a) {
     }
   }
   if (!(r.total > 0.0)) return;
+  if (h.t == 0.0f) {   // (whatever q is: all that p has over it is there)
+    if (part == 0 && threadIdx.x == 0) a.tokens[row] = r.best;
+    return;
+  }
   const int token = a.drafts[row];
-  const bool rest = row != end - 1;
-  const float *q = rest && a.probs ? a.probs + size_t(row) * a.probs_stride : nullptr;
-  const bool q_aligned = q && reinterpret_cast<size_t>(q) % 16 == 0;
-  const RowOf<T> x(a, row);
-  // weights of a piece: of p, of p without the drafted token, or of what p has over q
-  enum Kind { kAll, kWithout, kOver };
-  const auto weights = [&](int c, Kind kind, double (&w)[E]) {
-    float v[E];
-    x.load(c, v);
-    const int i0 = c * E - x.lead;
-    float u[E];
-    if (kind == kOver) {
-      if (q_aligned && x.lead == 0 && i0 + E <= a.vocab) {
-        load_floats<E>(q + i0, u);
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) u[e] = i0 + e >= 0 && i0 + e < a.vocab ? q[i0 + e] : 0.0f;
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      w[e] = h.t > 0.0f ? weight_of(v[e], r.top, h.by) : i0 + e == r.best ? 1.0 : 0.0;
-      if (kind == kOver) w[e] = fmax(w[e] - double(u[e]) * r.total, 0.0);
-      else if (kind == kWithout && i0 + e == token) w[e] = 0.0;
-    }
-  };
-  // the sum of a part's weights, of every thread's J pieces (mine) and over the workgroup
-  const auto part_sum = [&](int part, Kind kind, double (&mine)[J]) {
+  const bool rest = row != end - 1, known = token >= 0 && token < a.vocab;
+  const bool over = rest && a.probs;
+  if (!over && part != 0) return;
+  const Piece<T> x(a, row, r, h);
+  double *sums = a.rest + size_t(s) * a.n_parts;
+  const Part *parts = a.parts + size_t(row) * a.n_parts;
+  double mine[J];
+  // the sum of every thread's pieces over the workgroup
+  const auto block_sum = [&]() __attribute__((always_inline)) {
     double all = 0.0;
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-      double w[E];
-      weights(part * (J * kThreads) + j * kThreads + int(threadIdx.x), kind, w);
-      mine[j] = 0.0;
-#pragma unroll
-      for (int e = 0; e < E; ++e) mine[j] += w[e];
-      all += mine[j];
-    }
-    all = wave_sum(all);
-    __syncthreads();
+    for (int j = 0; j < J; ++j) all += mine[j];
+    all = wave_sum(all, lane);
     if (lane == 0) scan[0][wave] = all;
     __syncthreads();
     all = scan[0][0];
@@ -323,11 +368,13 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(VerifyArgs a) {
     __syncthreads();
     return all;
   };
-  double mine[J];
-  Kind kind = q ? kOver : rest && token >= 0 && token < a.vocab ? kWithout : kAll;
-  double *sums = a.rest + size_t(s) * a.n_parts;
-  if (kind == kOver) {
-    const double sum = part_sum(part, kind, mine);
+  bool from_rest = over;   // weights are those of p - q
+  int skip = -1;           // the token that p is to lack, its part and what is left of that
+  int lacking = -1;
+  double less = 0.0;
+  if (over) {
+    x.template sums<true, J>(part, -1, mine);
+    const double sum = block_sum();
     if (threadIdx.x == 0) {
       __hip_atomic_store(sums + part, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       __threadfence();
@@ -336,87 +383,99 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(VerifyArgs a) {
     __syncthreads();
     if (!joins) return;
     __threadfence();
-  } else if (part != 0) {
-    return;
+  } else if (rest && known) {
+    // (the difference keeps 42 bits, or the part is summed without the token)
+    skip = token;
+    lacking = (token + x.lead) / (PART * E);
+    const double with = part_weight(parts[lacking], r, h);
+    less = with - weight_of(float(x.x[token]), r.top, h);
+    if (!(less > with * 0x1p-10)) {
+      x.template sums<false, J>(lacking, skip, mine);
+      less = block_sum();
+    }
   }
   // Parts' sums in order, and the first that the threshold falls into: a wave, 64
   // parts at a time.
-  const int without = kind == kWithout ? (token + x.lead) / (J * kThreads * E) : -1;   // the part that lacks a token
-  double less = 0.0;
-  if (without >= 0) less = part_sum(without, kWithout, mine);
-  const Part *parts = a.parts + size_t(row) * a.n_parts;
   for (int again = 0; again < 2; ++again) {
     if (wave == 0) {
-      const auto sum_of = [&](int i) {
+      const auto sum_of = [&](int i) __attribute__((always_inline)) {
         if (i >= a.n_parts) return 0.0;
-        if (kind == kOver) return __hip_atomic_load(sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (i == without && kind == kWithout) return less;
-        if (h.t == 0.0f) return parts[i].best == r.best && parts[i].top == r.top ? 1.0 : 0.0;
-        return parts[i].sum * weight_of(parts[i].top, r.top, h.by);
+        if (from_rest) return __hip_atomic_load(sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        return i == lacking ? less : part_weight(parts[i], r, h);
       };
-      double all = 0.0;
-      for (int i = 0; i < a.n_parts; i += kWave) all += wave_sum(sum_of(i + lane));
+      const double v0 = sum_of(lane);
+      double all = wave_sum(v0, lane);
+      for (int i = kWave; i < a.n_parts; i += kWave) all += wave_sum(sum_of(i + lane), lane);
       int found = -1, behind = -1;
       double target = double(a.uniforms[row].y) * all, before = 0.0;
       for (int i = 0; i < a.n_parts && found < 0; i += kWave) {
-        const double v = sum_of(i + lane), upto = before + wave_scan(v, lane);
+        const double v = i == 0 ? v0 : sum_of(i + lane), upto = before + wave_scan(v);
         const uint64_t past = __builtin_amdgcn_ballot_w64(v > 0.0 && upto > target), some = __builtin_amdgcn_ballot_w64(v > 0.0);
         if (past) {
           found = __builtin_ctzll(past);
-          target -= __shfl(upto - v, found);
+          target -= lane_value(upto - v, found);
           found += i;
         } else {
           if (some) behind = i + 63 - __builtin_clzll(some);
-          before = __shfl(upto, kWave - 1);
+          before = lane_value(upto, kWave - 1);
         }
       }
       if (found < 0) found = behind, target = INFINITY;   // (rounding, or a number of 1 and more: the last)
-      if (lane == 0) chosen = all > 0.0 ? found : -1, chosen_sum = target, at = 0x7FFFFFFF, last = -1;
+      if (lane == 0) chosen = all > 0.0 ? found : -1, chosen_target = target, at = 0x7FFFFFFF, last = -1;
     }
     __syncthreads();
     if (chosen >= 0) break;
-    // nothing is left of p - q: from p
-    kind = kAll;
+    // nothing is left: from p
+    from_rest = false;
+    skip = lacking = -1;
     __syncthreads();
   }
   if (chosen < 0) return;   // (p weighs something)
-  const double target = chosen_sum;
-  part_sum(chosen, kind, mine);
+  // the first piece past the threshold (or the last with a weight), then in it the
+  // element, by the piece's thread
+  const double target = chosen_target;
+  if (from_rest) x.template sums<true, J>(chosen, -1, mine);
+  else x.template sums<false, J>(chosen, skip, mine);
   double upto[J];
 #pragma unroll
   for (int j = 0; j < J; ++j) {
-    upto[j] = wave_scan(mine[j], lane);
+    upto[j] = wave_scan(mine[j]);
     if (lane == kWave - 1) scan[j][wave] = upto[j];
   }
   __syncthreads();
-  double before = 0.0;
+  double before = 0.0, base = 0.0;
+  int past = 0x7FFFFFFF, behind = -1;
 #pragma unroll
   for (int j = 0; j < J; ++j) {
-    double base = before;
+    double here = base;   // all before this wave's pieces of round j
 #pragma unroll
     for (int v = 0; v < kWaves; ++v) {
-      if (v < wave) base += scan[j][v];
-      before += scan[j][v];
+      if (v < wave) here += scan[j][v];
+      base += scan[j][v];
     }
-    const int c = chosen * (J * kThreads) + j * kThreads + int(threadIdx.x);
     if (mine[j] > 0.0) {
-      double w[E];
-      weights(c, kind, w);
-      double sum = base + (upto[j] - mine[j]);
-      const bool here = base + upto[j] > target;
-      int end_at = -1, found = -1;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        sum += w[e];
-        if (w[e] > 0.0) end_at = c * E - x.lead + e;
-        if (found < 0 && sum > target) found = c * E - x.lead + e;
-      }
-      if (here) atomicMin(&at, found >= 0 ? found : end_at);
-      atomicMax(&last, end_at);
+      behind = j * kThreads + int(threadIdx.x);
+      if (past == 0x7FFFFFFF && here + upto[j] > target) past = behind, before = here + (upto[j] - mine[j]);
     }
   }
+  if (past < 0x7FFFFFFF) atomicMin(&at, past);
+  if (behind >= 0) atomicMax(&last, behind);
   __syncthreads();
-  if (threadIdx.x == 0) a.tokens[row] = at < 0x7FFFFFFF ? at : last;
+  const int piece = at < 0x7FFFFFFF ? at : last;
+  if (piece < 0 || piece % kThreads != int(threadIdx.x)) return;
+  double w[E];
+  const int c = chosen * PART + piece;
+  if (from_rest) x.template weights<true>(c, -1, w);
+  else x.template weights<false>(c, skip, w);
+  int token_at = -1;
+  bool done = false;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    before += w[e];
+    if (!done && w[e] > 0.0) token_at = c * E - x.lead + e;
+    done = done || (piece == past && w[e] > 0.0 && before > target);
+  }
+  a.tokens[row] = token_at;
 }
 
 int launch_err(const char *what) {
@@ -432,11 +491,11 @@ int check_sizes(const lmx_drafts *d, int type) {
   return LMX_OK;
 }
 
-// Pieces of 16 bytes a thread: parts of 8 while that still makes four workgroups a
+// Pieces of 16 bytes a thread: parts of 4 while that still makes four workgroups a
 // CU, else of 2.
 int pieces_of(size_t rows, size_t vocab, int type) {
-  const size_t part = kThreads * 8 * (16 / type_bytes(type));
-  return rows * (vocab / part) >= 1024 ? 8 : 2;
+  const size_t part = kThreads * 4 * (16 / type_bytes(type));
+  return rows * (vocab / part) >= 1024 ? 4 : 2;
 }
 size_t parts_of(size_t rows, size_t vocab, int type) {
   const size_t e = 16 / type_bytes(type), part = kThreads * e * pieces_of(rows, vocab, type);
@@ -453,7 +512,7 @@ int launch(const VerifyArgs &a, hipStream_t st) {
 }
 template <class T>
 int launch(const VerifyArgs &a, int pieces, hipStream_t st) {
-  return pieces == 8 ? launch<T, 8>(a, st) : launch<T, 2>(a, st);
+  return pieces == 4 ? launch<T, 4>(a, st) : launch<T, 2>(a, st);
 }
 
 struct Layout { size_t rest, tickets, all; };
