@@ -135,20 +135,27 @@ struct RowOf {
   int lead, vocab;
   __device__ __forceinline__ RowOf(const VerifyArgs &a, int row)
       : x(static_cast<const T *>(a.logits) + size_t(row) * a.stride), lead(int(reinterpret_cast<size_t>(x) / sizeof(T) % E)), vocab(a.vocab) {}
+  typedef uint32_t Raw __attribute__((ext_vector_type(4)));
+  typedef T Values __attribute__((ext_vector_type(E)));
   // (elements past the row's ends: -inf, which weighs nothing)
-  __device__ __forceinline__ void load(int c, float (&v)[E]) const {
+  __device__ __forceinline__ Raw raw(int c) const {
     const int i = c * E - lead;
-    if (i >= 0 && i + E <= vocab) {
-      load_floats<E>(x + i, v);
-    } else {
+    if (i >= 0 && i + E <= vocab) return *reinterpret_cast<const Raw *>(x + i);
+    Values v;
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[e] = -INFINITY;
-      if (i < vocab)
+    for (int e = 0; e < E; ++e) v[e] = T(-INFINITY);
+    if (i < vocab)
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (i + e >= 0 && i + e < vocab) v[e] = float(x[i + e]);
-    }
+      for (int e = 0; e < E; ++e)
+        if (i + e >= 0 && i + e < vocab) v[e] = x[i + e];
+    return __builtin_bit_cast(Raw, v);
   }
+  static __device__ __forceinline__ void floats(Raw r, float (&v)[E]) {
+    const Values u = __builtin_bit_cast(Values, r);
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = float(u[e]);
+  }
+  __device__ __forceinline__ void load(int c, float (&v)[E]) const { floats(raw(c), v); }
 };
 
 // Sums, largest and first of the largest of each part of each row: J pieces a
@@ -162,40 +169,56 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(VerifyArgs a) {
   const int part = int(blockIdx.y), row = int(blockIdx.x), lane = threadIdx.x & (kWave - 1), wave = int(threadIdx.x) / kWave;
   const RowOf<T> r(a, row);
   const int c0 = part * (J * kThreads) + int(threadIdx.x);
-  float v[J][E];
+  typename RowOf<T>::Raw raw[J];
+  const int i0 = part * (J * kThreads * E) - r.lead;
+  if (i0 >= 0 && i0 + J * kThreads * E <= a.vocab) {   // the whole part is inside the row
+    const typename RowOf<T>::Raw *from = reinterpret_cast<const typename RowOf<T>::Raw *>(r.x + i0) + threadIdx.x;
 #pragma unroll
-  for (int j = 0; j < J; ++j) r.load(c0 + j * kThreads, v[j]);
+    for (int j = 0; j < J; ++j) raw[j] = from[j * kThreads];
+  } else {
+#pragma unroll
+    for (int j = 0; j < J; ++j) raw[j] = r.raw(c0 + j * kThreads);
+  }
   const int s = sequence_of(a.offsets, a.n_seqs, row, lane);
   if (s < 0 || row >= a.offsets[s + 1]) return;
   const Heat h = heat_of(a, s);
   if (part == 0 && threadIdx.x == 0 && row == max(a.offsets[s], 0)) a.tickets[s] = 0;
-  float top = -INFINITY;
-  bool nan = false;
+  float top = -INFINITY;   // (a NaN stays)
 #pragma unroll
-  for (int j = 0; j < J; ++j)
+  for (int j = 0; j < J; ++j) {
+    float v[E];
+    r.floats(raw[j], v);
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      nan |= v[j][e] != v[j][e];
-      top = fmaxf(top, v[j][e]);
-    }
+    for (int e = 0; e < E; ++e) top = __builtin_elementwise_maximum(top, v[e]);
+  }
+  const bool nan = top != top;
   top = wave_max(top, lane);
   if (lane == 0) tops[wave] = top;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) top = fmaxf(top, tops[w]);
+  // (from the packed values again: as floats they would take the registers of half the waves)
+#pragma unroll
+  for (int j = 0; j < J; ++j) asm volatile("" : "+v"(raw[j]));
   double sum = 0.0;
   int first = 0x7FFFFFFF;
   if (h.t > 0.0f) {
 #pragma unroll
-    for (int j = 0; j < J; ++j)
+    for (int j = 0; j < J; ++j) {
+      float v[E];
+      r.floats(raw[j], v);
 #pragma unroll
-      for (int e = 0; e < E; ++e) sum += weight_of(v[j][e], top, h);
+      for (int e = 0; e < E; ++e) sum += weight_of(v[e], top, h);
+    }
   } else {
 #pragma unroll
-    for (int j = 0; j < J; ++j)
+    for (int j = 0; j < J; ++j) {
+      float v[E];
+      r.floats(raw[j], v);
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        if (v[j][e] == top) first = min(first, (c0 + j * kThreads) * E - r.lead + e);
+        if (v[e] == top) first = min(first, (c0 + j * kThreads) * E - r.lead + e);
+    }
     first = wave_min(first, lane);
   }
   if (nan || top == INFINITY) sum = __builtin_nan("");
@@ -215,22 +238,26 @@ struct Row {
   int best;
 };
 // A part's weights in a row's units.
-__device__ __forceinline__ double part_weight(const Part &p, const Row &r, const Heat &h) { return p.sum * weight_of(p.top, r.top, h); }
-// By a wave, each lane with its first part (of lane `lane`) in `first`.
-__device__ __forceinline__ Row row_of(const Part *p, int n, const Part &first, const Heat &h, int lane) {
+__device__ __forceinline__ double part_weight(const Part &p, float top, const Heat &h) { return p.sum * weight_of(p.top, top, h); }
+// By a wave, each lane with its first part (of lane `lane`) in `first`; share: that part's weights.
+__device__ __forceinline__ Row row_of(const Part *p, int n, const Part &first, const Heat &h, int lane, double &share) {
   Row r{0.0, first.top, 0x7FFFFFFF};
   for (int i = lane + kWave; i < n; i += kWave) r.top = fmaxf(r.top, p[i].top);
   r.top = wave_max(r.top, lane);
-  const auto add = [&](const Part &q) {
-    r.total += h.t > 0.0f || q.sum != q.sum ? q.sum * weight_of(q.top, r.top, h) : 0.0;
-    if (q.top == r.top) r.best = min(r.best, q.best);
-  };
-  add(first);
-  for (int i = lane + kWave; i < n; i += kWave) add(p[i]);
-  r.total = wave_sum(r.total, lane);
-  if (h.t == 0.0f) {
+  if (h.t > 0.0f) {
+    share = part_weight(first, r.top, h);
+    r.total = share;
+    for (int i = lane + kWave; i < n; i += kWave) r.total += part_weight(p[i], r.top, h);
+    r.total = wave_sum(r.total, lane);
+  } else {
+    bool bad = first.sum != first.sum;
+    if (first.top == r.top) r.best = first.best;
+    for (int i = lane + kWave; i < n; i += kWave) {
+      bad |= p[i].sum != p[i].sum;
+      if (p[i].top == r.top) r.best = min(r.best, p[i].best);
+    }
     r.best = wave_min(r.best, lane);
-    if (r.total == 0.0) r.total = 1.0;
+    r.total = __builtin_amdgcn_ballot_w64(bad) ? 0.0 : 1.0;
   }
   if (r.top == -INFINITY || !(r.total > 0.0)) r.total = 0.0;
   return r;
@@ -280,18 +307,48 @@ struct Piece : RowOf<T> {
   }
 };
 
+// The place among up to 64 parts a time, of n, where a wave's sums of weights first
+// pass u times all of them: the part, and what is left of the threshold in it
+// (infinite: its last token with a weight).  v0: the lane's first sum, of(i): part i's.
+struct Place {
+  int part;   // -1: nothing weighs anything
+  double target;
+};
+template <class F>
+__device__ __forceinline__ Place place_of(int n, double u, double v0, int lane, F of) {
+  double all = wave_sum(v0, lane);
+  for (int i = kWave; i < n; i += kWave) all += wave_sum(i + lane < n ? of(i + lane) : 0.0, lane);
+  if (!(all > 0.0)) return {-1, 0.0};
+  const double target = u * all;
+  double before = 0.0;
+  int behind = -1;
+  for (int i = 0; i < n; i += kWave) {
+    const double v = i == 0 ? v0 : i + lane < n ? of(i + lane) : 0.0, upto = before + wave_scan(v);
+    const uint64_t some = __builtin_amdgcn_ballot_w64(v > 0.0), past = some & __builtin_amdgcn_ballot_w64(upto > target);
+    if (past) {
+      const int found = __builtin_ctzll(past);
+      return {i + found, target - lane_value(upto - v, found)};
+    }
+    if (some) behind = i + 63 - __builtin_clzll(some);
+    before = lane_value(upto, kWave - 1);
+  }
+  return {behind, INFINITY};   // (rounding, or a number of 1 and more)
+}
+
 // A workgroup a sequence, or one for each part where q may be needed: each finds
-// the row that the sequence stops at, four rows at a time.  The token there: parts'
-// sums are known, or, of p - q, taken by the sequence's workgroups; the last of them
-// finds the part that the threshold falls into, then the element in it.
+// the row that the sequence stops at, four rows at a time, a wave each.  The token
+// there: parts' sums are known, or, of p - q, taken by the sequence's workgroups;
+// the row's wave (or the last workgroup) finds the part that the threshold falls into,
+// the workgroup the element in it.  What it costs is its chain of loads: offsets,
+// then parts' sums and drafts, then the drafted tokens' logits, then the part found.
 template <class T, int J>
 __global__ __launch_bounds__(kThreads) void pick_kernel(VerifyArgs a) {
   constexpr int E = RowOf<T>::E, PART = J * kThreads;   // pieces of a part
   __shared__ Row rows[kWaves];
   __shared__ int stops[kWaves];
   __shared__ double scan[J][kWaves];
-  __shared__ double chosen_target;
-  __shared__ int chosen, at, last, joins;
+  __shared__ Place place;
+  __shared__ int at, last, joins;
   const int s = int(blockIdx.x), part = int(blockIdx.y), lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
   const int begin = max(a.offsets[s], 0), end = min(a.offsets[s + 1], a.n_rows);
@@ -300,58 +357,51 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(VerifyArgs a) {
     if (part == 0 && threadIdx.x == 0) a.accepted[s] = 0;
     return;
   }
-  int row = begin;
-  Row r;
+  int row = begin, owner, token = -1;
+  double share = 0.0, weight = 0.0;   // of this wave's row: the lane's part's, the drafted token's
+  bool known = false;
+  float2 u = {0.0f, 0.0f};
   for (;; row += kWaves) {
     const int mine = row + wave;
     if (mine < end) {
-      // (parts and token on their way at once, then the token's logit and share)
       const Part *parts = a.parts + size_t(mine) * a.n_parts;
       const Part first = lane < a.n_parts ? parts[lane] : Part{0.0, -INFINITY, 0x7FFFFFFF};
-      const int token = a.drafts[mine];
-      const double u = a.uniforms[mine].x;
-      const bool drafted = mine != end - 1 && token >= 0 && token < a.vocab;
-      float l = 0.0f, q = 1.0f;
-      if (drafted) {
+      token = a.drafts[mine];
+      u = a.uniforms[mine];
+      known = mine != end - 1 && token >= 0 && token < a.vocab;
+      float l = -INFINITY, q = 1.0f;
+      if (known) {
         l = float((static_cast<const T *>(a.logits) + size_t(mine) * a.stride)[token]);
         if (a.probs) q = a.probs[size_t(mine) * a.probs_stride + token];
       }
-      const Row x = row_of(parts, a.n_parts, first, h, lane);
-      const double w = h.t > 0.0f ? weight_of(l, x.top, h) : token == x.best ? 1.0 : 0.0;
-      const bool go = drafted && x.total > 0.0 && u * double(q) * x.total < w;
+      const Row x = row_of(parts, a.n_parts, first, h, lane, share);
+      weight = h.t > 0.0f ? weight_of(l, x.top, h) : token == x.best ? 1.0 : 0.0;
+      const bool go = known && x.total > 0.0 && double(u.x) * double(q) * x.total < weight;
       if (lane == 0) rows[wave] = x, stops[wave] = !go;
     } else if (lane == 0) {
       stops[wave] = 1;
     }
     __syncthreads();
-    int n = 0;
-    while (n < kWaves && !stops[n]) ++n;
-    if (n < kWaves) {   // (the last row stops)
-      row += n;
-      r = rows[n];
-      break;
-    }
+    owner = 0;
+    while (owner < kWaves && !stops[owner]) ++owner;
+    if (owner < kWaves) break;   // (the last row stops)
     __syncthreads();
   }
+  row += owner;
+  const Row r = rows[owner];
   if (part == 0) {
     for (int i = begin + int(threadIdx.x); i < end; i += kThreads)
       if (i != row) a.tokens[i] = i < row ? a.drafts[i] : -1;
     if (threadIdx.x == 0) {
       a.accepted[s] = row - begin;
-      if (!(r.total > 0.0)) a.tokens[row] = -1;
+      // (greedily: whatever q is, all that p has over it is there)
+      if (!(r.total > 0.0) || h.t == 0.0f) a.tokens[row] = r.total > 0.0 ? r.best : -1;
     }
   }
-  if (!(r.total > 0.0)) return;
-  if (h.t == 0.0f) {   // (whatever q is: all that p has over it is there)
-    if (part == 0 && threadIdx.x == 0) a.tokens[row] = r.best;
-    return;
-  }
-  const int token = a.drafts[row];
-  const bool rest = row != end - 1, known = token >= 0 && token < a.vocab;
-  const bool over = rest && a.probs;
+  if (!(r.total > 0.0) || h.t == 0.0f) return;
+  const bool over = row != end - 1 && a.probs;
   if (!over && part != 0) return;
   const Piece<T> x(a, row, r, h);
-  double *sums = a.rest + size_t(s) * a.n_parts;
   const Part *parts = a.parts + size_t(row) * a.n_parts;
   double mine[J];
   // the sum of every thread's pieces over the workgroup
@@ -369,10 +419,10 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(VerifyArgs a) {
     return all;
   };
   bool from_rest = over;   // weights are those of p - q
-  int skip = -1;           // the token that p is to lack, its part and what is left of that
-  int lacking = -1;
-  double less = 0.0;
+  int skip = -1;           // the token that p is to lack
+  if (threadIdx.x == 0) at = 0x7FFFFFFF, last = -1;
   if (over) {
+    double *sums = a.rest + size_t(s) * a.n_parts;
     x.template sums<true, J>(part, -1, mine);
     const double sum = block_sum();
     if (threadIdx.x == 0) {
@@ -383,59 +433,53 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(VerifyArgs a) {
     __syncthreads();
     if (!joins) return;
     __threadfence();
-  } else if (rest && known) {
-    // (the difference keeps 42 bits, or the part is summed without the token)
-    skip = token;
-    lacking = (token + x.lead) / (PART * E);
-    const double with = part_weight(parts[lacking], r, h);
-    less = with - weight_of(float(x.x[token]), r.top, h);
-    if (!(less > with * 0x1p-10)) {
-      x.template sums<false, J>(lacking, skip, mine);
-      less = block_sum();
+    if (wave == owner) {
+      const auto of = [&](int i) __attribute__((always_inline)) { return __hip_atomic_load(sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+      const Place p = place_of(a.n_parts, double(u.y), lane < a.n_parts ? of(lane) : 0.0, lane, of);
+      if (lane == 0) place = p;
+    }
+    __syncthreads();
+    if (place.part < 0) from_rest = false;   // nothing is left: from p
+    __syncthreads();
+  } else {
+    // the part that lacks the drafted token: the difference keeps 42 bits, or it is
+    // summed without the token
+    __shared__ int without;
+    if (wave == owner) {
+      const int lacking = known ? (token + x.lead) / (PART * E) : -1;
+      const double with = lane == lacking ? share : lacking >= kWave ? part_weight(parts[lacking], r.top, h) : INFINITY;
+      const bool lost = lacking >= 0 && __builtin_amdgcn_ballot_w64(!(with - weight > with * 0x1p-10) && with < INFINITY) != 0;
+      if (lane == 0) without = known ? token : -1, joins = lost;
+    }
+    __syncthreads();
+    skip = without;
+    if (joins) {
+      x.template sums<false, J>((skip + x.lead) / (PART * E), skip, mine);
+      weight = block_sum();
     }
   }
-  // Parts' sums in order, and the first that the threshold falls into: a wave, 64
-  // parts at a time.
-  for (int again = 0; again < 2; ++again) {
-    if (wave == 0) {
-      const auto sum_of = [&](int i) __attribute__((always_inline)) {
-        if (i >= a.n_parts) return 0.0;
-        if (from_rest) return __hip_atomic_load(sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        return i == lacking ? less : part_weight(parts[i], r, h);
-      };
-      const double v0 = sum_of(lane);
-      double all = wave_sum(v0, lane);
-      for (int i = kWave; i < a.n_parts; i += kWave) all += wave_sum(sum_of(i + lane), lane);
-      int found = -1, behind = -1;
-      double target = double(a.uniforms[row].y) * all, before = 0.0;
-      for (int i = 0; i < a.n_parts && found < 0; i += kWave) {
-        const double v = i == 0 ? v0 : sum_of(i + lane), upto = before + wave_scan(v);
-        const uint64_t past = __builtin_amdgcn_ballot_w64(v > 0.0 && upto > target), some = __builtin_amdgcn_ballot_w64(v > 0.0);
-        if (past) {
-          found = __builtin_ctzll(past);
-          target -= lane_value(upto - v, found);
-          found += i;
-        } else {
-          if (some) behind = i + 63 - __builtin_clzll(some);
-          before = lane_value(upto, kWave - 1);
-        }
+  if (!from_rest) {
+    for (int again = 0; again < 2; ++again) {
+      if (wave == owner) {
+        const int lacking = skip >= 0 ? (skip + x.lead) / (PART * E) : -1;
+        const auto less = [&](int i, double v) __attribute__((always_inline)) { return i != lacking ? v : joins && !over ? weight : v - weight; };
+        const auto of = [&](int i) __attribute__((always_inline)) { return less(i, part_weight(parts[i], r.top, h)); };
+        const Place p = place_of(a.n_parts, double(u.y), lane < a.n_parts ? less(lane, share) : 0.0, lane, of);
+        if (lane == 0) place = p;
       }
-      if (found < 0) found = behind, target = INFINITY;   // (rounding, or a number of 1 and more: the last)
-      if (lane == 0) chosen = all > 0.0 ? found : -1, chosen_target = target, at = 0x7FFFFFFF, last = -1;
+      __syncthreads();
+      if (place.part >= 0) break;
+      skip = -1;   // nothing is left without the token: from p
+      __syncthreads();
     }
-    __syncthreads();
-    if (chosen >= 0) break;
-    // nothing is left: from p
-    from_rest = false;
-    skip = lacking = -1;
-    __syncthreads();
+    if (place.part < 0) return;   // (p weighs something)
   }
-  if (chosen < 0) return;   // (p weighs something)
   // the first piece past the threshold (or the last with a weight), then in it the
   // element, by the piece's thread
-  const double target = chosen_target;
-  if (from_rest) x.template sums<true, J>(chosen, -1, mine);
-  else x.template sums<false, J>(chosen, skip, mine);
+  const double target = place.target;
+  const int c0 = place.part * PART;
+  if (from_rest) x.template sums<true, J>(place.part, -1, mine);
+  else x.template sums<false, J>(place.part, skip, mine);
   double upto[J];
 #pragma unroll
   for (int j = 0; j < J; ++j) {
@@ -464,15 +508,14 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(VerifyArgs a) {
   const int piece = at < 0x7FFFFFFF ? at : last;
   if (piece < 0 || piece % kThreads != int(threadIdx.x)) return;
   double w[E];
-  const int c = chosen * PART + piece;
-  if (from_rest) x.template weights<true>(c, -1, w);
-  else x.template weights<false>(c, skip, w);
+  if (from_rest) x.template weights<true>(c0 + piece, -1, w);
+  else x.template weights<false>(c0 + piece, skip, w);
   int token_at = -1;
   bool done = false;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     before += w[e];
-    if (!done && w[e] > 0.0) token_at = c * E - x.lead + e;
+    if (!done && w[e] > 0.0) token_at = (c0 + piece) * E - x.lead + e;
     done = done || (piece == past && w[e] > 0.0 && before > target);
   }
   a.tokens[row] = token_at;
@@ -494,8 +537,8 @@ int check_sizes(const lmx_drafts *d, int type) {
 // Pieces of 16 bytes a thread: parts of 4 while that still makes four workgroups a
 // CU, else of 2.
 int pieces_of(size_t rows, size_t vocab, int type) {
-  const size_t part = kThreads * 4 * (16 / type_bytes(type));
-  return rows * (vocab / part) >= 1024 ? 4 : 2;
+  const size_t part = kThreads * 8 * (16 / type_bytes(type));
+  return rows * (vocab / part) >= 1024 ? 8 : 2;
 }
 size_t parts_of(size_t rows, size_t vocab, int type) {
   const size_t e = 16 / type_bytes(type), part = kThreads * e * pieces_of(rows, vocab, type);
@@ -512,7 +555,7 @@ int launch(const VerifyArgs &a, hipStream_t st) {
 }
 template <class T>
 int launch(const VerifyArgs &a, int pieces, hipStream_t st) {
-  return pieces == 4 ? launch<T, 4>(a, st) : launch<T, 2>(a, st);
+  return pieces == 8 ? launch<T, 8>(a, st) : launch<T, 2>(a, st);
 }
 
 struct Layout { size_t rest, tickets, all; };
