@@ -37,9 +37,12 @@ struct VerifyArgs {
   double *rest;       // [n_seqs][n_parts] sums of what p has over q, where a sequence needs them
   unsigned *tickets;  // [n_seqs], zero when a pick begins
   int n_parts;
+  int groups;         // workgroups of a sequence where q may be needed
 };
 
-constexpr int kThreads = 256, kWaves = kThreads / kWave;
+// A part of a row is what a wave takes at a time: kPieces pieces of 16 bytes a lane.
+constexpr int kPieces = 4, kPart = kPieces * kWave;   // (pieces of a part)
+constexpr int kStatsThreads = 256, kThreads = 512, kWaves = kThreads / kWave;
 
 // Sums over a wave, the same bits in every lane, and inclusive sums over its lanes
 // (without LDS: a shuffle of 64 bits takes two trips through it).
@@ -126,109 +129,101 @@ __device__ __forceinline__ double weight_of(float l, float top, const Heat &h) {
   return ldexp(p, int(uint32_t(__builtin_bit_cast(uint64_t, n))));
 }
 
-// A row's elements in pieces of 16 bytes: piece c holds elements c E - lead .. + E - 1,
-// so that pieces are aligned wherever the row begins.
+// A row's elements in pieces of 16 bytes, E of them from element c E on, whatever
+// the row's alignment (the loads need none).  Elements past the row's end are -inf,
+// which weighs nothing.
 template <class T>
 struct RowOf {
   static constexpr int E = 16 / int(sizeof(T));
-  const T *x;
-  int lead, vocab;
-  __device__ __forceinline__ RowOf(const VerifyArgs &a, int row)
-      : x(static_cast<const T *>(a.logits) + size_t(row) * a.stride), lead(int(reinterpret_cast<size_t>(x) / sizeof(T) % E)), vocab(a.vocab) {}
-  typedef uint32_t Raw __attribute__((ext_vector_type(4)));
   typedef T Values __attribute__((ext_vector_type(E)));
-  // (elements past the row's ends: -inf, which weighs nothing)
-  __device__ __forceinline__ Raw raw(int c) const {
-    const int i = c * E - lead;
-    if (i >= 0 && i + E <= vocab) return *reinterpret_cast<const Raw *>(x + i);
+  typedef T Anywhere __attribute__((ext_vector_type(E), aligned(sizeof(T))));
+  const T *x;
+  int vocab;
+  __device__ __forceinline__ RowOf(const VerifyArgs &a, int row) : x(static_cast<const T *>(a.logits) + size_t(row) * a.stride), vocab(a.vocab) {}
+  __device__ __forceinline__ Values piece(int c) const {
+    const int i = c * E;
+    if (i + E <= vocab) return *reinterpret_cast<const Anywhere *>(x + i);
     Values v;
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = T(-INFINITY);
-    if (i < vocab)
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (i + e >= 0 && i + e < vocab) v[e] = x[i + e];
-    return __builtin_bit_cast(Raw, v);
+    for (int e = 0; e < E; ++e) v[e] = i + e < vocab ? x[i + e] : T(-INFINITY);
+    return v;
   }
-  static __device__ __forceinline__ void floats(Raw r, float (&v)[E]) {
-    const Values u = __builtin_bit_cast(Values, r);
+  // A part's pieces, all on their way at once.
+  __device__ __forceinline__ void part(int part, int lane, Values (&v)[kPieces]) const {
+    const bool whole = (part + 1) * (kPart * E) <= vocab;
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = float(u[e]);
+    for (int j = 0; j < kPieces; ++j) {
+      const int c = part * kPart + j * kWave + lane;
+      if (whole) v[j] = *reinterpret_cast<const Anywhere *>(x + c * E);
+      else v[j] = piece(c);
+    }
   }
-  __device__ __forceinline__ void load(int c, float (&v)[E]) const { floats(raw(c), v); }
 };
 
-// Sums, largest and first of the largest of each part of each row: J pieces a
-// thread.
-template <class T, int J>
-__global__ __launch_bounds__(kThreads) void stats_kernel(VerifyArgs a) {
+// Sums, largest and first of the largest of each part of each row, a wave a run of
+// parts, the next of them on its way while one is summed.  Bound by the vector unit:
+// 24 operations an element (64 x 0..7 drafts, 151936 logits, bf16).
+template <class T>
+__global__ __launch_bounds__(kStatsThreads) void stats_kernel(VerifyArgs a) {
+  typedef typename RowOf<T>::Values Values;
   constexpr int E = RowOf<T>::E;
-  __shared__ float tops[kWaves];
-  __shared__ double sums[kWaves];
-  __shared__ int firsts[kWaves];
-  const int part = int(blockIdx.y), row = int(blockIdx.x), lane = threadIdx.x & (kWave - 1), wave = int(threadIdx.x) / kWave;
-  const RowOf<T> r(a, row);
-  const int c0 = part * (J * kThreads) + int(threadIdx.x);
-  typename RowOf<T>::Raw raw[J];
-  const int i0 = part * (J * kThreads * E) - r.lead;
-  if (i0 >= 0 && i0 + J * kThreads * E <= a.vocab) {   // the whole part is inside the row
-    const typename RowOf<T>::Raw *from = reinterpret_cast<const typename RowOf<T>::Raw *>(r.x + i0) + threadIdx.x;
+  const int lane = threadIdx.x & (kWave - 1);
+  const size_t waves = size_t(gridDim.x) * (kStatsThreads / kWave), units = size_t(a.n_rows) * a.n_parts;
+  const size_t wave = size_t(blockIdx.x) * (kStatsThreads / kWave) + __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
+  const size_t each = units / waves, more = units % waves;   // (the first `more` waves take one more)
+  size_t left = each + (wave < more);
+  const size_t begin = wave * each + min(wave, more);
+  int row = int(begin / a.n_parts), part = int(begin % a.n_parts), known = -1, s = -1;
+  if (left == 0) return;
+  Values next[kPieces];
+  RowOf<T>(a, row).part(part, lane, next);
+  Heat h{};
+  bool mine = false;   // whether the row is any sequence's
+  while (true) {
+    Values x[kPieces];
 #pragma unroll
-    for (int j = 0; j < J; ++j) raw[j] = from[j * kThreads];
-  } else {
-#pragma unroll
-    for (int j = 0; j < J; ++j) raw[j] = r.raw(c0 + j * kThreads);
-  }
-  const int s = sequence_of(a.offsets, a.n_seqs, row, lane);
-  if (s < 0 || row >= a.offsets[s + 1]) return;
-  const Heat h = heat_of(a, s);
-  if (part == 0 && threadIdx.x == 0 && row == max(a.offsets[s], 0)) a.tickets[s] = 0;
-  float top = -INFINITY;   // (a NaN stays)
-#pragma unroll
-  for (int j = 0; j < J; ++j) {
-    float v[E];
-    r.floats(raw[j], v);
-#pragma unroll
-    for (int e = 0; e < E; ++e) top = __builtin_elementwise_maximum(top, v[e]);
-  }
-  const bool nan = top != top;
-  top = wave_max(top, lane);
-  if (lane == 0) tops[wave] = top;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) top = fmaxf(top, tops[w]);
-  // (from the packed values again: as floats they would take the registers of half the waves)
-#pragma unroll
-  for (int j = 0; j < J; ++j) asm volatile("" : "+v"(raw[j]));
-  double sum = 0.0;
-  int first = 0x7FFFFFFF;
-  if (h.t > 0.0f) {
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      float v[E];
-      r.floats(raw[j], v);
-#pragma unroll
-      for (int e = 0; e < E; ++e) sum += weight_of(v[e], top, h);
+    for (int j = 0; j < kPieces; ++j) x[j] = next[j];
+    const int this_row = row, this_part = part;
+    if (++part == a.n_parts) part = 0, ++row;
+    if (--left) RowOf<T>(a, row).part(part, lane, next);
+    if (this_row != known) {
+      known = this_row;
+      s = sequence_of(a.offsets, a.n_seqs, known, lane);
+      mine = s >= 0 && known < a.offsets[s + 1];
+      if (mine) {
+        h = heat_of(a, s);
+        if (lane == 0 && known == max(a.offsets[s], 0)) a.tickets[s] = 0;
+      }
     }
-  } else {
+    if (mine) {
+      float top = -INFINITY;   // (a NaN stays)
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-      float v[E];
-      r.floats(raw[j], v);
+      for (int j = 0; j < kPieces; ++j)
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (v[e] == top) first = min(first, (c0 + j * kThreads) * E - r.lead + e);
+        for (int e = 0; e < E; ++e) top = __builtin_elementwise_maximum(top, float(x[j][e]));
+      const bool nan = top != top;
+      top = wave_max(top, lane);
+      double sum = 0.0;
+      int first = 0x7FFFFFFF;
+      if (h.t > 0.0f) {
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j)
+#pragma unroll
+          for (int e = 0; e < E; ++e) sum += weight_of(float(x[j][e]), top, h);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j)
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (float(x[j][e]) == top) first = min(first, (this_part * kPart + j * kWave + lane) * E + e);
+        first = wave_min(first, lane);
+      }
+      if (nan || top == INFINITY) sum = __builtin_nan("");
+      sum = wave_sum(sum, lane);
+      if (lane == 0) a.parts[size_t(this_row) * a.n_parts + this_part] = Part{sum, top, first};
     }
-    first = wave_min(first, lane);
+    if (left == 0) return;
   }
-  if (nan || top == INFINITY) sum = __builtin_nan("");
-  sum = wave_sum(sum, lane);
-  if (lane == 0) sums[wave] = sum, firsts[wave] = first;
-  __syncthreads();
-  if (threadIdx.x != 0) return;
-#pragma unroll
-  for (int w = 1; w < kWaves; ++w) sum += sums[w], first = min(first, firsts[w]);
-  a.parts[size_t(row) * a.n_parts + part] = Part{sum, top, first};
 }
 
 // A row's distribution: weights over `total`.
@@ -267,43 +262,58 @@ __device__ __forceinline__ Row row_of(const Part *p, int n, const Part &first, c
 // but for `skip`.
 template <class T>
 struct Piece : RowOf<T> {
-  using RowOf<T>::E, RowOf<T>::lead, RowOf<T>::vocab;
+  using RowOf<T>::E, RowOf<T>::vocab;
+  typedef float Shares __attribute__((ext_vector_type(E)));
+  typedef float AnyShares __attribute__((ext_vector_type(E), aligned(4)));
   const Row &r;
   const Heat &h;
   const float *q;
-  bool q_aligned;
   __device__ __forceinline__ Piece(const VerifyArgs &a, int row, const Row &r, const Heat &h)
-      : RowOf<T>(a, row), r(r), h(h), q(a.probs + size_t(row) * a.probs_stride), q_aligned(lead == 0 && reinterpret_cast<size_t>(q) % 16 == 0) {}
+      : RowOf<T>(a, row), r(r), h(h), q(a.probs + size_t(row) * a.probs_stride) {}
+  __device__ __forceinline__ Shares shares(int c) const {
+    const int i = c * E;
+    if (i + E <= vocab) return *reinterpret_cast<const AnyShares *>(q + i);
+    Shares v;
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = i + e < vocab ? q[i + e] : 0.0f;
+    return v;
+  }
+  __device__ __forceinline__ double over(T l, float share) const { return fmax(fma(double(share), -r.total, weight_of(float(l), r.top, h)), 0.0); }
   template <bool OVER>
   __device__ __forceinline__ void weights(int c, int skip, double (&w)[E]) const {
-    float v[E], u[E];
-    const int i0 = c * E - lead;
-    if constexpr (OVER) {
-      if (q_aligned && i0 + E <= vocab) {
-        load_floats<E>(q + i0, u);
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) u[e] = i0 + e >= 0 && i0 + e < vocab ? q[i0 + e] : 0.0f;
-      }
-    }
-    this->load(c, v);
+    const typename RowOf<T>::Values v = this->piece(c);
+    Shares u;
+    if constexpr (OVER) u = shares(c);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      w[e] = weight_of(v[e], r.top, h);
-      if constexpr (OVER) w[e] = fmax(fma(double(u[e]), -r.total, w[e]), 0.0);
-      else if (i0 + e == skip) w[e] = 0.0;
+      if constexpr (OVER) w[e] = over(v[e], u[e]);
+      else w[e] = c * E + e == skip ? 0.0 : weight_of(float(v[e]), r.top, h);
     }
   }
-  template <bool OVER, int J>
-  __device__ __forceinline__ void sums(int part, int skip, double (&mine)[J]) const {
+  // The sum of a part's weights, by a wave.
+  template <bool OVER>
+  __device__ __forceinline__ double part_sum(int part, int skip, int lane) const {
+    typename RowOf<T>::Values v[kPieces];
+    Shares u[kPieces];
+    if constexpr (OVER) {
+      const bool whole = (part + 1) * (kPart * E) <= vocab;
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-      double w[E];
-      weights<OVER>((part * J + j) * kThreads + int(threadIdx.x), skip, w);
-      mine[j] = 0.0;
-#pragma unroll
-      for (int e = 0; e < E; ++e) mine[j] += w[e];
+      for (int j = 0; j < kPieces; ++j) {
+        const int c = part * kPart + j * kWave + lane;
+        if (whole) u[j] = *reinterpret_cast<const AnyShares *>(q + c * E);
+        else u[j] = shares(c);
+      }
     }
+    this->part(part, lane, v);
+    double all = 0.0;
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j)
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if constexpr (OVER) all += over(v[j][e], u[j][e]);
+        else all += (part * kPart + j * kWave + lane) * E + e == skip ? 0.0 : weight_of(float(v[j][e]), r.top, h);
+      }
+    return wave_sum(all, lane);
   }
 };
 
@@ -335,26 +345,28 @@ __device__ __forceinline__ Place place_of(int n, double u, double v0, int lane, 
   return {behind, INFINITY};   // (rounding, or a number of 1 and more)
 }
 
-// A workgroup a sequence, or one for each part where q may be needed: each finds
-// the row that the sequence stops at, four rows at a time, a wave each.  The token
-// there: parts' sums are known, or, of p - q, taken by the sequence's workgroups;
-// the row's wave (or the last workgroup) finds the part that the threshold falls into,
-// the workgroup the element in it.  What it costs is its chain of loads: offsets,
-// then parts' sums and drafts, then the drafted tokens' logits, then the part found.
-template <class T, int J>
+// A workgroup a sequence, or, where q may be needed, some: each finds the row that
+// the sequence stops at, a wave a row at a time.  The token there: parts' sums are
+// known, or, of p - q, taken by the sequence's workgroups; the row's wave (of the last
+// workgroup) finds the part that the threshold falls into, the workgroup the
+// element in it.  What it costs is its chain of loads: offsets, then parts' sums
+// and drafts, then the drafted tokens' logits, then the part found.
+template <class T>
 __global__ __launch_bounds__(kThreads) void pick_kernel(VerifyArgs a) {
-  constexpr int E = RowOf<T>::E, PART = J * kThreads;   // pieces of a part
+  constexpr int E = RowOf<T>::E;
+  static_assert(kPart <= kThreads, "a piece a thread");
   __shared__ Row rows[kWaves];
   __shared__ int stops[kWaves];
-  __shared__ double scan[J][kWaves];
+  constexpr int kNear = 2 * kWaves;
+  __shared__ double scan[kWaves], near[kNear];   // (sums of one workgroup's few parts stay here)
   __shared__ Place place;
-  __shared__ int at, last, joins;
-  const int s = int(blockIdx.x), part = int(blockIdx.y), lane = threadIdx.x & (kWave - 1);
+  __shared__ int at, last, joins, without;
+  const int s = int(blockIdx.x), group = int(blockIdx.y), lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
   const int begin = max(a.offsets[s], 0), end = min(a.offsets[s + 1], a.n_rows);
   const Heat h = heat_of(a, s);
   if (begin >= end) {
-    if (part == 0 && threadIdx.x == 0) a.accepted[s] = 0;
+    if (group == 0 && threadIdx.x == 0) a.accepted[s] = 0;
     return;
   }
   int row = begin, owner, token = -1;
@@ -389,7 +401,7 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(VerifyArgs a) {
   }
   row += owner;
   const Row r = rows[owner];
-  if (part == 0) {
+  if (group == 0) {
     for (int i = begin + int(threadIdx.x); i < end; i += kThreads)
       if (i != row) a.tokens[i] = i < row ? a.drafts[i] : -1;
     if (threadIdx.x == 0) {
@@ -400,125 +412,99 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(VerifyArgs a) {
   }
   if (!(r.total > 0.0) || h.t == 0.0f) return;
   const bool over = row != end - 1 && a.probs;
-  if (!over && part != 0) return;
+  if (!over && group != 0) return;
   const Piece<T> x(a, row, r, h);
   const Part *parts = a.parts + size_t(row) * a.n_parts;
-  double mine[J];
-  // the sum of every thread's pieces over the workgroup
-  const auto block_sum = [&]() __attribute__((always_inline)) {
-    double all = 0.0;
-#pragma unroll
-    for (int j = 0; j < J; ++j) all += mine[j];
-    all = wave_sum(all, lane);
-    if (lane == 0) scan[0][wave] = all;
-    __syncthreads();
-    all = scan[0][0];
-#pragma unroll
-    for (int v = 1; v < kWaves; ++v) all += scan[0][v];
-    __syncthreads();
-    return all;
-  };
+  if (threadIdx.x == 0) at = 0x7FFFFFFF, last = -1;
   bool from_rest = over;   // weights are those of p - q
   int skip = -1;           // the token that p is to lack
-  if (threadIdx.x == 0) at = 0x7FFFFFFF, last = -1;
   if (over) {
     double *sums = a.rest + size_t(s) * a.n_parts;
-    x.template sums<true, J>(part, -1, mine);
-    const double sum = block_sum();
-    if (threadIdx.x == 0) {
-      __hip_atomic_store(sums + part, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      __threadfence();
-      joins = atomicAdd(a.tickets + s, 1u) == unsigned(a.n_parts - 1);
+    for (int part = group * kWaves + wave; part < a.n_parts; part += a.groups * kWaves) {
+      const double sum = x.template part_sum<true>(part, -1, lane);
+      if (lane != 0) continue;
+      if (a.groups == 1 && part < kNear) near[part] = sum;
+      else __hip_atomic_store(sums + part, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
+    // (The sums go past the caches and are there before the ticket is taken; a fence
+    // would write back the whole L2, 100 us in all for 64 sequences' workgroups.)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (!joins) return;
-    __threadfence();
+    if (a.groups > 1) {
+      if (threadIdx.x == 0)
+        joins = __hip_atomic_fetch_add(a.tickets + s, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == unsigned(a.groups - 1);
+      __syncthreads();
+      if (!joins) return;
+    }
     if (wave == owner) {
-      const auto of = [&](int i) __attribute__((always_inline)) { return __hip_atomic_load(sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+      const auto of = [&](int i) __attribute__((always_inline)) {
+        return a.groups == 1 && i < kNear ? near[i] : __hip_atomic_load(sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      };
       const Place p = place_of(a.n_parts, double(u.y), lane < a.n_parts ? of(lane) : 0.0, lane, of);
       if (lane == 0) place = p;
     }
     __syncthreads();
-    if (place.part < 0) from_rest = false;   // nothing is left: from p
+    from_rest = place.part >= 0;   // (nothing is left: from p)
     __syncthreads();
-  } else {
-    // the part that lacks the drafted token: the difference keeps 42 bits, or it is
-    // summed without the token
-    __shared__ int without;
+  }
+  if (!from_rest) {
     if (wave == owner) {
-      const int lacking = known ? (token + x.lead) / (PART * E) : -1;
-      const double with = lane == lacking ? share : lacking >= kWave ? part_weight(parts[lacking], r.top, h) : INFINITY;
-      const bool lost = lacking >= 0 && __builtin_amdgcn_ballot_w64(!(with - weight > with * 0x1p-10) && with < INFINITY) != 0;
-      if (lane == 0) without = known ? token : -1, joins = lost;
+      // the part that lacks the drafted token: the difference keeps 42 bits, or it
+      // is summed without the token
+      int lacking = -1;
+      double less = 0.0;
+      if (!over && known) {
+        lacking = token / (kPart * E);
+        const double with = lacking < kWave ? lane_value(share, lacking) : part_weight(parts[lacking], r.top, h);
+        less = with - weight;
+        if (!(less > with * 0x1p-10)) less = x.template part_sum<false>(lacking, token, lane);
+      }
+      const auto of = [&](int i) __attribute__((always_inline)) { return i == lacking ? less : part_weight(parts[i], r.top, h); };
+      const double v0 = lane < a.n_parts ? lane == lacking ? less : share : 0.0;
+      Place p = place_of(a.n_parts, double(u.y), v0, lane, of);
+      if (p.part < 0) {   // nothing is left without the token: from p
+        lacking = -1;
+        p = place_of(a.n_parts, double(u.y), lane < a.n_parts ? share : 0.0, lane, of);
+      }
+      if (lane == 0) place = p, without = lacking >= 0 ? token : -1;
     }
     __syncthreads();
     skip = without;
-    if (joins) {
-      x.template sums<false, J>((skip + x.lead) / (PART * E), skip, mine);
-      weight = block_sum();
-    }
-  }
-  if (!from_rest) {
-    for (int again = 0; again < 2; ++again) {
-      if (wave == owner) {
-        const int lacking = skip >= 0 ? (skip + x.lead) / (PART * E) : -1;
-        const auto less = [&](int i, double v) __attribute__((always_inline)) { return i != lacking ? v : joins && !over ? weight : v - weight; };
-        const auto of = [&](int i) __attribute__((always_inline)) { return less(i, part_weight(parts[i], r.top, h)); };
-        const Place p = place_of(a.n_parts, double(u.y), lane < a.n_parts ? less(lane, share) : 0.0, lane, of);
-        if (lane == 0) place = p;
-      }
-      __syncthreads();
-      if (place.part >= 0) break;
-      skip = -1;   // nothing is left without the token: from p
-      __syncthreads();
-    }
     if (place.part < 0) return;   // (p weighs something)
   }
-  // the first piece past the threshold (or the last with a weight), then in it the
-  // element, by the piece's thread
+  // The first piece past the threshold (or the last with a weight), then in it the
+  // element: a piece a thread.
   const double target = place.target;
-  const int c0 = place.part * PART;
-  if (from_rest) x.template sums<true, J>(place.part, -1, mine);
-  else x.template sums<false, J>(place.part, skip, mine);
-  double upto[J];
+  const int piece = place.part * kPart + int(threadIdx.x);
+  double w[E], mine = 0.0;
+  if (threadIdx.x < kPart) {
+    if (from_rest) x.template weights<true>(piece, -1, w);
+    else x.template weights<false>(piece, skip, w);
 #pragma unroll
-  for (int j = 0; j < J; ++j) {
-    upto[j] = wave_scan(mine[j]);
-    if (lane == kWave - 1) scan[j][wave] = upto[j];
+    for (int e = 0; e < E; ++e) mine += w[e];
   }
+  const double upto = wave_scan(mine);
+  if (lane == kWave - 1) scan[wave] = upto;
   __syncthreads();
-  double before = 0.0, base = 0.0;
-  int past = 0x7FFFFFFF, behind = -1;
+  double before = upto - mine;
 #pragma unroll
-  for (int j = 0; j < J; ++j) {
-    double here = base;   // all before this wave's pieces of round j
-#pragma unroll
-    for (int v = 0; v < kWaves; ++v) {
-      if (v < wave) here += scan[j][v];
-      base += scan[j][v];
-    }
-    if (mine[j] > 0.0) {
-      behind = j * kThreads + int(threadIdx.x);
-      if (past == 0x7FFFFFFF && here + upto[j] > target) past = behind, before = here + (upto[j] - mine[j]);
-    }
-  }
-  if (past < 0x7FFFFFFF) atomicMin(&at, past);
-  if (behind >= 0) atomicMax(&last, behind);
+  for (int v = 0; v < kWaves; ++v)
+    if (v < wave) before += scan[v];
+  // (what precedes a thread and with it is, but for rounding, what precedes the next)
+  const bool past = mine > 0.0 && before + mine > target;
+  if (past) atomicMin(&at, int(threadIdx.x));
+  if (mine > 0.0) atomicMax(&last, int(threadIdx.x));
   __syncthreads();
-  const int piece = at < 0x7FFFFFFF ? at : last;
-  if (piece < 0 || piece % kThreads != int(threadIdx.x)) return;
-  double w[E];
-  if (from_rest) x.template weights<true>(c0 + piece, -1, w);
-  else x.template weights<false>(c0 + piece, skip, w);
-  int token_at = -1;
+  if (int(threadIdx.x) != (at < 0x7FFFFFFF ? at : last)) return;
+  int found = -1;
   bool done = false;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     before += w[e];
-    if (!done && w[e] > 0.0) token_at = (c0 + piece) * E - x.lead + e;
-    done = done || (piece == past && w[e] > 0.0 && before > target);
+    if (!done && w[e] > 0.0) found = piece * E + e;
+    done = done || (past && w[e] > 0.0 && before > target);
   }
-  a.tokens[row] = token_at;
+  a.tokens[row] = found;
 }
 
 int launch_err(const char *what) {
@@ -534,33 +520,32 @@ int check_sizes(const lmx_drafts *d, int type) {
   return LMX_OK;
 }
 
-// Pieces of 16 bytes a thread: parts of 4 while that still makes four workgroups a
-// CU, else of 2.
-int pieces_of(size_t rows, size_t vocab, int type) {
-  const size_t part = kThreads * 8 * (16 / type_bytes(type));
-  return rows * (vocab / part) >= 1024 ? 8 : 2;
-}
-size_t parts_of(size_t rows, size_t vocab, int type) {
-  const size_t e = 16 / type_bytes(type), part = kThreads * e * pieces_of(rows, vocab, type);
-  return (vocab + e - 1 + part - 1) / part;   // (wherever in a piece a row begins)
+size_t parts_of(size_t vocab, int type) {
+  const size_t part = kPart * (16 / type_bytes(type));
+  return (vocab + part - 1) / part;
 }
 
-template <class T, int J>
+template <class T>
 int launch(const VerifyArgs &a, hipStream_t st) {
-  if (a.n_rows) stats_kernel<T, J><<<dim3(unsigned(a.n_rows), unsigned(a.n_parts)), kThreads, 0, st>>>(a);
+  // (four waves a SIMD, each with a few parts to go through; two or eight take as long)
+  const size_t units = size_t(a.n_rows) * a.n_parts, most = 256 * 16;
+  if (units) stats_kernel<T><<<unsigned((std::min(units, most) + 3) / 4), kStatsThreads, 0, st>>>(a);
   const int r = launch_err("verify");
   if (r) return r;
-  pick_kernel<T, J><<<dim3(unsigned(a.n_seqs), a.probs ? unsigned(a.n_parts) : 1u), kThreads, 0, st>>>(a);
+  pick_kernel<T><<<dim3(unsigned(a.n_seqs), unsigned(a.groups)), kThreads, 0, st>>>(a);
   return launch_err("verify pick");
 }
-template <class T>
-int launch(const VerifyArgs &a, int pieces, hipStream_t st) {
-  return pieces == 8 ? launch<T, 8>(a, st) : launch<T, 2>(a, st);
+
+// Workgroups of a sequence for p - q: a part a wave, as long as that is four
+// workgroups a CU at most (one where it has two parts a wave).
+int groups_of(const VerifyArgs &a) {
+  if (!a.probs || a.n_parts <= 2 * kWaves) return 1;
+  return std::max(1, std::min((a.n_parts + kWaves - 1) / kWaves, 1024 / a.n_seqs));
 }
 
 struct Layout { size_t rest, tickets, all; };
 Layout layout(const lmx_drafts *d, int type) {
-  const size_t parts = parts_of(d->n_rows, d->vocab, type);
+  const size_t parts = parts_of(d->vocab, type);
   Layout l{};
   l.rest = d->n_rows * parts * sizeof(Part);
   l.tickets = l.rest + d->n_seqs * parts * sizeof(double);
@@ -611,13 +596,13 @@ int lmx_verify_drafts(const lmx_drafts *d, int type, const void *logits, size_t 
   char *work = static_cast<char *>(workspace);
   a.parts = reinterpret_cast<Part *>(work), a.rest = reinterpret_cast<double *>(work + l.rest);
   a.tickets = reinterpret_cast<unsigned *>(work + l.tickets);
-  a.n_parts = int(parts_of(d->n_rows, d->vocab, type));
-  const int pieces = pieces_of(d->n_rows, d->vocab, type);
+  a.n_parts = int(parts_of(d->vocab, type));
+  a.groups = groups_of(a);
   hipStream_t st = static_cast<hipStream_t>(stream);
   switch (type) {
-  case LMX_F32: return launch<float>(a, pieces, st);
-  case LMX_F16: return launch<f16>(a, pieces, st);
-  default: return launch<bf16>(a, pieces, st);
+  case LMX_F32: return launch<float>(a, st);
+  case LMX_F16: return launch<f16>(a, st);
+  default: return launch<bf16>(a, st);
   }
 }
 
