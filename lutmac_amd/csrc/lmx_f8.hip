@@ -22,7 +22,6 @@ namespace {
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
-typedef float v16f __attribute__((ext_vector_type(16)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
@@ -36,9 +35,11 @@ struct F8Args {
   const void *bias, *x;
   void *y;
   int rows, cols, batch, Kp, steps;
-  int Bp;            // batch padded to whole 16-byte pieces
+  int Bp;            // batch padded to 64
   uint8_t *codes;    // [batch][Kp]
   float *scales;     // [steps][Bp]
+  int splits;        // parts of k, each with sums of its own to join
+  float *sums;       // [splits][batch][rows]
 };
 
 // Eight neighbouring elements of a row of x (zeros past its end); vec: the row
@@ -84,12 +85,12 @@ __device__ __forceinline__ uint2 block_codes(const float (&v)[8], int lane, floa
 }
 
 // Codes and scales of x: 16 lanes a block.
-template <class T>
-__global__ __launch_bounds__(256) void f8_codes_kernel(F8Args a) {
+template <class T, int NT>
+__global__ __launch_bounds__(NT) void f8_codes_kernel(F8Args a) {
   const int lane = threadIdx.x & (kWave - 1), row = int(blockIdx.x);
   const T *x = static_cast<const T *>(a.x) + size_t(row) * a.cols;
   const bool vec = reinterpret_cast<size_t>(x) % 16 == 0;
-  for (int k = int(threadIdx.x) * 8; k < a.Kp; k += 256 * 8) {   // (whole groups of 16 lanes)
+  for (int k = int(threadIdx.x) * 8; k < a.Kp; k += NT * 8) {   // (whole groups of 16 lanes)
     float v[8], s;
     load8(x, k, a.cols, vec, v);
     const uint2 c = block_codes(v, lane, s);
@@ -124,26 +125,273 @@ __device__ __forceinline__ float scalar_load(const float *p) {
   return *(const __attribute__((address_space(4))) float *)(p);
 }
 
+// 128-byte rows in LDS: piece p (16 bytes) of row r lies at p ^ (r / 2 mod 8), so
+// that the 16 lanes of a read's phase touch all 64 banks once.
+__device__ __forceinline__ int piece_place(int row, int piece) { return 16 * (piece ^ (row >> 1 & 7)); }
+// Where lane `lane` of a load of 8 rows reads row `row` (the last one past it).
+__device__ __forceinline__ int piece_offset(int row, int last, int stride, int lane) {
+  return min(row, last) * stride + piece_place(row, lane % 8);
+}
+
+// One step of 16 rows as a matrix instruction's operand: lane (i, g) holds bytes
+// 16 g .. and 64 + 16 g .. of row i (any 32 bytes do, if both operands' are the same).
+struct Operand {
+  v4i a, b;
+  __device__ __forceinline__ void cut(int left, int g) { a = cut_piece(a, left - 16 * g), b = cut_piece(b, left - 64 - 16 * g); }
+};
 __device__ __forceinline__ v8h halves(int lo, int hi) {   // 8 codes -> fp16, exactly
   const v2h a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true),
             c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
   return v8h{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
+// What the instructions take: the codes, or for fp32 results fp16.
+template <bool EXACT>
+struct Factor {
+  v8i v;
+  __device__ __forceinline__ explicit Factor(const Operand &o) : v(__builtin_shufflevector(o.a, o.b, 0, 1, 2, 3, 4, 5, 6, 7)) {}
+  Factor() = default;
+};
+template <>
+struct Factor<true> {
+  v8h v[4];
+  __device__ __forceinline__ explicit Factor(const Operand &o)
+      : v{halves(o.a[0], o.a[1]), halves(o.a[2], o.a[3]), halves(o.b[0], o.b[1]), halves(o.b[2], o.b[3])} {}
+  Factor() = default;
+};
+// The sums of a block of 128: lane (j, g) gets weight rows 4 g .. + 3 of activation row j.
+__device__ __forceinline__ v4f products(const Factor<false> &w, const Factor<false> &x) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, x.v, v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0, 0, 0, 0);
+}
+__device__ __forceinline__ v4f products(const Factor<true> &w, const Factor<true> &x) {
+  v4f p = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int q = 0; q < 4; ++q) p = __builtin_amdgcn_mfma_f32_16x16x32_f16(w.v[q], x.v[q], p, 0, 0, 0);
+  return p;
+}
+__device__ __forceinline__ void add_scaled(v4f &acc, const v4f &p, float f) {
+#pragma unroll
+  for (int v = 0; v < 4; ++v) acc[v] = fmaf(p[v], f, acc[v]);
+}
 
+// Biases of four neighbouring weight rows (past the last: its own).
+template <class T>
+__device__ __forceinline__ v4f biases(const F8Args &a, int n) {
+  v4f f = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (const T *b = static_cast<const T *>(a.bias)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = float(b[min(n + i, a.rows - 1)]);
+  }
+  return f;
+}
+// Four neighbouring outputs y[m][n .. n + 3]; whole groups go out in one store where y allows it (vec).
+template <class T>
+__device__ __forceinline__ void store4(const F8Args &a, int m, int n, const v4f s, bool vec) {
+  if (m >= a.batch || n >= a.rows) return;
+  T *y = static_cast<T *>(a.y) + size_t(m) * a.rows + n;
+  if (vec) {   // (then rows are whole groups)
+    const float f[4] = {s[0], s[1], s[2], s[3]};
+    store_floats<4>(y, f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < a.rows) y[i] = T(s[i]);
+  }
+}
+template <class T>
+__device__ __forceinline__ bool vector_rows(const F8Args &a) {
+  return a.rows % 4 == 0 && reinterpret_cast<size_t>(a.y) % (4 * sizeof(T)) == 0;
+}
+
+// ---------------------------------------------------------------------------
+// One to four rows of activations, one launch: a workgroup takes 16 weight rows,
+// its W waves the k-steps w, w + W, ..., each through U LDS buffers of its own that
+// are filled straight from memory U - 1 steps ahead, so that no wave waits for
+// another before the end.  Every workgroup makes the codes itself, in LDS while its
+// first weights are on their way (R >= batch rows, a power of two; at most 16 values
+// a thread, which stay in registers), which saves a launch and the trip through memory.
+constexpr int rows_buffers(int waves) { return waves == 16 ? 3 : 4; }
+template <class T, int W, int R>
+__global__ __launch_bounds__(W *kWave) void f8_rows_kernel(F8Args a) {
+  constexpr bool EXACT = std::is_same<T, float>::value;
+  constexpr int U = rows_buffers(W), RB = 16 * kStep;
+  __shared__ v4f part[W][kWave];
+  extern __shared__ __attribute__((aligned(1024))) char lds[];   // the waves' buffers, codes [batch][Kp + 16], factors [batch][steps]
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
+  const int i = lane & 15, g = lane >> 4, row0 = int(blockIdx.x) * 16;
+  char *mine = lds + wave * (U * RB), *codes = lds + W * U * RB;
+  float *factors = reinterpret_cast<float *>(codes + a.batch * (a.Kp + 16));
+  constexpr int KEEP = 2, TR = W * kWave / R;   // threads of an activation row
+  const int am = int(threadIdx.x) / TR, k0 = int(threadIdx.x) % TR * 8;
+  const float *ws = a.w_scale + size_t(row0 / kStep) * a.steps;
+  float v[KEEP][8], wf[KEEP];
+  {
+    const T *x = static_cast<const T *>(a.x) + size_t(min(am, a.batch - 1)) * a.cols;
+    const bool vec = reinterpret_cast<size_t>(x) % 16 == 0;
+#pragma unroll
+    for (int j = 0; j < KEEP; ++j) {
+      load8(x, k0 + j * TR * 8, a.cols, vec, v[j]);
+      wf[j] = ws[min((k0 + j * TR * 8) / kStep, a.steps - 1)];
+    }
+  }
+  const auto wbuf = weight_buffer(a, row0);
+  int won[2];
+#pragma unroll
+  for (int n = 0; n < 2; ++n) won[n] = piece_offset(8 * n + lane / 8, a.rows - 1 - row0, int(a.w_stride), lane);
+  const int turns = wave < a.steps ? (a.steps - 1 - wave) / W + 1 : 0;
+  const auto fill = [&](int buf, int t) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n) buffer_to_lds(wbuf, mine + buf * RB + n * 1024, won[n], (wave + t * W) * kStep);
+  };
+#pragma unroll
+  for (int t = 0; t < U - 1; ++t)
+    if (t < turns) fill(t, t);
+  if (am < a.batch) {
+#pragma unroll
+    for (int j = 0; j < KEEP; ++j) {
+      const int k = k0 + j * TR * 8;
+      if (k < a.Kp) {   // (whole groups of 16 lanes)
+        float s;
+        const uint2 c = block_codes(v[j], lane, s);
+        *reinterpret_cast<uint2 *>(codes + am * (a.Kp + 16) + k) = c;
+        if (lane % 16 == 0) factors[am * a.steps + k / kStep] = s * wf[j];
+      }
+    }
+  }
+  lds_barrier();
+  const int m = min(i, a.batch - 1);
+  const char *xc = codes + m * (a.Kp + 16) + 16 * g;
+  const float *fc = factors + m * a.steps;
+  v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  int buf = 0;
+  for (int t = 0; t < turns; ++t) {
+    if (t + U - 1 <= turns) wait_loads<(U - 2) * 2>();
+    else wait_loads<0>();
+    const int step = wave + t * W;
+    const char *at = mine + buf * RB + i * kStep;
+    Operand w = {*reinterpret_cast<const v4i *>(at + piece_place(i, g)), *reinterpret_cast<const v4i *>(at + piece_place(i, 4 + g))};
+    const Operand x = {*reinterpret_cast<const v4i *>(xc + step * kStep), *reinterpret_cast<const v4i *>(xc + step * kStep + 64)};
+    const float f = fc[step];
+    if (t + U - 1 < turns) fill(buf == 0 ? U - 1 : buf - 1, t + U - 1);   // (the buffer of the step before, whose products are made)
+    if (a.cols - step * kStep < kStep) w.cut(a.cols - step * kStep, g);
+    add_scaled(acc, products(Factor<EXACT>(w), Factor<EXACT>(x)), f);
+    buf = buf == U - 1 ? 0 : buf + 1;
+  }
+  part[wave][lane] = acc;
+  const v4f bias = biases<T>(a, row0 + 4 * g);
+  __syncthreads();
+  if (wave != 0) return;
+#pragma unroll
+  for (int v = 1; v < W; ++v) acc += part[v][lane];
+  store4<T>(a, i, row0 + 4 * g, acc + bias, vector_rows<T>(a));
+}
+
+// ---------------------------------------------------------------------------
+// Some rows of activations (up to 16 G) and so few weight rows that tiles of
+// 64 x 64 leave CUs idle: 16 R weight rows a workgroup, its W waves the k-steps w,
+// w + W, ..., each through U LDS buffers of its own as above (weights, codes, the
+// codes' scales).
+template <class T, int W, int R, int G, int U>
+__global__ __launch_bounds__(W *kWave) void f8_few_kernel(F8Args a) {
+  constexpr bool EXACT = std::is_same<T, float>::value;
+  constexpr int CB = (R + G) * 16 * kStep, RB = CB + 64 * 4;   // bytes of a buffer: weights, codes, 64 scales
+  constexpr int LOADS = 2 * (R + G) + 1;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
+  const int i = lane & 15, g = lane >> 4, row0 = int(blockIdx.x) * (16 * R);
+  const auto wbuf = weight_buffer(a, row0);
+  const auto xbuf = __builtin_amdgcn_make_buffer_rsrc(a.codes, 0, a.batch * a.Kp, 0x00020000);
+  const auto sbuf = __builtin_amdgcn_make_buffer_rsrc(a.scales, 0, a.steps * a.Bp * 4, 0x00020000);
+  int won[2 * R], xon[2 * G];   // (a load instruction: 8 rows)
+#pragma unroll
+  for (int n = 0; n < 2 * R; ++n) won[n] = piece_offset(8 * n + lane / 8, a.rows - 1 - row0, int(a.w_stride), lane);
+#pragma unroll
+  for (int n = 0; n < 2 * G; ++n) xon[n] = piece_offset(8 * n + lane / 8, a.batch - 1, a.Kp, lane);
+  char *mine = lds + wave * (U * RB);
+  const int turns = wave < a.steps ? (a.steps - 1 - wave) / W + 1 : 0;
+  const auto fill = [&](int buf, int t) {
+    const int k = (wave + t * W) * kStep;
+#pragma unroll
+    for (int n = 0; n < 2 * R; ++n) buffer_to_lds(wbuf, mine + buf * RB + n * 1024, won[n], k);
+#pragma unroll
+    for (int n = 0; n < 2 * G; ++n) buffer_to_lds(xbuf, mine + buf * RB + (2 * R + n) * 1024, xon[n], k);
+    buffer_to_lds<4>(sbuf, mine + buf * RB + CB, 4 * lane, (wave + t * W) * a.Bp * 4);
+  };
+#pragma unroll
+  for (int t = 0; t < U - 1; ++t)
+    if (t < turns) fill(t, t);
+  const float *ws = a.w_scale + size_t(row0 / kStep) * a.steps;
+  float wf = scalar_load(ws + min(wave, a.steps - 1));
+  v4f acc[R][G];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int n = 0; n < G; ++n) acc[r][n] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  int buf = 0;
+  for (int t = 0; t < turns; ++t) {
+    if (t + U - 1 <= turns) wait_loads<(U - 2) * LOADS>();
+    else wait_loads<0>();
+    const int step = wave + t * W;
+    const char *at = mine + buf * RB + i * kStep;
+    const int pa = piece_place(i, g), pb = piece_place(i, 4 + g);
+    Operand w[R], x[G];
+    float f[G];
+#pragma unroll
+    for (int r = 0; r < R; ++r) w[r] = {*reinterpret_cast<const v4i *>(at + r * 16 * kStep + pa), *reinterpret_cast<const v4i *>(at + r * 16 * kStep + pb)};
+#pragma unroll
+    for (int n = 0; n < G; ++n) {
+      x[n] = {*reinterpret_cast<const v4i *>(at + (R + n) * 16 * kStep + pa), *reinterpret_cast<const v4i *>(at + (R + n) * 16 * kStep + pb)};
+      f[n] = *reinterpret_cast<const float *>(mine + buf * RB + CB + 4 * (16 * n + i)) * wf;
+    }
+    wf = scalar_load(ws + min(step + W, a.steps - 1));
+    if (t + U - 1 < turns) fill(buf == 0 ? U - 1 : buf - 1, t + U - 1);   // (the buffer of the step before, whose products are made)
+    if (a.cols - step * kStep < kStep)
+#pragma unroll
+      for (int r = 0; r < R; ++r) w[r].cut(a.cols - step * kStep, g);
+    Factor<EXACT> wv[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) wv[r] = Factor<EXACT>(w[r]);
+#pragma unroll
+    for (int n = 0; n < G; ++n) {
+      const Factor<EXACT> xv(x[n]);
+#pragma unroll
+      for (int r = 0; r < R; ++r) add_scaled(acc[r][n], products(wv[r], xv), f[n]);
+    }
+    buf = buf == U - 1 ? 0 : buf + 1;
+  }
+  __syncthreads();   // every wave is done with its buffers
+  v4f(*part)[R * G][kWave] = reinterpret_cast<v4f(*)[R * G][kWave]>(lds);
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int n = 0; n < G; ++n) part[wave][r * G + n][lane] = acc[r][n];
+  __syncthreads();
+  for (int q = wave; q < R * G; q += W) {
+    const int r = q / G, m = 16 * (q % G) + i, row = row0 + 16 * r + 4 * g;
+    v4f sum = part[0][q][lane];
+#pragma unroll
+    for (int v = 1; v < W; ++v) sum += part[v][q][lane];
+    store4<T>(a, m, row, sum + biases<T>(a, row), vector_rows<T>(a));
+  }
+}
+
+// ---------------------------------------------------------------------------
 // Many rows of activations: BN weight rows x BM activation rows per workgroup,
 // WN x WM waves, a block of 128 k per step through S LDS buffers that are filled
-// straight from memory S - 1 steps ahead.  A row's 16-byte pieces lie in LDS at p ^
-// (row / 2 mod 8), so that the 16 lanes of a read's phase touch all 64 banks once.
-// Each step's products are summed apart and enter the result with the step's two
-// scales.
-template <class T, int BN, int BM, int WN, int WM, int S>
-__global__ __launch_bounds__(WN *WM *kWave) __attribute__((amdgpu_waves_per_eu(BN *BM / (WN * WM) > 8192 ? 1 : 2))) void f8_tile_kernel(F8Args a) {
+// straight from memory S - 1 steps ahead.  Each step's products are summed apart and
+// enter the result with the step's two scales: 4 fused products of the vector unit for each matrix
+// instruction, half its time.
+//
+// PART: workgroup (tile, part) takes part blockIdx.y of k and leaves its sums for
+// f8_join_kernel: where tiles are few and k is long.
+template <class T, bool PART, int BN, int BM, int WN, int WM, int S>
+__global__ __launch_bounds__(WN *WM *kWave) __attribute__((amdgpu_waves_per_eu(2))) void f8_tile_kernel(F8Args a) {
   constexpr bool EXACT = std::is_same<T, float>::value;
-  constexpr int W = WN * WM, TN = BN / WN / 32, TM = BM / WM / 32;
-  constexpr int RB = (BN + BM) * kStep;   // bytes of a buffer: weights, then codes
-  static_assert(BN / WN <= kStep && kStep % (BN / WN) == 0, "a wave's weight rows share a scale");
+  constexpr int W = WN * WM, NW = BN / WN, MW = BM / WM, TN = NW / 16, TM = MW / 16;
+  constexpr int CB = (BN + BM) * kStep, RB = CB + BM * 4;   // bytes of a buffer: weights, codes, the codes' scales
+  constexpr int SL = BM / 4 / W;   // lanes of a wave that load scales
+  static_assert(NW <= kStep && kStep % NW == 0, "a wave's weight rows share a scale");
+  static_assert(SL * 4 * W == BM && SL <= kWave, "a load for the scales");
   extern __shared__ __attribute__((aligned(1024))) char lds[];
-  const auto swizzle = [](int row) { return (row >> 1) & 7; };
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / kWave);
   const int wn = wave % WN, wm = wave / WN;
   // Workgroups go round the 8 XCDs, each with an L2 of its own: XCD x takes the
@@ -158,138 +406,133 @@ __global__ __launch_bounds__(WN *WM *kWave) __attribute__((amdgpu_waves_per_eu(B
   const auto xbuf = __builtin_amdgcn_make_buffer_rsrc(a.codes + size_t(m0) * a.Kp, 0,
                                                       int(min(size_t(a.batch - m0) * a.Kp, size_t(0x7FFFFFFF))), 0x00020000);
   // One load instruction of a wave: 1 KB, 8 rows.
-  constexpr int LN = BN / 8 / W, LM = BM / 8 / W;
+  constexpr int LN = BN / 8 / W, LM = BM / 8 / W, LOADS = LN + LM + 1;
   static_assert(LN * 8 * W == BN && LM * 8 * W == BM, "whole instructions");
-  const int lr = lane / 8, lp = lane % 8;
   int won[LN], wom[LM];
 #pragma unroll
-  for (int j = 0; j < LN; ++j) {
-    const int r = (j * W + wave) * 8 + lr;
-    won[j] = min(r, a.rows - 1 - row0) * int(a.w_stride) + 16 * (lp ^ swizzle(r));
-  }
+  for (int j = 0; j < LN; ++j) won[j] = piece_offset((j * W + wave) * 8 + lane / 8, a.rows - 1 - row0, int(a.w_stride), lane);
 #pragma unroll
-  for (int j = 0; j < LM; ++j) {
-    const int r = (j * W + wave) * 8 + lr;
-    wom[j] = min(r, a.batch - 1 - m0) * a.Kp + 16 * (lp ^ swizzle(r));
-  }
-  const auto fill = [&](int buf, int k) {
+  for (int j = 0; j < LM; ++j) wom[j] = piece_offset((j * W + wave) * 8 + lane / 8, a.batch - 1 - m0, a.Kp, lane);
+  const int son = min(m0 + 4 * (wave * SL + lane), a.Bp - 4) * 4;   // (what is past the batch reaches no output)
+  const auto fill = [&](int buf, int s) {
 #pragma unroll
-    for (int j = 0; j < LN; ++j) buffer_to_lds(wbuf, lds + buf * RB + (j * W + wave) * 1024, won[j], k);
+    for (int j = 0; j < LN; ++j) buffer_to_lds(wbuf, lds + buf * RB + (j * W + wave) * 1024, won[j], s * kStep);
 #pragma unroll
-    for (int j = 0; j < LM; ++j) buffer_to_lds(xbuf, lds + buf * RB + BN * kStep + (j * W + wave) * 1024, wom[j], k);
+    for (int j = 0; j < LM; ++j) buffer_to_lds(xbuf, lds + buf * RB + BN * kStep + (j * W + wave) * 1024, wom[j], s * kStep);
+    const auto sbuf = __builtin_amdgcn_make_buffer_rsrc(a.scales + size_t(s) * a.Bp, 0, a.Bp * 4, 0x00020000);
+    if (lane < SL) buffer_to_lds(sbuf, lds + buf * RB + CB + wave * SL * 16, son, 0);
   };
-  v16f acc[TN][TM];
+  v4f acc[TN][TM];
 #pragma unroll
   for (int n = 0; n < TN; ++n)
 #pragma unroll
-    for (int m = 0; m < TM; ++m)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) acc[n][m][v] = 0.0f;
-  const int i = lane & 31, h = lane >> 5;
-  const int n_first = row0 + wn * (BN / WN);
+    for (int m = 0; m < TM; ++m) acc[n][m] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  const int i = lane & 15, g = lane >> 4;
+  const int n_first = row0 + wn * NW;
   const float *ws = a.w_scale + size_t(min(n_first, a.rows - 1) / kStep) * a.steps;
-  int xm[TM];
-#pragma unroll
-  for (int m = 0; m < TM; ++m) xm[m] = min(m0 + wm * (BM / WM) + 32 * m + i, a.batch - 1);
+  int steps = a.steps, s0 = 0;
+  if constexpr (PART) {
+    const int part = int(blockIdx.y);
+    s0 = int(unsigned(a.steps) * unsigned(part) / unsigned(a.splits));
+    steps = int(unsigned(a.steps) * unsigned(part + 1) / unsigned(a.splits)) - s0;
+  }
 #pragma unroll
   for (int s = 0; s < S - 1; ++s)
-    if (s < a.steps) fill(s, s * kStep);
+    if (s < steps) fill(s, s0 + s);
+  float wf = scalar_load(ws + s0);
   int buf = 0;
-  for (int s = 0; s < a.steps; ++s) {
-    float f[TM];
-    const float wf = scalar_load(ws + s);
-#pragma unroll
-    for (int m = 0; m < TM; ++m) f[m] = a.scales[size_t(s) * a.Bp + xm[m]] * wf;
-    wait_loads<0>();
+  const int pa = piece_place(i, g), pb = piece_place(i, 4 + g);
+  for (int s = 0; s < steps; ++s) {
+    if (s + S - 1 <= steps) wait_loads<(S - 2) * LOADS>();
+    else wait_loads<0>();
     lds_barrier();   // (a wave is there once its reads of the step before are done)
-    if (s + S - 1 < a.steps) fill(buf == 0 ? S - 1 : buf - 1, (s + S - 1) * kStep);
-    const char *wl = lds + buf * RB + (wn * (BN / WN) + i) * kStep;
-    const char *xl = lds + buf * RB + BN * kStep + (wm * (BM / WM) + i) * kStep;
-    v4i wp[TN][4], xp[TM][4];   // pieces 2 q + h
+    if (s + S - 1 < steps) fill(buf == 0 ? S - 1 : buf - 1, s0 + s + S - 1);
+    const char *wl = lds + buf * RB + (wn * NW + i) * kStep, *xl = lds + buf * RB + (BN + wm * MW + i) * kStep;
+    const float *sl = reinterpret_cast<const float *>(lds + buf * RB + CB) + wm * MW + i;
+    Factor<EXACT> wv[TN];
+    const int left = a.cols - (s0 + s) * kStep;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int at = 16 * ((2 * q + h) ^ swizzle(i));
-#pragma unroll
-      for (int n = 0; n < TN; ++n) wp[n][q] = *reinterpret_cast<const v4i *>(wl + n * 32 * kStep + at);
-#pragma unroll
-      for (int m = 0; m < TM; ++m) xp[m][q] = *reinterpret_cast<const v4i *>(xl + m * 32 * kStep + at);
+    for (int n = 0; n < TN; ++n) {
+      Operand w = {*reinterpret_cast<const v4i *>(wl + n * 16 * kStep + pa), *reinterpret_cast<const v4i *>(wl + n * 16 * kStep + pb)};
+      if (left < kStep) w.cut(left, g);
+      wv[n] = Factor<EXACT>(w);
     }
-    const int left = a.cols - s * kStep;
-    if (left < kStep) {
+    const float wnow = wf;
+    wf = scalar_load(ws + min(s0 + s + 1, a.steps - 1));
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
+    for (int m = 0; m < TM; ++m) {
+      const Factor<EXACT> xv(Operand{*reinterpret_cast<const v4i *>(xl + m * 16 * kStep + pa), *reinterpret_cast<const v4i *>(xl + m * 16 * kStep + pb)});
+      const float f = sl[16 * m] * wnow;
+      v4f p[TN];
 #pragma unroll
-        for (int n = 0; n < TN; ++n) wp[n][q] = cut_piece(wp[n][q], left - 16 * (2 * q + h));
+      for (int n = 0; n < TN; ++n) p[n] = products(wv[n], xv);
+#pragma unroll
+      for (int n = 0; n < TN; ++n) add_scaled(acc[n][m], p[n], f);
     }
-#pragma unroll
-    for (int n = 0; n < TN; ++n)
-#pragma unroll
-      for (int m = 0; m < TM; ++m) {
-        v16f p;
-#pragma unroll
-        for (int v = 0; v < 16; ++v) p[v] = 0.0f;
-        if constexpr (EXACT) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-#pragma unroll
-            for (int o = 0; o < 4; o += 2)
-              p = __builtin_amdgcn_mfma_f32_32x32x16_f16(halves(wp[n][q][o], wp[n][q][o + 1]), halves(xp[m][q][o], xp[m][q][o + 1]), p, 0, 0, 0);
-        } else {
-#pragma unroll
-          for (int q = 0; q < 4; q += 2) {
-            const v8i w8 = __builtin_shufflevector(wp[n][q], wp[n][q + 1], 0, 1, 2, 3, 4, 5, 6, 7),
-                      x8 = __builtin_shufflevector(xp[m][q], xp[m][q + 1], 0, 1, 2, 3, 4, 5, 6, 7);
-            p = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w8, x8, p, 0, 0, 0, 0, 0, 0);
-          }
-        }
-#pragma unroll
-        for (int v = 0; v < 16; ++v) acc[n][m][v] = fmaf(p[v], f[m], acc[n][m][v]);
-      }
     buf = buf == S - 1 ? 0 : buf + 1;
   }
-  // The sums leave through LDS, 32 activation rows of the wave at a time, so
-  // that stores are whole lines of y.
-  constexpr int NW = BN / WN, LD = NW * int(sizeof(T)) + 16;   // a row in LDS, apart by banks
-  static_assert(W * 32 * LD <= S * RB, "the rows fit in the buffers");
+  // The sums leave through LDS, 16 activation rows of the wave at a time, so that
+  // stores are whole lines of y.
+  typedef typename std::conditional<PART, float, T>::type Out;
+  constexpr int LD = NW * int(sizeof(Out)) + 16;   // a row in LDS, apart by banks
+  static_assert(W * 16 * LD <= S * RB, "the rows fit in the buffers");
   lds_barrier();   // every wave is done with the buffers
-  char *out = lds + wave * (32 * LD);
-  constexpr int V = 16 / int(sizeof(T)), LPR = NW / V;   // elements of a store, lanes of a row
-  T *base = static_cast<T *>(a.y);
-  const T *bias = static_cast<const T *>(a.bias);
+  char *out = lds + wave * (16 * LD);
+  constexpr int V = 16 / int(sizeof(Out)), LPR = NW / V;   // elements of a store, lanes of a row
+  Out *base = PART ? reinterpret_cast<Out *>(a.sums) + size_t(blockIdx.y) * a.batch * a.rows : static_cast<Out *>(a.y);
+  v4f bias[TN];
+#pragma unroll
+  for (int n = 0; n < TN; ++n) bias[n] = PART ? v4f{0.0f, 0.0f, 0.0f, 0.0f} : biases<T>(a, n_first + 16 * n + 4 * g);
   const bool vec = a.rows % V == 0 && reinterpret_cast<size_t>(base) % 16 == 0;
 #pragma unroll
   for (int m = 0; m < TM; ++m) {
-    const int m1 = m0 + wm * (BM / WM) + 32 * m;
+    const int m1 = m0 + wm * MW + 16 * m;
     if (m1 >= a.batch) break;
 #pragma unroll
-    for (int n = 0; n < TN; ++n)
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const int at = 32 * n + 8 * b + 4 * h;
-        float o[4];
-#pragma unroll
-        for (int v = 0; v < 4; ++v)
-          o[v] = acc[n][m][4 * b + v] + (bias ? float(bias[min(n_first + at + v, a.rows - 1)]) : 0.0f);
-        store_floats<4>(reinterpret_cast<T *>(out + i * LD) + at, o);
-      }
+    for (int n = 0; n < TN; ++n) {
+      const v4f o = acc[n][m] + bias[n];
+      const float f[4] = {o[0], o[1], o[2], o[3]};
+      store_floats<4>(reinterpret_cast<Out *>(out + i * LD) + 16 * n + 4 * g, f);
+    }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    T *y = base + size_t(m1) * a.rows + n_first;
+    Out *y = base + size_t(m1) * a.rows + n_first;
     if (vec) {
-      typedef T vecT __attribute__((ext_vector_type(V)));
+      typedef Out vecT __attribute__((ext_vector_type(V)));
 #pragma unroll
-      for (int q = 0; q < 32 * LPR / kWave; ++q) {
+      for (int q = 0; q < (16 * LPR + kWave - 1) / kWave; ++q) {
         const int r = q * (kWave / LPR) + lane / LPR, n = lane % LPR * V;
-        if (m1 + r < a.batch && n_first + n < a.rows)
-          *reinterpret_cast<vecT *>(y + size_t(r) * a.rows + n) = *reinterpret_cast<const vecT *>(out + r * LD + n * sizeof(T));
+        if (r < 16 && m1 + r < a.batch && n_first + n < a.rows)
+          *reinterpret_cast<vecT *>(y + size_t(r) * a.rows + n) = *reinterpret_cast<const vecT *>(out + r * LD + n * sizeof(Out));
       }
     } else {
-      for (int q = 0; q < 32 * NW / kWave; ++q) {
+      for (int q = 0; q < 16 * NW / kWave; ++q) {
         const int at = q * kWave + lane, r = at / NW, n = at % NW;
-        if (m1 + r < a.batch && n_first + n < a.rows) y[size_t(r) * a.rows + n] = *reinterpret_cast<const T *>(out + r * LD + n * sizeof(T));
+        if (m1 + r < a.batch && n_first + n < a.rows) y[size_t(r) * a.rows + n] = *reinterpret_cast<const Out *>(out + r * LD + n * sizeof(Out));
       }
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
+}
+
+// y from the parts' sums, four weight rows of an activation row per thread.
+template <class T>
+__global__ __launch_bounds__(256) void f8_join_kernel(F8Args a) {
+  const int quads = (a.rows + 3) / 4;
+  const size_t at = size_t(blockIdx.x) * 256 + threadIdx.x;
+  if (at >= size_t(quads) * a.batch) return;
+  const int m = int(at / quads), n = int(at % quads) * 4;
+  const float *p = a.sums + size_t(m) * a.rows + n;
+  v4f s = biases<T>(a, n);
+#pragma unroll 8
+  for (int q = 0; q < a.splits; ++q, p += size_t(a.batch) * a.rows) {
+    if (a.rows % 4 == 0) {
+      s += *reinterpret_cast<const v4f *>(p);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[i] += n + i < a.rows ? p[i] : 0.0f;
+    }
+  }
+  store4<T>(a, m, n, s, vector_rows<T>(a));
 }
 
 // ---- host side ----
@@ -305,27 +548,122 @@ int allow_lds(const void *kernel, size_t bytes) {
   return e == hipSuccess ? LMX_OK : fail(LMX_ERR_HIP, "LDS of an f8 kernel: %s", hipGetErrorString(e));
 }
 
-template <class T, int BN, int BM, int WN, int WM, int S>
+size_t tile_count(size_t rows, size_t batch, size_t side) { return (rows + side - 1) / side * ((batch + side - 1) / side); }
+
+// Up to 64 activation rows go to f8_few_kernel, unless tiles of 64 x 64 are just
+// one round of the CUs.
+enum class FewShape { none, rows16, rows32, rows64 };
+FewShape few_shape(size_t rows, size_t batch) {
+  const size_t tiles = tile_count(rows, batch, 64);
+  if (batch > 64 || (batch > 16 && tiles >= 192 && tiles <= 256)) return FewShape::none;
+  if (batch > 16 && rows > 16384) return FewShape::rows64;
+  return batch > 32 && rows > 4096 ? FewShape::rows32 : FewShape::rows16;
+}
+
+// Parts of k for other calls of few tiles: as many as bring the 64 x 64 tiles to
+// one per CU, of 8 steps at least, if they are three.
+int split_count(size_t rows, size_t cols, size_t batch) {
+  if (few_shape(rows, batch) != FewShape::none) return 1;
+  const size_t tiles = tile_count(rows, batch, 64), steps = round_up(cols, kStep) / kStep;
+  const size_t parts = tiles ? std::min<size_t>(256 / tiles, steps / 8) : 1;
+  return parts < 3 ? 1 : int(parts);
+}
+
+// More waves share a row tile's k where the tiles alone leave CUs idle.
+int rows_waves(const F8Args &a) {
+  const int tiles = (a.rows + 15) / 16;
+  return tiles <= 256 ? 16 : tiles <= 768 ? 8 : 4;
+}
+
+template <class T, int W, int R>
+int launch_rows(const F8Args &a, hipStream_t st) {
+  constexpr size_t ring = W * rows_buffers(W) * 16 * kStep, most = ring + 1024 * W + 16 * R + 4 * R * 1024 * W / R / kStep;
+  if (const int r = allow_lds(reinterpret_cast<const void *>(&f8_rows_kernel<T, W, R>), most)) return r;
+  f8_rows_kernel<T, W, R><<<unsigned((a.rows + 15) / 16), W * kWave, ring + size_t(a.batch) * (a.Kp + 16 + 4 * a.steps), st>>>(a);
+  return launch_err("f8 linear");
+}
+template <class T, int R>
+int launch_rows(const F8Args &a, hipStream_t st) {
+  switch (rows_waves(a)) {
+  case 16: return launch_rows<T, 16, R>(a, st);
+  case 8: return launch_rows<T, 8, R>(a, st);
+  default: return launch_rows<T, 4, R>(a, st);
+  }
+}
+
+// Whether every workgroup makes the codes itself: up to 4 rows, as long as that
+// is two rounds of a workgroup's threads, and not too often for nothing.
+int row_slots(const F8Args &a) { return a.batch <= 2 ? a.batch : 4; }
+bool in_one_launch(const F8Args &a) {
+  return a.batch <= 4 && row_slots(a) * a.Kp <= 1024 * rows_waves(a) && (a.batch == 1 || a.rows <= 32768);
+}
+
+template <class T, bool PART, int BN, int BM, int WN, int WM, int S>
 int launch_tile(const F8Args &a, hipStream_t st) {
-  constexpr size_t lds = S * (BN + BM) * kStep;
-  if (const int r = allow_lds(reinterpret_cast<const void *>(&f8_tile_kernel<T, BN, BM, WN, WM, S>), lds)) return r;
+  constexpr size_t lds = S * ((BN + BM) * kStep + BM * 4);
+  const auto kernel = &f8_tile_kernel<T, PART, BN, BM, WN, WM, S>;
+  if (const int r = allow_lds(reinterpret_cast<const void *>(kernel), lds)) return r;
   const size_t tiles = size_t((a.rows + BN - 1) / BN) * size_t((a.batch + BM - 1) / BM);
   if (tiles > (1u << 30)) return fail(LMX_ERR_INVALID_ARGUMENT, "%d x %d outputs", a.rows, a.batch);
-  f8_tile_kernel<T, BN, BM, WN, WM, S><<<unsigned(round_up(tiles, 8)), WN * WM * kWave, lds, st>>>(a);
+  kernel<<<dim3(unsigned(round_up(tiles, 8)), unsigned(a.splits)), WN * WM * kWave, lds, st>>>(a);
   return launch_err("f8 linear");
+}
+
+template <class T, int W, int R, int G>
+int launch_few(const F8Args &a, hipStream_t st) {
+  constexpr size_t lds = W * 3 * ((R + G) * 16 * kStep + 256);
+  if (const int r = allow_lds(reinterpret_cast<const void *>(&f8_few_kernel<T, W, R, G, 3>), lds)) return r;
+  f8_few_kernel<T, W, R, G, 3><<<unsigned((a.rows + 16 * R - 1) / (16 * R)), W * kWave, lds, st>>>(a);
+  return launch_err("f8 linear");
+}
+template <class T>
+int launch_few(const F8Args &a, hipStream_t st) {
+  const int G = (a.batch + 15) / 16;
+  switch (few_shape(a.rows, a.batch)) {
+  case FewShape::rows64: return G == 2 ? launch_few<T, 2, 4, 2>(a, st) : G == 3 ? launch_few<T, 2, 4, 3>(a, st) : launch_few<T, 2, 4, 4>(a, st);
+  case FewShape::rows32: return G == 3 ? launch_few<T, 4, 2, 3>(a, st) : launch_few<T, 4, 2, 4>(a, st);
+  default:
+    return G == 1 ? launch_few<T, 4, 1, 1>(a, st) : G == 2 ? launch_few<T, 4, 1, 2>(a, st) : G == 3 ? launch_few<T, 4, 1, 3>(a, st)
+                                                                                      : launch_few<T, 4, 1, 4>(a, st);
+  }
 }
 
 template <class T>
 int launch_linear(const F8Args &a, hipStream_t st) {
-  f8_codes_kernel<T><<<unsigned(a.batch), 256, 0, st>>>(a);
-  const int r = launch_err("f8 codes");
-  return r ? r : launch_tile<T, 64, 64, 2, 2, 4>(a, st);
+  if (in_one_launch(a)) {
+    switch (row_slots(a)) {
+    case 1: return launch_rows<T, 1>(a, st);
+    case 2: return launch_rows<T, 2>(a, st);
+    default: return launch_rows<T, 4>(a, st);
+    }
+  }
+  // (few long rows: 1024 threads a row)
+  if (a.Kp > 2048 && a.batch < 512) f8_codes_kernel<T, 1024><<<unsigned(a.batch), 1024, 0, st>>>(a);
+  else f8_codes_kernel<T, 256><<<unsigned(a.batch), 256, 0, st>>>(a);
+  int r = launch_err("f8 codes");
+  if (r) return r;
+  if (few_shape(a.rows, a.batch) != FewShape::none) return launch_few<T>(a, st);
+  if (a.splits > 1) {
+    if ((r = launch_tile<T, true, 64, 64, 2, 2, 4>(a, st))) return r;
+    f8_join_kernel<T><<<unsigned((size_t(a.batch) * ((a.rows + 3) / 4) + 255) / 256), 256, 0, st>>>(a);
+    return launch_err("f8 join");
+  }
+  // The largest tiles that still fill most of the CUs, as larger ones read less
+  // from the L2s.
+  const size_t rows = a.rows, batch = a.batch;
+  if (!std::is_same<T, float>::value && tile_count(rows, batch, 256) >= 192) return launch_tile<T, false, 256, 256, 4, 2, 2>(a, st);
+  if (tile_count(rows, batch, 128) >= 160) return launch_tile<T, false, 128, 128, 2, 2, 2>(a, st);
+  return launch_tile<T, false, 64, 64, 2, 2, 4>(a, st);
 }
 
-// Scales, then codes.
-size_t padded(size_t batch) { return round_up(batch, 4); }
+// Scales, codes and, of a call that splits k, its parts' sums.
+size_t padded(size_t batch) { return round_up(batch, 64); }
 size_t codes_at(size_t cols, size_t batch) { return round_up(round_up(cols, kStep) / kStep * padded(batch) * sizeof(float), 256); }
-size_t f8_workspace(size_t cols, size_t batch) { return codes_at(cols, batch) + batch * round_up(cols, kStep); }
+size_t sums_at(size_t cols, size_t batch) { return codes_at(cols, batch) + round_up(batch * round_up(cols, kStep), 256); }
+size_t f8_workspace(size_t rows, size_t cols, size_t batch) {
+  const int splits = split_count(rows, cols, batch);
+  return sums_at(cols, batch) + (splits > 1 ? size_t(splits) * batch * rows * sizeof(float) : 0);
+}
 
 }  // namespace
 }  // namespace lmx
@@ -339,7 +677,7 @@ int lmx_linear_f8_workspace(size_t rows, size_t cols, size_t batch, int type, si
   if (!type_bytes(type)) return fail(LMX_ERR_UNSUPPORTED_FORMAT, "unknown element type %d", type);
   if (rows == 0 || rows > (1u << 24) || cols == 0 || cols > 131072 || batch > (1u << 22))
     return fail(LMX_ERR_INVALID_ARGUMENT, "%zu x %zu, %zu vectors: rows 1..2^24, cols 1..131072, at most 2^22 vectors", rows, cols, batch);
-  *bytes = f8_workspace(cols, batch);
+  *bytes = f8_workspace(rows, cols, batch);
   return LMX_OK;
 }
 
@@ -366,6 +704,8 @@ int lmx_linear_f8(const uint8_t *w, size_t w_stride, const float *w_scale, const
   a.Bp = int(padded(batch));
   a.scales = static_cast<float *>(workspace);
   a.codes = static_cast<uint8_t *>(workspace) + codes_at(cols, batch);
+  a.splits = split_count(rows, cols, batch);
+  a.sums = reinterpret_cast<float *>(static_cast<char *>(workspace) + sums_at(cols, batch));
   hipStream_t st = static_cast<hipStream_t>(stream);
   switch (type) {
   case LMX_F32: return launch_linear<float>(a, st);

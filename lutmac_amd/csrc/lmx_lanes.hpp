@@ -110,12 +110,15 @@ __device__ __forceinline__ unsigned long long wave_max_key(unsigned long long ke
   else return key;
 }
 
-// 16 bytes per lane from a buffer straight to LDS, lane l's at lds + 16 l (the
+// N (4 or 16) bytes per lane from a buffer straight to LDS, lane l's at lds + N l (the
 // host pass, which emits no device code, rejects the builtin).
+template <int N = 16>
 __device__ __forceinline__ void buffer_to_lds(__amdgpu_buffer_rsrc_t buf, char *lds, int at, int base) {
 #ifdef __HIP_DEVICE_COMPILE__
   typedef __attribute__((address_space(3))) void lds_void;
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(buf, (lds_void *)lds, 16, at, base, 0, 0);
+  static_assert(N == 4 || N == 16, "sizes of such a load");
+  if constexpr (N == 16) __builtin_amdgcn_raw_ptr_buffer_load_lds(buf, (lds_void *)lds, 16, at, base, 0, 0);
+  else __builtin_amdgcn_raw_ptr_buffer_load_lds(buf, (lds_void *)lds, 4, at, base, 0, 0);
 #endif
 }
 template <int N>
