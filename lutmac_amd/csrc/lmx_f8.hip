@@ -429,7 +429,6 @@ __global__ __launch_bounds__(WN *WM *kWave) __attribute__((amdgpu_waves_per_eu(2
     for (int m = 0; m < TM; ++m) acc[n][m] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
   const int i = lane & 15, g = lane >> 4;
   const int n_first = row0 + wn * NW;
-  const float *ws = a.w_scale + size_t(min(n_first, a.rows - 1) / kStep) * a.steps;
   int steps = a.steps, s0 = 0;
   if constexpr (PART) {
     const int part = int(blockIdx.y);
@@ -439,35 +438,63 @@ __global__ __launch_bounds__(WN *WM *kWave) __attribute__((amdgpu_waves_per_eu(2
 #pragma unroll
   for (int s = 0; s < S - 1; ++s)
     if (s < steps) fill(s, s0 + s);
-  float wf = scalar_load(ws + s0);
+  // (the weights' scales of a wave's rows, one of BN / 128 runs, wait in LDS)
+  float *wsl = reinterpret_cast<float *>(lds + S * RB) + wn * NW / kStep * a.steps;
+  for (int s = int(threadIdx.x); s < (BN + kStep - 1) / kStep * steps; s += W * kWave) {
+    const int run = s / steps, at = s - run * steps;
+    reinterpret_cast<float *>(lds + S * RB)[run * a.steps + at] =
+        a.w_scale[size_t(min(row0 + run * kStep, a.rows - 1) / kStep) * a.steps + s0 + at];
+  }
   int buf = 0;
   const int pa = piece_place(i, g), pb = piece_place(i, 4 + g);
+  const int tail = a.cols % kStep != 0 && s0 + steps == a.steps ? steps - 1 : -1;   // the step that ends inside a block
   for (int s = 0; s < steps; ++s) {
     if (s + S - 1 <= steps) wait_loads<(S - 2) * LOADS>();
     else wait_loads<0>();
     lds_barrier();   // (a wave is there once its reads of the step before are done)
-    if (s + S - 1 < steps) fill(buf == 0 ? S - 1 : buf - 1, s0 + s + S - 1);
+    if (s == tail) {   // past the last column there may be anything, a NaN too
+      const int left = a.cols - (s0 + s) * kStep;
+      for (int r = int(threadIdx.x); r < BN; r += W * kWave)
+        for (int q = left / 16; q < 8; ++q) {
+          v4i *piece = reinterpret_cast<v4i *>(lds + buf * RB + r * kStep + piece_place(r, q));
+          *piece = cut_piece(*piece, left - 16 * q);
+        }
+      lds_barrier();
+    }
+    // What the first product needs is read first; then, in this order, an activation
+    // operand ahead and matrix instructions with the vector unit's work on those before.
     const char *wl = lds + buf * RB + (wn * NW + i) * kStep, *xl = lds + buf * RB + (BN + wm * MW + i) * kStep;
     const float *sl = reinterpret_cast<const float *>(lds + buf * RB + CB) + wm * MW + i;
+    const auto read = [&](const char *from, int n) __attribute__((always_inline)) {
+      return Operand{*reinterpret_cast<const v4i *>(from + n * 16 * kStep + pa), *reinterpret_cast<const v4i *>(from + n * 16 * kStep + pb)};
+    };
+    Operand w[TN], x = read(xl, 0), ahead{};
+    w[0] = read(wl, 0);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int n = 1; n < TN; ++n) w[n] = read(wl, n);
+    float f[TM];
+    const float wnow = wsl[s];
+#pragma unroll
+    for (int m = 0; m < TM; ++m) f[m] = sl[16 * m];
+    __builtin_amdgcn_sched_barrier(0);
+    v4f p[2][TN];
     Factor<EXACT> wv[TN];
-    const int left = a.cols - (s0 + s) * kStep;
 #pragma unroll
-    for (int n = 0; n < TN; ++n) {
-      Operand w = {*reinterpret_cast<const v4i *>(wl + n * 16 * kStep + pa), *reinterpret_cast<const v4i *>(wl + n * 16 * kStep + pb)};
-      if (left < kStep) w.cut(left, g);
-      wv[n] = Factor<EXACT>(w);
-    }
-    const float wnow = wf;
-    wf = scalar_load(ws + min(s0 + s + 1, a.steps - 1));
+    for (int m = 0; m <= TM; ++m) {
+      if (m + 1 < TM) ahead = read(xl, m + 1);
+      Factor<EXACT> xv{};
+      if (m < TM) xv = Factor<EXACT>(x);
+      const float fm = m > 0 ? f[m - 1] * wnow : 0.0f;
 #pragma unroll
-    for (int m = 0; m < TM; ++m) {
-      const Factor<EXACT> xv(Operand{*reinterpret_cast<const v4i *>(xl + m * 16 * kStep + pa), *reinterpret_cast<const v4i *>(xl + m * 16 * kStep + pb)});
-      const float f = sl[16 * m] * wnow;
-      v4f p[TN];
-#pragma unroll
-      for (int n = 0; n < TN; ++n) p[n] = products(wv[n], xv);
-#pragma unroll
-      for (int n = 0; n < TN; ++n) add_scaled(acc[n][m], p[n], f);
+      for (int n = 0; n < TN; ++n) {
+        if (m == 0) wv[n] = Factor<EXACT>(w[n]);
+        if (m < TM) p[m % 2][n] = products(wv[n], xv);
+        if (m > 0) add_scaled(acc[n][m - 1], p[(m + 1) % 2][n], fm);
+        if (EXACT ? n == TN - 1 : true) __builtin_amdgcn_sched_barrier(0);
+      }
+      x = ahead;
+      if (m == 0 && s + S - 1 < steps) fill(buf == 0 ? S - 1 : buf - 1, s0 + s + S - 1);
     }
     buf = buf == S - 1 ? 0 : buf + 1;
   }
@@ -600,7 +627,7 @@ bool in_one_launch(const F8Args &a) {
 
 template <class T, bool PART, int BN, int BM, int WN, int WM, int S>
 int launch_tile(const F8Args &a, hipStream_t st) {
-  constexpr size_t lds = S * ((BN + BM) * kStep + BM * 4);
+  const size_t lds = S * ((BN + BM) * kStep + BM * 4) + (BN + kStep - 1) / kStep * a.steps * 4;   // (at most 8 KB of scales)
   const auto kernel = &f8_tile_kernel<T, PART, BN, BM, WN, WM, S>;
   if (const int r = allow_lds(reinterpret_cast<const void *>(kernel), lds)) return r;
   const size_t tiles = size_t((a.rows + BN - 1) / BN) * size_t((a.batch + BM - 1) / BM);
@@ -651,7 +678,8 @@ int launch_linear(const F8Args &a, hipStream_t st) {
   // The largest tiles that still fill most of the CUs, as larger ones read less
   // from the L2s.
   const size_t rows = a.rows, batch = a.batch;
-  if (!std::is_same<T, float>::value && tile_count(rows, batch, 256) >= 192) return launch_tile<T, false, 256, 256, 4, 2, 2>(a, st);
+  if constexpr (!std::is_same<T, float>::value)
+    if (tile_count(rows, batch, 256) >= 192) return launch_tile<T, false, 256, 256, 4, 2, 2>(a, st);
   if (tile_count(rows, batch, 128) >= 160) return launch_tile<T, false, 128, 128, 2, 2, 2>(a, st);
   return launch_tile<T, false, 64, 64, 2, 2, 4>(a, st);
 }
