@@ -578,17 +578,20 @@ int allow_lds(const void *kernel, size_t bytes) {
 size_t tile_count(size_t rows, size_t batch, size_t side) { return (rows + side - 1) / side * ((batch + side - 1) / side); }
 
 // Up to 64 activation rows go to f8_few_kernel, unless tiles of 64 x 64 are just
-// one round of the CUs.
-enum class FewShape { none, rows16, rows32, rows64 };
+// one round of the CUs; 32 weight rows a workgroup read the codes less often (us in a
+// graph, bf16, tiles / 16 weight rows / 32: 16 x 2048 -> 2048 10.7 / 5.6 / -, 48 x 8960 ->
+// 1536 31 / 15.9 / 18.8, 48 x 2048 -> 8192 12.3 / 11.5 / 9.5, 48 x 8192 -> 24576 62 / 74 /
+// 60, 48 x 2048 -> 16384, one round, 14.3 / 19.5 / 14.9).
+enum class FewShape { none, rows16, rows32 };
 FewShape few_shape(size_t rows, size_t batch) {
   const size_t tiles = tile_count(rows, batch, 64);
   if (batch > 64 || (batch > 16 && tiles >= 192 && tiles <= 256)) return FewShape::none;
-  if (batch > 16 && rows > 16384) return FewShape::rows64;
-  return batch > 32 && rows > 4096 ? FewShape::rows32 : FewShape::rows16;
+  return batch > 16 && rows > 4096 ? FewShape::rows32 : FewShape::rows16;
 }
 
 // Parts of k for other calls of few tiles: as many as bring the 64 x 64 tiles to
-// one per CU, of 8 steps at least, if they are three.
+// one per CU, of 8 steps at least, if they are three (us, in one part / in parts:
+// 100 x 8960 -> 1536 in 5 31.6 / 17.8, 200 x 8192 -> 1024 in 4 29.8 / 18.7).
 int split_count(size_t rows, size_t cols, size_t batch) {
   if (few_shape(rows, batch) != FewShape::none) return 1;
   const size_t tiles = tile_count(rows, batch, 64), steps = round_up(cols, kStep) / kStep;
@@ -596,7 +599,9 @@ int split_count(size_t rows, size_t cols, size_t batch) {
   return parts < 3 ? 1 : int(parts);
 }
 
-// More waves share a row tile's k where the tiles alone leave CUs idle.
+// More waves share a row tile's k where the tiles alone leave CUs idle (us, 4 / 8 /
+// 16 waves: 1 x 8192 -> 2048 10.8 / 7.0 / 6.9, 1 x 2048 -> 8192 6.0 / 5.7 / 7.1, 1 x 2048 ->
+// 16384 8.9 / 10.0 / 12.6).
 int rows_waves(const F8Args &a) {
   const int tiles = (a.rows + 15) / 16;
   return tiles <= 256 ? 16 : tiles <= 768 ? 8 : 4;
@@ -619,7 +624,9 @@ int launch_rows(const F8Args &a, hipStream_t st) {
 }
 
 // Whether every workgroup makes the codes itself: up to 4 rows, as long as that
-// is two rounds of a workgroup's threads, and not too often for nothing.
+// is two rounds of a workgroup's threads, and not too often for nothing (us,
+// itself / codes in a launch before: 1 x 2048 -> 16384 8.9 / 11.4, 2 x 2048 -> 16384 10.5 /
+// 11.3, 4 x 2048 -> 2048 3.9 / 5.6, 2 x 2048 -> 65536 32.9 / 30.9).
 int row_slots(const F8Args &a) { return a.batch <= 2 ? a.batch : 4; }
 bool in_one_launch(const F8Args &a) {
   return a.batch <= 4 && row_slots(a) * a.Kp <= 1024 * rows_waves(a) && (a.batch == 1 || a.rows <= 32768);
@@ -646,13 +653,10 @@ int launch_few(const F8Args &a, hipStream_t st) {
 template <class T>
 int launch_few(const F8Args &a, hipStream_t st) {
   const int G = (a.batch + 15) / 16;
-  switch (few_shape(a.rows, a.batch)) {
-  case FewShape::rows64: return G == 2 ? launch_few<T, 2, 4, 2>(a, st) : G == 3 ? launch_few<T, 2, 4, 3>(a, st) : launch_few<T, 2, 4, 4>(a, st);
-  case FewShape::rows32: return G == 3 ? launch_few<T, 4, 2, 3>(a, st) : launch_few<T, 4, 2, 4>(a, st);
-  default:
-    return G == 1 ? launch_few<T, 4, 1, 1>(a, st) : G == 2 ? launch_few<T, 4, 1, 2>(a, st) : G == 3 ? launch_few<T, 4, 1, 3>(a, st)
-                                                                                      : launch_few<T, 4, 1, 4>(a, st);
-  }
+  if (few_shape(a.rows, a.batch) == FewShape::rows32)
+    return G == 2 ? launch_few<T, 4, 2, 2>(a, st) : G == 3 ? launch_few<T, 4, 2, 3>(a, st) : launch_few<T, 4, 2, 4>(a, st);
+  return G == 1 ? launch_few<T, 4, 1, 1>(a, st) : G == 2 ? launch_few<T, 4, 1, 2>(a, st) : G == 3 ? launch_few<T, 4, 1, 3>(a, st)
+                                                                                            : launch_few<T, 4, 1, 4>(a, st);
 }
 
 template <class T>
@@ -676,7 +680,9 @@ int launch_linear(const F8Args &a, hipStream_t st) {
     return launch_err("f8 join");
   }
   // The largest tiles that still fill most of the CUs, as larger ones read less
-  // from the L2s.
+  // from the L2s (us, bf16, 256 / 128 / 64: 2048 x 2048 -> 8192 41 / 51 / 82, 1024 x 2048 ->
+  // 8192 37 / 29 / 48, 256 x 2048 -> 16384 37 / 25 / 28, 517 x 1400 -> 3001 28 / 17.5 / 12.9;
+  // fp32, 128 / 64: 2048 x 2048 -> 8192 76 / 109; its operands as fp16 leave no registers for 256).
   const size_t rows = a.rows, batch = a.batch;
   if constexpr (!std::is_same<T, float>::value)
     if (tile_count(rows, batch, 256) >= 192) return launch_tile<T, false, 256, 256, 4, 2, 2>(a, st);

@@ -59,20 +59,42 @@ __device__ __forceinline__ void block_sums(uint32_t (&v)[N], uint32_t (&base)[N]
 __device__ __forceinline__ uint32_t pages_of(uint32_t tokens) { return (tokens + kPage - 1) / kPage; }
 
 // n pages between a table row (from its entry `first` on) and the stack (from its
-// place `top` down): f(table entry, stack place) for each, by the thread itself
-// or, of many, by its wave.
-template <class F>
-__device__ __forceinline__ void each_page(uint32_t n, size_t first, uint32_t top, F f) {
-  if (n <= kWave)
-    for (uint32_t j = 0; j < n; ++j) f(first + j, top - j);
-  uint64_t many = __builtin_amdgcn_ballot_w64(n > kWave);
+// place `top` down), taken from it or (PUSH) given back.  One or two by the thread
+// itself; of more, a wave's lanes take those of kAtOnce sequences at a time, their
+// loads on the way together (1000 sequences of 31 pages in one workgroup: 41 us
+// thread by thread, 24 so, bound by what a CU issues: some 50 operations a sequence).
+constexpr int kAtOnce = 8;
+template <bool PUSH>
+__device__ __forceinline__ void move_pages(const PagesArgs &a, uint32_t n, size_t first, uint32_t top) {
+  const auto take = [&](size_t entry, uint32_t place) __attribute__((always_inline)) { return PUSH ? a.pages[entry] : a.free_pages[place]; };
+  const auto give = [&](size_t entry, uint32_t place, int page) __attribute__((always_inline)) {
+    a.pages[entry] = PUSH ? -1 : page;
+    if (PUSH && place < uint32_t(a.n_pages)) a.free_pages[place] = page;   // (pages freed twice may be more than there are)
+  };
+  if (n <= 2)
+    for (uint32_t j = 0; j < n; ++j) give(first + j, top - j, take(first + j, top - j));
+  const uint32_t lane = threadIdx.x & (kWave - 1);
+  uint64_t many = __builtin_amdgcn_ballot_w64(n > 2);
   while (many) {
-    const int from = __builtin_ctzll(many);
-    many &= many - 1;
-    const auto pick = [from](uint32_t v) { return uint32_t(__builtin_amdgcn_readlane(int(v), from)); };
-    const uint32_t all = pick(n), t = pick(top);
-    const size_t e = size_t(pick(uint32_t(first >> 32))) << 32 | pick(uint32_t(first));
-    for (uint32_t j = threadIdx.x & (kWave - 1); j < all; j += kWave) f(e + j, t - j);
+    uint32_t all[kAtOnce], tops[kAtOnce], most = 0;
+    size_t firsts[kAtOnce];
+#pragma unroll
+    for (int q = 0; q < kAtOnce; ++q) {
+      const int from = many ? __builtin_ctzll(many) : 0;
+      const auto pick = [from](uint32_t v) __attribute__((always_inline)) { return uint32_t(__builtin_amdgcn_readlane(int(v), from)); };
+      all[q] = many ? pick(n) : 0, tops[q] = pick(top);
+      firsts[q] = size_t(pick(uint32_t(first >> 32))) << 32 | pick(uint32_t(first));
+      most = max(most, all[q]);
+      many &= many - 1;
+    }
+    for (uint32_t j = lane; j < most; j += kWave) {
+      int page[kAtOnce];   // (those of no use: the first entry or place, as some page moves there is one)
+#pragma unroll
+      for (int q = 0; q < kAtOnce; ++q) page[q] = take(j < all[q] ? firsts[q] + j : 0, j < all[q] ? tops[q] - j : 0);
+#pragma unroll
+      for (int q = 0; q < kAtOnce; ++q)
+        if (j < all[q]) give(firsts[q] + j, tops[q] - j, page[q]);
+    }
   }
 }
 
@@ -99,7 +121,7 @@ __device__ __forceinline__ int last_at_most(const int *v, int n, int r) {
 
 // One workgroup over all sequences, a thread each, kThreads of them at a time:
 // the sums of new tokens, pages and granted tokens are all that couples them.
-// ROWS: places the rows as well.
+// ROWS: moves the pages and places the rows as well.
 template <bool ROWS>
 __global__ __launch_bounds__(kThreads) void extend_kernel(PagesArgs a) {
   __shared__ uint32_t waves[2][kWaves], used;
@@ -128,9 +150,8 @@ __global__ __launch_bounds__(kThreads) void extend_kernel(PagesArgs a) {
     // (a sequence that gets pages is behind none that needed some and got none)
     const uint32_t take = yes ? need : 0;
     if (take) atomicMax(&used, v[1]);
-    each_page(take, size_t(s) * a.max_pages + first, have - 1 - (v[1] - need),
-              [&](size_t entry, uint32_t place) { a.pages[entry] = a.free_pages[place]; });
     if constexpr (ROWS) {
+      move_pages<false>(a, take, size_t(s) * a.max_pages + first, have - 1 - (v[1] - need));
       begin[threadIdx.x] = int(g[0]) - (yes ? int(add) : 0);
       start[threadIdx.x] = int(old);
       __syncthreads();
@@ -146,12 +167,104 @@ __global__ __launch_bounds__(kThreads) void extend_kernel(PagesArgs a) {
   if (threadIdx.x == 0) *a.n_free = int(have - used);
 }
 
-// The rows of the call, where they are many.
+// The new pages of a call of many rows, once it is known who gets them: up to
+// kMovers workgroups, which sum anew what precedes their sequences.  (A workgroup of its
+// own for each few sequences, since one CU issues too little for them all.)
+constexpr int kMovers = 64;
+__global__ __launch_bounds__(256) void new_pages_kernel(PagesArgs a) {
+  __shared__ uint32_t sums[2][4];
+  const int lane = threadIdx.x & (kWave - 1), wave = int(threadIdx.x) / kWave;
+  const int share = ((a.n_seqs + int(gridDim.x) - 1) / int(gridDim.x) + kWave - 1) / kWave * kWave;
+  const int begin = min(int(blockIdx.x) * share, a.n_seqs), end = min(begin + share, a.n_seqs);
+  if (begin == end) return;
+  struct Taken { uint32_t first, need; };
+  const auto taken = [&](int s) __attribute__((always_inline)) {
+    const uint32_t got = uint32_t(a.granted[s]), now = uint32_t(max(a.lengths[s], 0)), first = pages_of(now - got);
+    return Taken{first, got ? pages_of(now) - first : 0};
+  };
+  uint32_t before = 0, all = 0;
+  for (int s = int(threadIdx.x); s < a.n_seqs; s += 256) {
+    const uint32_t need = taken(s).need;
+    all += need;
+    if (s < begin) before += need;
+  }
+#pragma unroll
+  for (int d = kWave / 2; d; d /= 2) all += __shfl_xor(all, d), before += __shfl_xor(before, d);
+  if (lane == 0) sums[0][wave] = before, sums[1][wave] = all;
+  __syncthreads();
+  before = sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3];
+  uint32_t top = uint32_t(*a.n_free) + sums[1][0] + sums[1][1] + sums[1][2] + sums[1][3] - 1 - before;   // of the next sequence
+  // every wave goes over the workgroup's sequences, and moves the pages of a quarter of each 64
+  for (int s0 = begin; s0 < end; s0 += kWave) {
+    const int s = s0 + lane;
+    const Taken t = s < end ? taken(s) : Taken{0, 0};
+    uint32_t upto = t.need;
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+      const uint32_t o = __shfl_up(upto, d);
+      if (lane >= d) upto += o;
+    }
+    move_pages<false>(a, lane / 16 == wave ? t.need : 0, size_t(s) * a.max_pages + t.first, top - (upto - t.need));
+    top -= __shfl(upto, kWave - 1);
+  }
+}
+
+// The last sequence whose first row is at most r (the first row is 0), by a wave.
+__device__ __forceinline__ int wave_search(const int *offsets, int n, int r) {
+  const int lane = threadIdx.x & (kWave - 1);
+  int lo = 0;
+  while (n > 1) {
+    const int step = (n + kWave - 1) / kWave, i = lane * step;
+    const int c = __builtin_popcountll(__builtin_amdgcn_ballot_w64(i < n && offsets[lo + min(i, n - 1)] <= r));
+    lo += (c - 1) * step;
+    n = min(step, n - (c - 1) * step);
+  }
+  return lo;
+}
+
+// The rows of the call, where they are many, kEach neighbours a thread: 12 bytes
+// written a row.
+constexpr int kEach = 4;
 __global__ __launch_bounds__(256) void rows_kernel(PagesArgs a) {
-  const int r = int(blockIdx.x * 256 + threadIdx.x);
-  if (r >= a.offsets[a.n_seqs]) return;
-  const int s = last_at_most(a.offsets, a.n_seqs, r);
-  place_row(a, r, s, a.lengths[s] - a.offsets[s + 1] + r);
+  const int rows = a.offsets[a.n_seqs], first = int(blockIdx.x * 256 + (threadIdx.x & ~(kWave - 1))) * kEach;
+  if (first >= rows) return;   // (the wave's)
+  const int lo = wave_search(a.offsets, a.n_seqs, first), hi = wave_search(a.offsets, a.n_seqs, min(first + kWave * kEach, rows) - 1);
+  const int r0 = first + int(threadIdx.x & (kWave - 1)) * kEach;
+  if (r0 >= rows) return;
+  int s = lo + last_at_most(a.offsets + lo, hi - lo + 1, r0), end = a.offsets[s + 1], pos = a.lengths[s] - end + r0, page = 0, known = -1;
+  int at[kEach];
+  long long slot[kEach];
+  const int n = min(kEach, rows - r0);
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    if (j >= n) break;
+    if (r0 + j >= end) {   // the next sequence that has rows
+      do end = a.offsets[++s + 1];
+      while (r0 + j >= end);
+      pos = a.lengths[s] - end + r0 + j;
+      known = -1;
+    }
+    if (a.slots && pos / kPage != known) known = pos / kPage, page = a.pages[size_t(s) * a.max_pages + known];
+    at[j] = pos;
+    slot[j] = page < 0 ? -1 : (long long)page * kPage + pos % kPage;
+    ++pos;
+  }
+  if (n == kEach && reinterpret_cast<size_t>(a.positions) % 16 == 0) {
+    *reinterpret_cast<int4 *>(a.positions + r0) = make_int4(at[0], at[1], at[2], at[3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+      if (j < n) a.positions[r0 + j] = at[j];
+  }
+  if (!a.slots) return;
+  if (n == kEach && reinterpret_cast<size_t>(a.slots) % 16 == 0) {
+    *reinterpret_cast<longlong2 *>(a.slots + r0) = make_longlong2(slot[0], slot[1]);
+    *reinterpret_cast<longlong2 *>(a.slots + r0 + 2) = make_longlong2(slot[2], slot[3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+      if (j < n) a.slots[r0 + j] = slot[j];
+  }
 }
 
 __global__ __launch_bounds__(kThreads) void trim_kernel(PagesArgs a) {
@@ -168,21 +281,18 @@ __global__ __launch_bounds__(kThreads) void trim_kernel(PagesArgs a) {
     c.gone = uint32_t(min(size_t(pages_of(old)), a.max_pages)) - c.kept;
     return c;
   };
-  uint32_t all[1] = {0};   // pages of the whole call
-  for (int s0 = 0; s0 < a.n_seqs; s0 += kThreads) {
+  uint32_t all[1] = {0}, before[1] = {0};   // pages of the whole call, and up to here
+  for (int s0 = 0; a.n_seqs > kThreads && s0 < a.n_seqs; s0 += kThreads) {
     uint32_t v[1] = {cut(s0 + int(threadIdx.x)).gone};
     block_sums<1>(v, all, waves);
   }
-  uint32_t before[1] = {0};
   for (int s0 = 0; s0 < a.n_seqs; s0 += kThreads) {
     const int s = s0 + int(threadIdx.x);
     const Cut c = cut(s);
     uint32_t v[1] = {c.gone};
     block_sums<1>(v, before, waves);
-    each_page(c.gone, size_t(s) * a.max_pages + c.kept, have + all[0] - 1 - (v[0] - c.gone), [&](size_t entry, uint32_t place) {
-      if (place < uint32_t(a.n_pages)) a.free_pages[place] = a.pages[entry];   // (pages freed twice may be more than there are)
-      a.pages[entry] = -1;
-    });
+    if (a.n_seqs <= kThreads) all[0] = before[0];
+    move_pages<true>(a, c.gone, size_t(s) * a.max_pages + c.kept, have + all[0] - 1 - (v[0] - c.gone));
     if (c.live) a.lengths[s] = int(c.keep);
   }
   if (threadIdx.x == 0) *a.n_free = int(min(add_sat(have, all[0]), uint32_t(a.n_pages)));
@@ -244,7 +354,10 @@ int lmx_kv8_extend(const lmx_kv8_pages *pages, const int32_t *new_tokens, size_t
   }
   extend_kernel<false><<<1, kThreads, 0, st>>>(a);
   if ((r = launch_err("kv8 extend"))) return r;
-  rows_kernel<<<unsigned((n_rows + 255) / 256), 256, 0, st>>>(a);
+  if (pages->n_seqs == 0) return LMX_OK;
+  new_pages_kernel<<<unsigned(std::min<size_t>((pages->n_seqs + kWave - 1) / kWave, kMovers)), 256, 0, st>>>(a);
+  if ((r = launch_err("kv8 extend pages"))) return r;
+  rows_kernel<<<unsigned((n_rows + 256 * kEach - 1) / (256 * kEach)), 256, 0, st>>>(a);
   return launch_err("kv8 extend rows");
 }
 
