@@ -95,7 +95,7 @@ class Both:
 
 
 @pytest.mark.parametrize("n,most,rows", [(1, 1, 8), (1, 700, 4096), (3, 200, 600), (64, 5, 320), (1000, 3, 2500), (1024, 2, 3000), (1025, 70, 30000),
-                                         (2500, 9, 20000), (40, 9000, 200000), (5000, 1, 5000)])
+                                         (2500, 9, 20000), (40, 9000, 200000), (5000, 1, 5000), (9000, 9, 30000)])
 def test_steps(cuda, n, most, rows):
     """Some steps of growing and shrinking; tight rows and pages leave some out."""
     rng = random.Random(n + most)
