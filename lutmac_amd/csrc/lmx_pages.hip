@@ -60,10 +60,10 @@ __device__ __forceinline__ uint32_t pages_of(uint32_t tokens) { return (tokens +
 
 // n pages between a table row (from its entry `first` on) and the stack (from its
 // place `top` down), taken from it or (PUSH) given back.  One or two by the thread
-// itself; of more, a wave's lanes take those of kAtOnce sequences at a time, their
-// loads on the way together (1000 sequences of 31 pages in one workgroup: 41 us
-// thread by thread, 24 so, bound by what a CU issues: some 50 operations a sequence).
-constexpr int kAtOnce = 8;
+// itself, of up to kLong by 16 lanes, kAtOnce times 4 sequences at a time with their
+// loads on the way together, of more by the wave (1000 sequences of 31 pages in one
+// workgroup: 41 us thread by thread, 17 a wave for each, 11 so).
+constexpr int kAtOnce = 4, kLong = 128;
 template <bool PUSH>
 __device__ __forceinline__ void move_pages(const PagesArgs &a, uint32_t n, size_t first, uint32_t top) {
   const auto take = [&](size_t entry, uint32_t place) __attribute__((always_inline)) { return PUSH ? a.pages[entry] : a.free_pages[place]; };
@@ -73,27 +73,53 @@ __device__ __forceinline__ void move_pages(const PagesArgs &a, uint32_t n, size_
   };
   if (n <= 2)
     for (uint32_t j = 0; j < n; ++j) give(first + j, top - j, take(first + j, top - j));
-  const uint32_t lane = threadIdx.x & (kWave - 1);
-  uint64_t many = __builtin_amdgcn_ballot_w64(n > 2);
-  while (many) {
-    uint32_t all[kAtOnce], tops[kAtOnce], most = 0;
-    size_t firsts[kAtOnce];
+  const int lane = threadIdx.x & (kWave - 1);
+  for (uint64_t huge = __builtin_amdgcn_ballot_w64(n > kLong); huge; huge &= huge - 1) {
+    const int src = __builtin_ctzll(huge);
+    const uint32_t count = __shfl(n, src), from = __shfl(top, src);
+    const size_t entry = size_t(__shfl(uint32_t(first >> 32), src)) << 32 | __shfl(uint32_t(first), src);
+    for (uint32_t j = uint32_t(lane); j < count; j += 4 * kWave) {
+      int page[4];
 #pragma unroll
-    for (int q = 0; q < kAtOnce; ++q) {
-      const int from = many ? __builtin_ctzll(many) : 0;
-      const auto pick = [from](uint32_t v) __attribute__((always_inline)) { return uint32_t(__builtin_amdgcn_readlane(int(v), from)); };
-      all[q] = many ? pick(n) : 0, tops[q] = pick(top);
-      firsts[q] = size_t(pick(uint32_t(first >> 32))) << 32 | pick(uint32_t(first));
-      most = max(most, all[q]);
-      many &= many - 1;
+      for (int b = 0; b < 4; ++b) page[b] = take(entry + min(j + b * kWave, count - 1), from - min(j + b * kWave, count - 1));
+#pragma unroll
+      for (int b = 0; b < 4; ++b) asm volatile("" ::"v"(page[b]));
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        if (j + b * kWave < count) give(entry + j + b * kWave, from - (j + b * kWave), page[b]);
     }
-    for (uint32_t j = lane; j < most; j += kWave) {
-      int page[kAtOnce];   // (those of no use: the first entry or place, as some page moves there is one)
+  }
+  const uint32_t big = n > 2 && n <= kLong ? n : 0;
+  const uint64_t many = __builtin_amdgcn_ballot_w64(big != 0);
+  for (int q0 = 0; q0 < kWave; q0 += 4 * kAtOnce) {
+    if (!(many >> q0 & ((uint64_t(1) << (4 * kAtOnce)) - 1))) continue;
+    uint32_t count[kAtOnce], from[kAtOnce];
+    size_t entry[kAtOnce];
 #pragma unroll
-      for (int q = 0; q < kAtOnce; ++q) page[q] = take(j < all[q] ? firsts[q] + j : 0, j < all[q] ? tops[q] - j : 0);
+    for (int b = 0; b < kAtOnce; ++b) {
+      const int src = q0 + 4 * b + lane / 16;
+      count[b] = __shfl(big, src), from[b] = __shfl(top, src);
+      entry[b] = size_t(__shfl(uint32_t(first >> 32), src)) << 32 | __shfl(uint32_t(first), src);
+    }
+    for (uint32_t j = uint32_t(lane) % 16;; j += 32) {
+      bool more = false;
+      int page[2 * kAtOnce];   // (those of no use: the first entry or place, as some page moves there is one)
 #pragma unroll
-      for (int q = 0; q < kAtOnce; ++q)
-        if (j < all[q]) give(firsts[q] + j, tops[q] - j, page[q]);
+      for (int b = 0; b < 2 * kAtOnce; ++b) {
+        const uint32_t i = j + 16 * (b % 2);
+        const bool yes = i < count[b / 2];
+        page[b] = take(yes ? entry[b / 2] + i : 0, yes ? from[b / 2] - i : 0);
+        more |= i + 32 < count[b / 2];
+      }
+      // (all here before the first store: else each store's branch would wait for the store before)
+#pragma unroll
+      for (int b = 0; b < 2 * kAtOnce; ++b) asm volatile("" ::"v"(page[b]));
+#pragma unroll
+      for (int b = 0; b < 2 * kAtOnce; ++b) {
+        const uint32_t i = j + 16 * (b % 2);
+        if (i < count[b / 2]) give(entry[b / 2] + i, from[b / 2] - i, page[b]);
+      }
+      if (!__builtin_amdgcn_ballot_w64(more)) break;
     }
   }
 }
