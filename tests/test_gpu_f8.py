@@ -97,7 +97,8 @@ def test_linear_f8_large(cuda, dtype, rows, cols, batch):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-@pytest.mark.parametrize("rows,cols,batch", [(70, 131072, 2), (64, 20000, 70), (16, 131071, 1), (130, 60001, 20)])
+@pytest.mark.parametrize("rows,cols,batch", [(70, 131072, 2), (64, 20000, 70), (16, 131071, 1), (130, 60001, 20),
+                                             (1000, 8300, 33), (17, 30001, 64), (300, 5000, 9)])
 def test_linear_f8_long(cuda, dtype, rows, cols, batch):
     a = make(rows, cols, batch, dtype, 8)
     check(*a, L.linear_f8(a[0], a[1], a[2], bias=a[3]))
