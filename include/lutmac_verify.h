@@ -27,7 +27,7 @@ extern "C" {
 /* Rows offsets[s] .. offsets[s + 1] - 1 of a call are sequence s's: row by row the
  * target's logits, drafts[r] the token drafted at row r (the last row of a sequence has none: its entry
  * is not looked at), so a sequence with n drafted tokens has n + 1 rows.
- * Offsets do not decrease; rows of no sequence are neither read nor written. */
+ * Offsets do not decrease; rows of no sequence reach nothing and their tokens stay. */
 typedef struct {
   const int32_t *offsets;   /* [n_seqs + 1] */
   const int32_t *drafts;    /* [n_rows] */
@@ -57,6 +57,7 @@ int lmx_verify_drafts_workspace(const lmx_drafts *d, int type, size_t *bytes);
  * number is within some 2^-40 of a border.
  * logits: elements of `type`, row r at logits + r * stride (elements; at least
  * vocab), aligned to an element; probs fp32, row r at probs + r * probs_stride.
+ * accepted and tokens overlap no input.
  * workspace: lmx_verify_drafts_workspace bytes, 16-byte aligned, in any state;
  * calls that may overlap in time need workspaces of their own. */
 int lmx_verify_drafts(const lmx_drafts *d, int type, const void *logits, size_t stride,

@@ -582,6 +582,7 @@ int lmx_verify_drafts(const lmx_drafts *d, int type, const void *logits, size_t 
        reinterpret_cast<size_t>(probs) | reinterpret_cast<size_t>(accepted) | reinterpret_cast<size_t>(tokens)) % 4 ||
       reinterpret_cast<size_t>(d->uniforms) % 8 || reinterpret_cast<size_t>(logits) % e)
     return fail(LMX_ERR_INVALID_ARGUMENT, "pointers must be aligned to their elements, uniforms to their pairs");
+  if (d->n_rows && tokens == d->drafts) return fail(LMX_ERR_INVALID_ARGUMENT, "tokens and drafts are the same memory");
   if (d->n_rows > 1 && (stride < d->vocab || stride >> 40 || (probs && (probs_stride < d->vocab || probs_stride >> 40))))
     return fail(LMX_ERR_INVALID_ARGUMENT, "row strides %zu and %zu of rows of %zu", stride, probs_stride, d->vocab);
   if (need && (!workspace || workspace_bytes < need || reinterpret_cast<size_t>(workspace) % 16))

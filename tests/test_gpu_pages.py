@@ -163,6 +163,19 @@ def test_nothing_to_give(cuda, n, max_pages, pages, rows):
     b.trim([1] * n)
 
 
+def test_arguments_that_are_one(cuda):
+    """Sequences that end drop their own lengths; counts asked and granted in one tensor."""
+    for n in (5, 3000):
+        b = Both(n, 4, 2 * n, 2 * n)
+        new = torch.full((n,), 3, dtype=torch.int32, device="cuda")
+        positions = torch.zeros(2 * n, dtype=torch.int32, device="cuda")
+        _, granted, _, _ = b.held.extend(new, positions, granted=new)
+        assert granted is new and new.tolist() == [3 if 3 * (s + 1) <= 2 * n else 0 for s in range(n)]
+        b.held.trim(b.held.lengths)
+        assert not b.held.lengths.any() and int(b.held.n_free) == 2 * n and (b.held.pages == -1).all()
+        assert torch.equal(b.held.free.sort()[0].cpu(), torch.arange(2 * n, dtype=torch.int32))
+
+
 def test_one_long_sequence(cuda):
     """A prompt of many pages beside single tokens; slots past 2^31."""
     b = Both(3, 6000, 7000, 300000)

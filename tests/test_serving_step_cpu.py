@@ -94,7 +94,7 @@ def drafts(**kw):
     return L.DraftsC(*[d[n] for n, _ in L.DraftsC._fields_])
 
 
-def verify(d=None, kind=L.F32, x=A, xs=1000, q=A, qs=1000, accepted=A, tokens=A, work=A, size=1 << 30):
+def verify(d=None, kind=L.F32, x=A, xs=1000, q=A, qs=1000, accepted=A, tokens=2 * A, work=A, size=1 << 30):
     d = d or drafts()
     return L.lib().lmx_verify_drafts(ctypes.addressof(d), kind, x, xs, q, qs, accepted, tokens, work, size, None)
 
@@ -107,7 +107,7 @@ def test_bad_drafts(bad):
 
 
 @pytest.mark.parametrize("bad", [dict(x=None), dict(x=A + 2), dict(xs=999), dict(xs=1 << 41), dict(q=A + 2), dict(qs=999), dict(accepted=None),
-                                 dict(accepted=A + 2), dict(tokens=None), dict(tokens=A + 1), dict(work=None), dict(work=A + 8),
+                                 dict(accepted=A + 2), dict(tokens=None), dict(tokens=A + 1), dict(tokens=A), dict(work=None), dict(work=A + 8),
                                  dict(size=16)], ids=str)
 def test_bad_verify(bad):
     assert verify(**bad) == L.ERR_INVALID_ARGUMENT
