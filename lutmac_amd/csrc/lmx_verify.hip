@@ -358,7 +358,7 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(VerifyArgs a) {
   static_assert(kPart <= kThreads, "a piece a thread");
   __shared__ Row rows[kWaves];
   __shared__ int stops[kWaves];
-  constexpr int kNear = 2 * kWaves;
+  constexpr int kNear = kWaves;
   __shared__ double scan[kWaves], near[kNear];   // (sums of one workgroup's few parts stay here)
   __shared__ Place place;
   __shared__ int at, last, joins, without;
@@ -538,9 +538,9 @@ int launch(const VerifyArgs &a, hipStream_t st) {
 }
 
 // Workgroups of a sequence for p - q: a part a wave, as long as that is four
-// workgroups a CU at most (one where it has two parts a wave).
+// workgroups a CU at most (9 sequences of 16 parts: one workgroup each 16.5 us, two 14.4).
 int groups_of(const VerifyArgs &a) {
-  if (!a.probs || a.n_parts <= 2 * kWaves) return 1;
+  if (!a.probs || a.n_parts <= kWaves) return 1;
   return std::max(1, std::min((a.n_parts + kWaves - 1) / kWaves, 1024 / a.n_seqs));
 }
 
