@@ -210,10 +210,7 @@ int lmx_weight_codes_i8(const lmx_weight *w, int8_t *codes, size_t w_stride,
  * with amax <= 448 s (at least 2^-126), so that x / s is exact; c = x / s rounded
  * to e4m3 (ties to even), and
  *   y[b][r] = sum_j s[b][j] w_scale[r / 128][j] (sum of c w over k of block j) + bias[r],
- * rounded once to y's type.  Sums are fp32, for fp32 x with every product exact;
- * for the 16-bit types the products of the 128 k that one matrix instruction
- * takes lose what lies below 2^-13 of their largest (about 2^-16 of y; half a
- * step of fp16 is 2^-11).
+ * rounded once to y's type.  Every product of codes is exact, sums are fp32.
  * w: codes, row r at w + r * w_stride (w and w_stride multiples of 16, the
  * stride at most 262144; cols any number up to 131072; the bytes between cols and
  * w_stride are not used); w_scale contiguous, [ceil(rows / 128)][ceil(cols / 128)];

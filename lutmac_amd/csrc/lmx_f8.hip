@@ -2,11 +2,14 @@
 // weights with a scale per 128 x 128 block, activations rounded to e4m3 with a
 // power of two per row and 128 columns, their products on the matrix cores.
 //
-// The fp8 matrix instructions align the products that they sum to the largest and
-// drop what lies below 2^-13 of it: 1.3e-5 of the result for normal data, far below
-// half a step of a 16-bit result (2^-9, 2^-12 on average), far above that of fp32.
-// Results in fp32 therefore come from the fp16 instructions, which hold an e4m3
-// number exactly and sum in fp32, at half the rate.
+// The products are made by the fp16 matrix instructions, which hold an e4m3 number
+// exactly and sum in fp32.  The fp8 ones take half the time, but of every eight
+// neighbouring k they drop what lies below 2^-13 of the largest product (measured:
+// seven small ones beside a large one vanish): up to 7 * 2^-13 of a sum of one
+// sign, more than half a step of fp16 and, near a border, a whole step of bf16.
+// What that costs: nothing to speak of up to 64 rows, where the weights' bytes bound
+// the call, a tenth to a third up to 1000, the matrix cores' factor of two beyond
+// (8192 x 2048 -> 16384 275 us with the fp8 instructions, 490 so).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -20,7 +23,6 @@ namespace lmx {
 namespace {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
-typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
@@ -149,25 +151,15 @@ __device__ __forceinline__ v8h halves(int lo, int hi) {   // 8 codes -> fp16, ex
             c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
   return v8h{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
-// What the instructions take: the codes, or for fp32 results fp16.
-template <bool EXACT>
+// The operand as the instructions take it.
 struct Factor {
-  v8i v;
-  __device__ __forceinline__ explicit Factor(const Operand &o) : v(__builtin_shufflevector(o.a, o.b, 0, 1, 2, 3, 4, 5, 6, 7)) {}
-  Factor() = default;
-};
-template <>
-struct Factor<true> {
   v8h v[4];
   __device__ __forceinline__ explicit Factor(const Operand &o)
       : v{halves(o.a[0], o.a[1]), halves(o.a[2], o.a[3]), halves(o.b[0], o.b[1]), halves(o.b[2], o.b[3])} {}
   Factor() = default;
 };
 // The sums of a block of 128: lane (j, g) gets weight rows 4 g .. + 3 of activation row j.
-__device__ __forceinline__ v4f products(const Factor<false> &w, const Factor<false> &x) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, x.v, v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0, 0, 0, 0);
-}
-__device__ __forceinline__ v4f products(const Factor<true> &w, const Factor<true> &x) {
+__device__ __forceinline__ v4f products(const Factor &w, const Factor &x) {
   v4f p = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int q = 0; q < 4; ++q) p = __builtin_amdgcn_mfma_f32_16x16x32_f16(w.v[q], x.v[q], p, 0, 0, 0);
@@ -214,11 +206,10 @@ __device__ __forceinline__ bool vector_rows(const F8Args &a) {
 // another before the end.  Every workgroup makes the codes itself, in LDS while its
 // first weights are on their way (R >= batch rows, a power of two; at most 16 values
 // a thread, which stay in registers), which saves a launch and the trip through memory
-// (1 x 2048 -> 16384 7.2 us, 4.7 TB/s).
+// (1 x 2048 -> 16384 7.6 us, 4.4 TB/s).
 constexpr int rows_buffers(int waves) { return waves == 16 ? 3 : 4; }
 template <class T, int W, int R>
 __global__ __launch_bounds__(W *kWave) void f8_rows_kernel(F8Args a) {
-  constexpr bool EXACT = std::is_same<T, float>::value;
   constexpr int U = rows_buffers(W), RB = 16 * kStep;
   __shared__ v4f part[W][kWave];
   extern __shared__ __attribute__((aligned(1024))) char lds[];   // the waves' buffers, codes [batch][Kp + 16], factors [batch][steps]
@@ -279,7 +270,7 @@ __global__ __launch_bounds__(W *kWave) void f8_rows_kernel(F8Args a) {
     const float f = fc[step];
     if (t + U - 1 < turns) fill(buf == 0 ? U - 1 : buf - 1, t + U - 1);   // (the buffer of the step before, whose products are made)
     if (a.cols - step * kStep < kStep) w.cut(a.cols - step * kStep, g);
-    add_scaled(acc, products(Factor<EXACT>(w), Factor<EXACT>(x)), f);
+    add_scaled(acc, products(Factor(w), Factor(x)), f);
     buf = buf == U - 1 ? 0 : buf + 1;
   }
   part[wave][lane] = acc;
@@ -295,12 +286,11 @@ __global__ __launch_bounds__(W *kWave) void f8_rows_kernel(F8Args a) {
 // Some rows of activations (up to 16 G) and so few weight rows that tiles of
 // 64 x 64 leave CUs idle: 16 R weight rows a workgroup, its W waves the k-steps w,
 // w + W, ..., each through U LDS buffers of its own as above (weights, codes, the
-// codes' scales; 48 x 8960 -> 1536 7.5 us).  Where that is few workgroups, blockIdx.y takes a part of k: the parts'
+// codes' scales; 48 x 8960 -> 1536 9.2 us).  Where that is few workgroups, blockIdx.y takes a part of k: the parts'
 // sums go past the caches, and the last workgroup of a row tile to finish adds them in
 // their order.
 template <class T, int W, int R, int G, int U>
 __global__ __launch_bounds__(W *kWave) void f8_few_kernel(F8Args a) {
-  constexpr bool EXACT = std::is_same<T, float>::value;
   constexpr int CB = (R + G) * 16 * kStep, RB = CB + 64 * 4;   // bytes of a buffer: weights, codes, 64 scales
   constexpr int LOADS = 2 * (R + G) + 1;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
@@ -356,12 +346,12 @@ __global__ __launch_bounds__(W *kWave) void f8_few_kernel(F8Args a) {
     if (a.cols - step * kStep < kStep)
 #pragma unroll
       for (int r = 0; r < R; ++r) w[r].cut(a.cols - step * kStep, g);
-    Factor<EXACT> wv[R];
+    Factor wv[R];
 #pragma unroll
-    for (int r = 0; r < R; ++r) wv[r] = Factor<EXACT>(w[r]);
+    for (int r = 0; r < R; ++r) wv[r] = Factor(w[r]);
 #pragma unroll
     for (int n = 0; n < G; ++n) {
-      const Factor<EXACT> xv(x[n]);
+      const Factor xv(x[n]);
 #pragma unroll
       for (int r = 0; r < R; ++r) add_scaled(acc[r][n], products(wv[r], xv), f[n]);
     }
@@ -419,17 +409,13 @@ __global__ __launch_bounds__(W *kWave) void f8_few_kernel(F8Args a) {
 // Many rows of activations: BN weight rows x BM activation rows per workgroup,
 // WN x WM waves, a block of 128 k per step through S LDS buffers that are filled
 // straight from memory S - 1 steps ahead.  Each step's products are summed apart and
-// enter the result with the step's two scales: 4 fused products of the vector unit for each matrix
-// instruction, half its time.  8192 x 2048 -> 16384 takes 253 to 302 us (the clock falls
-// under load), 2.2 to 1.8 PFLOP/s, matrix cores busy 0.49 and the vector unit 0.40 of
-// the cycles, 128 KB of results a tile written meanwhile; with the operands of the
-// first product not read first 288.
+// enter the result with the step's two scales.  8192 x 2048 -> 16384 takes 465 to 530 us (the
+// clock falls under load), 1.2 to 1.0 PFLOP/s, the rate of a library's fp16 product.
 //
 // PART: workgroup (tile, part) takes part blockIdx.y of k and leaves its sums for
 // f8_join_kernel: where tiles are few and k is long.
 template <class T, bool PART, int BN, int BM, int WN, int WM, int S>
 __global__ __launch_bounds__(WN *WM *kWave) __attribute__((amdgpu_waves_per_eu(2))) void f8_tile_kernel(F8Args a) {
-  constexpr bool EXACT = std::is_same<T, float>::value;
   constexpr int W = WN * WM, NW = BN / WN, MW = BM / WM, TN = NW / 16, TM = MW / 16;
   constexpr int CB = (BN + BM) * kStep, RB = CB + BM * 4;   // bytes of a buffer: weights, codes, the codes' scales
   constexpr int SL = BM / 4 / W;   // lanes of a wave that load scales
@@ -523,20 +509,20 @@ __global__ __launch_bounds__(WN *WM *kWave) __attribute__((amdgpu_waves_per_eu(2
     for (int m = 0; m < TM; ++m) f[m] = sl[16 * m];
     __builtin_amdgcn_sched_barrier(0);
     v4f p[2][TN];
-    Factor<EXACT> wv[TN];
+    Factor wv[TN];
 #pragma unroll
     for (int m = 0; m <= TM; ++m) {
       if (m + 1 < TM) ahead = read(xl, m + 1);
-      Factor<EXACT> xv{};
-      if (m < TM) xv = Factor<EXACT>(x);
+      Factor xv{};
+      if (m < TM) xv = Factor(x);
       const float fm = m > 0 ? f[m - 1] * wnow : 0.0f;
 #pragma unroll
       for (int n = 0; n < TN; ++n) {
-        if (m == 0) wv[n] = Factor<EXACT>(w[n]);
+        if (m == 0) wv[n] = Factor(w[n]);
         if (m < TM) p[m % 2][n] = products(wv[n], xv);
         if (m > 0) add_scaled(acc[n][m - 1], p[(m + 1) % 2][n], fm);
-        if (EXACT ? n == TN - 1 : true) __builtin_amdgcn_sched_barrier(0);
       }
+      __builtin_amdgcn_sched_barrier(0);
       x = ahead;
       if (m == 0 && s + S - 1 < steps) fill(buf == 0 ? S - 1 : buf - 1, s0 + s + S - 1);
     }
@@ -623,9 +609,8 @@ size_t tile_count(size_t rows, size_t batch, size_t side) { return (rows + side 
 
 // Up to 64 activation rows go to f8_few_kernel, unless tiles of 64 x 64 are just
 // one round of the CUs; 32 weight rows a workgroup read the codes less often (us in a
-// graph, bf16, tiles / 16 weight rows / 32: 16 x 2048 -> 2048 10.7 / 5.6 / -, 48 x 8960 ->
-// 1536 31 / 15.9 / 18.8, 48 x 2048 -> 8192 12.3 / 11.5 / 9.5, 48 x 8192 -> 24576 62 / 74 /
-// 60, 48 x 2048 -> 16384, one round, 14.3 / 19.5 / 14.9).
+// graph, bf16, tiles / 16 weight rows / 32: 48 x 2048 -> 4096 13.9 / 7.7 / 8.7, 48 x 2048 ->
+// 8192 14.4 / 11.9 / 9.9, 48 x 2048 -> 16384, one round, 15.7 / 20.3 / 16.1).
 enum class FewShape { none, rows16, rows32 };
 FewShape few_shape(size_t rows, size_t batch) {
   const size_t tiles = tile_count(rows, batch, 64);
@@ -635,8 +620,8 @@ FewShape few_shape(size_t rows, size_t batch) {
 
 // Parts of k for f8_few_kernel's 16 weight rows: as many as bring its workgroups to
 // one per CU, of 16 steps at least (us, in one part / in parts: 48 x 8960 -> 1536 in 2
-// 15.9 / 12.7, 16 x 8960 -> 1536 12.0 / 10.4, 48 x 4096 -> 2048 in 2 9.5 / 9.0, 48 x 4096 -> 1024 in
-// 2 7.7 / 8.1).
+// 15.8 / 12.8, 16 x 8960 -> 1536 in 2 11.8 / 10.5, 48 x 4096 -> 2048 in 2 9.8 / 9.2, 48 x 4096 -> 1024 in
+// 2 8.6 / 8.6).
 int few_parts(size_t rows, size_t cols) {
   const size_t tiles = (rows + 15) / 16, steps = round_up(cols, kStep) / kStep;
   return int(std::max<size_t>(1, std::min<size_t>(256 / tiles, steps / 16)));
@@ -644,7 +629,7 @@ int few_parts(size_t rows, size_t cols) {
 
 // Parts of k for other calls of few tiles: as many as bring the 64 x 64 tiles to
 // one per CU, of 8 steps at least, if they are three (us, in one part / in parts:
-// 100 x 8960 -> 1536 in 5 31.6 / 17.8, 200 x 8192 -> 1024 in 4 29.8 / 18.7).
+// 100 x 8960 -> 1536 in 5 42 / 19.5, 200 x 8192 -> 1024 in 4 40 / 20.9).
 int split_count(size_t rows, size_t cols, size_t batch) {
   if (few_shape(rows, batch) != FewShape::none) return few_shape(rows, batch) == FewShape::rows16 ? few_parts(rows, cols) : 1;
   const size_t tiles = tile_count(rows, batch, 64), steps = round_up(cols, kStep) / kStep;
@@ -653,8 +638,8 @@ int split_count(size_t rows, size_t cols, size_t batch) {
 }
 
 // More waves share a row tile's k where the tiles alone leave CUs idle (us, 4 / 8 /
-// 16 waves: 1 x 8192 -> 2048 10.8 / 7.0 / 6.9, 1 x 2048 -> 8192 6.0 / 5.7 / 7.1, 1 x 2048 ->
-// 16384 8.9 / 10.0 / 12.6).
+// 16 waves: 1 x 8192 -> 2048 - / 7.3 / 7.0, 1 x 2048 -> 8192 6.1 / 5.9 / 7.5, 1 x 2048 ->
+// 16384 9.1 / 10.4 / 13.3).
 int rows_waves(const F8Args &a) {
   const int tiles = (a.rows + 15) / 16;
   return tiles <= 256 ? 16 : tiles <= 768 ? 8 : 4;
@@ -678,8 +663,8 @@ int launch_rows(const F8Args &a, hipStream_t st) {
 
 // Whether every workgroup makes the codes itself: up to 4 rows, as long as that
 // is two rounds of a workgroup's threads, and not too often for nothing (us,
-// itself / codes in a launch before: 1 x 2048 -> 16384 8.9 / 11.4, 2 x 2048 -> 16384 10.5 /
-// 11.3, 4 x 2048 -> 2048 3.9 / 5.6, 2 x 2048 -> 65536 32.9 / 30.9).
+// itself / codes in a launch before: 1 x 2048 -> 16384 9.2 / 11.8, 2 x 2048 -> 16384 11.1 /
+// 12.0, 4 x 2048 -> 2048 4.0 / 5.7, 2 x 2048 -> 65536 33.3 / 31.8).
 int row_slots(const F8Args &a) { return a.batch <= 2 ? a.batch : 4; }
 bool in_one_launch(const F8Args &a) {
   return a.batch <= 4 && row_slots(a) * a.Kp <= 1024 * rows_waves(a) && (a.batch == 1 || a.rows <= 32768);
@@ -732,14 +717,11 @@ int launch_linear(const F8Args &a, hipStream_t st) {
     f8_join_kernel<T><<<unsigned((size_t(a.batch) * ((a.rows + 3) / 4) + 255) / 256), 256, 0, st>>>(a);
     return launch_err("f8 join");
   }
-  // The largest tiles that still fill most of the CUs, as larger ones read less
-  // from the L2s (us, bf16, 256 / 128 / 64: 2048 x 2048 -> 8192 41 / 51 / 82, 1024 x 2048 ->
-  // 8192 37 / 29 / 48, 256 x 2048 -> 16384 37 / 25 / 28, 517 x 1400 -> 3001 28 / 17.5 / 12.9;
-  // fp32, 128 / 64: 2048 x 2048 -> 8192 76 / 109; its operands as fp16 leave no registers for 256).
-  const size_t rows = a.rows, batch = a.batch;
-  if constexpr (!std::is_same<T, float>::value)
-    if (tile_count(rows, batch, 256) >= 192) return launch_tile<T, false, 256, 256, 4, 2, 2>(a, st);
-  if (tile_count(rows, batch, 128) >= 160) return launch_tile<T, false, 128, 128, 2, 2, 2>(a, st);
+  // The larger tiles where they still fill most of the CUs, as they read less from the
+  // L2s (us, bf16, 128 / 64: 2048 x 2048 -> 8192 70 / 106, 1024 x 2048 -> 8192 40 / 58, 256 x
+  // 2048 -> 16384 28 / 33, 512 x 2048 -> 4096 26 / 19.6, 517 x 1400 -> 3001 21 / 15.7; 256 x
+  // 128 take 498 for 8192 x 2048 -> 16384 where 128 x 128 take 500).
+  if (tile_count(a.rows, a.batch, 128) >= 160) return launch_tile<T, false, 128, 128, 2, 2, 2>(a, st);
   return launch_tile<T, false, 64, 64, 2, 2, 4>(a, st);
 }
 
