@@ -123,7 +123,8 @@ int lmx_kv8_attention(const lmx_kv8_cache *cache, const lmx_kv8_batch *batch,
 typedef struct {
   int32_t *pages;      /* [n_seqs][max_pages] */
   int32_t *lengths;    /* [n_seqs] */
-  int32_t *free_pages; /* [n_pages], the stack: the last of the first n_free[0] is on top */
+  int32_t *free_pages; /* [n_pages], the stack of pages 0 .. n_pages - 1 that nobody has: the last of the
+                          first n_free[0] is on top */
   int32_t *n_free;     /* [1] */
   size_t n_seqs;       /* <= 2^20 */
   size_t max_pages;    /* <= 2^24 */
@@ -151,7 +152,10 @@ int lmx_kv8_extend(const lmx_kv8_pages *pages, const int32_t *new_tokens, size_t
  * sequence s: drafts that were rejected, or a sequence that has ended.  Pages that
  * hold none of its tokens any more go back to the stack (their table entries
  * become -1), those of the first sequence on top and of each sequence the earliest, so
- * that taking back what one lmx_kv8_extend granted restores the stack. */
+ * that taking back what one lmx_kv8_extend granted restores the stack.  Entries that
+ * are no pages (outside 0 .. n_pages - 1: places that the caller gave up before) become
+ * -1 too and reach nothing.  (Not so in a call that finds a length past its table row,
+ * which these calls never make: there all entries go back as they are.) */
 int lmx_kv8_trim(const lmx_kv8_pages *pages, const int32_t *drop, void *stream);
 
 /* Rotates rows to their positions: for row r and each head of q ([n_heads]

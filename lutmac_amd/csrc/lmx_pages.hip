@@ -62,13 +62,17 @@ __device__ __forceinline__ uint32_t pages_of(uint32_t tokens) { return (tokens +
 // place `top` down), taken from it or (PUSH) given back.  One or two by the thread
 // itself, of up to kLong by 16 lanes, kAtOnce times 4 sequences at a time with their
 // loads on the way together, of more by the wave (1000 sequences of 31 pages in one
-// workgroup: 41 us thread by thread, 17 a wave for each, 11 so).
+// workgroup: 41 us thread by thread, 17 a wave for each, 11 so).  Returns whether what this
+// thread gave back held an entry that is no page.
 constexpr int kAtOnce = 4, kLong = 128;
+__device__ __forceinline__ bool is_page(const PagesArgs &a, int page) { return uint32_t(page) < uint32_t(a.n_pages); }
 template <bool PUSH>
-__device__ __forceinline__ void move_pages(const PagesArgs &a, uint32_t n, size_t first, uint32_t top) {
+__device__ __forceinline__ bool move_pages(const PagesArgs &a, uint32_t n, size_t first, uint32_t top) {
+  bool hole = false;
   const auto take = [&](size_t entry, uint32_t place) __attribute__((always_inline)) { return PUSH ? a.pages[entry] : a.free_pages[place]; };
   const auto give = [&](size_t entry, uint32_t place, int page) __attribute__((always_inline)) {
     a.pages[entry] = PUSH ? -1 : page;
+    if (PUSH) hole |= !is_page(a, page);
     if (PUSH && place < uint32_t(a.n_pages)) a.free_pages[place] = page;   // (pages freed twice may be more than there are)
   };
   if (n <= 2)
@@ -122,6 +126,7 @@ __device__ __forceinline__ void move_pages(const PagesArgs &a, uint32_t n, size_
       if (!__builtin_amdgcn_ballot_w64(more)) break;
     }
   }
+  return hole;
 }
 
 // Row r is the token at `pos` of sequence s.
@@ -296,13 +301,16 @@ __global__ __launch_bounds__(256) void rows_kernel(PagesArgs a) {
 
 __global__ __launch_bounds__(kThreads) void trim_kernel(PagesArgs a) {
   __shared__ uint32_t waves[1][kWaves];
+  __shared__ int holes;
   const uint32_t have = uint32_t(min(max(*a.n_free, 0), a.n_pages));
-  struct Cut { uint32_t keep, kept, gone; bool live; };
+  if (threadIdx.x == 0) holes = 0;
+  struct Cut { uint32_t keep, kept, gone; bool live, past; };   // past: longer than the table row
   const auto cut = [&](int s) {
     Cut c{};
     c.live = s < a.n_seqs;
     if (!c.live) return c;
     const uint32_t old = uint32_t(max(a.lengths[s], 0)), drop = uint32_t(max(a.count[s], 0));
+    c.past = old > a.max_pages * kPage;
     c.keep = old - min(old, drop);
     c.kept = uint32_t(min(size_t(pages_of(c.keep)), a.max_pages));
     c.gone = uint32_t(min(size_t(pages_of(old)), a.max_pages)) - c.kept;
@@ -319,10 +327,25 @@ __global__ __launch_bounds__(kThreads) void trim_kernel(PagesArgs a) {
     uint32_t v[1] = {c.gone};
     block_sums<1>(v, before, waves);
     if (a.n_seqs <= kThreads) all[0] = before[0];
-    move_pages<true>(a, c.gone, size_t(s) * a.max_pages + c.kept, have + all[0] - 1 - (v[0] - c.gone));
+    const bool hole = move_pages<true>(a, c.gone, size_t(s) * a.max_pages + c.kept, have + all[0] - 1 - (v[0] - c.gone));
+    if (hole | c.past) atomicOr(&holes, int(hole) | 2 * int(c.past));
     if (c.live) a.lengths[s] = int(c.keep);
   }
-  if (threadIdx.x == 0) *a.n_free = int(min(add_sat(have, all[0]), uint32_t(a.n_pages)));
+  __syncthreads();
+  const uint32_t end = min(add_sat(have, all[0]), uint32_t(a.n_pages));
+  uint32_t pages[1] = {end - have};
+  if (holes == 1) {   // what is no page leaves the stack again (a chunk is read before any of it is written)
+    pages[0] = 0;
+    for (uint32_t p0 = have; p0 < end; p0 += kThreads) {
+      const uint32_t p = p0 + threadIdx.x;
+      const int page = p < end ? a.free_pages[p] : -1;
+      const bool ok = is_page(a, page);
+      uint32_t v[1] = {ok};
+      block_sums<1>(v, pages, waves);
+      if (ok) a.free_pages[have + v[0] - 1] = page;
+    }
+  }
+  if (threadIdx.x == 0) *a.n_free = int(have + pages[0]);
 }
 
 int launch_err(const char *what) {
