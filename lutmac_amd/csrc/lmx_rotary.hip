@@ -73,11 +73,15 @@ __device__ __forceinline__ void turn_unit(const RotaryArgs &a, const T *in, T *o
   }
 }
 
-// A workgroup a row, its threads the units of all heads, two each at most 512 wide:
-// bound by memory (16384 rows of 40 heads of 128, bf16: 61 us, 5.6 TB/s; 64 rows 2.7).
+// A workgroup a row, its up to 512 threads the units of all heads, shared evenly: bound by
+// memory (16384 rows of 40 heads of 128, bf16: 61 us, 5.6 TB/s; 64 rows 2.7).  Workgroups
+// lie in two dimensions, as one takes fewer than 2^32 threads.
+constexpr int kGroups = 1 << 20, kThreads = 512;
 template <class T, int E, bool INTER>
-__global__ __launch_bounds__(1024) void rotary_kernel(RotaryArgs a) {
-  const int row = int(blockIdx.x), pos = a.positions[row];
+__global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
+  const int row = int(blockIdx.y) * kGroups + int(blockIdx.x);
+  if (row >= a.rows) return;
+  const int pos = a.positions[row];
   if (pos < 0 || pos >= a.rope_n) return;
   const float2 *rope = a.rope + size_t(pos) * (a.rd / 2);
   const int total = (a.heads[0] + a.heads[1]) * a.units;
@@ -97,9 +101,9 @@ int launch(RotaryArgs a, hipStream_t st) {
   a.units = a.turning + (a.hd - a.rd) / E;
   // (exact while units * at < 2^31: at most 1024 units, 2048 heads)
   a.unit_inv = ((1u << 31) + a.units - 1) / a.units;
-  const size_t total = size_t(a.heads[0] + a.heads[1]) * a.units, rounds = (total + 511) / 512;
+  const size_t total = size_t(a.heads[0] + a.heads[1]) * a.units, rounds = (total + kThreads - 1) / kThreads;
   const unsigned threads = unsigned(round_up((total + rounds - 1) / rounds, kWave));
-  rotary_kernel<T, E, INTER><<<unsigned(a.rows), threads, 0, st>>>(a);
+  rotary_kernel<T, E, INTER><<<dim3(unsigned(std::min(a.rows, kGroups)), unsigned((a.rows + kGroups - 1) / kGroups)), threads, 0, st>>>(a);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? LMX_OK : fail(LMX_ERR_LAUNCH_FAILED, "rotary launch: %s", hipGetErrorString(e));
 }
