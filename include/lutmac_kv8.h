@@ -164,11 +164,13 @@ int lmx_kv8_trim(const lmx_kv8_pages *pages, const int32_t *drop, void *stream);
  * a s + b c) with (c, s) = rope[positions[r]][pair]; the rest is copied.
  * rope [rope_positions][rotary_dim / 2] pairs, 8-byte aligned.  interleaved 0: the
  * pairs are (d, d + rotary_dim / 2), as the reference's apply_rope has them
- * (embedding.cpp:36-75); 1: (2 d, 2 d + 1).  inverse 1: by -s, which undoes it and
- * is its gradient.  Rows whose position is negative or not below rope_positions are
+ * (embedding.cpp:36-75); 1: (2 d, 2 d + 1).  inverse 1: by -s, the transpose, which
+ * is its gradient, and undoes it where c^2 + s^2 = 1 (of a table whose pairs are m
+ * long, as some scalings make them, there and back is m^2).  Rows whose position is negative or not below rope_positions are
  * left out: neither read nor written.  q_out may be q, k_out k (with the same
- * stride); else they do not overlap.  Computed in fp32 and rounded once.  At most 1024 heads each, head_dim at most 1024,
- * rotary_dim even and at most head_dim; strides count elements and are at least a row's (rows <= 1: any);
+ * stride); else they do not overlap.  Computed in fp32 and rounded once.
+ * At most 2^24 rows, fewer than 2^31 rope_positions, 1024 heads each, head_dim at most 1024, rotary_dim even and
+ * at most head_dim; strides count elements and are at least a row's (rows <= 1: any);
  * alignment that of the elements (16 bytes, and sizes that are whole groups of 16
  * bytes, are faster). */
 int lmx_rotary(int type, const void *q, size_t q_stride, void *q_out, size_t q_out_stride,

@@ -86,7 +86,8 @@ def rotate(q, k, positions, rope, interleaved=False, inverse=False, q_out=None, 
     """lmx_rotary: q [rows, heads, head_dim] and k [rows, kv_heads, head_dim] (or None)
     turned to positions int32 [rows] by rope fp32 [positions, pairs, 2] (rope_table), the
     first 2 * pairs elements of each head, the rest copied; pairs lie half that apart or,
-    interleaved, side by side.  inverse: turned back, which is also the gradient.
+    interleaved, side by side.  inverse: by -sin, the gradient, which also turns back
+    what a table with cos^2 + sin^2 = 1 turned (a yarn table's `attention` comes in twice).
     Returns (q_out, k_out), which may be q and k (default new tensors; rows whose
     position the table lacks are not written).  Rows may lie any stride apart."""
     return on_stream(stream, torch_module().rotate, q, k, positions, rope, interleaved, inverse, q_out, k_out)
