@@ -607,14 +607,24 @@ int allow_lds(const void *kernel, size_t bytes) {
 
 size_t tile_count(size_t rows, size_t batch, size_t side) { return (rows + side - 1) / side * ((batch + side - 1) / side); }
 
-// Up to 64 activation rows go to f8_few_kernel, unless tiles of 64 x 64 are just
-// one round of the CUs; 32 weight rows a workgroup read the codes less often (us in a
-// graph, bf16, tiles / 16 weight rows / 32: 48 x 2048 -> 4096 13.9 / 7.7 / 8.7, 48 x 2048 ->
-// 8192 14.4 / 11.9 / 9.9, 48 x 2048 -> 16384, one round, 15.7 / 20.3 / 16.1).
+// Up to 64 activation rows go to f8_few_kernel, unless they are more than 32 and tiles of
+// 64 x 64 are three quarters of a round of the CUs or more: then its 16 or 32 weight rows
+// a workgroup read the codes too often.  32 read them less often than 16 where they still fill the
+// chip.  (us in a graph, bf16, tiles / 16 weight rows / 32:
+//   48 x 2048 ->  4096 13.9 /  7.7 /  8.7    64 x 2048 ->  4096 14.0 /  8.4 /  9.4
+//   48 x 2048 ->  8192 14.4 / 11.9 /  9.9    64 x 2048 ->  8192 14.5 / 13.3 / 10.7
+//   48 x 2048 -> 12288 14.8 / 16.0 / 14.7    64 x 2048 -> 12288 14.9 / 18.1 / 16.2
+//   48 x 2048 -> 16384 15.7 / 20.3 / 16.1    64 x 2048 -> 16384 15.9 / 22.7 / 17.5
+//   48 x 2048 -> 20000 20.4 / 24.0 / 20.4    64 x 2048 -> 20000 20.8 / 27.1 / 22.5
+//   48 x 2048 -> 32768 23.5 / 36.6 / 27.2    64 x 2048 -> 32768 24.1 / 41.4 / 29.9
+//   48 x 2048 -> 65536 43.6 / 68.1 / 49.5    64 x 2048 -> 65536 44.1 / 78.2 / 55.0
+//   64 x 8192 -> 24576 68.2 / 85.4 / 67.8    64 x 8192 -> 32768 75.6 / 110.7 / 86.5
+//   24 x 2048 -> 16384 15.4 / 14.6 / 13.5    24 x 2048 -> 32768 23.1 / 23.8 / 22.9
+//   24 x 2048 -> 65536 43.0 / 40.6 / 41.2    32 x 8192 -> 32768 74.0 / 77.3 / 74.7;
+// the other way: 32 x 512 -> 32768 10.2 / 13.3 / 13.2.)
 enum class FewShape { none, rows16, rows32 };
 FewShape few_shape(size_t rows, size_t batch) {
-  const size_t tiles = tile_count(rows, batch, 64);
-  if (batch > 64 || (batch > 16 && tiles >= 192 && tiles <= 256)) return FewShape::none;
+  if (batch > 64 || (batch > 32 && tile_count(rows, batch, 64) >= 192)) return FewShape::none;
   return batch > 16 && rows > 4096 ? FewShape::rows32 : FewShape::rows16;
 }
 
@@ -717,11 +727,11 @@ int launch_linear(const F8Args &a, hipStream_t st) {
     f8_join_kernel<T><<<unsigned((size_t(a.batch) * ((a.rows + 3) / 4) + 255) / 256), 256, 0, st>>>(a);
     return launch_err("f8 join");
   }
-  // The larger tiles where they still fill most of the CUs, as they read less from the
+  // The larger tiles where they are not half empty and still fill most of the CUs, as they read less from the
   // L2s (us, bf16, 128 / 64: 2048 x 2048 -> 8192 70 / 106, 1024 x 2048 -> 8192 40 / 58, 256 x
-  // 2048 -> 16384 28 / 33, 512 x 2048 -> 4096 26 / 19.6, 517 x 1400 -> 3001 21 / 15.7; 256 x
+  // 2048 -> 16384 28 / 33, 512 x 2048 -> 4096 26 / 19.6, 517 x 1400 -> 3001 21 / 15.7, 64 x 2048 -> 32768 30 / 24; 256 x
   // 128 take 498 for 8192 x 2048 -> 16384 where 128 x 128 take 500).
-  if (tile_count(a.rows, a.batch, 128) >= 160) return launch_tile<T, false, 128, 128, 2, 2, 2>(a, st);
+  if (a.batch > 64 && tile_count(a.rows, a.batch, 128) >= 160) return launch_tile<T, false, 128, 128, 2, 2, 2>(a, st);
   return launch_tile<T, false, 64, 64, 2, 2, 4>(a, st);
 }
 
