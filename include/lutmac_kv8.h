@@ -144,7 +144,10 @@ typedef struct {
  *   and tokens;
  *   positions [n_rows], slots [n_rows] (or NULL): each row's position in its
  *   sequence, and page * 64 + position % 64 (-1 where the row's page is negative).
- *   Rows from offsets[n_seqs] on stay as they are. */
+ *   Rows from offsets[n_seqs] on stay as they are.
+ * Rows are those granted: where a sequence is refused, the rows of those behind it move
+ * up, and what a program laid out by what it asked for (tokens, drafts) has to be taken
+ * from there: row r of sequence s, the (r - offsets[s])-th of its new tokens. */
 int lmx_kv8_extend(const lmx_kv8_pages *pages, const int32_t *new_tokens, size_t n_rows,
                    int32_t *offsets, int32_t *granted, int32_t *positions,
                    int64_t *slots, void *stream);

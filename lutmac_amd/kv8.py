@@ -18,6 +18,7 @@ call follows what they hold at each replay.
 back those that are dropped, without the host:
 
     offsets, granted, positions, _ = held.extend(new, positions)
+    at = asked_rows(asked, offsets, rows)         # of tokens laid out by what was asked
     q, k = rotate(q, k, positions, rope)          # (or let append rotate)
     cache.append(k, v, offsets, held.lengths, held.pages)
     out = cache.attend(q, offsets, held.lengths, held.pages)
@@ -93,6 +94,19 @@ def rotate(q, k, positions, rope, interleaved=False, inverse=False, q_out=None, 
     return on_stream(stream, torch_module().rotate, q, k, positions, rope, interleaved, inverse, q_out, k_out)
 
 
+def asked_rows(asked, offsets, rows):
+    """Where each of a step's rows lies among rows that were laid out before it was known
+    who is granted: offsets int32 [sequences + 1] as ``KvPages.extend`` gives them, asked
+    int32 [sequences] the first row of each sequence there.  Returns int64 [rows] (0
+    for rows behind the last), to index tokens and drafts with: a refused sequence's
+    rows are left out and those behind it move up.  Nothing is read on the host."""
+    if not asked.numel():
+        return torch.zeros(rows, dtype=torch.int64, device=offsets.device)
+    r = torch.arange(rows, dtype=offsets.dtype, device=offsets.device)
+    s = (torch.searchsorted(offsets, r, right=True) - 1).clamp_(0, asked.numel() - 1)
+    return torch.where(r < offsets[-1], asked[s] + r - offsets[s], 0).long()
+
+
 class KvPages:
     """Whose pages are whose, on the device: pages int32 [sequences, max_pages] as
     ``append`` and ``attend`` take them, lengths int32 [sequences], free int32 [pages]
@@ -122,7 +136,8 @@ class KvPages:
         (as many rows as the step has room for) and slots int64 [rows] (or None) receive
         each row's position and page * 64 + position % 64; rows past the last stay as they
         are.  Returns (offsets [sequences + 1], granted [sequences], positions, slots): a
-        sequence gets all its tokens or none."""
+        sequence gets all its tokens or none, and the rows of one that gets none are not
+        there (asked_rows)."""
         offsets, granted = on_stream(stream, self._ops.kv8_extend, *self._tensors, new, positions, slots, offsets, granted)
         return offsets, granted, positions, slots
 
