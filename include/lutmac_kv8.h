@@ -158,7 +158,13 @@ int lmx_kv8_extend(const lmx_kv8_pages *pages, const int32_t *new_tokens, size_t
  * that taking back what one lmx_kv8_extend granted restores the stack.  Entries that
  * are no pages (outside 0 .. n_pages - 1: places that the caller gave up before) become
  * -1 too and reach nothing.  (Not so in a call that finds a length past its table row,
- * which these calls never make: there all entries go back as they are.) */
+ * which these calls never make: there all entries go back as they are.)
+ * Caches are not touched.  Where dropped tokens were appended, the kept tokens of
+ * their last block of 16 were rounded to the scale that the dropped ones asked for
+ * (by half of it at most, beside half of their own: lmx_kv8_append), and a dropped token that was not finite
+ * leaves NaN in the block until it starts anew.  For a cache as if the dropped tokens had never been
+ * there, a program copies the block that the sequence's next token falls into (codes and
+ * scales, unless it is empty) before it appends, puts it back after the trim, and appends the kept rows again. */
 int lmx_kv8_trim(const lmx_kv8_pages *pages, const int32_t *drop, void *stream);
 
 /* Rotates rows to their positions: for row r and each head of q ([n_heads]

@@ -2,7 +2,8 @@
  * lutmac_verify.h -- verification of drafted tokens (C ABI): which of the tokens
  * that a cheaper model proposed a program keeps, and the token that follows them, so
  * that what comes out is distributed as if every token had been sampled from the
- * target model.
+ * target model whose logits are given (what a cache makes of tokens that were
+ * dropped again: lmx_kv8_trim).
  *
  * The reference samples one token at a time from its logits (Model::sample,
  * src/model.cpp:455-490); this is the same choice for several positions of many
