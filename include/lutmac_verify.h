@@ -50,11 +50,14 @@ int lmx_verify_drafts_workspace(const lmx_drafts *d, int type, size_t *bytes);
  * whose weights with those of the tokens before it exceed u1 times the sum of all.
  *   accepted [n_seqs]: drafted tokens kept; tokens [n_rows]: row by row the
  *   accepted tokens, then the sampled one, then -1.  (No rows: 0 and nothing.)
+ * A drafted token outside 0 .. vocab - 1 is not accepted, but it is no mark of
+ * "nothing drafted": the token is sampled from max(0, p - q) of the row's probs all
+ * the same (probs NULL: from p).  A sequence with fewer drafts has fewer rows.
  * A temperature of 0 (or below, or NaN) is the limit: p is 1 for the first of the
  * largest logits.  Logits of -inf have p = 0; a row whose logits are all -inf,
- * or with a NaN or +inf, accepts nothing and gives the token -1.  A drafted token
- * outside 0 .. vocab - 1 is not accepted.  Everything is computed in 64 bits from the
- * given numbers, so that tokens do not depend on how sums are ordered but where a
+ * or with a NaN or +inf, accepts nothing and gives the token -1.  Everything is summed
+ * and compared in 64 bits from the given numbers, each e^x to 2^-44 of itself, so
+ * that tokens are those of exact arithmetic, and do not depend on how sums are ordered, but where a
  * number is within some 2^-40 of a border.
  * logits: elements of `type`, row r at logits + r * stride (elements; at least
  * vocab), aligned to an element; probs fp32, row r at probs + r * probs_stride.
