@@ -43,6 +43,17 @@ void check(int status) {
   if (status != LMX_OK) raise_lmx(status, lmx_last_error());
 }
 
+// A type as torch's users know it (the names inside torch are others).
+const char *dtype_name(at::ScalarType t) {
+  switch (t) {
+  case at::kChar: return "int8";
+  case at::kInt: return "int32";
+  case at::kLong: return "int64";
+  case at::kFloat: return "float32";
+  case at::kFloat8_e4m3fn: return "float8_e4m3fn";
+  default: return c10::toString(t);
+  }
+}
 std::string text(const at::Tensor &t) {
   std::string s = std::string(c10::toString(t.scalar_type())) + " [";
   for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.size(i));
@@ -277,7 +288,7 @@ struct Linear {
         bias(args[3] != Py_None ? &tensor("bias", args[3]) : nullptr), given(args[4] != Py_None ? &tensor("y", args[4]) : nullptr),
         type(type_of("x", x)) {
     if (w.dim() != 2 || w.scalar_type() != codes || w.stride(1) != 1)
-      bad("w", w, std::string(c10::toString(codes)) + " [rows, cols] with neighbouring columns side by side");
+      bad("w", w, std::string(dtype_name(codes)) + " [rows, cols] with neighbouring columns side by side");
     rows = w.size(0), cols = w.size(1);
     if (x.dim() == 0 || x.size(-1) != cols || !x.is_contiguous()) bad("x", x, "contiguous, " + std::to_string(cols) + " values a row");
   }
@@ -353,7 +364,7 @@ const at::Tensor &whole(const char *name, PyObject *o, at::ScalarType type, at::
   if (t.scalar_type() != type || !has_sizes(t, sizes) || !t.is_contiguous()) {
     std::string s;
     for (const int64_t n : sizes) s += (s.empty() ? "" : ", ") + std::to_string(n);
-    bad(name, t, std::string("contiguous ") + c10::toString(type) + " [" + s + "]");
+    bad(name, t, std::string("contiguous ") + dtype_name(type) + " [" + s + "]");
   }
   return t;
 }
