@@ -210,7 +210,8 @@ int lmx_weight_codes_i8(const lmx_weight *w, int8_t *codes, size_t w_stride,
  * with amax <= 448 s (at least 2^-126), so that x / s is exact; c = x / s rounded
  * to e4m3 (ties to even), and
  *   y[b][r] = sum_j s[b][j] w_scale[r / 128][j] (sum of c w over k of block j) + bias[r],
- * rounded once to y's type.  Every product of codes is exact, sums are fp32.
+ * rounded once to y's type.  Every product of codes is exact, sums are fp32; s w_scale
+ * is formed in fp32 (beyond its range a block is infinite or NaN, below 2^-126 it loses bits).
  * w: codes, row r at w + r * w_stride (w and w_stride multiples of 16, the
  * stride at most 262144; cols any number up to 131072; the bytes between cols and
  * w_stride are not used); w_scale contiguous, [ceil(rows / 128)][ceil(cols / 128)];

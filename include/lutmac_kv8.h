@@ -143,7 +143,7 @@ typedef struct {
  *   pages: the new pages, taken from the top of the stack in the order of sequences
  *   and tokens;
  *   positions [n_rows], slots [n_rows] (or NULL): each row's position in its
- *   sequence, and page * 64 + position % 64 (-1 where the row's page is negative).
+ *   sequence, and page * 64 + position % 64 (-1 where the row's page is negative); n_rows at most 2^24.
  *   Rows from offsets[n_seqs] on stay as they are.
  * Rows are those granted: where a sequence is refused, the rows of those behind it move
  * up, and what a program laid out by what it asked for (tokens, drafts) has to be taken
