@@ -123,12 +123,12 @@ int lmx_kv8_attention(const lmx_kv8_cache *cache, const lmx_kv8_batch *batch,
 typedef struct {
   int32_t *pages;      /* [n_seqs][max_pages] */
   int32_t *lengths;    /* [n_seqs] */
-  int32_t *free_pages; /* [n_pages], the stack of pages 0 .. n_pages - 1 that nobody has: the last of the
-                          first n_free[0] is on top */
+  int32_t *free_pages; /* [n_pages], the stack of pages that nobody has (any that are not negative, each
+                          once): the last of the first n_free[0] is on top */
   int32_t *n_free;     /* [1] */
   size_t n_seqs;       /* <= 2^20 */
   size_t max_pages;    /* <= 2^24 */
-  size_t n_pages;      /* < 2^31 */
+  size_t n_pages;      /* places of the stack, < 2^31 */
 } lmx_kv8_pages;
 
 /* Makes room for new_tokens[s] tokens of every sequence s (none where it is 0 or
@@ -156,8 +156,8 @@ int lmx_kv8_extend(const lmx_kv8_pages *pages, const int32_t *new_tokens, size_t
  * hold none of its tokens any more go back to the stack (their table entries
  * become -1), those of the first sequence on top and of each sequence the earliest, so
  * that taking back what one lmx_kv8_extend granted restores the stack.  Entries that
- * are no pages (outside 0 .. n_pages - 1: places that the caller gave up before) become
- * -1 too and reach nothing.  (Not so in a call that finds a length past its table row,
+ * are no pages (negative: places that the caller gave up before) become -1 too and
+ * reach nothing.  (Not so in a call that finds a length past its table row,
  * which these calls never make: there all entries go back as they are.)
  * Caches are not touched.  Where dropped tokens were appended, the kept tokens of
  * their last block of 16 were rounded to the scale that the dropped ones asked for

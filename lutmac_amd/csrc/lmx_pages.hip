@@ -63,16 +63,15 @@ __device__ __forceinline__ uint32_t pages_of(uint32_t tokens) { return (tokens +
 // itself, of up to kLong by 16 lanes, kAtOnce times 4 sequences at a time with their
 // loads on the way together, of more by the wave (1000 sequences of 31 pages in one
 // workgroup: 41 us thread by thread, 17 a wave for each, 11 so).  Returns whether what this
-// thread gave back held an entry that is no page.
+// thread gave back held an entry that is no page (negative).
 constexpr int kAtOnce = 4, kLong = 128;
-__device__ __forceinline__ bool is_page(const PagesArgs &a, int page) { return uint32_t(page) < uint32_t(a.n_pages); }
 template <bool PUSH>
 __device__ __forceinline__ bool move_pages(const PagesArgs &a, uint32_t n, size_t first, uint32_t top) {
   bool hole = false;
   const auto take = [&](size_t entry, uint32_t place) __attribute__((always_inline)) { return PUSH ? a.pages[entry] : a.free_pages[place]; };
   const auto give = [&](size_t entry, uint32_t place, int page) __attribute__((always_inline)) {
     a.pages[entry] = PUSH ? -1 : page;
-    if (PUSH) hole |= !is_page(a, page);
+    if (PUSH) hole |= page < 0;
     if (PUSH && place < uint32_t(a.n_pages)) a.free_pages[place] = page;   // (pages freed twice may be more than there are)
   };
   if (n <= 2)
@@ -339,7 +338,7 @@ __global__ __launch_bounds__(kThreads) void trim_kernel(PagesArgs a) {
     for (uint32_t p0 = have; p0 < end; p0 += kThreads) {
       const uint32_t p = p0 + threadIdx.x;
       const int page = p < end ? a.free_pages[p] : -1;
-      const bool ok = is_page(a, page);
+      const bool ok = page >= 0;
       uint32_t v[1] = {ok};
       block_sums<1>(v, pages, waves);
       if (ok) a.free_pages[have + v[0] - 1] = page;

@@ -144,7 +144,7 @@ class KvPages:
     def trim(self, drop, stream=None):
         """lmx_kv8_trim: takes the last drop int32 [sequences] tokens back, and frees the
         pages that hold none any more.  A sequence ends with drop = its length.  Entries
-        of the table that are no pages (given up by the caller) are not freed.  Caches
+        of the table that are no pages (negative: given up by the caller) are not freed.  Caches
         are not touched: the last block of kept tokens stays rounded to the scale that the
         dropped ones had asked for (NaN, where they were not finite)."""
         on_stream(stream, self._ops.kv8_trim, *self._tensors, drop)

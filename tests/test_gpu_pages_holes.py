@@ -1,4 +1,4 @@
-"""Page tables with entries that are no pages (the caller took some out: a window that
+"""Page tables with entries that are no pages (negative: the caller took some out: a window that
 moved on, a prefix put elsewhere): lmx_kv8_trim gives back the others alone, so that no
 later sequence is granted a page that is none."""
 import random
@@ -30,13 +30,13 @@ def test_holes(cuda, n, most, share):
     for s in range(n):
         for j in range(-(-lengths[s] // PAGE)):
             if rng.random() < share:
-                table[s][j] = rng.choice([-1, -1, -5, pages, 2 ** 31 - 1, -2 ** 31])
+                table[s][j] = rng.choice([-1, -1, -5, -2 ** 31])
     held.pages.copy_(i32(table))
     drop = [rng.choice([0, lengths[s], rng.randint(0, lengths[s])]) for s in range(n)]
     gone = []
     for s in range(n):
         a, b = -(-(lengths[s] - drop[s]) // PAGE), -(-lengths[s] // PAGE)
-        gone += [p for p in table[s][a:b] if 0 <= p < pages]
+        gone += [p for p in table[s][a:b] if p >= 0]
         table[s][a:b] = [-1] * (b - a)
     held.trim(i32(drop))
     free += gone[::-1]
@@ -53,6 +53,23 @@ def test_holes(cuda, n, most, share):
     assert (slots[: int(offsets[-1])] >= 0).all()
     mine = held.pages[held.pages >= 0]
     assert mine.unique().numel() == mine.numel() == sum(-(-g // PAGE) for g in granted.tolist())
+
+
+@pytest.mark.parametrize("first", [1, 1000, 2 ** 31 - 41])
+def test_pages_of_other_numbers(cuda, first):
+    """A stack of pages that do not begin at 0 (a part of a cache, one without its page 0)."""
+    held = kv8.KvPages.empty(5, 4, 40)
+    held.free.add_(first)
+    was = held.free.clone()
+    lengths = [200, 1, 64, 0, 256]
+    held.extend(i32(lengths), torch.zeros(1000, dtype=torch.int32, device="cuda"))
+    assert held.pages[0].tolist() == list(range(first, first + 4))
+    held.trim(i32(lengths))
+    assert int(held.n_free) == 40 and torch.equal(held.free, was)
+    held.extend(i32(lengths), torch.zeros(1000, dtype=torch.int32, device="cuda"))
+    held.pages[0, 1] = -1
+    held.trim(i32(lengths))
+    assert int(held.n_free) == 39 and held.free[:39].tolist() == [p for p in was.tolist() if p != first + 1]
 
 
 def test_replays(cuda):
